@@ -239,6 +239,7 @@ def prepare(case, seed):
         i32 = dict(dtype=torch.int32, device="cuda")
         K = 2 * W
         st["cand"] = (torch.empty(B, K, device="cuda"), torch.empty(B, K, **i32), torch.empty(B, K, **i32))
+        st["work"] = torch.empty(B * W * (V // 2048 + 2) * (16 + 8 * K), dtype=torch.uint8, device="cuda")   # (what pieces of the rows have found)
         st["next"] = (torch.empty(B, W, device="cuda"), torch.empty(B, W, **i32), torch.empty(B, W, **i32))
     else:
         _, _, n_kv, D = MODELS[case["model"]][:4]
@@ -471,7 +472,7 @@ def _run_own(st, k):
                           window=st["window"])
         return st["out"]
     if k == "beam":
-        L.beam_select(st["logits"], st["scores"], st["case"]["beams"], st["stops"], *st["cand"], *st["next"])
+        L.beam_select(st["logits"], st["scores"], st["case"]["beams"], st["stops"], *st["cand"], *st["next"], st["work"])
         names = ("score", "token", "row", "next_score", "next_token", "next_row")
         return dict(zip(names, st["cand"] + st["next"]))
     if k == "fork":
