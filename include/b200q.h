@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define B200Q_VERSION 7
+#define B200Q_VERSION 8
 
 #define B200Q_OK 0
 #define B200Q_EINVAL (-1)   /* bad argument / unsupported shape            */
@@ -641,9 +641,84 @@ int b200q_sandwich_close(float* x_dev, const void* y_dev, int y_f32, int splits,
  * + eps) * w in the model dtype */
 int b200q_pass_begin(float* x_dev, const float* x0_dev, const float* step_dev, float* keep_dev, const float* w_dev,
                      void* out_dev, int T, int W, float eps, int dtype, void* stream);
+/* ---- a cache in 4 bits (kv4_ops.cu, kv4_attn.cu; layout and conversions: kv4.cuh) --------------------------------------------
+ * Sixteen neighbouring values of a head share a scale byte (five bits of exponent, three of mantissa: the upper byte of a half
+ * without its sign); a value is sign, two bits of exponent, one of mantissa: 0, .5, 1, 1.5, 2, 3, 4, 6 times the scale.  The
+ * scale is a sixth of the group's largest magnitude, rounded to nearest (even), from 2^-17 to 10240; values are rounded to
+ * nearest (even code).  Magnitudes above 61440 and infinities are held as 61440; a group with a NaN reads back as NaN.
+ * A layer is [num_blocks][n_kv] pages of 18 D bytes (16 tokens of a head: keys' codes, their scales, values' codes, their
+ * scales), 16-byte aligned; block tables, slots and tiles are those of the 16-bit cache.  D in {64, 128, 256}, block_size 16. */
+
+/* bytes of a page of all heads, 18 D n_kv; B200Q_EINVAL for sizes that there are none of */
+int64_t b200q_kv4_page_bytes(int n_kv, int D);
+/* b200q_rope_kvwrite into a 4-bit cache: q is rotated in place, rotated k and v are quantised into their slots; slot < 0: no
+ *     write, what lies there stays */
+int b200q_rope_kvwrite_q4(void* qkv_dev, const void* cos_sin_dev, const int32_t* positions_dev, const int32_t* slot_mapping_dev,
+                          void* kv4_layer_dev, int T, int n_q, int n_kv, int D, int block_size, void* stream);
+/* pages as pages of the 16-bit cache, exactly: page i of kv_out ([n_pages][2][n_kv][16][D] bf16, pieces permuted as there) is
+ *     page pages[i] of the 4-bit layer */
+int b200q_kv4_unpack(const void* kv4_layer_dev, const int32_t* pages_dev, int n_pages, void* kv_out_dev, int n_kv, int D,
+                     int block_size, void* stream);
+/* b200q_decode_attn_ex over a 4-bit cache (GQA group <= 8).  A sequence of no tokens gives zeros.  q rows 16-byte aligned. */
+int b200q_decode_attn_q4(const void* q_dev, int q_stride, void* out_dev, const void* kv4_layer_dev, const int32_t* block_table_dev,
+                         int bt_stride, const int32_t* ctx_lens_dev, int n_seqs, int n_q, int n_kv, int D, int block_size,
+                         float scale, float softcap, int window, void* stream);
+/* b200q_prefill_attn_seqs over a 4-bit cache.  The workspace (256-byte aligned, of b200q_prefill_attn_q4_workspace bytes for the
+ *     block table's n_seqs rows of bt_stride entries) holds the pages that the portions see as 16-bit ones; what is in it need not
+ *     be kept between calls.  GQA group <= 8, at D = 256 <= 4. */
+int64_t b200q_prefill_attn_q4_workspace(int n_seqs, int bt_stride, int n_kv, int D);
+int b200q_prefill_attn_q4(const void* q_dev, int q_stride, void* out_dev, const void* kv4_layer_dev, const int32_t* block_table_dev,
+                          int bt_stride, int n_seqs, const int32_t* tiles_dev, int n_tiles, int n_q, int n_kv, int D, int block_size,
+                          float scale, float softcap, int window, void* workspace_dev, int64_t workspace_bytes, void* stream);
+
+/* ---- beams (beam.cu) and their pages (pages.cu) ----------------------------------------------------------------------------
+ * Row r of a group of beams is r = group * beams + beam everywhere: logits, scores, block tables. */
+
+/* The K best continuations of every group (beams <= K <= 64, beams <= 32, V >= K): of the scores[r] + logits[r, v] - log sum_v exp
+ *     logits[r, v] of a group's rows the K largest, best first, of equal ones the lowest row, then the lowest token.  cand_* [groups, K]:
+ *     the value (fp32; compared in 64 bits), v, r.  next_* [groups, beams]: the first `beams` of them whose token is none of
+ *     stops[n_stops]; where there are fewer, value -infinity, token 0, the group's first row.  A row whose score is not finite, or
+ *     whose logits are all -infinity or one +infinity, counts as -infinity throughout; a NaN logit as -infinity.
+ *     next_scores may be scores.  logits and workspace are 16-byte aligned; the workspace need not be kept between calls. */
+int64_t b200q_beam_select_workspace(int groups, int beams, int64_t V, int K);
+int b200q_beam_select(const void* logits_dev, const float* scores_dev, int groups, int beams, int64_t V, const int32_t* stops_dev,
+                      int n_stops, int K, float* cand_scores_dev, int32_t* cand_tokens_dev, int32_t* cand_rows_dev,
+                      float* next_scores_dev, int32_t* next_tokens_dev, int32_t* next_rows_dev, void* workspace_dev,
+                      int64_t workspace_bytes, void* stream);
+/* Pages of any paged cache.  refs[p] (int32 [num_blocks]) is how many rows of block tables hold page p, 0: it is free; a row of
+ *     len tokens holds the first ceil(len / block_size) entries of its row (lens beyond the table's width count as its width).
+ *
+ * New row i (n_new of them) continues old row parents[i] of lens[parents[i]] tokens (outside 0 .. n_old - 1: it is empty and holds
+ *     nothing): it holds its parent's pages, and the page that its next token goes to is its own.  That is the lowest free page where
+ *     its parent's last page is full; the last page itself for the first row of a parent if no other row held it; else the lowest
+ *     free page, and pairs[i] = {the parent's last page, that page} says what is to be copied (b200q_pages_copy; {-1, -1}: nothing).
+ *     Free pages go out in the order of the rows; pages that become free by this call are free for later ones.  slots[i] =
+ *     page * block_size + place of the next token, -1 where there is none.  Old rows hold nothing any more: refs is kept up.
+ *     status[0] = pages that were missing (0: all is well; else nothing has changed, slots are -1), status[1] = rows whose table is
+ *     full (slot -1; they hold their parent's pages).  Entries of table_out behind a row's pages stay as they are; it must not
+ *     overlap `table`.  n_old, n_new <= 16384, block_size 16. */
+int b200q_pages_fork(const int32_t* table_dev, const int32_t* lens_dev, int n_old, const int32_t* parents_dev, int n_new, int bt_stride,
+                     int32_t* refs_dev, int num_blocks, int block_size, int32_t* table_out_dev, int32_t* slots_dev, int32_t* pairs_dev,
+                     int32_t* status_dev, void* stream);
+/* rows r with ends[r] != 0 (NULL: all) give back what they hold */
+int b200q_pages_free(const int32_t* table_dev, const int32_t* lens_dev, const int32_t* ends_dev, int n_rows, int bt_stride,
+                     int32_t* refs_dev, int num_blocks, int block_size, void* stream);
+/* page pairs[i][1] <- page pairs[i][0] in every layer, for i < n_pairs (and < *count_dev unless NULL); pairs with a number outside
+ *     0 .. num_blocks - 1 are passed over.  Layer l begins layer_stride * l bytes into kv.  No page may be both read and written. */
+int b200q_pages_copy(void* kv_dev, const int32_t* pairs_dev, int n_pairs, const int32_t* count_dev, int64_t page_bytes, int n_layers,
+                     int64_t layer_stride, int num_blocks, void* stream);
+/* Moves the pages in use to the front: status = {n, m}, n pages are in use, and the m of them behind page n - 1 go, in order, to the m
+ *     free ones before: pairs[0 .. m - 1] (room for num_blocks / 2 + 1) for b200q_pages_copy.  map[p] = page p's new number, -1: it was free.
+ *     table_out = the rows' entries renumbered (others stay; may be `table`); refs_out = counts of the new numbers (may be `refs`). */
+int b200q_pages_compact(const int32_t* table_dev, const int32_t* lens_dev, int n_rows, int bt_stride, const int32_t* refs_dev,
+                        int num_blocks, int block_size, int32_t* table_out_dev, int32_t* refs_out_dev, int32_t* map_dev,
+                        int32_t* pairs_dev, int32_t* status_dev, void* stream);
+/* test hook: so many CTAs share a sequence and head in b200q_decode_attn_q4 (0: chosen) */
+int b200q_decode_attn_q4_set_splits(int splits);
+
 /* nonzero once a kernel's bounded wait has run out in this process (its outputs are then missing or wrong); engine steps report
- * it as B200Q_ECUDA.  Calls return before their kernels run: who calls b200q_gemm_* (up to 128 rows), b200q_prefill_attn* or the
- * layered attention directly asks here once the stream has been waited for. */
+ * it as B200Q_ECUDA.  Calls return before their kernels run: who calls b200q_gemm_* (up to 128 rows), b200q_prefill_attn*,
+ * b200q_decode_attn_q4 or the layered attention directly asks here once the stream has been waited for. */
 int b200q_wait_failures(void);
 
 /* ------------------------------------------------------------------------------------

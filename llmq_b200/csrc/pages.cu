@@ -1,0 +1,458 @@
+// pages.cu — pages of a paged cache between sequences: forks, ends, copies and moves.
+//
+// A cache's pages are numbered; a sequence's row of the block table names its pages; refs[p] says how many rows hold page p, 0: it is free.
+// That is all the state there is, so that a step's selection of beams needs no answer from the GPU before the next step can be enqueued.
+//   fork     rows become continuations of other rows.  Pages are shared; the page that a row's next token goes to is its own: the lowest free
+//            one where the old ones are full, the old last one for its first continuation if nobody else holds it, a copy for all others.
+//   free     rows end.
+//   copy     pages (all layers) as a list of pairs says.
+//   compact  the pages in use move to the front of the pool, as few of them as that takes.
+// Bound: fork and compact by latency (chains of a few dependent reads; a cluster of CTAs works on all rows and all pages at once, its
+// barriers between the steps), copies by the pages' bytes.  Results follow from the arguments alone: page numbers are given out in order of
+// rows and pages, counts change by atomic additions of whole numbers.
+#include "layered_common.cuh"
+#include "tcgen05.cuh"
+
+namespace b200q {
+
+constexpr int PG_THREADS = 1024, PG_CTAS = 8, PG_ROWS = 16384, PG_BLOCK = 16;
+
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// sum over the threads before this one, and over all (every thread of the CTA calls it)
+__device__ __forceinline__ int block_prefix(int v, int* total, int* scratch /* 33 */) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) scratch[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    int s = scratch[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += y;
+    }
+    scratch[lane] = s;
+  }
+  __syncthreads();
+  const int before = (warp ? scratch[warp - 1] : 0) + x - v;
+  *total = scratch[31];
+  __syncthreads();
+  return before;
+}
+
+// the share of [0, n) of this CTA of the cluster, cut at multiples of 4 (refs is read four at a time)
+struct PageShare {
+  int from, to;
+  __device__ __forceinline__ PageShare(int n) {
+    const int per = ((n + (int)gridDim.x - 1) / (int)gridDim.x + 3) / 4 * 4;
+    from = min(n, (int)blockIdx.x * per);
+    to = min(n, from + per);
+  }
+};
+// pages p .. p + 3 (those in [.., to)): their counts, others -1
+__device__ __forceinline__ int4 counts_of(const int32_t* refs, int p, int to, bool vec) {
+  if (vec && p + 4 <= to) return *reinterpret_cast<const int4*>(refs + p);
+  return make_int4(p < to ? refs[p] : -1, p + 1 < to ? refs[p + 1] : -1, p + 2 < to ? refs[p + 2] : -1, p + 3 < to ? refs[p + 3] : -1);
+}
+
+// one number per CTA of the cluster: the sums of those before this CTA and of all (every thread calls it; box: two ints, `turn` 0, 1, ...)
+__device__ __forceinline__ int cluster_prefix(int v, int* total, int* box, int turn) {
+  if (gridDim.x == 1) {
+    *total = v;
+    return 0;
+  }
+  if (threadIdx.x == 0) box[turn & 1] = v;
+  cluster_sync_all();
+  int before = 0, all = 0;
+  for (int c = 0; c < (int)gridDim.x; ++c) {
+    const int x = (int)ld_cluster_u32(mapa_shared(box + (turn & 1), c));
+    before += c < (int)blockIdx.x ? x : 0;
+    all += x;
+  }
+  *total = all;
+  return before;
+}
+__device__ __forceinline__ void rows_sync() {
+  if (gridDim.x == 1)
+    __syncthreads();
+  else
+    cluster_sync_all();
+}
+
+struct ForkArgs {
+  const int32_t *table, *lens, *parents;
+  int32_t *refs, *table_out, *slots;
+  int2* pairs;
+  int32_t* status;
+  int n_old, n_new, stride, num_blocks;
+};
+
+__global__ void __launch_bounds__(PG_THREADS, 1) pages_fork_kernel(ForkArgs a) {
+  follow_previous(a.table, a.lens, a.parents, a.refs, a.table_out, a.slots, a.pairs, a.status);
+  extern __shared__ int32_t rows[];
+  int32_t *first = rows, *count = rows + a.n_old, *fresh = rows + 2 * a.n_old;  // per old row; new rows that need a page, in order
+  __shared__ int scratch[33], box[2], no_column_s;
+  const int tid = threadIdx.x;
+  for (int i = tid; i < a.n_old; i += PG_THREADS) {
+    first[i] = 0x7fffffff;
+    count[i] = 0;
+  }
+  if (tid == 0) no_column_s = 0;
+  __syncthreads();
+  for (int i = tid; i < a.n_new; i += PG_THREADS) {
+    const int p = a.parents[i];
+    if (p >= 0 && p < a.n_old) {
+      atomicMin(first + p, i);
+      atomicAdd(count + p, 1);
+    }
+  }
+  __syncthreads();
+  const int most = a.stride * PG_BLOCK;
+  auto len_of = [&](int p) { return min(max(a.lens[p], 0), most); };
+  // ---- who needs a page (every CTA finds this out for all rows: it is a few reads per row, and nobody has to be told)
+  int n_fresh = 0;
+  for (int i0 = 0; i0 < a.n_new; i0 += PG_THREADS) {
+    const int i = i0 + tid, p = i < a.n_new ? a.parents[i] : -1;
+    bool need = false;
+    if (p >= 0 && p < a.n_old) {
+      const int len = len_of(p), last = len / PG_BLOCK;
+      if (last >= a.stride) {
+        if (blockIdx.x == 0) atomicAdd(&no_column_s, 1);
+      } else if (len % PG_BLOCK == 0) {
+        need = true;
+      } else {
+        const int page = a.table[(long long)p * a.stride + last];
+        need = !(first[p] == i && page >= 0 && page < a.num_blocks && a.refs[page] == 1);
+      }
+    }
+    int all;
+    const int before = block_prefix(need, &all, scratch);
+    if (need) fresh[n_fresh + before] = i;
+    n_fresh += all;
+  }
+  // ---- the free pages of this CTA's share, and of all
+  const PageShare share(a.num_blocks);
+  const bool vec = (reinterpret_cast<uintptr_t>(a.refs) & 15) == 0;
+  int mine = 0;
+  for (int p = share.from + 4 * tid; p < share.to; p += 4 * PG_THREADS) {
+    const int4 c = counts_of(a.refs, p, share.to, vec);
+    mine += (c.x == 0) + (c.y == 0) + (c.z == 0) + (c.w == 0);
+  }
+  int here, free_all;
+  block_prefix(mine, &here, scratch);
+  int rank = cluster_prefix(here, &free_all, box, 0);
+  const bool enough = free_all >= n_fresh;
+  if (blockIdx.x == 0 && tid == 0) {
+    a.status[0] = enough ? 0 : n_fresh - free_all;
+    a.status[1] = no_column_s;
+  }
+  if (!enough) {  // nothing changes, and nobody has a place to write to
+    for (int i = blockIdx.x * PG_THREADS + tid; i < a.n_new; i += gridDim.x * PG_THREADS) {
+      a.slots[i] = -1;
+      a.pairs[i] = make_int2(-1, -1);
+    }
+    if (gridDim.x > 1) cluster_sync_all();  // (a peer may still read this CTA's number)
+    return;
+  }
+  // ---- the k-th free page goes to the k-th row that needs one
+  for (int p0 = share.from; p0 < share.to && rank < n_fresh; p0 += 4 * PG_THREADS) {
+    const int p = p0 + 4 * tid;
+    const int4 c = p < share.to ? counts_of(a.refs, p, share.to, vec) : make_int4(-1, -1, -1, -1);
+    const bool is_free[4] = {c.x == 0, c.y == 0, c.z == 0, c.w == 0};
+    int all;
+    int k = rank + block_prefix(is_free[0] + is_free[1] + is_free[2] + is_free[3], &all, scratch);
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      if (is_free[x]) {
+        if (k < n_fresh) {
+          const int i = fresh[k], from = a.parents[i], len = len_of(from), last = len / PG_BLOCK;
+          a.refs[p + x] = 1;
+          a.table_out[(long long)i * a.stride + last] = p + x;
+          a.slots[i] = (p + x) * PG_BLOCK + len % PG_BLOCK;
+          a.pairs[i] = len % PG_BLOCK ? make_int2(a.table[(long long)from * a.stride + last], p + x) : make_int2(-1, -1);
+        }
+        ++k;
+      }
+    rank += all;
+  }
+  rows_sync();  // all free pages have been looked for: counts may change
+  // ---- tables of the new rows, slots of those that keep a page; then what the old rows' pages gain and lose.  A warp to a row
+  const int warp = (blockIdx.x * PG_THREADS + tid) >> 5, warps = (gridDim.x * PG_THREADS) >> 5, lane = tid & 31;
+  for (int i = warp; i < a.n_new; i += warps) {
+    const int p = a.parents[i];
+    if (p < 0 || p >= a.n_old) {
+      if (lane == 0) {
+        a.slots[i] = -1;
+        a.pairs[i] = make_int2(-1, -1);
+      }
+      continue;
+    }
+    const int len = len_of(p), last = len / PG_BLOCK;
+    const int32_t* from = a.table + (long long)p * a.stride;
+    int32_t* to = a.table_out + (long long)i * a.stride;
+    for (int c = lane; c < last; c += 32) to[c] = from[c];
+    if (lane == 0) {
+      if (last >= a.stride) {
+        a.slots[i] = -1;
+        a.pairs[i] = make_int2(-1, -1);
+      } else if (len % PG_BLOCK) {
+        // who has it was decided by counts that may have changed since: the list of rows that need a page says it
+        int lo = 0, hi = n_fresh;
+        while (lo < hi) {
+          const int mid = (lo + hi) / 2;
+          if (fresh[mid] < i)
+            lo = mid + 1;
+          else
+            hi = mid;
+        }
+        if (lo == n_fresh || fresh[lo] != i) {
+          to[last] = from[last];
+          a.slots[i] = from[last] * PG_BLOCK + len % PG_BLOCK;
+          a.pairs[i] = make_int2(-1, -1);
+        }
+      }
+    }
+  }
+  for (int p = warp; p < a.n_old; p += warps) {
+    const int len = len_of(p), full = len / PG_BLOCK, kids = count[p];
+    const int32_t* row = a.table + (long long)p * a.stride;
+    if (kids != 1)
+      for (int c = lane; c < full; c += 32) {
+        const int page = row[c];
+        if (page >= 0 && page < a.num_blocks) atomicAdd(a.refs + page, kids - 1);
+      }
+    if (lane == 0 && len % PG_BLOCK) {
+      bool kept = false;
+      if (kids > 0) {
+        const int i = first[p];
+        int lo = 0, hi = n_fresh;
+        while (lo < hi) {
+          const int mid = (lo + hi) / 2;
+          if (fresh[mid] < i)
+            lo = mid + 1;
+          else
+            hi = mid;
+        }
+        kept = lo == n_fresh || fresh[lo] != i;
+      }
+      const int page = row[full];
+      if (!kept && page >= 0 && page < a.num_blocks) atomicAdd(a.refs + page, -1);
+    }
+  }
+  if (gridDim.x > 1) cluster_sync_all();  // (nobody leaves while a peer may read its number)
+}
+
+// A warp to a row.
+__global__ void __launch_bounds__(256) pages_free_kernel(const int32_t* table, const int32_t* lens, const int32_t* ends, int n, int stride,
+                                                         int32_t* refs, int num_blocks) {
+  follow_previous(table, lens, ends, refs);
+  const int lane = threadIdx.x & 31;
+  for (int r = blockIdx.x * 8 + (threadIdx.x >> 5); r < n; r += gridDim.x * 8) {
+    if (ends && ends[r] == 0) continue;
+    const int pages = min((max(lens[r], 0) + PG_BLOCK - 1) / PG_BLOCK, stride);
+    for (int c = lane; c < pages; c += 32) {
+      const int p = table[(long long)r * stride + c];
+      if (p >= 0 && p < num_blocks) atomicAdd(refs + p, -1);
+    }
+  }
+}
+
+// An item is COPY_BYTES of one layer's page (the last one of a page may be shorter): eight pieces of 16 bytes per thread on their way at once.
+constexpr int COPY_THREADS = 256, COPY_AT_ONCE = 8, COPY_BYTES = COPY_THREADS * COPY_AT_ONCE * 16;
+__global__ void __launch_bounds__(COPY_THREADS) pages_copy_kernel(uint8_t* kv, const int2* pairs, const int32_t* count, int n, long long page_bytes,
+                                                                  int n_layers, long long layer_stride, int num_blocks) {
+  follow_previous(kv, pairs, count);
+  const int parts = (int)((page_bytes + COPY_BYTES - 1) / COPY_BYTES);
+  const long long items = (long long)(count ? min(max(count[0], 0), n) : n) * n_layers * parts;
+  for (long long it = blockIdx.x; it < items; it += gridDim.x) {
+    const int part = (int)(it % parts), layer = (int)(it / parts % n_layers);
+    const int2 pr = pairs[it / parts / n_layers];
+    if (pr.x < 0 || pr.y < 0 || pr.x >= num_blocks || pr.y >= num_blocks) continue;
+    uint8_t* base = kv + layer * layer_stride + (long long)part * COPY_BYTES;
+    const uint4* from = reinterpret_cast<const uint4*>(base + pr.x * page_bytes);
+    uint4* to = reinterpret_cast<uint4*>(base + pr.y * page_bytes);
+    const int pieces = (int)min((long long)COPY_BYTES, page_bytes - (long long)part * COPY_BYTES) / 16;
+    uint4 v[COPY_AT_ONCE];
+#pragma unroll
+    for (int u = 0; u < COPY_AT_ONCE; ++u)
+      if (u * COPY_THREADS + (int)threadIdx.x < pieces) v[u] = ld_once_v4(from + u * COPY_THREADS + threadIdx.x);
+#pragma unroll
+    for (int u = 0; u < COPY_AT_ONCE; ++u)
+      if (u * COPY_THREADS + (int)threadIdx.x < pieces) st_v4(to + u * COPY_THREADS + threadIdx.x, v[u]);
+  }
+}
+
+struct CompactArgs {
+  const int32_t *table, *lens, *refs;
+  int32_t *table_out, *refs_out, *map;
+  int2* pairs;
+  int32_t* status;
+  int n_rows, stride, num_blocks;
+};
+
+// n pages are in use.  Of two counts of pages in use, before page p and before page n, follow the places: free page p < n is number
+// p - before(p) of those that are filled, page p >= n in use is number before(p) - before(n) of those that fill them.
+__global__ void __launch_bounds__(PG_THREADS, 1) pages_compact_kernel(CompactArgs a) {
+  follow_previous(a.table, a.lens, a.refs, a.table_out, a.refs_out, a.map, a.pairs, a.status);
+  __shared__ int scratch[33], box[2];
+  const int tid = threadIdx.x;
+  const PageShare share(a.num_blocks);
+  const bool vec = (reinterpret_cast<uintptr_t>(a.refs) & 15) == 0;
+  int mine = 0;
+  for (int p = share.from + 4 * tid; p < share.to; p += 4 * PG_THREADS) {
+    const int4 c = counts_of(a.refs, p, share.to, vec);
+    mine += (c.x > 0) + (c.y > 0) + (c.z > 0) + (c.w > 0);
+  }
+  int here, n, below_all;
+  block_prefix(mine, &here, scratch);
+  int before = cluster_prefix(here, &n, box, 0);
+  int below = 0;
+  for (int p = share.from + 4 * tid; p < min(share.to, n); p += 4 * PG_THREADS) {
+    const int4 c = counts_of(a.refs, p, min(share.to, n), vec);
+    below += (c.x > 0) + (c.y > 0) + (c.z > 0) + (c.w > 0);
+  }
+  block_prefix(below, &here, scratch);
+  cluster_prefix(here, &below_all, box, 1);
+  const int moves = n - below_all;
+  if (blockIdx.x == 0 && tid == 0) {
+    a.status[0] = n;
+    a.status[1] = moves;
+  }
+  for (int p0 = share.from; p0 < share.to; p0 += 4 * PG_THREADS) {
+    const int p = p0 + 4 * tid;
+    const int4 c4 = p < share.to ? counts_of(a.refs, p, share.to, vec) : make_int4(-1, -1, -1, -1);
+    const int c[4] = {c4.x, c4.y, c4.z, c4.w};
+    int all;
+    int k = before + block_prefix((c[0] > 0) + (c[1] > 0) + (c[2] > 0) + (c[3] > 0), &all, scratch);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int id = p + x;
+      if (id >= share.to || p >= share.to) continue;
+      if (c[x] > 0) {
+        if (id < n) {
+          a.map[id] = id;
+          a.refs_out[id] = c[x];
+        } else {
+          a.pairs[k - below_all].x = id;
+        }
+        ++k;
+      } else {
+        a.map[id] = -1;
+        if (id < n)
+          a.pairs[id - k].y = id;
+        else
+          a.refs_out[id] = 0;
+      }
+    }
+    before += all;
+  }
+  rows_sync();
+  const int at = blockIdx.x * PG_THREADS + tid, threads = gridDim.x * PG_THREADS;
+  for (int k = at; k < moves; k += threads) {
+    const int2 pr = a.pairs[k];
+    a.map[pr.x] = pr.y;
+    a.refs_out[pr.y] = a.refs[pr.x];
+    a.refs_out[pr.x] = 0;  // (refs_out may be refs)
+  }
+  rows_sync();
+  for (int r = at >> 5; r < a.n_rows; r += threads >> 5) {
+    const int pages = min((max(a.lens[r], 0) + PG_BLOCK - 1) / PG_BLOCK, a.stride);
+    for (int c = tid & 31; c < pages; c += 32) {
+      const int p = a.table[(long long)r * a.stride + c];
+      a.table_out[(long long)r * a.stride + c] = p >= 0 && p < a.num_blocks ? a.map[p] : -1;
+    }
+  }
+}
+
+// CTAs of a cluster: one where a thread has a few pages and a warp a few rows
+static int page_ctas(int num_blocks, long long entries) { return num_blocks <= 16384 && entries <= 8192 ? 1 : PG_CTAS; }
+
+}  // namespace b200q
+
+using namespace b200q;
+
+extern "C" {
+
+int b200q_pages_fork(const int32_t* table, const int32_t* lens, int n_old, const int32_t* parents, int n_new, int bt_stride, int32_t* refs,
+                     int num_blocks, int block_size, int32_t* table_out, int32_t* slots, int32_t* pairs, int32_t* status, void* stream) {
+  B200Q_CHECK_ARG(n_old >= 0 && n_new >= 0 && n_old <= PG_ROWS && n_new <= PG_ROWS && bt_stride > 0 && bt_stride <= (1 << 26) && num_blocks > 0 &&
+                      num_blocks <= (1 << 27) && block_size == PG_BLOCK,
+                  "pages_fork: bad shape n_old=%d n_new=%d (up to %d) bt_stride=%d num_blocks=%d block_size=%d (16)", n_old, n_new, PG_ROWS, bt_stride,
+                  num_blocks, block_size);
+  B200Q_CHECK_ARG(refs && status && (n_old == 0 || (table && lens)) && (n_new == 0 || (parents && table_out && slots && pairs)),
+                  "pages_fork: null argument");
+  B200Q_CHECK_ARG(n_old == 0 || n_new == 0 ||
+                      !(table_out < table + (long long)n_old * bt_stride && table < table_out + (long long)n_new * bt_stride),
+                  "pages_fork: the new table must not overlap the old one");
+  B200Q_CHECK_ARG((reinterpret_cast<uintptr_t>(pairs) & 7) == 0, "pages_fork: pairs must be 8-byte aligned");
+  const size_t smem = (2 * (size_t)n_old + n_new) * 4;
+  static bool ready[64];
+  int dev = 0;
+  B200Q_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !ready[dev]) {
+    B200Q_CUDA(cudaFuncSetAttribute(pages_fork_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * PG_ROWS * 4));
+    if (dev < 64) ready[dev] = true;
+  }
+  const int ctas = page_ctas(num_blocks, (long long)(n_old > n_new ? n_old : n_new) * bt_stride);
+  const ForkArgs a{table, lens, parents, refs, table_out, slots, (int2*)pairs, status, n_old, n_new, bt_stride, num_blocks};
+  B200Q_CUDA(launch_early(pages_fork_kernel, dim3(ctas), PG_THREADS, smem, as_stream(stream), ctas, a));
+  count_launch();
+  return B200Q_OK;
+}
+
+int b200q_pages_free(const int32_t* table, const int32_t* lens, const int32_t* ends, int n_rows, int bt_stride, int32_t* refs, int num_blocks,
+                     int block_size, void* stream) {
+  B200Q_CHECK_ARG(n_rows >= 0 && bt_stride >= 0 && num_blocks > 0 && num_blocks <= (1 << 27) && block_size == PG_BLOCK,
+                  "pages_free: bad shape n_rows=%d bt_stride=%d num_blocks=%d block_size=%d (16)", n_rows, bt_stride, num_blocks, block_size);
+  if (n_rows == 0 || bt_stride == 0) return B200Q_OK;
+  B200Q_CHECK_ARG(table && lens && refs, "pages_free: null argument");
+  const int blocks = (n_rows + 7) / 8;
+  B200Q_CUDA(launch_early(pages_free_kernel, dim3(blocks < 4096 ? blocks : 4096), 256, 0, as_stream(stream), 1, table, lens, ends, n_rows, bt_stride, refs,
+                          num_blocks));
+  count_launch();
+  return B200Q_OK;
+}
+
+int b200q_pages_copy(void* kv, const int32_t* pairs, int n_pairs, const int32_t* count, int64_t page_bytes, int n_layers, int64_t layer_stride,
+                     int num_blocks, void* stream) {
+  B200Q_CHECK_ARG(n_pairs >= 0 && page_bytes > 0 && page_bytes % 16 == 0 && page_bytes < (1ll << 31) && n_layers >= 0 && layer_stride % 16 == 0 &&
+                      num_blocks > 0,
+                  "pages_copy: bad shape n_pairs=%d page_bytes=%lld n_layers=%d layer_stride=%lld num_blocks=%d (bytes in multiples of 16)", n_pairs,
+                  (long long)page_bytes, n_layers, (long long)layer_stride, num_blocks);
+  if (n_pairs == 0 || n_layers == 0) return B200Q_OK;
+  B200Q_CHECK_ARG(kv && pairs, "pages_copy: null argument");
+  B200Q_CHECK_ARG((reinterpret_cast<uintptr_t>(kv) & 15) == 0 && (reinterpret_cast<uintptr_t>(pairs) & 7) == 0,
+                  "pages_copy: the cache must be 16-byte aligned, pairs 8-byte");
+  const long long items = (long long)n_pairs * n_layers * ((page_bytes + COPY_BYTES - 1) / COPY_BYTES);
+  const long long most = 8LL * num_sms();
+  B200Q_CUDA(launch_early(pages_copy_kernel, dim3((unsigned)(items < most ? items : most)), COPY_THREADS, 0, as_stream(stream), 1, (uint8_t*)kv,
+                          (const int2*)pairs, count, n_pairs, (long long)page_bytes, n_layers, (long long)layer_stride, num_blocks));
+  count_launch();
+  return B200Q_OK;
+}
+
+int b200q_pages_compact(const int32_t* table, const int32_t* lens, int n_rows, int bt_stride, const int32_t* refs, int num_blocks, int block_size,
+                        int32_t* table_out, int32_t* refs_out, int32_t* map, int32_t* pairs, int32_t* status, void* stream) {
+  B200Q_CHECK_ARG(n_rows >= 0 && bt_stride >= 0 && bt_stride <= (1 << 26) && num_blocks > 0 && num_blocks <= (1 << 27) && block_size == PG_BLOCK,
+                  "pages_compact: bad shape n_rows=%d bt_stride=%d num_blocks=%d block_size=%d (16)", n_rows, bt_stride, num_blocks, block_size);
+  B200Q_CHECK_ARG(refs && refs_out && map && pairs && status && (n_rows == 0 || bt_stride == 0 || (table && lens && table_out)),
+                  "pages_compact: null argument");
+  B200Q_CHECK_ARG((reinterpret_cast<uintptr_t>(pairs) & 7) == 0, "pages_compact: pairs must be 8-byte aligned");
+  const int ctas = page_ctas(num_blocks, (long long)n_rows * bt_stride);
+  const CompactArgs a{table, lens, refs, table_out, refs_out, map, (int2*)pairs, status, bt_stride > 0 ? n_rows : 0, bt_stride, num_blocks};
+  B200Q_CUDA(launch_early(pages_compact_kernel, dim3(ctas), PG_THREADS, 0, as_stream(stream), ctas, a));
+  count_launch();
+  return B200Q_OK;
+}
+
+}  // extern "C"

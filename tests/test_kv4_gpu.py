@@ -1,0 +1,258 @@
+"""The 4-bit paged cache (csrc/kv4_ops.cu, csrc/kv4_attn.cu) through the C ABI: what is written, what is read back, and attention over
+it for single tokens and for prompts, against plain 64-bit forms (tests/kv4_util.py)."""
+import pytest
+import torch
+
+from tests.kv4_util import BF, BS, attention, attention_close, held, make_cache, read_pages, rope_rows, write_rows
+
+pytestmark = pytest.mark.gpu
+
+
+def same(a, b):
+    return torch.equal(torch.nan_to_num(a.double().cpu(), nan=1e30), torch.nan_to_num(b.double().cpu(), nan=1e30))
+
+
+def hard_rows(T, n, g):
+    """rows whose groups are zeros, tiny, subnormal, huge, infinite, NaN or full of values on the borders between two codes"""
+    x = torch.randn(T, n, generator=g) * torch.exp2(torch.randint(-20, 18, (T, n // 16), generator=g).float()).repeat_interleave(16, 1)
+    x = x.to(BF).view(T, n // 16, 16)
+    border = torch.tensor([6.0, 0.25, -0.75, 1.25, -1.75, 2.5, -3.5, 5.0, 0.0, -0.0, 0.5, 1.5, 3.0, -4.0, 2.0, -6.0])
+    scale = torch.exp2(torch.randint(-12, 11, (T, n // 16, 1), generator=g).float()) * (1 + torch.randint(0, 8, (T, n // 16, 1), generator=g) / 8)
+    kind = torch.randint(0, 10, (T, n // 16), generator=g)
+    x[kind == 1] = (border * scale)[kind == 1].to(BF)
+    x[kind == 2] = 0.0
+    x[kind == 3] = 1e-7
+    x[kind == 4] = (border * scale)[kind == 4].to(BF) * 1.5   # largest magnitudes of 9, 10.5, ...: scales on borders
+    x[(kind == 5), 3] = float("inf")
+    x[(kind == 6), 7] = float("nan")
+    x[(kind == 7), 0] = -3e38
+    return x.reshape(T, n)
+
+
+@pytest.mark.parametrize("D,n_q,n_kv", [(64, 4, 2), (128, 3, 3), (128, 8, 1), (256, 4, 2), (64, 0, 1)])
+@pytest.mark.parametrize("T", [1, 7, 333])
+@pytest.mark.parametrize("hard", [False, True])
+def test_write(cuda, D, n_q, n_kv, T, hard):
+    from llmq_b200 import lib
+    g = torch.Generator().manual_seed(T + D)
+    n = (n_q + 2 * n_kv) * D
+    qkv = hard_rows(T, n, g) if hard else torch.randn(T, n, generator=g).to(BF)
+    positions = torch.randint(0, 5000, (T,), generator=g).to(torch.int32)
+    cos_sin = torch.randn(5000, D, generator=g).to(BF) if not hard else torch.cat([torch.ones(5000, D // 2), torch.zeros(5000, D // 2)], 1).to(BF)
+    blocks = T // 16 + 4
+    slots = torch.randperm(blocks * 16, generator=g)[:T].to(torch.int32)
+    if T > 2:
+        slots[1] = -1
+    start = torch.randint(0, 256, (blocks, n_kv, 18 * D), generator=g).to(torch.uint8)
+    q, k, v = rope_rows(qkv, cos_sin, positions, n_q, n_kv, D)
+    ref = start.clone()
+    write_rows(ref, slots, k, v, D)
+    x, cache = qkv.to(cuda), start.to(cuda)
+    lib.rope_kvwrite_q4(x, cos_sin.to(cuda), positions.to(cuda), slots.to(cuda), cache, n_q, n_kv, D, BS)
+    got = cache.cpu()
+    if n_q:
+        assert same(x[:, : n_q * D], q.reshape(T, -1))
+    assert torch.equal(x[:, n_q * D:].view(torch.int16).cpu(), qkv[:, n_q * D:].view(torch.int16))   # keys and values stay as they were
+    for a, b in zip(read_pages(got, D), read_pages(ref, D)):
+        assert same(a, b)
+    # (codes of a NaN's group say nothing; all other bytes are the same ones)
+    if not hard:
+        assert torch.equal(got, ref)
+
+
+@pytest.mark.parametrize("D,n_kv", [(64, 3), (128, 2), (256, 1)])
+@pytest.mark.parametrize("n", [1, 5, 700])
+def test_unpack(cuda, D, n_kv, n):
+    from llmq_b200 import lib
+    g = torch.Generator().manual_seed(n)
+    cache = torch.randint(0, 256, (900, n_kv, 18 * D), generator=g).to(torch.uint8)
+    pages = torch.randint(0, 900, (n,), generator=g).to(torch.int32)   # (pages may be named twice)
+    out = torch.full((n + 1, 2, n_kv, BS, D), 7.0, dtype=BF, device=cuda)
+    cache[:, :, 8 * D: 9 * D].clamp_(max=226)
+    cache[:, :, 17 * D:].clamp_(max=226)
+    lib.kv4_unpack(cache.to(cuda), pages.to(cuda), out, n_kv, D, BS)
+    k, v = read_pages(cache[pages.long()], D)
+    got = out.cpu()
+    assert (got[n] == 7).all()
+    i, c = torch.arange(16).view(16, 1), torch.arange(D).view(1, D)
+    at = ((c // 8) ^ (i & 7)) * 8 + c % 8
+    for which, x in ((0, k), (1, v)):
+        assert same(got[:n, which].gather(-1, at.expand(n, n_kv, 16, D)), x)
+
+
+CASES = [[1], [0, 1, 15, 16, 17], [31, 32, 33, 63, 64, 65, 100], [700, 3, 129], [4097], list(range(1, 80))]
+
+
+@pytest.mark.parametrize("D,n_q,n_kv", [(64, 8, 2), (64, 7, 1), (128, 8, 8), (128, 8, 1), (128, 6, 2), (256, 8, 2), (256, 8, 1)])
+@pytest.mark.parametrize("ctxs", CASES, ids=lambda c: f"{len(c)}x{max(c)}")
+@pytest.mark.parametrize("cap,window", [(0.0, 0), (20.0, 100), (0.0, 1), (0.0, 50)])
+def test_decode(cuda, D, n_q, n_kv, ctxs, cap, window):
+    from llmq_b200 import lib
+    cache, table, rows = make_cache(ctxs, n_kv, D, seed=len(ctxs) + D)
+    B = len(ctxs)
+    qkv = torch.randn(B, (n_q + 2 * n_kv) * D, generator=torch.Generator().manual_seed(7)).to(BF)
+    out = torch.full((B + 1, n_q * D), float("nan"), dtype=BF, device=cuda)
+    args = (cache.to(cuda), table.to(cuda), torch.tensor(ctxs, dtype=torch.int32, device=cuda), n_q, n_kv, D, BS, D ** -0.5)
+    for splits in (0, 1, 3, 16):
+        out.fill_(float("nan"))
+        lib.decode_attn_q4_set_splits(splits)
+        try:
+            lib.decode_attn_q4(qkv.to(cuda), out, *args, softcap=cap, window=window)
+        finally:
+            lib.decode_attn_q4_set_splits(0)
+        got = out.cpu()
+        assert torch.isnan(got[B].float()).all()
+        for i, c in enumerate(ctxs):
+            if c == 0:
+                assert (got[i] == 0).all()
+                continue
+            q = qkv[i: i + 1, : n_q * D].view(1, n_q, D)
+            ref, weight, size = attention(q, *rows[i], torch.tensor([c - 1]), D ** -0.5, cap, window)
+            attention_close(got[i].view(1, n_q, D), ref, weight, size, D, 2.0 ** -11, f"ctx {c}, {splits} CTAs")
+    assert lib.load().b200q_wait_failures() == 0
+
+
+@pytest.mark.parametrize("D,n_q,n_kv", [(64, 4, 1), (128, 8, 2), (256, 2, 1)])
+@pytest.mark.parametrize("q_size,kv_size,scale", [(1e4, 1.0, 1e-5), (1e-6, 30.0, 1e4), (1.0, 1e-3, 100.0), (3.0, 5000.0, 1e-5), (1.0, 1.0, -0.2), (1.0, 1.0, 0.0)])
+def test_decode_sizes_of_values(cuda, D, n_q, n_kv, q_size, kv_size, scale):
+    """queries beyond and below what a half holds, scales of keys and values at both ends, scores that fall instead of rise"""
+    from llmq_b200 import lib
+    ctxs = [300, 77]
+    cache, table, rows = make_cache(ctxs, n_kv, D, seed=3, spread=kv_size)
+    qkv = (q_size * torch.randn(2, (n_q + 2 * n_kv) * D, generator=torch.Generator().manual_seed(9))).to(BF)
+    out = torch.empty(2, n_q * D, dtype=BF, device=cuda)
+    lib.decode_attn_q4(qkv.to(cuda), out, cache.to(cuda), table.to(cuda), torch.tensor(ctxs, dtype=torch.int32, device=cuda), n_q, n_kv, D, BS, scale)
+    for i, c in enumerate(ctxs):
+        ref, weight, size = attention(qkv[i: i + 1, : n_q * D].view(1, n_q, D), *rows[i], torch.tensor([c - 1]), scale)
+        attention_close(out[i].view(1, n_q, D), ref, weight, size, D, 2.0 ** -11, f"ctx {c}")
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_decode_growing_scores(cuda, D):
+    """each page's scores beyond the ones before it: the running maximum moves all the way, by less and by more than its step"""
+    from llmq_b200 import lib
+    ctx, n_kv, n_q = 600, 1, 4
+    for step in (0.05, 0.3, 3.0):
+        g = torch.Generator().manual_seed(1)
+        k = (torch.randn(ctx, 1, D, generator=g) * 0.1 + step * torch.arange(ctx).view(ctx, 1, 1) / 16).to(BF)
+        v = torch.randn(ctx, 1, D, generator=g).to(BF)
+        cache = torch.zeros((ctx + 15) // 16, 1, 18 * D, dtype=torch.uint8)
+        write_rows(cache, torch.arange(ctx), k, v, D)
+        table = torch.arange((ctx + 15) // 16, dtype=torch.int32).view(1, -1)
+        qkv = (torch.rand(1, 6 * D, generator=g) + 0.5).to(BF)
+        out = torch.empty(1, n_q * D, dtype=BF, device=cuda)
+        lib.decode_attn_q4(qkv.to(cuda), out, cache.to(cuda), table.to(cuda), torch.tensor([ctx], dtype=torch.int32, device=cuda), n_q, n_kv, D, BS, 1 / D)
+        ref, weight, size = attention(qkv[:, : n_q * D].view(1, n_q, D), held(k).transpose(0, 1), held(v).transpose(0, 1), torch.tensor([ctx - 1]), 1 / D)
+        attention_close(out.view(1, n_q, D), ref, weight, size, D, 2.0 ** -11, f"step {step}")
+
+
+def test_decode_far_pages_and_many_rows(cuda):
+    """pages beyond 2^31 bytes of the cache; more sequences than one grid dimension takes, most of them empty"""
+    from llmq_b200 import lib
+    D, n_kv, n_q = 64, 8, 8
+    page = lib.kv4_page_bytes(n_kv, D)
+    blocks = 2 ** 31 // page + 300
+    ctxs = [200, 90]
+    small, table, rows = make_cache(ctxs, n_kv, D, seed=5)
+    cache = torch.zeros(blocks, n_kv, 18 * D, dtype=torch.uint8, device=cuda)
+    cache[blocks - small.shape[0]:] = small.to(cuda)
+    B = 65535 + 9
+    far = torch.zeros(B, table.shape[1], dtype=torch.int32)
+    far[0], far[B - 1] = table[0] + blocks - small.shape[0], table[1] + blocks - small.shape[0]
+    lens = torch.zeros(B, dtype=torch.int32)
+    lens[0], lens[B - 1] = 200, 90
+    qkv = torch.randn(B, (n_q + 2 * n_kv) * D, generator=torch.Generator().manual_seed(7)).to(BF)
+    out = torch.full((B, n_q * D), float("nan"), dtype=BF, device=cuda)
+    lib.decode_attn_q4(qkv.to(cuda), out, cache, far.to(cuda), lens.to(cuda), n_q, n_kv, D, BS, D ** -0.5)
+    got = out.cpu()
+    assert (got[1: B - 1] == 0).all()
+    for i, r in ((0, 0), (B - 1, 1)):
+        ref, weight, size = attention(qkv[i: i + 1, : n_q * D].view(1, n_q, D), *rows[r], torch.tensor([ctxs[r] - 1]), D ** -0.5)
+        attention_close(got[i].view(1, n_q, D), ref, weight, size, D, 2.0 ** -11)
+    # writing there
+    positions, slots = torch.tensor([3], dtype=torch.int32), torch.tensor([blocks * 16 - 1], dtype=torch.int32)
+    cos_sin = torch.cat([torch.ones(8, D // 2), torch.zeros(8, D // 2)], 1).to(BF)
+    lib.rope_kvwrite_q4(qkv[:1].to(cuda), cos_sin.to(cuda), positions.to(cuda), slots.to(cuda), cache, n_q, n_kv, D, BS)
+    k, v = read_pages(cache[-1].cpu(), D)
+    assert same(k[:, 15], held(qkv[0].view(-1, D)[n_q: n_q + n_kv])) and same(v[:, 15], held(qkv[0].view(-1, D)[n_q + n_kv:]))
+
+
+def tiles_of(portions):
+    tiles, row = [], 0
+    for i, (n, past) in enumerate(portions):
+        tiles += [[i, row + j, min(16, n - j), past + j] for j in range(0, n, 16)]
+        row += n
+    return torch.tensor(tiles, dtype=torch.int32), row
+
+
+@pytest.mark.parametrize("D,n_q,n_kv", [(64, 8, 2), (128, 8, 1), (128, 3, 3), (256, 8, 2)])
+@pytest.mark.parametrize("portions", [[(1, 0)], [(16, 0), (3, 40)], [(5, 11), (33, 0), (17, 100)], [(700, 0)], [(300, 77), (40, 1000)], [(12, 3)] * 40],
+                         ids=lambda p: f"{len(p)}x{max(n for n, _ in p)}")
+@pytest.mark.parametrize("cap,window", [(0.0, 0), (30.0, 90), (0.0, 7)])
+def test_prompts(cuda, D, n_q, n_kv, portions, cap, window):
+    from llmq_b200 import lib
+    cache, table, rows = make_cache([n + past for n, past in portions], n_kv, D, seed=len(portions) + D)
+    table = torch.cat([table, torch.zeros(table.shape[0], 3, dtype=torch.int32)], 1).contiguous()
+    tiles, T = tiles_of(portions)
+    qkv = torch.randn(T, (n_q + 2 * n_kv) * D, generator=torch.Generator().manual_seed(7)).to(BF)
+    out = torch.full((T + 1, n_q * D), float("nan"), dtype=BF, device=cuda)
+    size = lib.prefill_attn_q4_workspace(*table.shape, n_kv, D)
+    work = torch.full((size + 256,), 0xFF, dtype=torch.uint8, device=cuda)
+    lib.prefill_attn_q4(qkv.to(cuda), out, cache.to(cuda), table.to(cuda), tiles.to(cuda), n_q, n_kv, D, BS, D ** -0.5, work[:size], softcap=cap, window=window)
+    got = out.cpu()
+    assert torch.isnan(got[T].float()).all() and (work[size:] == 0xFF).all()
+    at = 0
+    for i, (n, past) in enumerate(portions):
+        q = qkv[at: at + n, : n_q * D].view(n, n_q, D)
+        ref, weight, sz = attention(q, *rows[i], torch.arange(past, past + n), D ** -0.5, cap, window)
+        # probabilities are bf16 here, a half step 2^-8
+        attention_close(got[at: at + n].view(n, n_q, D), ref, weight, sz, D, 2.0 ** -8, f"portion {i}")
+        at += n
+    assert lib.load().b200q_wait_failures() == 0
+
+
+def test_captured_and_on_another_stream(cuda):
+    """a write and the attention behind it, captured once and replayed over other inputs, beside the same on a stream of its own"""
+    from llmq_b200 import lib
+    D, n_q, n_kv, B = 128, 8, 2, 3
+    ctxs = [40, 17, 300]
+    cache, table, _ = make_cache(ctxs, n_kv, D, seed=11)
+    table = torch.cat([table, torch.zeros(B, 1, dtype=torch.int32)], 1).contiguous()
+    cos_sin = torch.randn(400, D, generator=torch.Generator().manual_seed(2)).to(BF).to(cuda)
+    g = torch.Generator().manual_seed(4)
+    steps = [torch.randn(B, (n_q + 2 * n_kv) * D, generator=g).to(BF) for _ in range(3)]
+
+    def state():
+        return {"cache": cache.to(cuda), "table": table.to(cuda), "qkv": torch.zeros(B, (n_q + 2 * n_kv) * D, dtype=BF, device=cuda),
+                "ctx": torch.tensor(ctxs, dtype=torch.int32, device=cuda), "pos": torch.zeros(B, dtype=torch.int32, device=cuda),
+                "slot": torch.zeros(B, dtype=torch.int32, device=cuda), "out": torch.zeros(B, n_q * D, dtype=BF, device=cuda)}
+
+    def call(s, **kw):
+        lib.rope_kvwrite_q4(s["qkv"], cos_sin, s["pos"], s["slot"], s["cache"], n_q, n_kv, D, BS, **kw)
+        lib.decode_attn_q4(s["qkv"], s["out"], s["cache"], s["table"], s["ctx"], n_q, n_kv, D, BS, D ** -0.5, **kw)
+
+    def place(s, x, lens):   # a token in the place of the last one
+        s["qkv"].copy_(x)
+        s["ctx"].copy_(torch.tensor(lens, dtype=torch.int32))
+        s["pos"].copy_(torch.tensor([n - 1 for n in lens], dtype=torch.int32))
+        s["slot"].copy_(torch.tensor([int(table[i, (n - 1) // 16]) * 16 + (n - 1) % 16 for i, n in enumerate(lens)], dtype=torch.int32))
+
+    a, b = state(), state()
+    place(a, steps[0], ctxs)
+    call(a)
+    torch.cuda.synchronize()
+    a = state()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(a)
+    other = torch.cuda.Stream()
+    for k, x in enumerate(steps):
+        lens = [n - k for n in ctxs]
+        place(a, x, lens)
+        place(b, x, lens)
+        torch.cuda.synchronize()
+        graph.replay()
+        call(b, stream=other)
+        torch.cuda.synchronize()
+        for name in ("out", "cache", "qkv"):
+            assert torch.equal(a[name].view(torch.uint8), b[name].view(torch.uint8)), name
