@@ -1,25 +1,18 @@
 // beam.cu — the best continuations of beams: for every group of W rows of logits, of t(w, v) = score_w + logit_wv - log sum_v exp(logit_wv)
 // the K largest of W V, of equal ones those with the lowest w V + v first; and the first W of them that do not end.
 //
-// Two kernels.  The first has a piece of a row per CTA, in registers: its maximum, the sum of its exponentials and its K best logits (a row's
-// order needs no logarithm).  The largest logit of each pair of threads gives a bound that K of the piece reach; what reaches it, K or a
-// few more, is ranked by counting.  The second has a group per CTA: sums to logarithms, best logits to scores, and again a bound (the K-th
+// Two kernels.  The first has a piece of a row per CTA and goes through it once: the sum of its exponentials and its K best logits (a row's
+// order needs no logarithm).  The largest logits of groups of threads give a bound that K of the first tile reach; what reaches it, K or a
+// few more, is ranked by counting, and the K-th best so far is the bound from there on.  The second has a group per CTA: sums to logarithms, best logits to scores, and again a bound (the K-th
 // best of the pieces' first entries), what reaches it, and ranks.
-// Scores that are compared across rows are 64 bits, and a row's sum of exponentials keeps about 2^-26: rows whose candidates are that close
-// would come in an order of rounding errors otherwise.
-// Bound: the logits, 2 bytes each, once; next to it the exponentials, some nine instructions a logit.
+// Scores that are compared across rows are 64 bits; a row's logarithm comes from sums whose terms are off by some 2^-23 in either direction.
+// Bound: the logits, 2 bytes each, once; next to it the exponentials, four instructions a logit, one of them of the unit that has a quarter
+// of the others' rate.
 #include "common.cuh"
 
 namespace b200q {
 
-constexpr int BEAM_THREADS = 256, BEAM_PAIRS = BEAM_THREADS / 2, BEAM_MOST_K = 64, BEAM_MOST_W = 32, BEAM_FOUND = 512;
-
-// what a piece tells the second kernel: beside `entries` [K] {logit as fp32 bits, token; -1: there is none}
-struct BeamPiece {
-  double sum;
-  float top;
-  int pad;
-};
+constexpr int BEAM_THREADS = 256, BEAM_MOST_K = 64, BEAM_MOST_W = 32, BEAM_FOUND = 512, BEAM_VECTORS = 256;
 
 __device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
   uint32_t r;
@@ -31,14 +24,37 @@ __device__ __forceinline__ uint32_t beam_order(uint32_t h) {
   if ((h & 0x7fffu) > 0x7f80u) h = 0xff80u;
   return (h & 0x8000u) ? 0xffffu ^ h : h | 0x8000u;
 }
-// e^d for d <= 0 (0 below e^-160, and for NaN): the product with log2(e) in two parts, so that the exponent's rounding does not show
-__device__ __forceinline__ float beam_exp(float d) {
-  d = fmaxf(d, -160.f);
-  const float hi = d * 1.44269504088896341f;
-  const float lo = fmaf(d, 1.44269504088896341f, -hi) + d * 1.925963033500e-8f;  // log2(e) - float(log2(e)) = 1.926e-8
-  float e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(hi));
-  return fmaf(e, lo * 0.693147180559945309f, e);
+// two numbers at once, as neighbouring registers (one issue slot)
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair_of(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 halves_of(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// sum += e^w of two logits.  The exponent's rounding, 2^-24 of it, and what the fp32 constant is off by follow from the logit alone and are the
+// same for the rows that are compared.
+__device__ __forceinline__ void add_exps(f32x2& sum, uint32_t w) {
+  constexpr float L = 1.44269504088896341f;
+  const float2 h = halves_of(mul2(pair_of(bf16_lo(w), bf16_hi(w)), pair_of(L, L)));
+  float x, y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x) : "f"(h.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(h.y));
+  sum = add2(sum, pair_of(x, y));
 }
 
 // logits 8 i .. 8 i + 7 of a row, those behind its end as -infinity.  Rows of a V that is no multiple of 8 begin anywhere: they are cut at the
@@ -86,77 +102,169 @@ struct BeamRow {
   }
 };
 
-// NV: vectors per thread; a piece is up to 8 * NV * 256 logits
-template <int NV, bool kAligned>
-__global__ void __launch_bounds__(BEAM_THREADS, NV == 8 ? 3 : 4) beam_rows_kernel(const bf16* logits, long long V, int K, long long row0, long long rows,
-                                                                                  int2* entries, BeamPiece* pieces) {
-  follow_previous(logits, entries, pieces);
+// the next place in a list in shared memory (few lanes at a time ask for one: no need to ask for all of them together)
+__device__ __forceinline__ int next_place(int* count) {
+  int at;
+  asm volatile("atom.shared.add.s32 %0, [%1], 1;" : "=r"(at) : "r"(smem_u32(count)) : "memory");
+  return at;
+}
+
+// A piece of a row, in tiles of TILE vectors; the next tile is on its way while one is looked at.
+constexpr int BEAM_NV = 4, TILE = BEAM_NV * BEAM_THREADS;
+template <bool kAligned>
+__global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* logits, long long V, int K, long long row0, long long rows,
+                                                                    int2* entries, double* logs) {
+  follow_previous(logits, entries, logs);
   const int tid = threadIdx.x, piece = blockIdx.x, n_pieces = gridDim.x;
   const long long row = row0 + blockIdx.y;
   const BeamRow<kAligned> x(logits, V, row, rows);
   const int vecs = (int)((V + 7) / 8), per = (vecs + n_pieces - 1) / n_pieces, v0 = min(vecs, piece * per), v1 = min(vecs, v0 + per);
   const uint4 none = make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
-  uint4 a[NV];
-#pragma unroll
-  for (int u = 0; u < NV; ++u) a[u] = v0 + u * BEAM_THREADS + tid < v1 ? x(v0 + u * BEAM_THREADS + tid) : none;
-
-  __shared__ float tops[BEAM_PAIRS];
-  __shared__ uint64_t found[BEAM_FOUND];
+  __shared__ float tops[BEAM_THREADS / 2];
+  __shared__ uint64_t found[BEAM_FOUND], best[BEAM_MOST_K];
   __shared__ double sums[BEAM_THREADS / 32];
-  __shared__ int n_found, bound_s;
-  __shared__ float top_s;
+  __shared__ uint4 vectors[BEAM_VECTORS];  // that hold a logit that reaches the bound, and which they are
+  __shared__ int vector_at[BEAM_VECTORS], n_vectors, n_found, bound_s;
   __shared__ uint64_t best_s[BEAM_THREADS / 32];
-  uint32_t m2 = 0xff80ff80u;
+  uint4 a[BEAM_NV];
 #pragma unroll
-  for (int u = 0; u < NV; ++u) m2 = max_bf16x2(m2, max_bf16x2(max_bf16x2(a[u].x, a[u].y), max_bf16x2(a[u].z, a[u].w)));
-  float mine = fmaxf(bf16_lo(m2), bf16_hi(m2));  // (max of a number and NaN is the number; -infinity was among them)
-  mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
-  if ((tid & 1) == 0) tops[tid >> 1] = mine;
-  if (tid == 0) n_found = 0;
-  __syncthreads();
-  if (tid < BEAM_PAIRS) {  // the K-th of the pairs' maxima, and the first
-    const float t = tops[tid];
-    int rank = 0;
-#pragma unroll 8
-    for (int i = 0; i < BEAM_PAIRS; ++i) rank += tops[i] > t || (tops[i] == t && i < tid);
-    if (rank == 0) top_s = t;
-    if (rank == K - 1) bound_s = __float_as_int(t);
-  }
-  __syncthreads();
-  const float top = top_s, bound = __int_as_float(bound_s);
-  // ---- the sum, and what reaches the bound
-  float sum = 0.f;
-  const bool finite = top > -INFINITY && top < INFINITY;
-  uint32_t reached = 0;  // bit u: vector u has a logit that reaches the bound
-  auto keep = [&](uint32_t h, int token) {
-    const int at = atomicAdd(&n_found, 1);
-    if (at < BEAM_FOUND) found[at] = ((uint64_t)beam_order(h) << 32) | (0xffffffffu - (uint32_t)token);
+  for (int u = 0; u < BEAM_NV; ++u) a[u] = v0 + u * BEAM_THREADS + tid < v1 ? x(v0 + u * BEAM_THREADS + tid) : none;
+  if (tid == 0) n_found = n_vectors = 0;
+  float bound = -INFINITY;
+  uint32_t top2 = 0xff80ff80u;
+  f32x2 sum = 0;
+  // the logits of the collected vectors that reach the bound, and the k0 in best: the K best of them into best, in order; the K-th is the new
+  // bound.  False: too many to look at
+  auto prune = [&](int k0) {
+    __syncthreads();
+    const int nv = n_vectors;
+    if (nv > 0 && nv <= BEAM_VECTORS)
+      for (int i = tid; i < 8 * nv; i += BEAM_THREADS) {
+        const uint32_t w = reinterpret_cast<const uint32_t*>(vectors)[i >> 1], h = i & 1 ? w >> 16 : w & 0xffffu;
+        const long long token = 8LL * vector_at[i >> 3] + (i & 7);
+        if (__uint_as_float(h << 16) >= bound && token < V) {
+          const int at = next_place(&n_found);
+          if (at < BEAM_FOUND) found[at] = ((uint64_t)beam_order(h) << 32) | (0xffffffffu - (uint32_t)token);
+        }
+      }
+    __syncthreads();
+    const int n = n_found;
+    if (nv == 0) return true;
+    if (nv > BEAM_VECTORS || n > BEAM_FOUND) return false;
+    uint64_t key[BEAM_FOUND / BEAM_THREADS + 1];
+    int rank[BEAM_FOUND / BEAM_THREADS + 1];
+#pragma unroll
+    for (int i = 0; i < BEAM_FOUND / BEAM_THREADS + 1; ++i) {
+      const int at = i * BEAM_THREADS + tid;
+      rank[i] = K;
+      if (at >= k0 + n) continue;
+      key[i] = at < k0 ? best[at] : found[at - k0];
+      rank[i] = at < k0 ? at : 0;
+#pragma unroll 4
+      for (int k = 0; k < n; ++k) rank[i] += found[k] > key[i];
+      if (at >= k0)
+#pragma unroll 4
+        for (int k = 0; k < k0; ++k) rank[i] += best[k] > key[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < BEAM_FOUND / BEAM_THREADS + 1; ++i)
+      if (rank[i] < K) best[rank[i]] = key[i];
+    if (tid == 0) n_found = n_vectors = 0;
+    __syncthreads();
+    return true;
   };
+  auto value_of = [](uint64_t key) {  // the logit of a key
+    const uint32_t o = (uint32_t)(key >> 32), h = (o & 0x8000u) ? o & 0x7fffu : 0xffffu ^ o;
+    return __uint_as_float(h << 16);
+  };
+  // a bound that K of the first tile reach: the K-th of the largest logits of groups of threads, at least twice as many as are wanted
+  {
+    uint32_t m = 0xff80ff80u;
 #pragma unroll
-  for (int u = 0; u < NV; ++u) {
-    const uint32_t w[4] = {a[u].x, a[u].y, a[u].z, a[u].w};
-    bool any = false;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      any |= bf16_lo(w[k]) >= bound || bf16_hi(w[k]) >= bound;
-      sum += beam_exp(bf16_lo(w[k]) - top);
-      sum += beam_exp(bf16_hi(w[k]) - top);
+    for (int u = 0; u < BEAM_NV; ++u) m = max_bf16x2(m, max_bf16x2(max_bf16x2(a[u].x, a[u].y), max_bf16x2(a[u].z, a[u].w)));
+    const int deep = K <= 16 ? 3 : K <= 32 ? 2 : 1, groups = BEAM_THREADS >> deep;
+    float mine = fmaxf(bf16_lo(m), bf16_hi(m));  // (max of a number and NaN is the number; -infinity was among them)
+    for (int o = 1; o < 1 << deep; o <<= 1) mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+    if ((tid & ((1 << deep) - 1)) == 0) tops[tid >> deep] = mine;
+    __syncthreads();
+    if (tid < groups) {
+      const float y = tops[tid];
+      int rank = 0;
+#pragma unroll 16
+      for (int i = 0; i < groups; ++i) rank += tops[i] > y || (tops[i] == y && i < tid);
+      if (rank == K - 1) bound_s = __float_as_int(y);
     }
-    reached |= any ? 1u << u : 0u;
+    __syncthreads();
+    bound = __int_as_float(bound_s);
   }
-  // (seldom: the vector once more, so that this is no code for every register)
-  for (; reached; reached &= reached - 1) {
-    const int c = v0 + (__ffs(reached) - 1) * BEAM_THREADS + tid;
-    if (c >= v1) break;
-    const uint4 v = x(c);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  auto look = [&](const uint4& v, int c) {
+    const uint32_t m = max_bf16x2(max_bf16x2(v.x, v.y), max_bf16x2(v.z, v.w));
+    top2 = max_bf16x2(top2, m);
+    if (fmaxf(bf16_lo(m), bf16_hi(m)) >= bound) {  // (seldom)
+      const int at = next_place(&n_vectors);
+      if (at < BEAM_VECTORS) {
+        vectors[at] = v;
+        vector_at[at] = c;
+      }
+    }
+    add_exps(sum, v.x);
+    add_exps(sum, v.y);
+    add_exps(sum, v.z);
+    add_exps(sum, v.w);
+  };
+  // Tiles that have a whole one behind them, which is asked for vector by vector as soon as this one's has been seen.  Behind tiles 0, 3, 15,
+  // ... only the K best so far matter.
+  int c = v0 + tid, kept = 0;
+  bool overflow = false;
+  auto settle = [&]() {
+    const bool fits = prune(kept);
+    kept = K;
+    overflow |= !fits || bound == -INFINITY;
+    bound = overflow ? INFINITY : value_of(best[K - 1]);  // (overflow: whatever is found from here on does not matter)
+  };
+  const int whole = max((v1 - v0) / TILE - 1, 0);
+  for (int t = 0, end = 1; t < whole; end *= 4) {
+    for (; t < min(end, whole); ++t, c += TILE)
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const uint32_t h = k & 1 ? w[k >> 1] >> 16 : w[k >> 1] & 0xffffu;
-      if (__uint_as_float(h << 16) >= bound && 8LL * c + k < V) keep(h, 8 * c + k);
+      for (int u = 0; u < BEAM_NV; ++u) {
+        look(a[u], c + u * BEAM_THREADS);
+        a[u] = x(c + TILE + u * BEAM_THREADS);
+      }
+    if (t < whole || v0 + (t + 1) * TILE < v1) settle();
+  }
+  // the last whole tile, which is there already, and what is behind it
+#pragma unroll
+  for (int u = 0; u < BEAM_NV; ++u)
+    if (c + u * BEAM_THREADS < v1) look(a[u], c + u * BEAM_THREADS);
+  for (c += TILE; c < v1; c += BEAM_THREADS) look(x(c), c);
+  settle();
+  const float2 halves = halves_of(sum);
+  float mine_sum = halves.x + halves.y;
+  // the largest logit: where the exponentials themselves would leave what fp32 holds, or the constant's own error would show, or a thread
+  // met NaN, once more by differences to it
+  float top = fmaxf(bf16_lo(top2), bf16_hi(top2));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  __syncthreads();
+  if ((tid & 31) == 0) tops[tid >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < BEAM_THREADS / 32; ++w) top = fmaxf(top, tops[w]);
+  const bool far = fabsf(top) > 32.f;
+  if (far || mine_sum != mine_sum) {
+    mine_sum = 0.f;
+    for (int c = v0 + tid; c < v1; c += BEAM_THREADS) {
+      const uint4 v = x(c);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float y = k & 1 ? bf16_hi(w[k >> 1]) : bf16_lo(w[k >> 1]);
+        if (y == y) mine_sum += far ? (y == top ? 1.f : expf(y - top)) : expf(y);
+      }
     }
   }
-  double d = finite ? (double)sum : 0.0;
+  double d = (double)mine_sum;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
   if ((tid & 31) == 0) sums[tid >> 5] = d;
@@ -165,51 +273,41 @@ __global__ void __launch_bounds__(BEAM_THREADS, NV == 8 ? 3 : 4) beam_rows_kerne
   if (tid == 0) {
     double s = 0.0;
     for (int w = 0; w < BEAM_THREADS / 32; ++w) s += sums[w];
-    pieces[out] = {s, top, 0};
+    // (-infinity: no logit; +infinity: one is)
+    logs[out] = fabsf(top) == INFINITY ? (double)top : log(s) + (far ? (double)top : 0.0);
   }
   int2* to = entries + out * K;
-  const int n = n_found;
-  auto tell = [&](int rank, uint64_t key) {
-    const uint32_t o = (uint32_t)(key >> 32), h = (o & 0x8000u) ? o & 0x7fffu : 0xffffu ^ o;
-    to[rank] = make_int2((int)(h << 16), (int)(0xffffffffu - (uint32_t)key));
-  };
-  if (bound > -INFINITY && n <= BEAM_FOUND) {  // (K and more reach the bound; the keys are all different)
-    for (int i = tid; i < n; i += BEAM_THREADS) {
-      const uint64_t key = found[i];
-      int rank = 0;
-      for (int k = 0; k < n; ++k) rank += found[k] > key;
-      if (rank < K) tell(rank, key);
-    }
+  auto tell = [&](int rank, uint64_t key) { to[rank] = make_int2(__float_as_int(value_of(key)), (int)(0xffffffffu - (uint32_t)key)); };
+  if (!overflow && v0 < v1) {  // (K and more reach the bound; the keys are all different)
+    if (tid < K) tell(tid, best[tid]);
     return;
   }
-  // Fewer than K pairs with a number above -infinity, or hundreds of equal logits: one after the other.
+  // Fewer than K groups with a number above -infinity, or hundreds of equal or ever larger logits: one after the other.
   uint64_t last = ~0ull;
   for (int k = 0; k < K; ++k) {
-    uint64_t best = 0;
-    auto look = [&](uint32_t h, int token) {
-      const uint64_t key = ((uint64_t)beam_order(h) << 32) | (0xffffffffu - (uint32_t)token);
-      if (key < last && key > best) best = key;
-    };
+    uint64_t most = 0;
     for (int c = v0 + tid; c < v1; c += BEAM_THREADS) {
       const uint4 v = x(c);
       const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (8LL * c + i < V) look(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu, 8 * c + i);
+      for (int i = 0; i < 8; ++i) {
+        const uint64_t key = ((uint64_t)beam_order(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu) << 32) | (0xffffffffu - (uint32_t)(8 * c + i));
+        if (8LL * c + i < V && key < last && key > most) most = key;
+      }
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) best = max(best, (uint64_t)__shfl_xor_sync(0xffffffffu, (unsigned long long)best, o));
-    if ((tid & 31) == 0) best_s[tid >> 5] = best;
+    for (int o = 16; o > 0; o >>= 1) most = max(most, (uint64_t)__shfl_xor_sync(0xffffffffu, (unsigned long long)most, o));
+    if ((tid & 31) == 0) best_s[tid >> 5] = most;
     __syncthreads();
-    for (int w = 0; w < BEAM_THREADS / 32; ++w) best = max(best, best_s[w]);
+    for (int w = 0; w < BEAM_THREADS / 32; ++w) most = max(most, best_s[w]);
     __syncthreads();
     if (tid == 0) {
-      if (best)
-        tell(k, best);
+      if (most)
+        tell(k, most);
       else
         to[k] = make_int2((int)0xff800000u, -1);
     }
-    last = best;  // (0: nothing is below it, so the rest is told to be none too)
+    last = most;  // (0: nothing is below it, so the rest is told to be none too)
   }
 }
 
@@ -217,7 +315,7 @@ struct BeamArgs {
   const float* scores;
   const int32_t* stops;
   const int2* entries;
-  const BeamPiece* pieces;
+  const double* logs;  // of a piece's sum of exponentials
   float *cand_scores, *next_scores;
   int32_t *cand_tokens, *cand_rows, *next_tokens, *next_rows;
   int W, K, n_pieces, n_stops;
@@ -229,9 +327,9 @@ __device__ __forceinline__ uint64_t order_double(double v) {
   return b >> 63 ? ~b : b | 0x8000000000000000ull;
 }
 
-constexpr int MERGE_THREADS = 512, HEADS = 256;
+constexpr int MERGE_THREADS = 512, HEADS = 128, MERGE_KEYS = 2048, MERGE_OWN = MERGE_KEYS / MERGE_THREADS;
 __global__ void __launch_bounds__(MERGE_THREADS) beam_groups_kernel(BeamArgs a) {
-  follow_previous(a.scores, a.stops, a.entries, a.pieces, a.cand_scores, a.next_scores, a.cand_tokens, a.cand_rows, a.next_tokens, a.next_rows);
+  follow_previous(a.scores, a.stops, a.entries, a.logs, a.cand_scores, a.next_scores, a.cand_tokens, a.cand_rows, a.next_tokens, a.next_rows);
   const int tid = threadIdx.x, W = a.W, K = a.K;
   const long long group = blockIdx.x, row0 = group * W;
   const int lists = W * a.n_pieces, n = lists * K;
@@ -241,74 +339,80 @@ __global__ void __launch_bounds__(MERGE_THREADS) beam_groups_kernel(BeamArgs a) 
   constexpr int FOUND = 1024;
   __shared__ uint64_t found_key[FOUND];
   __shared__ int found_place[FOUND];  // place among the group's n entries
-  __shared__ uint64_t heads[HEADS];
+  __shared__ uint64_t heads[HEADS], keys[MERGE_KEYS];
   __shared__ double out_t[BEAM_MOST_K];
   __shared__ int out_token[BEAM_MOST_K], out_row[BEAM_MOST_K];
   const int2* entries = a.entries + row0 * a.n_pieces * K;
-  const BeamPiece* pieces = a.pieces + row0 * a.n_pieces;
+  const double* logs = a.logs + row0 * a.n_pieces;
+  const bool held = n <= MERGE_KEYS;  // every thread has its entries, asked for before the rows' logarithms are known
+  int2 mine[MERGE_OWN];
+#pragma unroll
+  for (int i = 0; i < MERGE_OWN; ++i)
+    if (held && i * MERGE_THREADS + tid < n) mine[i] = entries[i * MERGE_THREADS + tid];
   for (int w = tid >> 5; w < W; w += MERGE_THREADS / 32) {
     const int lane = tid & 31;
-    float top = -INFINITY;
-    for (int p = lane; p < a.n_pieces; p += 32) top = fmaxf(top, pieces[w * a.n_pieces + p].top);
+    const double s = (double)a.scores[row0 + w];
+    double top = -INFINITY;
+    for (int p = lane; p < a.n_pieces; p += 32) top = fmax(top, logs[w * a.n_pieces + p]);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    double sum = 0.0;
+    for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
     const bool finite = top > -INFINITY && top < INFINITY;
-    for (int p = lane; p < a.n_pieces && finite; p += 32) {
-      const BeamPiece b = pieces[w * a.n_pieces + p];
-      if (b.top > -INFINITY) sum += b.sum * exp((double)b.top - (double)top);
-    }
+    double sum = 0.0;
+    for (int p = lane; p < a.n_pieces && finite; p += 32) sum += exp(logs[w * a.n_pieces + p] - top);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) {
-      const double s = (double)a.scores[row0 + w];
-      const double t = finite && s > -INFINITY && s < INFINITY ? s - ((double)top + log(sum)) : -INFINITY;
-      shift[w] = t;
-    }
+    if (lane == 0) shift[w] = finite && s > -INFINITY && s < INFINITY ? s - (top + log(sum)) : -INFINITY;
   }
   if (tid == 0) {
     n_found = 0;
     bound_s = 0;
   }
   __syncthreads();
-  // an entry's score; of rows without candidates the first list stands for tokens 0 .. K - 1 at -infinity
-  auto entry = [&](int i, int& w, int& token) -> double {
+  // entry e at place i: its score; of rows without candidates the first list stands for tokens 0 .. K - 1 at -infinity
+  auto score_of = [&](int2 e, int i, int& w, int& token) -> double {
     const int list = i / K;
     w = list / a.n_pieces;
-    const int2 e = entries[i];
     token = e.y;
     if (shift[w] == -INFINITY) token = list % a.n_pieces == 0 ? i % K : -1;
     const float x = __int_as_float(e.x);
     return shift[w] == -INFINITY || !(x > -INFINITY) ? -INFINITY : shift[w] + (double)x;
   };
-  // ---- a bound that K candidates reach.  Of K lists and more: the K-th of the largest first entries of up to 256 classes of lists; of
-  // fewer: the least of the entries that are K together.
+  auto entry = [&](int i, int& w, int& token) { return score_of(entries[i], i, w, token); };
+  auto key_of = [&](int2 e, int i) -> uint64_t {
+    int w, token;
+    const double t = score_of(e, i, w, token);
+    return token >= 0 ? order_double(t) : 0;
+  };
+#pragma unroll
+  for (int i = 0; i < MERGE_OWN; ++i)
+    if (held && i * MERGE_THREADS + tid < n) keys[i * MERGE_THREADS + tid] = key_of(mine[i], i * MERGE_THREADS + tid);
+  __syncthreads();
+  // ---- a bound that K candidates reach: the K-th best of the first entries of each list, so many that they are up to 128 together; of more
+  // lists, the K-th of the largest first entries of 128 classes of lists
   {
-    const int classes = min(lists, HEADS), deep = lists >= K ? 0 : (K + lists - 1) / lists - 1;
-    uint64_t mine = 0;
-    if (tid < classes)
-      for (int l = tid; l < lists; l += classes) {
-        int w, token;
-        const double t = entry(l * K + deep, w, token);
-        mine = max(mine, token >= 0 ? order_double(t) : 0);
-      }
-    if (tid < HEADS) heads[tid] = mine;
+    const int deep = min(K, max(1, HEADS / lists)), heads_n = min(lists * deep, HEADS);
+    uint64_t best = 0;
+    if (tid < heads_n) {
+      const int first = tid / deep * K + tid % deep, step = heads_n / deep * K;
+      for (int i = first; i < n; i += step) best = max(best, held ? keys[i] : key_of(entries[i], i));
+    }
+    if (tid < HEADS) heads[tid] = best;
     __syncthreads();
-    if (tid < classes) {
+    if (tid < heads_n) {
       int rank = 0;
-      for (int i = 0; i < classes; ++i) rank += heads[i] > mine || (heads[i] == mine && i < tid);
-      if (rank == min(K, classes) - 1) bound_s = mine;
+#pragma unroll 8
+      for (int i = 0; i < heads_n; ++i) rank += heads[i] > best || (heads[i] == best && i < tid);
+      if (rank == min(K, heads_n) - 1) bound_s = best;
     }
     __syncthreads();
   }
-  const uint64_t bound = bound_s;
+  const uint64_t bound = max(bound_s, (uint64_t)1);
   for (int i = tid; i < n; i += MERGE_THREADS) {
-    int w, token;
-    const double t = entry(i, w, token);
-    if (token >= 0 && order_double(t) >= bound) {
-      const int at = atomicAdd(&n_found, 1);
+    const uint64_t key = held ? keys[i] : key_of(entries[i], i);
+    if (key >= bound) {
+      const int at = next_place(&n_found);
       if (at < FOUND) {
-        found_key[at] = order_double(t);
+        found_key[at] = key;
         found_place[at] = i;
       }
     }
@@ -403,11 +507,21 @@ __global__ void __launch_bounds__(MERGE_THREADS) beam_groups_kernel(BeamArgs a) 
   }
 }
 
-// Pieces of a row: of 16384 logits where the rows alone fill the chip, else of 4096
-static int beam_vectors(long long rows, long long V) { return rows * ((V + 16383) / 16384) >= 2 * 148 ? 8 : 2; }
+// Pieces of a row: the least time of the SM that has most CTAs, each its logits (five CTAs at once are as fast as an SM gets) and 11000 logits'
+// worth beside them, and of the lists that the second kernel has to look at.  384 rows of 256000 logits: 1 / 2 / 3 / 4 / 8 / 16 pieces 73.8 /
+// 62.5 / 58.3 / 62.4 / 67.4 / 81.8 us; 4 rows of 128256: 8 / 24 / 32 / 64 pieces 13.1 / 11.3 / 12.2 / 13.5 us.
 static int beam_pieces(long long rows, long long V) {
-  const long long most = beam_vectors(rows, V) * 8LL * BEAM_THREADS;
-  return (int)((V + most - 1) / most);
+  int best = 1;
+  double least = 1e30;
+  for (int p = 1; p <= 256 && (p == 1 || V / p >= 2048); ++p) {
+    const long long deep = (rows * p + 147) / 148;
+    const double t = (double)(deep > 5 ? deep : 5) * ((double)V / p) + deep * 11000.0 + 500.0 * p;
+    if (t < 0.98 * least) {
+      least = t;
+      best = p;
+    }
+  }
+  return best;
 }
 
 }  // namespace b200q
@@ -423,7 +537,7 @@ int64_t b200q_beam_select_workspace(int groups, int beams, int64_t V, int K) {
     return B200Q_EINVAL;
   }
   const int64_t pieces = (int64_t)groups * beams * beam_pieces((int64_t)groups * beams, V);
-  return pieces * (int64_t)(sizeof(BeamPiece) + K * sizeof(int2));
+  return pieces * (int64_t)(sizeof(double) + K * sizeof(int2));
 }
 
 int b200q_beam_select(const void* logits, const float* scores, int groups, int beams, int64_t V, const int32_t* stops, int n_stops, int K,
@@ -443,17 +557,16 @@ int b200q_beam_select(const void* logits, const float* scores, int groups, int b
   B200Q_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && (reinterpret_cast<uintptr_t>(logits) & 15) == 0,
                   "beam_select: logits and workspace must be 16-byte aligned");
   const int pieces = beam_pieces(rows, V);
-  BeamPiece* piece = (BeamPiece*)workspace;
-  int2* entries = (int2*)(piece + rows * pieces);
+  double* logs = (double*)workspace;
+  int2* entries = (int2*)(logs + rows * pieces);
   cudaStream_t st = as_stream(stream);
   for (int64_t r0 = 0; r0 < rows; r0 += 65535) {  // (a grid's second dimension ends there)
     const unsigned n = (unsigned)(rows - r0 < 65535 ? rows - r0 : 65535);
-    const bool wide = beam_vectors(rows, V) == 8;
-    auto kern = V % 8 ? (wide ? beam_rows_kernel<8, false> : beam_rows_kernel<2, false>) : wide ? beam_rows_kernel<8, true> : beam_rows_kernel<2, true>;
-    B200Q_CUDA(launch_early(kern, dim3(pieces, n), BEAM_THREADS, 0, st, 1, (const bf16*)logits, (long long)V, K, (long long)r0, (long long)rows, entries, piece));
+    auto kern = V % 8 ? beam_rows_kernel<false> : beam_rows_kernel<true>;
+    B200Q_CUDA(launch_early(kern, dim3(pieces, n), BEAM_THREADS, 0, st, 1, (const bf16*)logits, (long long)V, K, (long long)r0, (long long)rows, entries, logs));
     count_launch();
   }
-  const BeamArgs a{scores, stops, entries, piece, cand_scores, next_scores, cand_tokens, cand_rows, next_tokens, next_rows, beams, K, pieces, n_stops,
+  const BeamArgs a{scores, stops, entries, logs, cand_scores, next_scores, cand_tokens, cand_rows, next_tokens, next_rows, beams, K, pieces, n_stops,
                    (long long)V};
   B200Q_CUDA(launch_early(beam_groups_kernel, dim3(groups), MERGE_THREADS, 0, st, 1, a));
   count_launch();
