@@ -713,12 +713,12 @@ int b200q_pages_copy(void* kv_dev, const int32_t* pairs_dev, int n_pairs, const 
 int b200q_pages_compact(const int32_t* table_dev, const int32_t* lens_dev, int n_rows, int bt_stride, const int32_t* refs_dev,
                         int num_blocks, int block_size, int32_t* table_out_dev, int32_t* refs_out_dev, int32_t* map_dev,
                         int32_t* pairs_dev, int32_t* status_dev, void* stream);
-/* test hook: so many CTAs share a sequence and head in b200q_decode_attn_q4 (0: chosen) */
-int b200q_decode_attn_q4_set_splits(int splits);
+/* test hook: b200q_decode_attn_q4 gives a sequence's heads to warps whole (1), or pages evenly (0); -1: as B200Q_BATCH_INVARIANT says */
+int b200q_decode_attn_q4_set_whole(int whole);
 
 /* nonzero once a kernel's bounded wait has run out in this process (its outputs are then missing or wrong); engine steps report
- * it as B200Q_ECUDA.  Calls return before their kernels run: who calls b200q_gemm_* (up to 128 rows), b200q_prefill_attn*,
- * b200q_decode_attn_q4 or the layered attention directly asks here once the stream has been waited for. */
+ * it as B200Q_ECUDA.  Calls return before their kernels run: who calls b200q_gemm_* (up to 128 rows), b200q_prefill_attn* or the
+ * layered attention directly asks here once the stream has been waited for. */
 int b200q_wait_failures(void);
 
 /* ------------------------------------------------------------------------------------

@@ -792,19 +792,14 @@ struct SplitBuffer {
   int device = 0;
   cudaStream_t stream = nullptr;
   unsigned long long capture = 0;  // of the graph that owns it; 0: the stream does
+  int kind = 0;                    // 0: parts of split products, 1: pieces of attention (which parts may have to outlive)
   std::atomic<bool> free{false};   // the graph is gone
 };
 std::mutex g_split_mu;
 std::vector<SplitBuffer*> g_split;  // (entries stay: a graph's callback names its own)
 }  // namespace
 
-static int splitk_scratch(int splits, int M, int N, cudaStream_t st, float** out) {
-  const size_t need = (size_t)splits * M * N * sizeof(float);
-  B200Q_CHECK_ARG(need <= SPLIT_BYTES, "split-K scratch too small for M=%d N=%d splits=%d", M, N, splits);
-  if (need <= t_model_scratch.bytes) {
-    *out = (float*)t_model_scratch.p;
-    return B200Q_OK;
-  }
+int stream_scratch(int kind, size_t need, cudaStream_t st, float** out) {
   int device = 0;
   unsigned long long capture = 0;
   cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
@@ -821,7 +816,7 @@ static int splitk_scratch(int splits, int M, int N, cudaStream_t st, float** out
   std::lock_guard<std::mutex> lock(g_split_mu);
   SplitBuffer *own = nullptr, *spare = nullptr;
   for (SplitBuffer* b : g_split) {
-    if (b->device != device || b->bytes < need) continue;
+    if (b->device != device || b->bytes < need || b->kind != kind) continue;
     if (b->free.load()) {
       if (!spare || b->bytes < spare->bytes) spare = b;
     } else if (b->stream == st && b->capture == capture && (!own || b->bytes > own->bytes)) {
@@ -844,6 +839,7 @@ static int splitk_scratch(int splits, int M, int N, cudaStream_t st, float** out
       own->p = p;
       own->bytes = bytes;
       own->device = device;
+      own->kind = kind;
       own->free.store(true);
       g_split.push_back(own);
     }
@@ -859,6 +855,16 @@ static int splitk_scratch(int splits, int M, int N, cudaStream_t st, float** out
   }
   *out = (float*)own->p;
   return B200Q_OK;
+}
+
+static int splitk_scratch(int splits, int M, int N, cudaStream_t st, float** out) {
+  const size_t need = (size_t)splits * M * N * sizeof(float);
+  B200Q_CHECK_ARG(need <= SPLIT_BYTES, "split-K scratch too small for M=%d N=%d splits=%d", M, N, splits);
+  if (need <= t_model_scratch.bytes) {
+    *out = (float*)t_model_scratch.p;
+    return B200Q_OK;
+  }
+  return stream_scratch(0, need, st, out);
 }
 
 // (no other thread's product on the same stream between a product and the sum of its parts, whichever kernels they take)

@@ -2,9 +2,9 @@
 //
 //   out[s, h] = sum_j softmax_j(x(scale q . k_j)) v_j,  max(0, ctx - window) <= j < ctx,  x(y) = y or cap tanh(y / cap)
 //
-// Bound: 18 D bytes of a head's 16 tokens, and next to them the instructions that turn codes into operands: at the memory's rate an SM
-// meets 42 codes a clock.  So a code is touched by few instructions:
-//   * A page's part of one head arrives by one bulk copy in a ring that each warp has for itself; nobody waits for another warp.
+// Bound: 18 D bytes of a head's 16 tokens from memory, and as long as that takes the instructions that turn codes into operands: from shared
+// memory alone the loop below goes through 7.3 TB/s of pages (8 to 24 warps per SM alike; without the scales' multiplications 9.7, without
+// the conversions 8.0, without the matrix products 7.6), the memory gives 6.5.  So a code is touched by few instructions:
 //   * Scores are S^T = K Q^T: tokens are the rows of the 16 x 16 operand tile and heads of the group its 8 columns (a group of up to 8 fills
 //     them; with heads as rows half the tile would be zeros).  The page is laid out so that a lane's operand registers are the codes of 16
 //     consecutive bytes: one conversion and one multiplication by the scale (both exact) for two values, no shuffles, no transposes.
@@ -12,7 +12,11 @@
 //     before the conversion (half an instruction for two values).  P^T is S^T after movmatrix.
 //   * The running maximum moves only when a score is 2^4 above it, which a vote finds out; otherwise no lane asks another one for anything.
 //     Probabilities are fp16 with 2^8 for the maximum's place (up to 2^12), so that a probability of 2^-32 of the largest still counts.
+//   * A warp has its own pages on their way, by asynchronous copies; nobody waits for another warp.
 // Queries are divided by the power of two in their largest magnitude before they become fp16, which costs nothing that fp32 sums would keep.
+// 700 sequences of 33 to 1000 tokens, 32 / 8 heads of 128: 95.6 us, 4.5 TB/s (the memory's share 66 us); 22 of 16000: 85; 3 of 9000 to 16000,
+// heads of 64: 18.6.
+#include <mutex>
 #include <type_traits>
 
 #include "kv4.cuh"
@@ -58,16 +62,14 @@ struct Kv4Args {
   const uint8_t* kv;
   const int32_t* block_table;
   const int32_t* ctx_lens;
-  int* failed;  // set when a bounded wait runs out
   int q_stride, bt_stride, n_seqs, n_q, n_kv, G, window;
   float c0, c1;  // of a product: plain c0 = scale log2(e); capped c0 = 2 log2(e) scale / cap, c1 = cap log2(e)
 };
 
-// pages that a warp works on at once (one chain of scores, exponentials and outputs for 256 keys' values of D = 16), turns of them in flight
+// pages that a warp works on at once: a turn
 template <int D>
 struct Q4Cfg {
-  static constexpr int PAGES = 256 / D, STAGES = 3;
-  static constexpr int TURN = PAGES * Kv4<D>::BYTES, RING = STAGES * TURN;  // 4608, 13824
+  static constexpr int PAGES = 256 / D, TURN = PAGES * Kv4<D>::BYTES;  // 4608 bytes
 };
 
 // what a warp knows of the keys that it has seen: outputs times sums, per lane heads 2 t and 2 t + 1 (t = lane % 4)
@@ -80,45 +82,6 @@ struct Q4State {
     for (int i = 0; i < D / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     m[0] = m[1] = -INFINITY;
     l[0] = l[1] = 0.f;
-  }
-};
-
-// queries of one group as the product's second operand: lane (g, t) has those values of head g that lane (., t) reads of a key
-template <int D>
-struct Q4Query {
-  uint32_t b[D / 16][2];
-  float c[2];  // c0 times what heads 2 t, 2 t + 1 were divided by
-  __device__ __forceinline__ void load(const bf16* rows, int G, float c0, int lane) {
-    const int g = lane >> 2, t = lane & 3;
-    constexpr int PART = D == 256 ? 32 : D / 4, PARTS = D == 256 ? 2 : 1;  // consecutive values
-    float x[PARTS][PART];
-    float most = 0.f;
-#pragma unroll
-    for (int h = 0; h < PARTS; ++h)
-#pragma unroll
-      for (int i = 0; i < PART / 8; ++i) {
-        const uint4 v = g < G ? ld_v4(rows + (long long)g * D + h * 128 + t * PART + i * 8) : make_uint4(0, 0, 0, 0);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          x[h][8 * i + 2 * k] = bf16_lo(w[k]);
-          x[h][8 * i + 2 * k + 1] = bf16_hi(w[k]);
-          most = fmaxf(most, fmaxf(fabsf(bf16_lo(w[k])), fabsf(bf16_hi(w[k]))));
-        }
-      }
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -126), 126);
-    const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-#pragma unroll
-    for (int h = 0; h < PARTS; ++h)
-#pragma unroll
-      for (int s = 0; s < PART / 4; ++s) {
-        b[h * (PART / 4) + s][0] = pack_half2(x[h][4 * s] * down, x[h][4 * s + 1] * down);
-        b[h * (PART / 4) + s][1] = pack_half2(x[h][4 * s + 2] * down, x[h][4 * s + 3] * down);
-      }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) c[i] = c0 * __uint_as_float((uint32_t)(127 + __shfl_sync(0xffffffffu, e, 8 * t + 4 * i)) << 23);
   }
 };
 
@@ -142,6 +105,45 @@ __device__ __forceinline__ uint32_t lds_u16(uint32_t at) {
   asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at));
   return v;
 }
+
+// queries of one group as the product's second operand: lane (g, t) has those values of head g that lane (., t) reads of a key
+template <int D>
+struct Q4Query {
+  uint32_t b[D / 16][2];
+  float c[2];  // c0 times what heads 2 t, 2 t + 1 were divided by
+  __device__ __forceinline__ void load(uint32_t rows, int G, float c0, int lane) {  // [G][D] in shared memory
+    const int g = lane >> 2, t = lane & 3;
+    constexpr int PART = D == 256 ? 32 : D / 4, PARTS = D == 256 ? 2 : 1;  // consecutive values
+    float x[PARTS][PART];
+    float most = 0.f;
+#pragma unroll
+    for (int h = 0; h < PARTS; ++h)
+#pragma unroll
+      for (int i = 0; i < PART / 8; ++i) {
+        const uint4 v = g < G ? lds_v4(rows + (g * D + h * 128 + t * PART + i * 8) * 2) : make_uint4(0, 0, 0, 0);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          x[h][8 * i + 2 * k] = bf16_lo(w[k]);
+          x[h][8 * i + 2 * k + 1] = bf16_hi(w[k]);
+          most = fmaxf(most, fmaxf(fabsf(bf16_lo(w[k])), fabsf(bf16_hi(w[k]))));
+        }
+      }
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -126), 126);
+    const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+    for (int h = 0; h < PARTS; ++h)
+#pragma unroll
+      for (int s = 0; s < PART / 4; ++s) {
+        b[h * (PART / 4) + s][0] = pack_half2(x[h][4 * s] * down, x[h][4 * s + 1] * down);
+        b[h * (PART / 4) + s][1] = pack_half2(x[h][4 * s + 2] * down, x[h][4 * s + 3] * down);
+      }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) c[i] = c0 * __uint_as_float((uint32_t)(127 + __shfl_sync(0xffffffffu, e, 8 * t + 4 * i)) << 23);
+  }
+};
 
 // four k-steps' worth: 8 values of rows g (w0) and g + 8 (w1) are two k-steps
 __device__ __forceinline__ void q4_score_steps(float (&s)[4], uint32_t w0, uint32_t w1, uint32_t s0, uint32_t s1, const uint32_t (&b0)[2],
@@ -318,194 +320,414 @@ __device__ __forceinline__ void q4_turn(uint32_t at, const Q4Query<D>& q, Q4Stat
   }
 }
 
-// a warp's share of one sequence and head: pages wg, wg + n_warps, ... of those that hold visible keys, through the warp's own ring
+// ------------------------------------------------------------------------------------------------------------------------
+// All pages of all sequences and heads in one row (units: sequence, head, page; an item's begin and end count as two pages more, about what
+// they cost), and every warp of the chip a piece of it of the same length.  A warp streams through its piece as it comes, the next item's
+// pages and queries on their way while the last one's are worked on; items that lie in it whole are finished there, of those that go on in
+// the next warp's piece the states go to scratch, where the second kernel adds them up.  Ragged contexts, few long ones and many short ones
+// then take the same time per page.
+// ------------------------------------------------------------------------------------------------------------------------
+constexpr int Q4_BEGIN = 2;        // units of an item beside its pages
+constexpr int Q4_LEAST_SHARE = 8;  // units of a piece at least
 template <int D>
-struct Q4Share {
-  static constexpr int P = Q4Cfg<D>::PAGES, STAGES = Q4Cfg<D>::STAGES;
-  const int32_t* bt;
-  const uint8_t* kv;  // this head's page of block 0
-  int ctx, lo, page0, n, turns, wg, n_warps, ids_base, ids;
-  long long page_stride;
-  __device__ __forceinline__ void begin(const Kv4Args& a, int seq, int kvh, int wg_, int n_warps_, int lane) {
-    ctx = a.ctx_lens[seq];
-    wg = wg_;
-    n_warps = n_warps_;
-    ctx = min(max(ctx, 0), a.bt_stride * 16);
+struct Q4Stream {
+  static constexpr int WARPS = 4 /* the join kernel's too */, STAGES = 2 /* turns change them with ^ 1 */, CTAS = D == 256 ? 3 : 4;
+  static constexpr int TURN = Q4Cfg<D>::TURN;
+  // bytes of a stage: a turn's pages, and the group's queries for an item that begins with it
+  static int stage_bytes(int G) { return TURN + G * D * 2; }
+  static int smem(int G) { return WARPS * STAGES * stage_bytes(G); }
+};
+// an item's chain of pieces: warps from .. from + n - 1 of them; n = 0: none
+struct __align__(16) Q4Chain {
+  int seq, head, from, n;
+};
+struct Q4Item {
+  int seq, head, ctx, lo, page0, pages;
+};
+// scratch: two chains per warp (of the piece at its beginning, of the one at its end), then two pieces per warp, [G][D] outputs, [G] maxima, [G] sums
+__host__ __device__ inline long long q4_piece_floats(int G, int D) { return ((long long)G * (D + 2) + 3) / 4 * 4; }
+__host__ __device__ inline long long q4_chain_floats(int warps) { return 8LL * warps; }
+
+// sequence s: keys that count and the pages that hold them
+struct Q4Span {
+  int ctx, lo, page0, pages;
+  __device__ __forceinline__ Q4Span(const Kv4Args& a, int n) {
+    ctx = min(max(n, 0), a.bt_stride * 16);
     lo = a.window > 0 && ctx > a.window ? ctx - a.window : 0;
     page0 = lo / 16;
-    const int pages = (ctx + 15) / 16 - page0;
-    n = pages > wg ? (pages - wg + n_warps - 1) / n_warps : 0;
-    turns = (n + P - 1) / P;
-    page_stride = (long long)a.n_kv * Kv4<D>::BYTES;
-    kv = a.kv + (long long)kvh * Kv4<D>::BYTES;
-    bt = a.block_table + (long long)seq * a.bt_stride + page0 + wg;
-    ids_base = 0;
-    ids = lane < n ? bt[n_warps * lane] : 0;
+    pages = (ctx + 15) / 16 - page0;
   }
-  // whole warp; the pages of turn k into its place of the ring
-  __device__ __forceinline__ void fetch(int k, uint8_t* ring, uint64_t* bars, int lane) {
-    const int k0 = k * P;
-    if (k0 - ids_base >= 32) {
-      ids_base += 32;
-      ids = ids_base + lane < n ? bt[n_warps * (ids_base + lane)] : 0;
-    }
-    const int st = k % STAGES, count = min(P, n - k0);
-    int blk[P];
-#pragma unroll
-    for (int x = 0; x < P; ++x) blk[x] = __shfl_sync(0xffffffffu, ids, (k0 - ids_base + x) & 31);
-    if (lane == 0) {
-      mbar_expect_tx(bars + st, (uint32_t)(count * Kv4<D>::BYTES));
-#pragma unroll
-      for (int x = 0; x < P; ++x)
-        if (x < count) tma_bulk_g2s(ring + st * Q4Cfg<D>::TURN + x * Kv4<D>::BYTES, kv + blk[x] * page_stride, Kv4<D>::BYTES, bars + st);
-    }
-  }
-  __device__ __forceinline__ int first_key(int i) const { return (page0 + wg + n_warps * i) * 16; }
+  __device__ __forceinline__ int units() const { return pages > 0 ? pages + Q4_BEGIN : 0; }  // of a head
 };
 
-// WARPS warps of a CTA, and the gridDim.x CTAs of a cluster, share one sequence and head.
-constexpr int Q4_WARPS = 4, Q4_MOST_CTAS = 16;
-template <int D>
-struct Q4Smem {
-  static constexpr int TOTAL = Q4_WARPS * Q4Cfg<D>::RING + Q4_WARPS * Q4Cfg<D>::STAGES * 8;
-};
 template <int D, bool kCap>
-__global__ void __launch_bounds__(Q4_WARPS * 32, D == 256 ? 3 : 4) kv4_decode_kernel(Kv4Args a) {
-  follow_previous(a.q, a.out, a.kv, a.block_table, a.ctx_lens);
-  using C = Q4Cfg<D>;
+__global__ void __launch_bounds__(Q4Stream<D>::WARPS * 32, Q4Stream<D>::CTAS) kv4_stream_kernel(Kv4Args a, int stage_bytes, int whole_items, int least_share, float* scratch) {
+  follow_previous(a.q, a.out, a.kv, a.block_table, a.ctx_lens, scratch);
+  using C = Q4Stream<D>;
+  constexpr int P = Q4Cfg<D>::PAGES, STAGES = C::STAGES, THREADS = C::WARPS * 32;
   extern __shared__ __align__(128) uint8_t smem[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int splits = gridDim.x, split = blockIdx.x, seq = blockIdx.y, kvh = blockIdx.z;
-  uint8_t* ring = smem + warp * C::RING;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Q4_WARPS * C::RING) + warp * C::STAGES;
-  if (lane == 0) {
+  __shared__ uint32_t before[THREADS + 1];  // units of a head of the sequences before each thread's
+  __shared__ uint32_t warp_sum[C::WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const uint32_t ring = smem_u32(smem + warp * STAGES * stage_bytes);
+  // ---- where every thread's share of the sequences begins
+  const int per = (a.n_seqs + THREADS - 1) / THREADS;
+  {
+    uint32_t mine = 0;
+    const int s0 = threadIdx.x * per, s1 = min(a.n_seqs, s0 + per);
+#pragma unroll 8
+    for (int s = s0; s < s1; ++s) mine += Q4Span(a, a.ctx_lens[s]).units();
+    uint32_t sum = mine;
 #pragma unroll
-    for (int s = 0; s < C::STAGES; ++s) mbar_init(bars + s, 1);
-    mbar_fence_init();
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += y;
+    }
+    if (lane == 31) warp_sum[warp] = sum;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < C::WARPS; ++w)
+      if (w < warp) sum += warp_sum[w];
+    before[threadIdx.x + 1] = sum;
+    if (threadIdx.x == 0) before[0] = 0;
+    __syncthreads();
   }
-  __shared__ int dead;
-  if (threadIdx.x == 0) dead = 0;
-  __syncthreads();
-  Q4Share<D> w;
-  w.begin(a, seq, kvh, split * Q4_WARPS + warp, splits * Q4_WARPS, lane);
-  for (int k = 0; k < min(w.turns, C::STAGES); ++k) w.fetch(k, ring, bars, lane);
-  Q4Query<D> q;
-  q.load(a.q + (long long)seq * a.q_stride + (long long)kvh * a.G * D, a.G, a.c0, lane);
-  Q4State<D> st;
-  st.clear();
-  for (int k = 0; k < w.turns; ++k) {
-    const int stage = k % C::STAGES;
-    if (!__all_sync(0xffffffffu, mbar_wait_or_fail(bars + stage, (uint32_t)(k / C::STAGES) & 1u, &dead, a.failed))) break;
-    const uint32_t at = smem_u32(ring + stage * C::TURN);
-    int first[C::PAGES];
+  // ---- sequences of no keys
+  for (int s = blockIdx.x; s < a.n_seqs; s += gridDim.x)
+    if (a.ctx_lens[s] <= 0 || a.bt_stride == 0)
+      for (int i = threadIdx.x; i < a.n_q * D / 2; i += THREADS) reinterpret_cast<uint32_t*>(a.out + (long long)s * a.n_q * D)[i] = 0;
+  const long long units = (long long)before[THREADS] * a.n_kv;
+  const int w_at = blockIdx.x * C::WARPS + warp, n_warps = gridDim.x * C::WARPS;
+  // (a division of 64 bits is some 100 instructions: only where 32 do not hold the units)
+  const int share = max(units >> 32 ? (int)((units + n_warps - 1) / n_warps) : (int)(((uint32_t)units + (uint32_t)n_warps - 1u) / (uint32_t)n_warps), least_share);
+  const long long piece0 = (long long)w_at * share;
+  long long u0 = piece0, u1 = min(u0 + share, units);
+  Q4Chain* chains = reinterpret_cast<Q4Chain*>(scratch) + 2 * w_at;
+  float* pieces = scratch + q4_chain_floats(n_warps) + 2 * w_at * q4_piece_floats(a.G, D);
+  if (lane < 2) chains[lane] = {0, 0, 0, 0};
+  __syncwarp();
+  if (u0 >= u1) return;
+  // ---- the sequence that has unit u, and its first unit
+  auto find = [&](long long u, long long& first) {
+    int c = 0;
 #pragma unroll
-    for (int x = 0; x < C::PAGES; ++x) first[x] = w.first_key(k * C::PAGES + x);
-    if (first[0] < w.lo || first[C::PAGES - 1] + 16 > w.ctx)
-      q4_turn<D, kCap, true>(at, q, st, a.c1, first, w.lo, w.ctx, lane);
-    else
-      q4_turn<D, kCap, false>(at, q, st, a.c1, first, w.lo, w.ctx, lane);
-    __syncwarp();
-    if (k + C::STAGES < w.turns) w.fetch(k + C::STAGES, ring, bars, lane);
-  }
-  // ---- this warp's state into its ring (all its copies have come): [head][D] | maxima [8] | sums [8]
-  float* mine = reinterpret_cast<float*>(ring);
-  const int g = lane >> 2, t = lane & 3;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    st.l[i] += __shfl_xor_sync(0xffffffffu, st.l[i], 4);
-    st.l[i] += __shfl_xor_sync(0xffffffffu, st.l[i], 8);
-    st.l[i] += __shfl_xor_sync(0xffffffffu, st.l[i], 16);
-    const int head = 2 * t + i;
-    if (head < a.G) {
-      float* to = mine + head * D + g * (D / 8);
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k) *reinterpret_cast<float2*>(to + 2 * k) = make_float2(st.o[k][i], st.o[k][2 + i]);
-      if (g == 0) {
-        mine[8 * D + head] = st.m[i];
-        mine[8 * D + 8 + head] = st.l[i];
+    for (int k = 0; k < THREADS / 32; ++k) c += __popc(__ballot_sync(0xffffffffu, (long long)before[32 * k + lane + 1] * a.n_kv <= u));
+    uint32_t at = before[c];
+    for (int s = c * per;; s += 32) {
+      uint32_t sum = per > 1 && s + lane < a.n_seqs ? Q4Span(a, a.ctx_lens[s + lane]).units() : 0;
+      if (per == 1) {
+        first = (long long)at * a.n_kv;
+        return s;
       }
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += y;
+      }
+      const int k = __popc(__ballot_sync(0xffffffffu, (long long)(at + sum) * a.n_kv <= u));
+      const uint32_t all = __shfl_sync(0xffffffffu, sum, 31), here = __shfl_sync(0xffffffffu, sum, max(k - 1, 0));
+      if (k < 32) {
+        first = (long long)(at + (k ? here : 0)) * a.n_kv;
+        return s + k;
+      }
+      at += all;
     }
+  };
+  long long seq_unit;
+  int seq = find(u0, seq_unit);
+  if (whole_items) {  // (B200Q_BATCH_INVARIANT: the items that begin in the piece, whole)
+    auto up = [&](long long u, int s, long long first) {
+      const uint32_t n = Q4Span(a, a.ctx_lens[s]).units();
+      return first + ((uint32_t)(u - first) + n - 1) / n * n;
+    };
+    long long first;
+    u0 = up(u0, seq, seq_unit);
+    if (u1 < units) {
+      const int s = find(u1, first);
+      u1 = up(u1, s, first);
+    }
+    if (u0 >= u1) return;
+    seq = find(u0, seq_unit);
   }
-  __syncthreads();
-  // ---- one state per CTA, in the first warp's place (an item is two values, which one thread reads and writes)
-  constexpr int RING_F = C::RING / 4;
-  float* all = reinterpret_cast<float*>(smem);
-  bf16* out = a.out + ((long long)seq * a.n_q + (long long)kvh * a.G) * D;
-  for (int idx = threadIdx.x * 2; idx < a.G * D; idx += Q4_WARPS * 64) {
-    const int r = idx / D;
-    float M = -INFINITY, den = 0.f;
-    float2 num = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int x = 0; x < Q4_WARPS; ++x) M = fmaxf(M, all[x * RING_F + 8 * D + r]);
-#pragma unroll
-    for (int x = 0; x < Q4_WARPS; ++x) {
-      const float mx = all[x * RING_F + 8 * D + r], wgt = mx == -INFINITY ? 0.f : q4_ex2(mx - M);
-      const float2 v = *reinterpret_cast<const float2*>(all + x * RING_F + idx);
-      num.x += wgt * v.x;
-      num.y += wgt * v.y;
-      den += wgt * all[x * RING_F + 8 * D + 8 + r];
+  // ---- pages on their way: of item (f_seq, f_head) from page f_page on; `left` units are not asked for yet.  What the other side has to know
+  // of an item goes through a small ring (the items of the turns in flight, and one more)
+  constexpr int ITEMS = 4;
+  static_assert(ITEMS > STAGES, "an item for every turn in flight");
+  __shared__ Q4Item items[C::WARPS][ITEMS];
+  int f_seq = seq, f_ctx = a.ctx_lens[seq], f_item = 0;
+  Q4Span f(a, f_ctx);
+  const uint32_t into = (uint32_t)(u0 - seq_unit);
+  int f_head = (int)(into / (uint32_t)f.units()), f_page = (int)(into - f_head * f.units()) - Q4_BEGIN, left = (int)(u1 - u0);
+  long long unit = u0 - (f_page + Q4_BEGIN);  // the item's first
+  if (f_page < 0) {  // (a piece that begins before the item's first page)
+    left += f_page;
+    f_page = 0;
+  }
+  if (left <= 0) return;  // (an item's begin and none of its pages)
+  bool fresh = true;      // the next turn is the first one of its item here
+  int f_stop = 0;
+  const int page_stride = a.n_kv * Kv4<D>::BYTES;
+  const uint8_t* f_kv = a.kv + (long long)f_head * Kv4<D>::BYTES;
+  const int32_t* f_row = a.block_table + (long long)f_seq * a.bt_stride + f.page0;
+  // numbers of the item's pages: 32 of them from ids_at on, the next 32, the first 32 of the sequence, and of the next sequence
+  auto ids_of = [&](const int32_t* row, int pages, int from) { return from + lane < pages ? row[from + lane] : 0; };
+  int ids_at = f_page;
+  int ids0 = ids_of(f_row, f.pages, 0), ids = ids_at ? ids_of(f_row, f.pages, ids_at) : ids0, ids_ahead = ids_of(f_row, f.pages, ids_at + 32);
+  int n_seq = 0, n_ctx = 0, n_ids = 0;  // the next sequence that has keys, once the last head of this one has begun
+  auto look_ahead = [&]() {
+    n_seq = f_seq;
+    do n_ctx = ++n_seq < a.n_seqs ? a.ctx_lens[n_seq] : 1; while (n_ctx <= 0);
+    if (n_seq < a.n_seqs) {
+      const Q4Span x(a, n_ctx);
+      n_ids = ids_of(a.block_table + (long long)n_seq * a.bt_stride + x.page0, x.pages, 0);
     }
-    if (splits > 1) {
-      *reinterpret_cast<float2*>(all + idx) = num;
-      if (idx % D == 0) {  // (the first warp's maxima and sums are still read: these go behind them)
-        all[8 * D + 16 + r] = M;
-        all[8 * D + 24 + r] = den;
+  };
+  auto begin_item = [&]() {
+    fresh = true;
+    if (lane == 0) items[warp][f_item % ITEMS] = {f_seq, f_head, f.ctx, f.lo, f.page0, f.pages};
+    ++f_item;
+    if (f_head == a.n_kv - 1) look_ahead();
+  };
+  auto next_item = [&]() {
+    f_page = 0;
+    f_kv += Kv4<D>::BYTES;
+    if (++f_head == a.n_kv) {
+      f_head = 0;
+      f_seq = n_seq;
+      f = Q4Span(a, n_ctx);
+      f_kv = a.kv;
+      f_row = a.block_table + (long long)f_seq * a.bt_stride + f.page0;
+      ids0 = n_ids;
+    }
+    ids_at = 0;
+    ids = ids0;
+    ids_ahead = ids_of(f_row, f.pages, 32);
+    begin_item();
+  };
+  // The next turn's pages into their stage: those of the item that are left, up to P of them.  Sixteen bytes per lane and copy, 512 in a row;
+  // a turn is nine copies.  (A bulk copy has to be told its addresses by one lane for all, some 40 instructions a page.)
+  constexpr int PIECES = Kv4<D>::BYTES / 16;  // of a page
+  auto copy_pages = [&](uint32_t to, int count) {
+    const uint8_t* from[P];
+#pragma unroll
+    for (int x = 0; x < P; ++x) from[x] = f_kv + lane * 16 + (long long)__shfl_sync(0xffffffffu, ids, f_page - ids_at + x) * page_stride;
+#pragma unroll
+    for (int k = 0; k < C::TURN / 512; ++k) {
+      const int x0 = 32 * k / PIECES, x1 = (32 * k + 31) / PIECES;  // the pages in which a copy's lanes lie
+      const bool second = x0 != x1 && lane >= x1 * PIECES - 32 * k;
+      const uint8_t* src = second ? from[x1] + 16 * (32 * k - x1 * PIECES) : from[x0] + 16 * (32 * k - x0 * PIECES);
+      if (count == P || (second ? x1 : x0) < count) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 512 * k), "l"(src) : "memory");
+    }
+  };
+  auto fetch_edge = [&](uint32_t to) {  // behind the last page, at an item's beginning and end, where the numbers are used up
+    if (left <= 0) return;
+    if (f_page - ids_at >= 32) {
+      ids_at += 32;
+      ids = ids_ahead;
+      ids_ahead = ids_of(f_row, f.pages, ids_at + 32);
+    }
+    const int count = min(P, min(f.pages - f_page, left));
+    copy_pages(to, count);
+    if (fresh) {
+      const uint8_t* q_rows = reinterpret_cast<const uint8_t*>(a.q + (long long)f_seq * a.q_stride + (long long)f_head * a.G * D);
+      for (int i = lane * 16; i < a.G * D * 2; i += 512)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to - lane * 16 + C::TURN + i), "l"(q_rows + i) : "memory");
+      fresh = false;
+    }
+    left -= count;
+    f_page += count;
+    if (f_page == f.pages) {
+      left -= Q4_BEGIN;  // (of the next item)
+      if (left > 0) next_item();
+    }
+    // up to here a turn is P pages of the same item whose numbers are there, and the next one begins behind it
+    f_stop = left > 0 && !fresh ? min(min(f.pages, f_page + left) - P, ids_at + 32 - P + 1) : 0;
+  };
+  auto fetch = [&](int stage) {
+    const uint32_t to = ring + stage * stage_bytes + lane * 16;
+    if (f_page < f_stop) {
+      copy_pages(to, P);
+      f_page += P;
+      left -= P;
+    } else {
+      fetch_edge(to);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  begin_item();
+  int page = f_page, to_do = left;  // the first item's pages begin here; units that have not been worked on, less the item's begin
+#pragma unroll
+  for (int s = 0; s < STAGES; ++s) fetch(s);
+  Q4Query<D> q;
+  Q4State<D> st;
+  int stage = 0, item = 0;
+  while (to_do > 0) {
+    __syncwarp();
+    const Q4Item it = items[warp][item++ % ITEMS];
+    const bool whole = page == 0;  // the item began in this piece
+    const int end = min(it.pages, page + to_do);
+    to_do -= end - page + Q4_BEGIN;
+    // turns whose keys all count begin from page `inner` up to `outer`
+    const int inner = it.lo > (it.page0 + page) * 16 ? page + 1 : page, outer = min(end - P, it.pages - P - 1);
+    for (bool first_turn = true; page < end; first_turn = false) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+      __syncwarp();
+      const uint32_t at = ring + stage * stage_bytes;
+      if (first_turn) {
+        q.load(at + C::TURN, a.G, a.c0, lane);
+        st.clear();
+      }
+      if (page >= inner && page <= outer) {
+        q4_turn<D, kCap, false>(at, q, st, a.c1, nullptr, 0, 0, lane);
+      } else {
+        int first[P];
+#pragma unroll
+        for (int x = 0; x < P; ++x) first[x] = page + x < end ? (it.page0 + page + x) * 16 : it.ctx;
+        q4_turn<D, kCap, true>(at, q, st, a.c1, first, it.lo, it.ctx, lane);
+      }
+      __syncwarp();
+      fetch(stage);
+      stage ^= 1;
+      page += P;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      st.l[i] += __shfl_xor_sync(0xffffffffu, st.l[i], 4);
+      st.l[i] += __shfl_xor_sync(0xffffffffu, st.l[i], 8);
+      st.l[i] += __shfl_xor_sync(0xffffffffu, st.l[i], 16);
+    }
+    if (whole && end == it.pages) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int head = 2 * t + i;
+        const float inv = st.l[i] > 0.f ? 1.f / st.l[i] : st.l[i];  // (NaN stays)
+        uint32_t* to = reinterpret_cast<uint32_t*>(a.out + ((long long)it.seq * a.n_q + (long long)it.head * a.G + head) * D) + g * (D / 16);
+        if (head < a.G)
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) to[k] = pack_bf16x2(st.o[k][i] * inv, st.o[k][2 + i] * inv);
       }
     } else {
-      const float inv = den > 0.f ? 1.f / den : den == 0.f ? 0.f : den;  // (NaN stays)
-      *reinterpret_cast<uint32_t*>(out + idx) = pack_bf16x2(num.x * inv, num.y * inv);
-    }
-  }
-  if (splits > 1) {
-    cluster_sync_all();
-    const int per = (a.G * D / 2 + splits - 1) / splits * 2;
-    for (int idx = split * per + threadIdx.x * 2; idx < min((split + 1) * per, a.G * D); idx += Q4_WARPS * 64) {
-      const int r = idx / D;
-      float M = -INFINITY, den = 0.f;
-      float2 num = make_float2(0.f, 0.f);
-      for (int x = 0; x < splits; ++x) M = fmaxf(M, ld_cluster_f32(mapa_shared(all + 8 * D + 16 + r, x)));
-      for (int x = 0; x < splits; ++x) {
-        const float mx = ld_cluster_f32(mapa_shared(all + 8 * D + 16 + r, x)), wgt = mx == -INFINITY ? 0.f : q4_ex2(mx - M);
-        const uint32_t from = mapa_shared(all + idx, x);
-        num.x += wgt * ld_cluster_f32(from);
-        num.y += wgt * ld_cluster_f32(from + 4);
-        den += wgt * ld_cluster_f32(mapa_shared(all + 8 * D + 24 + r, x));
+      const int slot = whole ? 1 : 0;  // (an item that ends in the next piece, or one that began in an earlier one)
+      float* to = pieces + slot * q4_piece_floats(a.G, D);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int head = 2 * t + i;
+        if (head < a.G) {
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) *reinterpret_cast<float2*>(to + head * D + g * (D / 8) + 2 * k) = make_float2(st.o[k][i], st.o[k][2 + i]);
+          if (g == 0) {
+            to[a.G * D + head] = st.m[i];
+            to[a.G * D + a.G + head] = st.l[i];
+          }
+        }
       }
-      const float inv = den > 0.f ? 1.f / den : den == 0.f ? 0.f : den;
-      *reinterpret_cast<uint32_t*>(out + idx) = pack_bf16x2(num.x * inv, num.y * inv);
+      if (lane == 0) {
+        // pages of the item before this warp's piece and behind it, and so the warps that have the first and the last one
+        const int ahead = max((int)(piece0 - (unit + Q4_BEGIN)), 0), behind = (int)(unit + Q4_BEGIN + it.pages - 1 - piece0);
+        const int from = w_at - (ahead + share - 1) / share;
+        chains[slot] = {it.seq, it.head, from, w_at + behind / share - from + 1};
+      }
     }
-    cluster_sync_all();  // nobody leaves while a peer still reads
+    unit += it.pages + Q4_BEGIN;
+    page = 0;
   }
 }
 
-int g_q4_splits = 0;  // test hook: > 0 forces the number of CTAs per sequence and head
+// The pieces of one item's chain: every warp of it has 64 threads here, and as many groups of them share the outputs, four of them to a thread; threads
+// that have no outputs of their own take a share of the pieces instead.
+constexpr int Q4_JOIN = 64;
+struct Q4Part {
+  float m = -INFINITY, l = 0.f;
+  float4 o = {0.f, 0.f, 0.f, 0.f};
+  __device__ __forceinline__ void add(const Q4Part& x) {
+    if (x.m == -INFINITY && x.l == 0.f) return;
+    const float top = fmaxf(m, x.m), old = m == -INFINITY ? 0.f : q4_ex2(m - top), now = x.m == -INFINITY ? 1.f : q4_ex2(x.m - top);
+    m = top;
+    l = l * old + x.l * now;
+    o = make_float4(o.x * old + x.o.x * now, o.y * old + x.o.y * now, o.z * old + x.o.z * now, o.w * old + x.o.w * now);
+  }
+};
+template <int D>
+__global__ void __launch_bounds__(8 * Q4_JOIN) kv4_join_kernel(const float* scratch, bf16* out, int n_q, int G) {
+  follow_previous(scratch, out);
+  // four warps' chains to a block, 64 threads to each of a warp's two
+  const int n_warps = gridDim.x * 4, tid = threadIdx.x % Q4_JOIN, w_at = blockIdx.x * 4 + threadIdx.x / (2 * Q4_JOIN), slot = threadIdx.x / Q4_JOIN % 2;
+  __shared__ float4 o_s[8 * Q4_JOIN];
+  __shared__ float2 ml_s[8 * Q4_JOIN];
+  const Q4Chain c = reinterpret_cast<const Q4Chain*>(scratch)[2 * w_at + slot];
+  if (!__syncthreads_or(c.n >= 2)) return;
+  const float* pieces = scratch + q4_chain_floats(n_warps);
+  const int size = (int)q4_piece_floats(G, D);
+  const int rank = w_at - c.from, quads = G * D / 4, per = c.n >= 2 ? (quads + c.n - 1) / c.n : 0, q_end = min(quads, (rank + 1) * per);
+  const int here = max(min(Q4_JOIN, q_end - rank * per), 0);
+  // threads side by side; the others go through the pieces beside them
+  const int width = here > 1 ? 1 << (32 - __clz(here - 1)) : 1, parts = Q4_JOIN / width, part = tid / width;
+  const bool shared = __syncthreads_or(c.n >= 2 && parts > 1);
+  const int rounds = (G * D / 8 + Q4_JOIN - 1) / Q4_JOIN;  // (for a chain of two; longer ones find nothing left to do)
+  for (int round = 0; round < rounds; ++round) {
+    const int quad = rank * per + round * Q4_JOIN + tid % width, head = quad * 4 / D;
+    const bool mine = c.n >= 2 && tid % width < here && quad < q_end;
+    Q4Part x;
+    if (mine)
+#pragma unroll 1
+      for (int p = part; p < c.n; p += parts) {
+        const float* from = pieces + (2LL * (c.from + p) + (p == 0)) * size;
+        Q4Part y;
+        y.m = from[G * D + head];
+        y.l = from[G * D + G + head];
+        y.o = *reinterpret_cast<const float4*>(from + 4 * quad);
+        x.add(y);
+      }
+    if (shared)
+      for (int o = Q4_JOIN / 2; o > 0; o >>= 1) {  // (all chains take the same steps; those within a chain's width add nothing)
+        o_s[threadIdx.x] = x.o;
+        ml_s[threadIdx.x] = make_float2(x.m, x.l);
+        __syncthreads();
+        if (mine && o >= width && part < o / width) {
+          Q4Part y;
+          y.m = ml_s[threadIdx.x + o].x;
+          y.l = ml_s[threadIdx.x + o].y;
+          y.o = o_s[threadIdx.x + o];
+          x.add(y);
+        }
+        __syncthreads();
+      }
+    if (mine && part == 0) {
+      const float inv = x.l > 0.f ? 1.f / x.l : x.l;
+      bf16* to = out + ((long long)c.seq * n_q + (long long)c.head * G) * D + 4 * quad;
+      *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(x.o.x * inv, x.o.y * inv), pack_bf16x2(x.o.z * inv, x.o.w * inv));
+    }
+  }
+}
+
+int g_q4_whole = -1;  // test hook: 1 / 0 give items to warps whole or not (-1: as B200Q_BATCH_INVARIANT says)
+static std::mutex g_q4_pair;  // no other thread's pieces on the same stream between a stream kernel and its join
 
 template <int D, bool kCap>
-static int launch_kv4_decode(const Kv4Args& a, cudaStream_t st) {
-  auto kern = kv4_decode_kernel<D, kCap>;
+static int launch_kv4_stream(const Kv4Args& a, cudaStream_t st) {
+  using C = Q4Stream<D>;
+  auto kern = kv4_stream_kernel<D, kCap>;
   static bool ready[64];
   int dev = 0;
   B200Q_CUDA(cudaGetDevice(&dev));
   if (dev >= 64 || !ready[dev]) {
-    B200Q_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Q4Smem<D>::TOTAL));
-    B200Q_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    B200Q_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem(8)));
     if (dev < 64) ready[dev] = true;
   }
-  const int pages = a.window > 0 && (a.window + 15) / 16 + 1 < a.bt_stride ? (a.window + 15) / 16 + 1 : a.bt_stride;
-  const long long items = (long long)a.n_seqs * a.n_kv;
-  int splits = 1;
-  while (!batch_invariant() && splits < Q4_MOST_CTAS && items * splits * 2 <= 4 * 148 && pages >= 2 * splits * Q4_WARPS * Q4Cfg<D>::PAGES) splits *= 2;
-  if (g_q4_splits > 0) splits = g_q4_splits;
-  for (int s0 = 0; s0 < a.n_seqs; s0 += 65535) {  // (a grid's second dimension ends there)
-    Kv4Args b = a;
-    b.n_seqs = a.n_seqs - s0 < 65535 ? a.n_seqs - s0 : 65535;
-    b.q += (long long)s0 * a.q_stride;
-    b.out += (long long)s0 * a.n_q * D;
-    b.block_table += (long long)s0 * a.bt_stride;
-    b.ctx_lens += s0;
-    B200Q_CUDA(launch_early(kern, dim3(splits, b.n_seqs, b.n_kv), Q4_WARPS * 32, Q4Smem<D>::TOTAL, st, splits, b));
-    count_launch();
-  }
+  const int ctas = C::CTAS * num_sms(), warps = ctas * C::WARPS;
+  // Items of up to 8 pages go to warps whole: adding up pieces costs as much as they do (one sequence of 64 tokens, 8 kv heads, 5.6 us, in
+  // pieces 9.5; 2800 of 128 tokens 96.5, in pieces 103.9).
+  const int width = a.window > 0 && (a.window + 15) / 16 + 1 < a.bt_stride ? (a.window + 15) / 16 + 1 : a.bt_stride;
+  const bool whole = g_q4_whole < 0 ? batch_invariant() || width <= 8 : g_q4_whole != 0;
+  float* scratch = nullptr;
+  const int rc = stream_scratch(1, (size_t)(q4_chain_floats(warps) + 2 * warps * q4_piece_floats(a.G, D)) * sizeof(float), st, &scratch);
+  if (rc) return rc;
+  std::lock_guard<std::mutex> together(g_q4_pair);
+  B200Q_CUDA(launch_early(kern, dim3(ctas), C::WARPS * 32, C::smem(a.G), st, 1, a, C::stage_bytes(a.G), (int)whole, whole ? 1 : Q4_LEAST_SHARE, scratch));
+  count_launch();
+  if (whole) return B200Q_OK;
+  B200Q_CUDA(launch_early(kv4_join_kernel<D>, dim3(ctas), 8 * Q4_JOIN, 0, st, 1, (const float*)scratch, a.out, a.n_q, a.G));
+  count_launch();
   return B200Q_OK;
 }
 
@@ -515,9 +737,9 @@ using namespace b200q;
 
 extern "C" {
 
-int b200q_decode_attn_q4_set_splits(int splits) {
-  B200Q_CHECK_ARG(splits >= 0 && splits <= Q4_MOST_CTAS, "decode_attn_q4: splits must be 0..%d", Q4_MOST_CTAS);
-  g_q4_splits = splits;
+int b200q_decode_attn_q4_set_whole(int whole) {
+  B200Q_CHECK_ARG(whole >= -1 && whole <= 1, "decode_attn_q4: whole must be -1..1");
+  g_q4_whole = whole;
   bump_tuning_epoch();
   return B200Q_OK;
 }
@@ -534,7 +756,7 @@ int b200q_decode_attn_q4(const void* q, int q_stride, void* out, const void* kv4
   B200Q_CHECK_ARG(q && out && kv4_layer && block_table && ctx_lens, "decode_attn_q4: null argument");
   B200Q_CHECK_ARG(q_stride % 8 == 0 && q_stride >= n_q * D && ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(kv4_layer)) & 15) == 0,
                   "decode_attn_q4: q (rows of q_stride=%d, a multiple of 8) and the cache must be 16-byte aligned", q_stride);
-  B200Q_CHECK_ARG((reinterpret_cast<uintptr_t>(out) & 3) == 0, "decode_attn_q4: out must be 4-byte aligned");
+  B200Q_CHECK_ARG((reinterpret_cast<uintptr_t>(out) & 7) == 0, "decode_attn_q4: out must be 8-byte aligned");
   const float log2e = 1.4426950408889634f;
   Kv4Args a{};
   a.q = (const bf16*)q;
@@ -551,16 +773,12 @@ int b200q_decode_attn_q4(const void* q, int q_stride, void* out, const void* kv4
   a.window = window;
   a.c0 = softcap > 0.f ? 2.f * log2e * scale / softcap : scale * log2e;
   a.c1 = softcap * log2e;
-  if (!wait_flag(&a.failed)) {
-    set_error("decode_attn_q4: no host memory for the wait flag");
-    return B200Q_ENOMEM;
-  }
   cudaStream_t st = as_stream(stream);
   auto run = [&](auto cap) {
     constexpr bool c = decltype(cap)::value;
-    if (D == 64) return launch_kv4_decode<64, c>(a, st);
-    if (D == 128) return launch_kv4_decode<128, c>(a, st);
-    return launch_kv4_decode<256, c>(a, st);
+    if (D == 64) return launch_kv4_stream<64, c>(a, st);
+    if (D == 128) return launch_kv4_stream<128, c>(a, st);
+    return launch_kv4_stream<256, c>(a, st);
   };
   return softcap > 0.f ? run(std::true_type{}) : run(std::false_type{});
 }

@@ -312,7 +312,7 @@ SIGNATURES = {
     "b200q_rope_kvwrite_q4": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
     "b200q_kv4_unpack": (_i, [_vp, _vp, _i, _vp, _i, _i, _i, _vp]),
     "b200q_decode_attn_q4": (_i, [_vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _f, _f, _i, _vp]),
-    "b200q_decode_attn_q4_set_splits": (_i, [_i]),
+    "b200q_decode_attn_q4_set_whole": (_i, [_i]),
     "b200q_prefill_attn_q4_workspace": (_i64, [_i, _i, _i, _i]),
     "b200q_prefill_attn_q4": (_i, [_vp, _i, _vp, _vp, _vp, _i, _i, _vp, _i, _i, _i, _i, _i, _f, _f, _i, _vp, _i64, _vp]),
     "b200q_beam_select_workspace": (_i64, [_i, _i, _i64, _i]),
@@ -662,8 +662,8 @@ def decode_attn_q4(qkv, out, kv4_layer, block_table, ctx_lens, n_q, n_kv, D, blo
                                       block_size, scale, softcap, window, s))
 
 
-def decode_attn_q4_set_splits(splits: int):
-    check(load().b200q_decode_attn_q4_set_splits(splits))
+def decode_attn_q4_set_whole(whole: int):
+    check(load().b200q_decode_attn_q4_set_whole(whole))
 
 
 def prefill_attn_q4_workspace(n_seqs, bt_stride, n_kv, D):

@@ -93,13 +93,13 @@ def test_decode(cuda, D, n_q, n_kv, ctxs, cap, window):
     qkv = torch.randn(B, (n_q + 2 * n_kv) * D, generator=torch.Generator().manual_seed(7)).to(BF)
     out = torch.full((B + 1, n_q * D), float("nan"), dtype=BF, device=cuda)
     args = (cache.to(cuda), table.to(cuda), torch.tensor(ctxs, dtype=torch.int32, device=cuda), n_q, n_kv, D, BS, D ** -0.5)
-    for splits in (0, 1, 3, 16):
+    for whole in (0, 1):
         out.fill_(float("nan"))
-        lib.decode_attn_q4_set_splits(splits)
+        lib.decode_attn_q4_set_whole(whole)
         try:
             lib.decode_attn_q4(qkv.to(cuda), out, *args, softcap=cap, window=window)
         finally:
-            lib.decode_attn_q4_set_splits(0)
+            lib.decode_attn_q4_set_whole(-1)
         got = out.cpu()
         assert torch.isnan(got[B].float()).all()
         for i, c in enumerate(ctxs):
@@ -108,7 +108,7 @@ def test_decode(cuda, D, n_q, n_kv, ctxs, cap, window):
                 continue
             q = qkv[i: i + 1, : n_q * D].view(1, n_q, D)
             ref, weight, size = attention(q, *rows[i], torch.tensor([c - 1]), D ** -0.5, cap, window)
-            attention_close(got[i].view(1, n_q, D), ref, weight, size, D, 2.0 ** -11, f"ctx {c}, {splits} CTAs")
+            attention_close(got[i].view(1, n_q, D), ref, weight, size, D, 2.0 ** -11, f"ctx {c}, whole {whole}")
     assert lib.load().b200q_wait_failures() == 0
 
 

@@ -46,7 +46,7 @@ def test_decode(change, word):
     a = dict(q=P, stride=1024, out=P, cache=P, table=P, bt=4, ctx=P, n=2, n_q=4, n_kv=2, D=128, block=16, scale=1.0, cap=0.0, window=0)
     a.update(change)
     refused(lib.load().b200q_decode_attn_q4(*a.values(), 0), word)
-    assert lib.load().b200q_decode_attn_q4_set_splits(17) == -1
+    assert lib.load().b200q_decode_attn_q4_set_whole(2) == -1
 
 
 @pytest.mark.parametrize("change,word", [(dict(D=256, n_q=16), "GQA"), (dict(n_q=18), "GQA"), (dict(bytes=100), "too small"), (dict(work=P + 128), "aligned"),
