@@ -88,26 +88,27 @@ __device__ __forceinline__ uint32_t kv4_scale_of(float most, bool nan) {
 }
 __device__ __forceinline__ float kv4_scale_value(uint32_t b) { return __half2float(__ushort_as_half((unsigned short)(b << 7))); }
 
-// Sixteen values (of a 16-bit float) to their codes and scale byte.  Quotients that are not on a border between two codes are 2^-11 and more
-// away from it (both have few bits): to multiples of 2^-13 they fall onto it exactly where they are on it, whatever the reciprocal rounds.
-__device__ __forceinline__ uint2 kv4_quantise(const float (&x)[16], uint32_t& scale) {
-  float most = 0.f;
-  bool nan = false;
+// Sixteen bf16 values to their codes and scale byte.  Quotients that are not on a border between two codes are 2^-11 and more away from it
+// (both have few bits): to multiples of 2^-13 they fall onto it exactly where they are on it, whatever the reciprocal rounds.
+__device__ __forceinline__ uint2 kv4_quantise(const uint4& x0, const uint4& x1, uint32_t& scale) {
+  const uint32_t x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+  uint32_t most = 0;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    most = fmaxf(most, fabsf(x[i]));
-    nan |= x[i] != x[i];
-  }
-  scale = kv4_scale_of(most, nan);
+  for (int i = 0; i < 8; ++i) asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(most) : "r"(x[i] & 0x7fff7fffu));
+  const float lo = bf16_lo(most), hi = bf16_hi(most);
+  const bool nan = lo != lo || hi != hi;
+  scale = kv4_scale_of(fmaxf(lo, hi), nan);
   const float r = __frcp_rn(kv4_scale_value(nan ? 1u : scale));
-  float y[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) y[i] = __fsub_rn(__fadd_rn(__fmul_rn(x[i], r), 1536.f), 1536.f);
-#pragma unroll
-  for (int i = 0; i < 16; ++i) y[i] = y[i] == 0.f ? copysignf(0.f, x[i]) : y[i];
   uint32_t w[2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < 2; ++i) {
+    float y[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t v = x[4 * i + k / 2];
+      const float f = k & 1 ? bf16_hi(v) : bf16_lo(v);
+      y[k] = copysignf(__fsub_rn(__fadd_rn(__fmul_rn(fabsf(f), r), 1536.f), 1536.f), f);  // (a zero keeps its sign)
+    }
     asm("{\n\t.reg .b8 a, b, c, d;\n\t"
         "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
         "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
@@ -115,8 +116,8 @@ __device__ __forceinline__ uint2 kv4_quantise(const float (&x)[16], uint32_t& sc
         "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
         "mov.b32 %0, {a, b, c, d};\n\t}"
         : "=r"(w[i])
-        : "f"(y[8 * i]), "f"(y[8 * i + 1]), "f"(y[8 * i + 2]), "f"(y[8 * i + 3]), "f"(y[8 * i + 4]), "f"(y[8 * i + 5]), "f"(y[8 * i + 6]),
-          "f"(y[8 * i + 7]));
+        : "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7]));
+  }
   return make_uint2(w[0], w[1]);
 }
 

@@ -1,26 +1,49 @@
 // kv4_ops.cu — writing the 4-bit cache (rotation and quantisation), reading its pages back as 16-bit ones, and prompt attention over it.
 // The page's layout and the conversions: kv4.cuh.
+#include <type_traits>
+
 #include "kv4.cuh"
 
 namespace b200q {
 
-__device__ __forceinline__ void floats_of(const uint4& v, float* x) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = bf16_lo(w[i]);
-    x[2 * i + 1] = bf16_hi(w[i]);
-  }
+// Two bf16 at once.  A product, a sum or a difference of two bf16 rounded to bf16 once is what fp32 arithmetic and a rounding behind it give
+// (products are exact in fp32; sums either are, or their fp32 rounding lies far below bf16's).
+__device__ __forceinline__ uint32_t mul_bf2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t add_bf2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t sub_bf2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// x1, x2 <- x1 cos - x2 sin, x2 cos + x1 sin, a rounding behind every operation
+__device__ __forceinline__ void turn_bf2(uint32_t& x1, uint32_t& x2, uint32_t c, uint32_t s) {
+  const uint32_t o1 = sub_bf2(mul_bf2(x1, c), mul_bf2(x2, s));
+  x2 = add_bf2(mul_bf2(x2, c), mul_bf2(x1, s));
+  x1 = o1;
+}
+__device__ __forceinline__ void turn_bf8(uint4& x1, uint4& x2, const uint4& c, const uint4& s) {
+  turn_bf2(x1.x, x2.x, c.x, s.x);
+  turn_bf2(x1.y, x2.y, c.y, s.y);
+  turn_bf2(x1.z, x2.z, c.z, s.z);
+  turn_bf2(x1.w, x2.w, c.w, s.w);
 }
 
 // ------------------------------------------------------------------------------------------------------------------------
 // Rotation of q and k (pairs i, i + D/2; a bf16 rounding behind every operation, as in elementwise.cu) and the write into 4-bit pages.
-// Items of a token: groups of 16 values of k with those they are paired with (two groups), groups of v, 8 + 8 values of q.  A thread has
-// its groups whole, so that no maximum crosses threads; rotated keys exist in registers only.
+// Items of a token: groups of 16 values of k with those they are paired with (two groups), groups of v, 8 + 8 values of q; a thread to an item,
+// so that no maximum crosses threads; rotated keys exist in registers only.
 // Bound: the rows' bytes (a cached token is 9/16 of a byte per value, a quarter of what the 16-bit write stores).
 // ------------------------------------------------------------------------------------------------------------------------
 template <int D>
-__global__ void __launch_bounds__(256) rope_kvwrite_q4_kernel(uint4* qkv, const uint4* cos_sin, const int32_t* positions, const int32_t* slot_mapping,
+__global__ void __launch_bounds__(512) rope_kvwrite_q4_kernel(uint4* qkv, const uint4* cos_sin, const int32_t* positions, const int32_t* slot_mapping,
                                                               uint8_t* kv_layer, int n_q, int n_kv) {
   follow_previous(qkv, cos_sin, positions, slot_mapping, kv_layer);
   constexpr int CPR = D / 8, HALF = CPR / 2;  // 16-byte pieces of a head's row, of half of it
@@ -30,55 +53,43 @@ __global__ void __launch_bounds__(256) rope_kvwrite_q4_kernel(uint4* qkv, const 
   const uint4* cs_row = cos_sin + (long long)positions[t] * CPR;
   const int token = slot & 15;
   uint8_t* page = kv_layer + (long long)(slot >> 4) * n_kv * Kv4<D>::BYTES;
-  const int k_items = slot >= 0 ? n_kv * (D / 32) : 0, v_items = slot >= 0 ? n_kv * (D / 16) : 0;
+  const int k_items = n_kv * (D / 32), v_items = n_kv * (D / 16);
   const int n_items = k_items + v_items + n_q * HALF;
-  auto turn = [](float x1, float x2, float c, float s, float& o1, float& o2) {
-    o1 = round_bf16(round_bf16(x1 * c) - round_bf16(x2 * s));
-    o2 = round_bf16(round_bf16(x2 * c) + round_bf16(x1 * s));
-  };
   for (int it = blockIdx.y * blockDim.x + threadIdx.x; it < n_items; it += gridDim.y * blockDim.x) {
     if (it < k_items) {
+      if (slot < 0) continue;
       const int h = it / (D / 32), p = it % (D / 32);  // groups p and p + D/32
       const uint4* src = row + (n_q + h) * CPR + 2 * p;
-      float a[16], b[16], c[16], s[16];
+      const uint4* cs = cs_row + 2 * p;
+      uint4 a[2], b[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        floats_of(ld_v4(src + i), a + 8 * i);
-        floats_of(ld_v4(src + HALF + i), b + 8 * i);
-        floats_of(ld_v4(cs_row + 2 * p + i), c + 8 * i);
-        floats_of(ld_v4(cs_row + HALF + 2 * p + i), s + 8 * i);
+        a[i] = ld_v4(src + i);
+        b[i] = ld_v4(src + HALF + i);
+        turn_bf8(a[i], b[i], ld_v4(cs + i), ld_v4(cs + HALF + i));
       }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) turn(a[i], b[i], c[i], s[i], a[i], b[i]);
       uint8_t* to = page + h * Kv4<D>::BYTES;
       const int r = kv4_key_row<D>(token);
       uint32_t scale;
-      *reinterpret_cast<uint2*>(to + kv4_key_code<D>(r, p)) = kv4_quantise(a, scale);
+      *reinterpret_cast<uint2*>(to + kv4_key_code<D>(r, p)) = kv4_quantise(a[0], a[1], scale);
       to[kv4_key_scale<D>(r, p)] = (uint8_t)scale;
-      *reinterpret_cast<uint2*>(to + kv4_key_code<D>(r, p + D / 32)) = kv4_quantise(b, scale);
+      *reinterpret_cast<uint2*>(to + kv4_key_code<D>(r, p + D / 32)) = kv4_quantise(b[0], b[1], scale);
       to[kv4_key_scale<D>(r, p + D / 32)] = (uint8_t)scale;
     } else if (it < k_items + v_items) {
+      if (slot < 0) continue;
       const int h = (it - k_items) / (D / 16), p = (it - k_items) % (D / 16);
       const uint4* src = row + (n_q + n_kv + h) * CPR + 2 * p;
-      float a[16];
-      floats_of(ld_v4(src), a);
-      floats_of(ld_v4(src + 1), a + 8);
       uint8_t* to = page + h * Kv4<D>::BYTES;
       uint32_t scale;
-      *reinterpret_cast<uint2*>(to + kv4_value_code<D>(token, p)) = kv4_quantise(a, scale);
+      *reinterpret_cast<uint2*>(to + kv4_value_code<D>(token, p)) = kv4_quantise(ld_v4(src), ld_v4(src + 1), scale);
       to[kv4_value_scale<D>(token, p)] = (uint8_t)scale;
     } else {
       const int h = (it - k_items - v_items) / HALF, c0 = (it - k_items - v_items) % HALF;
       uint4* at = row + h * CPR + c0;
-      float a[8], b[8], c[8], s[8];
-      floats_of(ld_v4(at), a);
-      floats_of(ld_v4(at + HALF), b);
-      floats_of(ld_v4(cs_row + c0), c);
-      floats_of(ld_v4(cs_row + HALF + c0), s);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) turn(a[i], b[i], c[i], s[i], a[i], b[i]);
-      st_v4(at, make_uint4(pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(a[4], a[5]), pack_bf16x2(a[6], a[7])));
-      st_v4(at + HALF, make_uint4(pack_bf16x2(b[0], b[1]), pack_bf16x2(b[2], b[3]), pack_bf16x2(b[4], b[5]), pack_bf16x2(b[6], b[7])));
+      uint4 a = ld_v4(at), b = ld_v4(at + HALF);
+      turn_bf8(a, b, ld_v4(cs_row + c0), ld_v4(cs_row + HALF + c0));
+      st_v4(at, a);
+      st_v4(at + HALF, b);
     }
   }
 }
@@ -86,50 +97,69 @@ __global__ void __launch_bounds__(256) rope_kvwrite_q4_kernel(uint4* qkv, const 
 // ------------------------------------------------------------------------------------------------------------------------
 // 4-bit pages as 16-bit ones (the layout of attn.cu: [2][n_kv][16][D], the 16-byte piece c of a row at c ^ (token & 7)).  Exact.
 // ------------------------------------------------------------------------------------------------------------------------
-// one head's page by the threads of a warp: an item is 8 values
+// One head's page by a warp, through its own place in shared memory (the page's bytes, 16 a lane): then an item is 8 values, 16 bytes out, and a
+// warp's stores are whole rows.
 template <int D>
-__device__ __forceinline__ void kv4_spread_head(const uint8_t* head, uint4* keys, uint4* values, int lane) {
-  constexpr int CPR = D / 8;
-#pragma unroll 4
-  for (int it = lane; it < 32 * CPR; it += 32) {
-    const int which = it / (16 * CPR), token = it / CPR % 16, c = it % CPR, p = c >> 1;
-    const int r = kv4_key_row<D>(token);
-    const uint32_t codes = *reinterpret_cast<const uint32_t*>(head + (which ? kv4_value_code<D>(token, p) : kv4_key_code<D>(r, p)) + (c & 1) * 4);
-    const uint32_t b = head[which ? kv4_value_scale<D>(token, p) : kv4_key_scale<D>(r, p)];
-    uint32_t h[4];
-    kv4_halves(codes, h);
-    const float s = kv4_scale_value(b);
-    uint32_t w[4];
+__device__ __forceinline__ void kv4_spread_head(const uint8_t* head, uint4* keys, uint4* values, uint8_t* stage, int lane) {
+  constexpr int CPR = D / 8, PIECES = Kv4<D>::BYTES / 16;
+  __syncwarp();
+  uint4 v[(PIECES + 31) / 32];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
-      w[i] = pack_bf16x2(f.x * s, f.y * s);
+  for (int i = 0; i < (PIECES + 31) / 32; ++i)
+    if (i * 32 + lane < PIECES) v[i] = ld_once_v4(head + (i * 32 + lane) * 16);
+#pragma unroll
+  for (int i = 0; i < (PIECES + 31) / 32; ++i)
+    if (i * 32 + lane < PIECES) st_v4(stage + (i * 32 + lane) * 16, v[i]);
+  __syncwarp();
+  auto part = [&](auto is_value) {
+    constexpr bool kValue = decltype(is_value)::value;
+    uint4* out = kValue ? values : keys;
+#pragma unroll 4
+    for (int it = lane; it < 16 * CPR; it += 32) {
+      const int token = it / CPR, c = it % CPR, p = c >> 1, r = kv4_key_row<D>(token);
+      const uint32_t codes = *reinterpret_cast<const uint32_t*>(stage + (kValue ? kv4_value_code<D>(token, p) : kv4_key_code<D>(r, p)) + (c & 1) * 4);
+      const uint32_t b = stage[kValue ? kv4_value_scale<D>(token, p) : kv4_key_scale<D>(r, p)];
+      uint32_t h[4];
+      kv4_halves(codes, h);
+      const float s = kv4_scale_value(b);
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+        w[i] = pack_bf16x2(f.x * s, f.y * s);
+      }
+      st_v4(out + token * CPR + (c ^ (token & 7)), make_uint4(w[0], w[1], w[2], w[3]));
     }
-    (which ? values : keys)[token * CPR + (c ^ (token & 7))] = make_uint4(w[0], w[1], w[2], w[3]);
-  }
+  };
+  part(std::false_type{});
+  part(std::true_type{});
 }
 
+constexpr int SPREAD_WARPS = 8;
 template <int D>
-__global__ void __launch_bounds__(128) kv4_unpack_kernel(const uint8_t* kv4, const int32_t* pages, int n_pages, uint4* out, int n_kv) {
+__global__ void __launch_bounds__(SPREAD_WARPS * 32) kv4_unpack_kernel(const uint8_t* kv4, const int32_t* pages, int n_pages, uint4* out, int n_kv) {
   follow_previous(kv4, pages, out);
+  __shared__ __align__(16) uint8_t stage[SPREAD_WARPS][Kv4<D>::BYTES];
+  const int warp = threadIdx.x >> 5;
   const long long items = (long long)n_pages * n_kv;
-  for (long long it = (long long)blockIdx.x * 4 + (threadIdx.x >> 5); it < items; it += (long long)gridDim.x * 4) {
+  for (long long it = (long long)blockIdx.x * SPREAD_WARPS + warp; it < items; it += (long long)gridDim.x * SPREAD_WARPS) {
     const long long i = it / n_kv;
-    const int h = (int)(it % n_kv);
+    const int h = (int)(it - i * n_kv);
     constexpr int ROWS = 16 * D / 8;
     uint4* keys = out + ((i * 2) * n_kv + h) * ROWS;
-    kv4_spread_head<D>(kv4 + ((long long)pages[i] * n_kv + h) * Kv4<D>::BYTES, keys, keys + (long long)n_kv * ROWS, threadIdx.x & 31);
+    kv4_spread_head<D>(kv4 + ((long long)pages[i] * n_kv + h) * Kv4<D>::BYTES, keys, keys + (long long)n_kv * ROWS, stage[warp], threadIdx.x & 31);
   }
 }
 
 // The pages that a step's portions see, spread out to a workspace in which column c of row r of the block table is page r * bt_stride + c.
-// A block has SPREAD_COLUMNS columns of one row; what a row needs it finds from the tiles (their first visible and their last key).
-constexpr int SPREAD_COLUMNS = 4;
+// A warp has one head of one page; what a row needs it finds from the tiles (their first visible and their last key).
 template <int D>
-__global__ void __launch_bounds__(256) kv4_spread_kernel(const uint8_t* kv4, const int32_t* block_table, int bt_stride, const int4* tiles, int n_tiles,
-                                                         int n_kv, int window, uint4* out, int32_t* table) {
+__global__ void __launch_bounds__(SPREAD_WARPS * 32) kv4_spread_kernel(const uint8_t* kv4, const int32_t* block_table, int bt_stride, const int4* tiles,
+                                                                       int n_tiles, int n_kv, int window, uint4* out, int32_t* table) {
   follow_previous(kv4, block_table, tiles, out, table);
-  const int row = blockIdx.y, c0 = blockIdx.x * SPREAD_COLUMNS;
+  __shared__ __align__(16) uint8_t stage[SPREAD_WARPS][Kv4<D>::BYTES];
+  const int row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int c = (blockIdx.x * SPREAD_WARPS + warp) / n_kv, h = (blockIdx.x * SPREAD_WARPS + warp) % n_kv;
   int lo = 0x7fffffff, hi = 0;
   for (int i = threadIdx.x; i < n_tiles; i += blockDim.x) {
     const int4 t = tiles[i];
@@ -152,16 +182,12 @@ __global__ void __launch_bounds__(256) kv4_spread_kernel(const uint8_t* kv4, con
   }
   __syncthreads();
   // (where a portion follows another of the same row, both are in [lo, hi))
-  const int first = max(s_lo / 16, c0), last = min(min((s_hi + 15) / 16, bt_stride), c0 + SPREAD_COLUMNS);
-  const int n = (last - first) * n_kv;
-  for (int it = threadIdx.x >> 5; it < n; it += 8) {
-    const int c = first + it / n_kv, h = it % n_kv;
-    const long long to = (long long)row * bt_stride + c;
-    constexpr int ROWS = 16 * D / 8;
-    uint4* keys = out + ((to * 2) * n_kv + h) * ROWS;
-    kv4_spread_head<D>(kv4 + ((long long)block_table[to] * n_kv + h) * Kv4<D>::BYTES, keys, keys + (long long)n_kv * ROWS, threadIdx.x & 31);
-    if (h == 0 && (threadIdx.x & 31) == 0) table[to] = (int32_t)to;
-  }
+  if (c < s_lo / 16 || c >= min((s_hi + 15) / 16, bt_stride)) return;
+  const long long to = (long long)row * bt_stride + c;
+  constexpr int ROWS = 16 * D / 8;
+  uint4* keys = out + ((to * 2) * n_kv + h) * ROWS;
+  kv4_spread_head<D>(kv4 + ((long long)block_table[to] * n_kv + h) * Kv4<D>::BYTES, keys, keys + (long long)n_kv * ROWS, stage[warp], lane);
+  if (h == 0 && lane == 0) table[to] = (int32_t)to;
 }
 
 static inline int64_t spread_pages_bytes(int64_t pages, int n_kv, int D) { return pages * (4LL * n_kv * 16 * D); }
@@ -202,8 +228,9 @@ int b200q_rope_kvwrite_q4(void* qkv, const void* cos_sin, const int32_t* positio
   B200Q_CHECK_ARG(qkv && cos_sin && positions && slot_mapping && kv4_layer, "rope_kvwrite_q4: null argument");
   B200Q_CHECK_ARG(((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(cos_sin) | reinterpret_cast<uintptr_t>(kv4_layer)) & 15) == 0,
                   "rope_kvwrite_q4: qkv, cos_sin and the cache must be 16-byte aligned");
-  const int items = n_kv * (D / 32) + n_kv * (D / 16) + n_q * (D / 16), blocks = T <= 320 ? (items + 127) / 128 : 1;
-  const int threads = blocks > 1 ? 128 : 256;
+  // A thread to an item; of few rows' items blocks of 128
+  const int items = n_kv * (D / 32) + n_kv * (D / 16) + n_q * (D / 16), most = T <= 320 ? 128 : 512, blocks = (items + most - 1) / most;
+  const int threads = ((items + blocks - 1) / blocks + 31) / 32 * 32;
   B200Q_KV4_DIMS("rope_kvwrite_q4", D,
                  B200Q_CUDA(launch_early(rope_kvwrite_q4_kernel<kD>, dim3(T, blocks), threads, 0, as_stream(stream), 1, (uint4*)qkv,
                                          (const uint4*)cos_sin, positions, slot_mapping, (uint8_t*)kv4_layer, n_q, n_kv)));
@@ -217,9 +244,9 @@ int b200q_kv4_unpack(const void* kv4_layer, const int32_t* pages, int n_pages, v
   if (n_pages == 0) return B200Q_OK;
   B200Q_CHECK_ARG(kv4_layer && pages && kv_out, "kv4_unpack: null argument");
   B200Q_CHECK_ARG(((reinterpret_cast<uintptr_t>(kv4_layer) | reinterpret_cast<uintptr_t>(kv_out)) & 15) == 0, "kv4_unpack: caches must be 16-byte aligned");
-  const long long items = (long long)n_pages * n_kv, blocks = (items + 3) / 4;
+  const long long items = (long long)n_pages * n_kv, blocks = (items + SPREAD_WARPS - 1) / SPREAD_WARPS;
   B200Q_KV4_DIMS("kv4_unpack", D,
-                 B200Q_CUDA(launch_early(kv4_unpack_kernel<kD>, dim3((unsigned)(blocks < 1 << 20 ? blocks : 1 << 20)), 128, 0, as_stream(stream), 1,
+                 B200Q_CUDA(launch_early(kv4_unpack_kernel<kD>, dim3((unsigned)(blocks < 1 << 20 ? blocks : 1 << 20)), SPREAD_WARPS * 32, 0, as_stream(stream), 1,
                                          (const uint8_t*)kv4_layer, pages, n_pages, (uint4*)kv_out, n_kv)));
   count_launch();
   return B200Q_OK;
@@ -253,7 +280,7 @@ int b200q_prefill_attn_q4(const void* q, int q_stride, void* out, const void* kv
   const int64_t pages = (int64_t)n_seqs * bt_stride;
   int32_t* table = (int32_t*)((uint8_t*)workspace + spread_pages_bytes(pages, n_kv, D));
   B200Q_KV4_DIMS("prefill_attn_q4", D,
-                 B200Q_CUDA(launch_early(kv4_spread_kernel<kD>, dim3((bt_stride + SPREAD_COLUMNS - 1) / SPREAD_COLUMNS, n_seqs), 256, 0, as_stream(stream),
+                 B200Q_CUDA(launch_early(kv4_spread_kernel<kD>, dim3((unsigned)(((int64_t)bt_stride * n_kv + SPREAD_WARPS - 1) / SPREAD_WARPS), n_seqs), SPREAD_WARPS * 32, 0, as_stream(stream),
                                          1, (const uint8_t*)kv4_layer, block_table, bt_stride, (const int4*)tiles, n_tiles, n_kv, window,
                                          (uint4*)workspace, table)));
   count_launch();
