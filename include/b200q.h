@@ -696,7 +696,7 @@ int b200q_beam_select(const void* logits_dev, const float* scores_dev, int group
  *     page * block_size + place of the next token, -1 where there is none.  Old rows hold nothing any more: refs is kept up.
  *     status[0] = pages that were missing (0: all is well; else nothing has changed, slots are -1), status[1] = rows whose table is
  *     full (slot -1; they hold their parent's pages).  Entries of table_out behind a row's pages stay as they are; it must not
- *     overlap `table`.  n_old, n_new <= 16384, block_size 16. */
+ *     overlap `table`.  n_old, n_new <= 8192, block_size 16. */
 int b200q_pages_fork(const int32_t* table_dev, const int32_t* lens_dev, int n_old, const int32_t* parents_dev, int n_new, int bt_stride,
                      int32_t* refs_dev, int num_blocks, int block_size, int32_t* table_out_dev, int32_t* slots_dev, int32_t* pairs_dev,
                      int32_t* status_dev, void* stream);

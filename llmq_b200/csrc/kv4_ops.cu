@@ -43,7 +43,7 @@ __device__ __forceinline__ void turn_bf8(uint4& x1, uint4& x2, const uint4& c, c
 // Bound: the rows' bytes (a cached token is 9/16 of a byte per value, a quarter of what the 16-bit write stores).
 // ------------------------------------------------------------------------------------------------------------------------
 template <int D>
-__global__ void __launch_bounds__(512) rope_kvwrite_q4_kernel(uint4* qkv, const uint4* cos_sin, const int32_t* positions, const int32_t* slot_mapping,
+__global__ void __launch_bounds__(128, 14) rope_kvwrite_q4_kernel(uint4* qkv, const uint4* cos_sin, const int32_t* positions, const int32_t* slot_mapping,
                                                               uint8_t* kv_layer, int n_q, int n_kv) {
   follow_previous(qkv, cos_sin, positions, slot_mapping, kv_layer);
   constexpr int CPR = D / 8, HALF = CPR / 2;  // 16-byte pieces of a head's row, of half of it
@@ -228,8 +228,9 @@ int b200q_rope_kvwrite_q4(void* qkv, const void* cos_sin, const int32_t* positio
   B200Q_CHECK_ARG(qkv && cos_sin && positions && slot_mapping && kv4_layer, "rope_kvwrite_q4: null argument");
   B200Q_CHECK_ARG(((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(cos_sin) | reinterpret_cast<uintptr_t>(kv4_layer)) & 15) == 0,
                   "rope_kvwrite_q4: qkv, cos_sin and the cache must be 16-byte aligned");
-  // A thread to an item; of few rows' items blocks of 128
-  const int items = n_kv * (D / 32) + n_kv * (D / 16) + n_q * (D / 16), most = T <= 320 ? 128 : 512, blocks = (items + most - 1) / most;
+  // A thread to an item, in blocks of up to 128 (4608 rows of 32 + 8 + 8 heads of 128 and reading them back: 26.7 us, in blocks of 192 27.3, of
+  // 384 31.3; 512 of heads of 64 3.3 / 4.5 / 4.4)
+  const int items = n_kv * (D / 32) + n_kv * (D / 16) + n_q * (D / 16), blocks = (items + 127) / 128;
   const int threads = ((items + blocks - 1) / blocks + 31) / 32 * 32;
   B200Q_KV4_DIMS("rope_kvwrite_q4", D,
                  B200Q_CUDA(launch_early(rope_kvwrite_q4_kernel<kD>, dim3(T, blocks), threads, 0, as_stream(stream), 1, (uint4*)qkv,

@@ -15,7 +15,7 @@
 
 namespace b200q {
 
-constexpr int PG_THREADS = 1024, PG_CTAS = 8, PG_ROWS = 16384, PG_BLOCK = 16;
+constexpr int PG_THREADS = 1024, PG_CTAS = 8, PG_ROWS = 8192, PG_BLOCK = 16;
 
 __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
   uint32_t v;
@@ -35,7 +35,7 @@ __device__ __forceinline__ int block_prefix(int v, int* total, int* scratch /* 3
   if (lane == 31) scratch[warp] = x;
   __syncthreads();
   if (warp == 0) {
-    int s = scratch[lane];
+    int s = lane < (int)blockDim.x / 32 ? scratch[lane] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, s, o);
@@ -89,6 +89,23 @@ __device__ __forceinline__ void rows_sync() {
     cluster_sync_all();
 }
 
+// entries 0 .. n - 1 of a table, eight of a thread at once: what `read` gives for those of (row, column) goes to `write`, unless it is NO_ENTRY
+constexpr int NO_ENTRY = -0x7fffffff - 1;
+template <typename R, typename W>
+__device__ __forceinline__ void for_entries(int n, int stride, int at, int threads, R&& read, W&& write) {
+  for (int e0 = at; e0 < n; e0 += 8 * threads) {
+    int v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int e = e0 + u * threads, i = e / stride;
+      v[u] = e < n ? read(i, e - i * stride) : NO_ENTRY;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (v[u] != NO_ENTRY) write(e0 + u * threads, v[u]);
+  }
+}
+
 struct ForkArgs {
   const int32_t *table, *lens, *parents;
   int32_t *refs, *table_out, *slots;
@@ -100,38 +117,46 @@ struct ForkArgs {
 __global__ void __launch_bounds__(PG_THREADS, 1) pages_fork_kernel(ForkArgs a) {
   follow_previous(a.table, a.lens, a.parents, a.refs, a.table_out, a.slots, a.pairs, a.status);
   extern __shared__ int32_t rows[];
-  int32_t *first = rows, *count = rows + a.n_old, *fresh = rows + 2 * a.n_old;  // per old row; new rows that need a page, in order
+  // per old row: its first continuation, how many, its length; per new row: its parent (-1: none); the new rows that need a page, in order
+  int32_t *first = rows, *count = first + a.n_old, *lens = count + a.n_old, *parent = lens + a.n_old, *fresh = parent + a.n_new;
   __shared__ int scratch[33], box[2], no_column_s;
-  const int tid = threadIdx.x;
-  for (int i = tid; i < a.n_old; i += PG_THREADS) {
+  const int tid = threadIdx.x, nt = blockDim.x;
+  const int most = a.stride * PG_BLOCK;
+  // counts of this CTA's share of the pages, asked for before anything else; of a share that is one round of the threads they stay in registers
+  const PageShare share(a.num_blocks);
+  const bool vec = (reinterpret_cast<uintptr_t>(a.refs) & 15) == 0, one_round = share.to - share.from <= 4 * nt;
+  const int p_mine = share.from + 4 * tid;
+  const int4 c_mine = one_round && p_mine < share.to ? counts_of(a.refs, p_mine, share.to, vec) : make_int4(-1, -1, -1, -1);
+  for (int i = tid; i < a.n_old; i += nt) {
     first[i] = 0x7fffffff;
     count[i] = 0;
+    lens[i] = min(max(a.lens[i], 0), most);
+  }
+  for (int i = tid; i < a.n_new; i += nt) {
+    const int p = a.parents[i];
+    parent[i] = p >= 0 && p < a.n_old ? p : -1;
   }
   if (tid == 0) no_column_s = 0;
   __syncthreads();
-  for (int i = tid; i < a.n_new; i += PG_THREADS) {
-    const int p = a.parents[i];
-    if (p >= 0 && p < a.n_old) {
-      atomicMin(first + p, i);
-      atomicAdd(count + p, 1);
+  for (int i = tid; i < a.n_new; i += nt)
+    if (parent[i] >= 0) {
+      atomicMin(first + parent[i], i);
+      atomicAdd(count + parent[i], 1);
     }
-  }
   __syncthreads();
-  const int most = a.stride * PG_BLOCK;
-  auto len_of = [&](int p) { return min(max(a.lens[p], 0), most); };
   // ---- who needs a page (every CTA finds this out for all rows: it is a few reads per row, and nobody has to be told)
   int n_fresh = 0;
-  for (int i0 = 0; i0 < a.n_new; i0 += PG_THREADS) {
-    const int i = i0 + tid, p = i < a.n_new ? a.parents[i] : -1;
+  for (int i0 = 0; i0 < a.n_new; i0 += nt) {
+    const int i = i0 + tid, p = i < a.n_new ? parent[i] : -1;
     bool need = false;
-    if (p >= 0 && p < a.n_old) {
-      const int len = len_of(p), last = len / PG_BLOCK;
+    if (p >= 0) {
+      const int len = lens[p], last = len / PG_BLOCK;
       if (last >= a.stride) {
         if (blockIdx.x == 0) atomicAdd(&no_column_s, 1);
       } else if (len % PG_BLOCK == 0) {
         need = true;
       } else {
-        const int page = a.table[(long long)p * a.stride + last];
+        const int page = a.table[p * a.stride + last];
         need = !(first[p] == i && page >= 0 && page < a.num_blocks && a.refs[page] == 1);
       }
     }
@@ -141,15 +166,12 @@ __global__ void __launch_bounds__(PG_THREADS, 1) pages_fork_kernel(ForkArgs a) {
     n_fresh += all;
   }
   // ---- the free pages of this CTA's share, and of all
-  const PageShare share(a.num_blocks);
-  const bool vec = (reinterpret_cast<uintptr_t>(a.refs) & 15) == 0;
-  int mine = 0;
-  for (int p = share.from + 4 * tid; p < share.to; p += 4 * PG_THREADS) {
-    const int4 c = counts_of(a.refs, p, share.to, vec);
-    mine += (c.x == 0) + (c.y == 0) + (c.z == 0) + (c.w == 0);
-  }
+  auto free_in = [](int4 c) { return (c.x == 0) + (c.y == 0) + (c.z == 0) + (c.w == 0); };
+  int mine = free_in(c_mine);
+  if (!one_round)
+    for (int p = p_mine; p < share.to; p += 4 * nt) mine += free_in(counts_of(a.refs, p, share.to, vec));
   int here, free_all;
-  block_prefix(mine, &here, scratch);
+  const int before_mine = block_prefix(mine, &here, scratch);
   int rank = cluster_prefix(here, &free_all, box, 0);
   const bool enough = free_all >= n_fresh;
   if (blockIdx.x == 0 && tid == 0) {
@@ -157,7 +179,7 @@ __global__ void __launch_bounds__(PG_THREADS, 1) pages_fork_kernel(ForkArgs a) {
     a.status[1] = no_column_s;
   }
   if (!enough) {  // nothing changes, and nobody has a place to write to
-    for (int i = blockIdx.x * PG_THREADS + tid; i < a.n_new; i += gridDim.x * PG_THREADS) {
+    for (int i = blockIdx.x * nt + tid; i < a.n_new; i += gridDim.x * nt) {
       a.slots[i] = -1;
       a.pairs[i] = make_int2(-1, -1);
     }
@@ -165,90 +187,75 @@ __global__ void __launch_bounds__(PG_THREADS, 1) pages_fork_kernel(ForkArgs a) {
     return;
   }
   // ---- the k-th free page goes to the k-th row that needs one
-  for (int p0 = share.from; p0 < share.to && rank < n_fresh; p0 += 4 * PG_THREADS) {
-    const int p = p0 + 4 * tid;
-    const int4 c = p < share.to ? counts_of(a.refs, p, share.to, vec) : make_int4(-1, -1, -1, -1);
-    const bool is_free[4] = {c.x == 0, c.y == 0, c.z == 0, c.w == 0};
-    int all;
-    int k = rank + block_prefix(is_free[0] + is_free[1] + is_free[2] + is_free[3], &all, scratch);
+  auto give = [&](int p, int4 c4, int k) {  // those of pages p .. p + 3 that are free, the first of them the k-th of all
+    const int c[4] = {c4.x, c4.y, c4.z, c4.w};
 #pragma unroll
     for (int x = 0; x < 4; ++x)
-      if (is_free[x]) {
+      if (c[x] == 0) {
         if (k < n_fresh) {
-          const int i = fresh[k], from = a.parents[i], len = len_of(from), last = len / PG_BLOCK;
+          const int i = fresh[k], from = parent[i], len = lens[from], last = len / PG_BLOCK;
           a.refs[p + x] = 1;
-          a.table_out[(long long)i * a.stride + last] = p + x;
+          a.table_out[i * a.stride + last] = p + x;
           a.slots[i] = (p + x) * PG_BLOCK + len % PG_BLOCK;
-          a.pairs[i] = len % PG_BLOCK ? make_int2(a.table[(long long)from * a.stride + last], p + x) : make_int2(-1, -1);
+          a.pairs[i] = len % PG_BLOCK ? make_int2(a.table[from * a.stride + last], p + x) : make_int2(-1, -1);
         }
         ++k;
       }
-    rank += all;
+  };
+  if (one_round) {
+    if (rank < n_fresh) give(p_mine, c_mine, rank + before_mine);
+  } else {
+    for (int p0 = share.from; p0 < share.to && rank < n_fresh; p0 += 4 * nt) {
+      const int p = p0 + 4 * tid;
+      const int4 c = p < share.to ? counts_of(a.refs, p, share.to, vec) : make_int4(-1, -1, -1, -1);
+      int all;
+      const int k = block_prefix(free_in(c), &all, scratch);
+      give(p, c, rank + k);
+      rank += all;
+    }
   }
   rows_sync();  // all free pages have been looked for: counts may change
-  // ---- tables of the new rows, slots of those that keep a page; then what the old rows' pages gain and lose.  A warp to a row
-  const int warp = (blockIdx.x * PG_THREADS + tid) >> 5, warps = (gridDim.x * PG_THREADS) >> 5, lane = tid & 31;
-  for (int i = warp; i < a.n_new; i += warps) {
-    const int p = a.parents[i];
-    if (p < 0 || p >= a.n_old) {
-      if (lane == 0) {
-        a.slots[i] = -1;
-        a.pairs[i] = make_int2(-1, -1);
-      }
-      continue;
+  // ---- tables of the new rows, slots of those that keep a page; then what the old rows' pages gain and lose
+  auto is_fresh = [&](int i) {  // (decided by counts that have changed since: the list of the rows that need a page says it)
+    int lo = 0, hi = n_fresh;
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (fresh[mid] < i)
+        lo = mid + 1;
+      else
+        hi = mid;
     }
-    const int len = len_of(p), last = len / PG_BLOCK;
-    const int32_t* from = a.table + (long long)p * a.stride;
-    int32_t* to = a.table_out + (long long)i * a.stride;
-    for (int c = lane; c < last; c += 32) to[c] = from[c];
-    if (lane == 0) {
-      if (last >= a.stride) {
-        a.slots[i] = -1;
-        a.pairs[i] = make_int2(-1, -1);
-      } else if (len % PG_BLOCK) {
-        // who has it was decided by counts that may have changed since: the list of rows that need a page says it
-        int lo = 0, hi = n_fresh;
-        while (lo < hi) {
-          const int mid = (lo + hi) / 2;
-          if (fresh[mid] < i)
-            lo = mid + 1;
-          else
-            hi = mid;
-        }
-        if (lo == n_fresh || fresh[lo] != i) {
-          to[last] = from[last];
-          a.slots[i] = from[last] * PG_BLOCK + len % PG_BLOCK;
-          a.pairs[i] = make_int2(-1, -1);
-        }
-      }
+    return lo < n_fresh && fresh[lo] == i;
+  };
+  const int at = blockIdx.x * nt + tid, threads = gridDim.x * nt;
+  for_entries(a.n_new * a.stride, a.stride, at, threads, [&](int i, int c) {
+    const int p = parent[i];
+    return p >= 0 && c < lens[p] / PG_BLOCK ? a.table[p * a.stride + c] : NO_ENTRY;
+  }, [&](int e, int page) { a.table_out[e] = page; });
+  for (int i = at; i < a.n_new; i += threads) {
+    const int p = parent[i], len = p >= 0 ? lens[p] : 0, last = len / PG_BLOCK;
+    if (p < 0 || last >= a.stride) {
+      a.slots[i] = -1;
+      a.pairs[i] = make_int2(-1, -1);
+    } else if (len % PG_BLOCK && !is_fresh(i)) {
+      const int page = a.table[p * a.stride + last];
+      a.table_out[i * a.stride + last] = page;
+      a.slots[i] = page * PG_BLOCK + len % PG_BLOCK;
+      a.pairs[i] = make_int2(-1, -1);
     }
   }
-  for (int p = warp; p < a.n_old; p += warps) {
-    const int len = len_of(p), full = len / PG_BLOCK, kids = count[p];
-    const int32_t* row = a.table + (long long)p * a.stride;
-    if (kids != 1)
-      for (int c = lane; c < full; c += 32) {
-        const int page = row[c];
-        if (page >= 0 && page < a.num_blocks) atomicAdd(a.refs + page, kids - 1);
-      }
-    if (lane == 0 && len % PG_BLOCK) {
-      bool kept = false;
-      if (kids > 0) {
-        const int i = first[p];
-        int lo = 0, hi = n_fresh;
-        while (lo < hi) {
-          const int mid = (lo + hi) / 2;
-          if (fresh[mid] < i)
-            lo = mid + 1;
-          else
-            hi = mid;
-        }
-        kept = lo == n_fresh || fresh[lo] != i;
-      }
-      const int page = row[full];
-      if (!kept && page >= 0 && page < a.num_blocks) atomicAdd(a.refs + page, -1);
+  // (both loops go through the old table: an entry counts for how many rows more or fewer hold its page now)
+  for_entries(a.n_old * a.stride, a.stride, at, threads, [&](int p, int c) {
+    const bool counts = count[p] != 1 && c < lens[p] / PG_BLOCK;
+    return counts ? a.table[p * a.stride + c] : NO_ENTRY;
+  }, [&](int e, int page) {
+    if (page >= 0 && page < a.num_blocks) atomicAdd(a.refs + page, count[e / a.stride] - 1);
+  });
+  for (int p = at; p < a.n_old; p += threads)
+    if (lens[p] % PG_BLOCK && !(count[p] > 0 && !is_fresh(first[p]))) {
+      const int page = a.table[p * a.stride + lens[p] / PG_BLOCK];
+      if (page >= 0 && page < a.num_blocks) atomicAdd(a.refs + page, -1);
     }
-  }
   if (gridDim.x > 1) cluster_sync_all();  // (nobody leaves while a peer may read its number)
 }
 
@@ -305,11 +312,11 @@ struct CompactArgs {
 __global__ void __launch_bounds__(PG_THREADS, 1) pages_compact_kernel(CompactArgs a) {
   follow_previous(a.table, a.lens, a.refs, a.table_out, a.refs_out, a.map, a.pairs, a.status);
   __shared__ int scratch[33], box[2];
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, nt = blockDim.x;
   const PageShare share(a.num_blocks);
   const bool vec = (reinterpret_cast<uintptr_t>(a.refs) & 15) == 0;
   int mine = 0;
-  for (int p = share.from + 4 * tid; p < share.to; p += 4 * PG_THREADS) {
+  for (int p = share.from + 4 * tid; p < share.to; p += 4 * nt) {
     const int4 c = counts_of(a.refs, p, share.to, vec);
     mine += (c.x > 0) + (c.y > 0) + (c.z > 0) + (c.w > 0);
   }
@@ -317,7 +324,7 @@ __global__ void __launch_bounds__(PG_THREADS, 1) pages_compact_kernel(CompactArg
   block_prefix(mine, &here, scratch);
   int before = cluster_prefix(here, &n, box, 0);
   int below = 0;
-  for (int p = share.from + 4 * tid; p < min(share.to, n); p += 4 * PG_THREADS) {
+  for (int p = share.from + 4 * tid; p < min(share.to, n); p += 4 * nt) {
     const int4 c = counts_of(a.refs, p, min(share.to, n), vec);
     below += (c.x > 0) + (c.y > 0) + (c.z > 0) + (c.w > 0);
   }
@@ -328,7 +335,7 @@ __global__ void __launch_bounds__(PG_THREADS, 1) pages_compact_kernel(CompactArg
     a.status[0] = n;
     a.status[1] = moves;
   }
-  for (int p0 = share.from; p0 < share.to; p0 += 4 * PG_THREADS) {
+  for (int p0 = share.from; p0 < share.to; p0 += 4 * nt) {
     const int p = p0 + 4 * tid;
     const int4 c4 = p < share.to ? counts_of(a.refs, p, share.to, vec) : make_int4(-1, -1, -1, -1);
     const int c[4] = {c4.x, c4.y, c4.z, c4.w};
@@ -357,7 +364,7 @@ __global__ void __launch_bounds__(PG_THREADS, 1) pages_compact_kernel(CompactArg
     before += all;
   }
   rows_sync();
-  const int at = blockIdx.x * PG_THREADS + tid, threads = gridDim.x * PG_THREADS;
+  const int at = blockIdx.x * nt + tid, threads = gridDim.x * nt;
   for (int k = at; k < moves; k += threads) {
     const int2 pr = a.pairs[k];
     a.map[pr.x] = pr.y;
@@ -365,17 +372,18 @@ __global__ void __launch_bounds__(PG_THREADS, 1) pages_compact_kernel(CompactArg
     a.refs_out[pr.x] = 0;  // (refs_out may be refs)
   }
   rows_sync();
-  for (int r = at >> 5; r < a.n_rows; r += threads >> 5) {
-    const int pages = min((max(a.lens[r], 0) + PG_BLOCK - 1) / PG_BLOCK, a.stride);
-    for (int c = tid & 31; c < pages; c += 32) {
-      const int p = a.table[(long long)r * a.stride + c];
-      a.table_out[(long long)r * a.stride + c] = p >= 0 && p < a.num_blocks ? a.map[p] : -1;
-    }
-  }
+  for_entries(a.n_rows * a.stride, a.stride, at, threads, [&](int r, int c) {
+    if (c >= min((max(a.lens[r], 0) + PG_BLOCK - 1) / PG_BLOCK, a.stride)) return NO_ENTRY;
+    const int p = a.table[r * a.stride + c];
+    return p >= 0 && p < a.num_blocks ? a.map[p] : -1;
+  }, [&](int e, int page) { a.table_out[e] = page; });
 }
 
-// CTAs of a cluster: one where a thread has a few pages and a warp a few rows
-static int page_ctas(int num_blocks, long long entries) { return num_blocks <= 16384 && entries <= 8192 ? 1 : PG_CTAS; }
+// a barrier of few warps is shorter: 256 threads where that is a page or an entry or so to each
+static int page_threads(int num_blocks, long long entries) { return num_blocks <= 1024 && entries <= 1024 ? 256 : PG_THREADS; }
+// CTAs of a cluster: one where a thread has a few pages and a few entries
+static int page_ctas(int num_blocks, long long entries) { return num_blocks <= 16384 && entries <= 16384 ? 1 : PG_CTAS; }
+constexpr long long PG_ENTRIES = 0x7fffffff - 8 * PG_CTAS * PG_THREADS;  // of a block table
 
 }  // namespace b200q
 
@@ -389,23 +397,24 @@ int b200q_pages_fork(const int32_t* table, const int32_t* lens, int n_old, const
                       num_blocks <= (1 << 27) && block_size == PG_BLOCK,
                   "pages_fork: bad shape n_old=%d n_new=%d (up to %d) bt_stride=%d num_blocks=%d block_size=%d (16)", n_old, n_new, PG_ROWS, bt_stride,
                   num_blocks, block_size);
+  B200Q_CHECK_ARG((long long)n_old * bt_stride <= PG_ENTRIES && (long long)n_new * bt_stride <= PG_ENTRIES, "pages_fork: tables of more than 2^31 entries");
   B200Q_CHECK_ARG(refs && status && (n_old == 0 || (table && lens)) && (n_new == 0 || (parents && table_out && slots && pairs)),
                   "pages_fork: null argument");
   B200Q_CHECK_ARG(n_old == 0 || n_new == 0 ||
                       !(table_out < table + (long long)n_old * bt_stride && table < table_out + (long long)n_new * bt_stride),
                   "pages_fork: the new table must not overlap the old one");
   B200Q_CHECK_ARG((reinterpret_cast<uintptr_t>(pairs) & 7) == 0, "pages_fork: pairs must be 8-byte aligned");
-  const size_t smem = (2 * (size_t)n_old + n_new) * 4;
+  const size_t smem = (3 * (size_t)n_old + 2 * (size_t)n_new) * 4;
   static bool ready[64];
   int dev = 0;
   B200Q_CUDA(cudaGetDevice(&dev));
   if (dev >= 64 || !ready[dev]) {
-    B200Q_CUDA(cudaFuncSetAttribute(pages_fork_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * PG_ROWS * 4));
+    B200Q_CUDA(cudaFuncSetAttribute(pages_fork_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 5 * PG_ROWS * 4));
     if (dev < 64) ready[dev] = true;
   }
   const int ctas = page_ctas(num_blocks, (long long)(n_old > n_new ? n_old : n_new) * bt_stride);
   const ForkArgs a{table, lens, parents, refs, table_out, slots, (int2*)pairs, status, n_old, n_new, bt_stride, num_blocks};
-  B200Q_CUDA(launch_early(pages_fork_kernel, dim3(ctas), PG_THREADS, smem, as_stream(stream), ctas, a));
+  B200Q_CUDA(launch_early(pages_fork_kernel, dim3(ctas), page_threads(num_blocks, (long long)(n_old > n_new ? n_old : n_new) * bt_stride), smem, as_stream(stream), ctas, a));
   count_launch();
   return B200Q_OK;
 }
@@ -445,12 +454,13 @@ int b200q_pages_compact(const int32_t* table, const int32_t* lens, int n_rows, i
                         int32_t* table_out, int32_t* refs_out, int32_t* map, int32_t* pairs, int32_t* status, void* stream) {
   B200Q_CHECK_ARG(n_rows >= 0 && bt_stride >= 0 && bt_stride <= (1 << 26) && num_blocks > 0 && num_blocks <= (1 << 27) && block_size == PG_BLOCK,
                   "pages_compact: bad shape n_rows=%d bt_stride=%d num_blocks=%d block_size=%d (16)", n_rows, bt_stride, num_blocks, block_size);
+  B200Q_CHECK_ARG((long long)n_rows * bt_stride <= PG_ENTRIES, "pages_compact: a table of more than 2^31 entries");
   B200Q_CHECK_ARG(refs && refs_out && map && pairs && status && (n_rows == 0 || bt_stride == 0 || (table && lens && table_out)),
                   "pages_compact: null argument");
   B200Q_CHECK_ARG((reinterpret_cast<uintptr_t>(pairs) & 7) == 0, "pages_compact: pairs must be 8-byte aligned");
   const int ctas = page_ctas(num_blocks, (long long)n_rows * bt_stride);
   const CompactArgs a{table, lens, refs, table_out, refs_out, map, (int2*)pairs, status, bt_stride > 0 ? n_rows : 0, bt_stride, num_blocks};
-  B200Q_CUDA(launch_early(pages_compact_kernel, dim3(ctas), PG_THREADS, 0, as_stream(stream), ctas, a));
+  B200Q_CUDA(launch_early(pages_compact_kernel, dim3(ctas), page_threads(num_blocks, (long long)n_rows * bt_stride), 0, as_stream(stream), ctas, a));
   count_launch();
   return B200Q_OK;
 }

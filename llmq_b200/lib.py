@@ -600,27 +600,38 @@ def argmax_bf16(logits, ids, stream=None):
 
 
 # ---- a cache in 4 bits, beams and their pages (include/b200q.h says what each computes) -----------------------------------
-# Tensors that are called int32, fp32 or bf16 have to be that, contiguous, and on the current device: the calls below look.
+# Types, devices and shapes of tensors are looked at, in as few calls as that takes: a small call's time is the host's.
 _TORCH = {}
 
 
-def _dtype(name):
-    if not _TORCH:
-        import torch
+def _types():
+    import torch
 
-        _TORCH.update(i=torch.int32, f=torch.float32, h=torch.bfloat16, torch=torch)
-    return _TORCH[name]
+    _TORCH.update(i=torch.int32, f=torch.float32, h=torch.bfloat16)
+    return _TORCH
 
 
-def _arg(t, dtype, what):
-    """data_ptr of a contiguous tensor of this type ("i", "f", "h": int32, fp32, bf16; None: any) on the current device"""
-    if dtype and t.dtype != _dtype(dtype):
-        raise ValueError(f"{what}: {t.dtype}, not {_dtype(dtype)}")
+def _refuse(t, kind, what, dev):
+    if kind and t.dtype is not (_TORCH or _types())[kind]:
+        raise ValueError(f"{what}: {t.dtype}, not {_TORCH[kind]}")
     if not (t.is_cuda and t.is_contiguous()):
         raise ValueError(f"{what}: a contiguous CUDA tensor is wanted")
-    if _device is not None and t.get_device() != _device():
-        raise ValueError(f"{what}: on device {t.get_device()}, and device {_device()} is the current one")
+    raise ValueError(f"{what}: on device {t.get_device()}, and device {dev} is the current one")
+
+
+def _arg(t, kind, what, dev=0):
+    """data_ptr of a contiguous tensor of this type ("i", "f", "h": int32, fp32, bf16; None: any) on device dev, the current one"""
+    if t.get_device() != dev or not t.is_contiguous() or (kind and t.dtype is not (_TORCH or _types())[kind]):
+        _refuse(t, kind, what, dev)
     return t.data_ptr()
+
+
+def _here(stream):
+    """(handle of `stream` or of the current one, the current device)"""
+    s = _stream(stream)
+    if _device is None:
+        _stream()
+    return s, _device()
 
 
 def _want(ok, what):
@@ -628,37 +639,41 @@ def _want(ok, what):
         raise ValueError(what)
 
 
-def kv4_page_bytes(n_kv, D):
-    """bytes of a page of the 4-bit cache (16 tokens, all heads of a layer)"""
-    n = int(load().b200q_kv4_page_bytes(n_kv, D))
+def _bytes(n):
     if n < 0:
         check(n)
-    return n
+    return int(n)
+
+
+def kv4_page_bytes(n_kv, D):
+    """bytes of a page of the 4-bit cache (16 tokens, all heads of a layer)"""
+    return _bytes(load().b200q_kv4_page_bytes(n_kv, D))
 
 
 def rope_kvwrite_q4(qkv, cos_sin, positions, slot_mapping, kv4_layer, n_q, n_kv, D, block_size, stream=None):
     """rope_kvwrite into a layer of the 4-bit cache ([num_blocks, n_kv, 18 D] bytes)"""
-    T, s = qkv.shape[0], _stream(stream)
-    _want(qkv.shape[1] == (n_q + 2 * n_kv) * D and positions.numel() == T and slot_mapping.numel() == T and cos_sin.shape[1] == D,
+    (T, width), (s, dev) = qkv.shape, _here(stream)
+    _want(width == (n_q + 2 * n_kv) * D and positions.numel() == T and slot_mapping.numel() == T and cos_sin.shape[1] == D,
           "rope_kvwrite_q4: rows of qkv, cos_sin, positions or slots do not fit the heads")
-    check(load().b200q_rope_kvwrite_q4(_arg(qkv, "h", "qkv"), _arg(cos_sin, "h", "cos_sin"), _arg(positions, "i", "positions"),
-                                       _arg(slot_mapping, "i", "slot_mapping"), _arg(kv4_layer, None, "kv4_layer"), T, n_q, n_kv, D, block_size, s))
+    check(load().b200q_rope_kvwrite_q4(_arg(qkv, "h", "qkv", dev), _arg(cos_sin, "h", "cos_sin", dev), _arg(positions, "i", "positions", dev),
+                                       _arg(slot_mapping, "i", "slot_mapping", dev), _arg(kv4_layer, None, "kv4_layer", dev), T, n_q, n_kv, D,
+                                       block_size, s))
 
 
 def kv4_unpack(kv4_layer, pages, kv_out, n_kv, D, block_size, stream=None):
     """pages of the 4-bit cache as pages of the 16-bit one: kv_out[i] = page pages[i]"""
-    n, s = pages.numel(), _stream(stream)
+    n, (s, dev) = pages.numel(), _here(stream)
     _want(kv_out.numel() >= n * 2 * n_kv * block_size * D, "kv4_unpack: kv_out is too small")
-    check(load().b200q_kv4_unpack(_arg(kv4_layer, None, "kv4_layer"), _arg(pages, "i", "pages"), n, _arg(kv_out, "h", "kv_out"), n_kv, D, block_size, s))
+    check(load().b200q_kv4_unpack(_arg(kv4_layer, None, "kv4_layer", dev), _arg(pages, "i", "pages", dev), n, _arg(kv_out, "h", "kv_out", dev), n_kv, D,
+                                  block_size, s))
 
 
 def decode_attn_q4(qkv, out, kv4_layer, block_table, ctx_lens, n_q, n_kv, D, block_size, scale, stream=None, softcap: float = 0.0, window: int = 0):
     """decode_attn over a layer of the 4-bit cache"""
-    n, s = ctx_lens.numel(), _stream(stream)
-    _want(qkv.shape[0] >= n and qkv.shape[1] >= n_q * D and block_table.shape[0] >= n and out.numel() >= n * n_q * D,
-          "decode_attn_q4: rows of qkv, out or the block table are missing")
-    check(load().b200q_decode_attn_q4(_arg(qkv, "h", "qkv"), qkv.shape[1], _arg(out, "h", "out"), _arg(kv4_layer, None, "kv4_layer"),
-                                      _arg(block_table, "i", "block_table"), block_table.shape[1], _arg(ctx_lens, "i", "ctx_lens"), n, n_q, n_kv, D,
+    n, (rows, width), (table, columns), (s, dev) = ctx_lens.numel(), qkv.shape, block_table.shape, _here(stream)
+    _want(rows >= n and width >= n_q * D and table >= n and out.numel() >= n * n_q * D, "decode_attn_q4: rows of qkv, out or the block table are missing")
+    check(load().b200q_decode_attn_q4(_arg(qkv, "h", "qkv", dev), width, _arg(out, "h", "out", dev), _arg(kv4_layer, None, "kv4_layer", dev),
+                                      _arg(block_table, "i", "block_table", dev), columns, _arg(ctx_lens, "i", "ctx_lens", dev), n, n_q, n_kv, D,
                                       block_size, scale, softcap, window, s))
 
 
@@ -668,77 +683,73 @@ def decode_attn_q4_set_whole(whole: int):
 
 def prefill_attn_q4_workspace(n_seqs, bt_stride, n_kv, D):
     """bytes of prefill_attn_q4's workspace for a block table of n_seqs rows and bt_stride columns"""
-    n = int(load().b200q_prefill_attn_q4_workspace(n_seqs, bt_stride, n_kv, D))
-    if n < 0:
-        check(n)
-    return n
+    return _bytes(load().b200q_prefill_attn_q4_workspace(n_seqs, bt_stride, n_kv, D))
 
 
 def prefill_attn_q4(qkv, out, kv4_layer, block_table, tiles, n_q, n_kv, D, block_size, scale, workspace, stream=None, softcap: float = 0.0,
                     window: int = 0):
     """prefill_attn over a layer of the 4-bit cache; workspace: a tensor of prefill_attn_q4_workspace(*block_table.shape, n_kv, D) bytes"""
-    s = _stream(stream)
-    _want(qkv.shape[1] >= n_q * D and tiles.shape[1] == 4, "prefill_attn_q4: rows of qkv or tiles do not fit")
-    check(load().b200q_prefill_attn_q4(_arg(qkv, "h", "qkv"), qkv.shape[1], _arg(out, "h", "out"), _arg(kv4_layer, None, "kv4_layer"),
-                                       _arg(block_table, "i", "block_table"), block_table.shape[1], block_table.shape[0], _arg(tiles, "i", "tiles"),
-                                       tiles.shape[0], n_q, n_kv, D, block_size, scale, softcap, window, _arg(workspace, None, "workspace"),
+    (rows, width), (table, columns), (n_tiles, four), (s, dev) = qkv.shape, block_table.shape, tiles.shape, _here(stream)
+    _want(width >= n_q * D and four == 4, "prefill_attn_q4: rows of qkv or tiles do not fit")
+    check(load().b200q_prefill_attn_q4(_arg(qkv, "h", "qkv", dev), width, _arg(out, "h", "out", dev), _arg(kv4_layer, None, "kv4_layer", dev),
+                                       _arg(block_table, "i", "block_table", dev), columns, table, _arg(tiles, "i", "tiles", dev), n_tiles, n_q, n_kv, D,
+                                       block_size, scale, softcap, window, _arg(workspace, None, "workspace", dev),
                                        workspace.numel() * workspace.element_size(), s))
 
 
 def beam_select_workspace(groups, beams, V, K):
     """bytes of beam_select's workspace"""
-    n = int(load().b200q_beam_select_workspace(groups, beams, V, K))
-    if n < 0:
-        check(n)
-    return n
+    return _bytes(load().b200q_beam_select_workspace(groups, beams, V, K))
 
 
 def beam_select(logits, scores, beams, stops, cand_scores, cand_tokens, cand_rows, next_scores, next_tokens, next_rows, workspace, stream=None):
     """the best continuations of groups of `beams` rows: logits bf16 [groups * beams, V], scores fp32 [groups * beams], cand_* [groups, K],
     next_* [groups, beams]"""
-    rows, V = logits.shape
-    groups, K, s = cand_scores.shape[0], cand_scores.shape[1], _stream(stream)
-    _want(rows == groups * beams and scores.numel() == rows and cand_tokens.shape == cand_scores.shape == cand_rows.shape
-          and next_scores.numel() == next_tokens.numel() == next_rows.numel() == rows, "beam_select: shapes do not fit groups of beams")
-    check(load().b200q_beam_select(_arg(logits, "h", "logits"), _arg(scores, "f", "scores"), groups, beams, V, _arg(stops, "i", "stops"), stops.numel(), K,
-                                   _arg(cand_scores, "f", "cand_scores"), _arg(cand_tokens, "i", "cand_tokens"), _arg(cand_rows, "i", "cand_rows"),
-                                   _arg(next_scores, "f", "next_scores"), _arg(next_tokens, "i", "next_tokens"), _arg(next_rows, "i", "next_rows"),
-                                   _arg(workspace, None, "workspace"), workspace.numel() * workspace.element_size(), s))
+    (rows, V), (groups, K), (s, dev) = logits.shape, cand_scores.shape, _here(stream)
+    n = groups * K
+    _want(rows == groups * beams and scores.numel() == rows and cand_tokens.numel() == n and cand_rows.numel() == n and next_scores.numel() == rows
+          and next_tokens.numel() == rows and next_rows.numel() == rows, "beam_select: shapes do not fit groups of beams")
+    check(load().b200q_beam_select(_arg(logits, "h", "logits", dev), _arg(scores, "f", "scores", dev), groups, beams, V, _arg(stops, "i", "stops", dev),
+                                   stops.numel(), K, _arg(cand_scores, "f", "cand_scores", dev), _arg(cand_tokens, "i", "cand_tokens", dev),
+                                   _arg(cand_rows, "i", "cand_rows", dev), _arg(next_scores, "f", "next_scores", dev),
+                                   _arg(next_tokens, "i", "next_tokens", dev), _arg(next_rows, "i", "next_rows", dev),
+                                   _arg(workspace, None, "workspace", dev), workspace.numel() * workspace.element_size(), s))
 
 
 def pages_fork(table, lens, parents, refs, table_out, slots, pairs, status, block_size=16, stream=None):
     """rows of table_out become continuations of rows parents[i] of `table` (lens[parents[i]] tokens), each with a page of its own for its
     next token; slots [n]: where that goes; pairs [n, 2]: what pages_copy has to copy; status [2]: pages missing, rows without a column"""
-    n, s = parents.numel(), _stream(stream)
-    _want(table.shape[1] == table_out.shape[1] and lens.numel() >= table.shape[0] and table_out.shape[0] >= n and slots.numel() >= n
-          and pairs.numel() >= 2 * n and status.numel() >= 2, "pages_fork: tables, slots, pairs or status are too small")
-    check(load().b200q_pages_fork(_arg(table, "i", "table"), _arg(lens, "i", "lens"), table.shape[0], _arg(parents, "i", "parents"), n, table.shape[1],
-                                  _arg(refs, "i", "refs"), refs.numel(), block_size, _arg(table_out, "i", "table_out"), _arg(slots, "i", "slots"),
-                                  _arg(pairs, "i", "pairs"), _arg(status, "i", "status"), s))
+    n, (old, columns), (new, columns_out), (s, dev) = parents.numel(), table.shape, table_out.shape, _here(stream)
+    _want(columns == columns_out and lens.numel() >= old and new >= n and slots.numel() >= n and pairs.numel() >= 2 * n and status.numel() >= 2,
+          "pages_fork: tables, slots, pairs or status are too small")
+    check(load().b200q_pages_fork(_arg(table, "i", "table", dev), _arg(lens, "i", "lens", dev), old, _arg(parents, "i", "parents", dev), n, columns,
+                                  _arg(refs, "i", "refs", dev), refs.numel(), block_size, _arg(table_out, "i", "table_out", dev),
+                                  _arg(slots, "i", "slots", dev), _arg(pairs, "i", "pairs", dev), _arg(status, "i", "status", dev), s))
 
 
 def pages_free(table, lens, refs, ends=None, block_size=16, stream=None):
     """rows with ends[r] != 0 (None: all rows) give back their pages"""
-    s = _stream(stream)
-    _want(lens.numel() >= table.shape[0] and (ends is None or ends.numel() >= table.shape[0]), "pages_free: lens or ends are too short")
-    check(load().b200q_pages_free(_arg(table, "i", "table"), _arg(lens, "i", "lens"), 0 if ends is None else _arg(ends, "i", "ends"), table.shape[0],
-                                  table.shape[1], _arg(refs, "i", "refs"), refs.numel(), block_size, s))
+    (rows, columns), (s, dev) = table.shape, _here(stream)
+    _want(lens.numel() >= rows and (ends is None or ends.numel() >= rows), "pages_free: lens or ends are too short")
+    check(load().b200q_pages_free(_arg(table, "i", "table", dev), _arg(lens, "i", "lens", dev), 0 if ends is None else _arg(ends, "i", "ends", dev), rows,
+                                  columns, _arg(refs, "i", "refs", dev), refs.numel(), block_size, s))
 
 
 def pages_copy(kv, pairs, count=None, stream=None):
     """page pairs[i, 1] <- page pairs[i, 0] in every layer of kv ([layers, num_blocks, ...]), the first count[0] pairs (None: all)"""
-    s = _stream(stream)
+    s, dev = _here(stream)
     _want(kv.dim() >= 2 and kv.numel() > 0, "pages_copy: kv is [layers, num_blocks, ...]")
-    page = kv.numel() // (kv.shape[0] * kv.shape[1]) * kv.element_size()
-    check(load().b200q_pages_copy(_arg(kv, None, "kv"), _arg(pairs, "i", "pairs"), pairs.numel() // 2, 0 if count is None else _arg(count, "i", "count"),
-                                  page, kv.shape[0], page * kv.shape[1], kv.shape[1], s))
+    layers, blocks = kv.shape[:2]
+    page = kv.numel() // (layers * blocks) * kv.element_size()
+    check(load().b200q_pages_copy(_arg(kv, None, "kv", dev), _arg(pairs, "i", "pairs", dev), pairs.numel() // 2,
+                                  0 if count is None else _arg(count, "i", "count", dev), page, layers, page * blocks, blocks, s))
 
 
 def pages_compact(table, lens, refs, table_out, refs_out, page_map, pairs, status, block_size=16, stream=None):
     """the pages in use move to the front of the pool: status = {pages in use, pages that move}; pairs for pages_copy (with status[1:])"""
-    s, n = _stream(stream), refs.numel()
-    _want(table.shape == table_out.shape and lens.numel() >= table.shape[0] and refs_out.numel() >= n and page_map.numel() >= n
+    n, (rows, columns), (s, dev) = refs.numel(), table.shape, _here(stream)
+    _want(table_out.numel() == rows * columns and lens.numel() >= rows and refs_out.numel() >= n and page_map.numel() >= n
           and pairs.numel() >= 2 * (n // 2 + 1) and status.numel() >= 2, "pages_compact: tables, counts, map, pairs or status are too small")
-    check(load().b200q_pages_compact(_arg(table, "i", "table"), _arg(lens, "i", "lens"), table.shape[0], table.shape[1], _arg(refs, "i", "refs"), n, block_size,
-                                     _arg(table_out, "i", "table_out"), _arg(refs_out, "i", "refs_out"), _arg(page_map, "i", "page_map"),
-                                     _arg(pairs, "i", "pairs"), _arg(status, "i", "status"), s))
+    check(load().b200q_pages_compact(_arg(table, "i", "table", dev), _arg(lens, "i", "lens", dev), rows, columns, _arg(refs, "i", "refs", dev), n,
+                                     block_size, _arg(table_out, "i", "table_out", dev), _arg(refs_out, "i", "refs_out", dev),
+                                     _arg(page_map, "i", "page_map", dev), _arg(pairs, "i", "pairs", dev), _arg(status, "i", "status", dev), s))
