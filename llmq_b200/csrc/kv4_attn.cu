@@ -648,51 +648,55 @@ struct Q4Part {
   }
 };
 template <int D>
-__global__ void __launch_bounds__(8 * Q4_JOIN) kv4_join_kernel(const float* scratch, bf16* out, int n_q, int G) {
+__global__ void __launch_bounds__(4 * Q4_JOIN) kv4_join_kernel(const float* scratch, bf16* out, int n_q, int G) {
   follow_previous(scratch, out);
-  // four warps' chains to a block, 64 threads to each of a warp's two
-  const int n_warps = gridDim.x * 4, tid = threadIdx.x % Q4_JOIN, w_at = blockIdx.x * 4 + threadIdx.x / (2 * Q4_JOIN), slot = threadIdx.x / Q4_JOIN % 2;
-  __shared__ float4 o_s[8 * Q4_JOIN];
-  __shared__ float2 ml_s[8 * Q4_JOIN];
+  // two warps' chains to a block, 64 threads to each of a warp's two
+  const int n_warps = gridDim.x * 2, tid = threadIdx.x % Q4_JOIN, w_at = blockIdx.x * 2 + threadIdx.x / (2 * Q4_JOIN), slot = threadIdx.x / Q4_JOIN % 2;
+  __shared__ Q4Part shared[4 * Q4_JOIN];
   const Q4Chain c = reinterpret_cast<const Q4Chain*>(scratch)[2 * w_at + slot];
-  if (!__syncthreads_or(c.n >= 2)) return;
+  if (c.n < 2) return;
   const float* pieces = scratch + q4_chain_floats(n_warps);
   const int size = (int)q4_piece_floats(G, D);
-  const int rank = w_at - c.from, quads = G * D / 4, per = c.n >= 2 ? (quads + c.n - 1) / c.n : 0, q_end = min(quads, (rank + 1) * per);
+  const int rank = w_at - c.from, quads = G * D / 4, per = (quads + c.n - 1) / c.n, q_end = min(quads, (rank + 1) * per);
   const int here = max(min(Q4_JOIN, q_end - rank * per), 0);
   // threads side by side; the others go through the pieces beside them
   const int width = here > 1 ? 1 << (32 - __clz(here - 1)) : 1, parts = Q4_JOIN / width, part = tid / width;
-  const bool shared = __syncthreads_or(c.n >= 2 && parts > 1);
-  const int rounds = (G * D / 8 + Q4_JOIN - 1) / Q4_JOIN;  // (for a chain of two; longer ones find nothing left to do)
-  for (int round = 0; round < rounds; ++round) {
-    const int quad = rank * per + round * Q4_JOIN + tid % width, head = quad * 4 / D;
-    const bool mine = c.n >= 2 && tid % width < here && quad < q_end;
+  for (int q0 = rank * per; q0 < q_end; q0 += Q4_JOIN) {
+    const int quad = q0 + tid % width, head = quad * 4 / D;
+    const bool mine = tid % width < here && quad < q_end;
     Q4Part x;
     if (mine)
-#pragma unroll 1
-      for (int p = part; p < c.n; p += parts) {
-        const float* from = pieces + (2LL * (c.from + p) + (p == 0)) * size;
-        Q4Part y;
-        y.m = from[G * D + head];
-        y.l = from[G * D + G + head];
-        y.o = *reinterpret_cast<const float4*>(from + 4 * quad);
-        x.add(y);
-      }
-    if (shared)
-      for (int o = Q4_JOIN / 2; o > 0; o >>= 1) {  // (all chains take the same steps; those within a chain's width add nothing)
-        o_s[threadIdx.x] = x.o;
-        ml_s[threadIdx.x] = make_float2(x.m, x.l);
-        __syncthreads();
-        if (mine && o >= width && part < o / width) {
-          Q4Part y;
-          y.m = ml_s[threadIdx.x + o].x;
-          y.l = ml_s[threadIdx.x + o].y;
-          y.o = o_s[threadIdx.x + o];
-          x.add(y);
+      for (int p0 = part; p0 < c.n; p0 += 4 * parts) {
+        Q4Part y[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int p = p0 + u * parts;
+          const float* from = pieces + (2LL * (c.from + p) + (p == 0)) * size;
+          if (p < c.n) {
+            y[u].m = from[G * D + head];
+            y[u].l = from[G * D + G + head];
+            y[u].o = *reinterpret_cast<const float4*>(from + 4 * quad);
+          }
         }
-        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < 4; ++u) x.add(y[u]);
       }
-    if (mine && part == 0) {
+    auto other = [&](int o) {  // of the thread o lanes away
+      Q4Part y;
+      y.m = __shfl_xor_sync(0xffffffffu, x.m, o);
+      y.l = __shfl_xor_sync(0xffffffffu, x.l, o);
+      y.o = make_float4(__shfl_xor_sync(0xffffffffu, x.o.x, o), __shfl_xor_sync(0xffffffffu, x.o.y, o), __shfl_xor_sync(0xffffffffu, x.o.z, o),
+                        __shfl_xor_sync(0xffffffffu, x.o.w, o));
+      return y;
+    };
+    for (int o = 16; o >= width; o /= 2) x.add(other(o));
+    if (parts > 1) {  // (two warps)
+      shared[threadIdx.x] = x;
+      asm volatile("bar.sync %0, 64;" ::"r"(1 + (int)threadIdx.x / Q4_JOIN) : "memory");
+      if (tid < 32) x.add(shared[threadIdx.x + 32]);
+      asm volatile("bar.sync %0, 64;" ::"r"(1 + (int)threadIdx.x / Q4_JOIN) : "memory");
+    }
+    if (mine && tid < width) {
       const float inv = x.l > 0.f ? 1.f / x.l : x.l;
       bf16* to = out + ((long long)c.seq * n_q + (long long)c.head * G) * D + 4 * quad;
       *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(x.o.x * inv, x.o.y * inv), pack_bf16x2(x.o.z * inv, x.o.w * inv));
@@ -726,7 +730,7 @@ static int launch_kv4_stream(const Kv4Args& a, cudaStream_t st) {
   B200Q_CUDA(launch_early(kern, dim3(ctas), C::WARPS * 32, C::smem(a.G), st, 1, a, C::stage_bytes(a.G), (int)whole, whole ? 1 : Q4_LEAST_SHARE, scratch));
   count_launch();
   if (whole) return B200Q_OK;
-  B200Q_CUDA(launch_early(kv4_join_kernel<D>, dim3(ctas), 8 * Q4_JOIN, 0, st, 1, (const float*)scratch, a.out, a.n_q, a.G));
+  B200Q_CUDA(launch_early(kv4_join_kernel<D>, dim3(warps / 2), 4 * Q4_JOIN, 0, st, 1, (const float*)scratch, a.out, a.n_q, a.G));
   count_launch();
   return B200Q_OK;
 }
