@@ -722,10 +722,13 @@ static int launch_kv4_stream(const Kv4Args& a, cudaStream_t st) {
   // Items of up to 8 pages go to warps whole: adding up pieces costs as much as they do (one sequence of 64 tokens, 8 kv heads, 5.6 us, in
   // pieces 9.5; 2800 of 128 tokens 96.5, in pieces 103.9).
   const int width = a.window > 0 && (a.window + 15) / 16 + 1 < a.bt_stride ? (a.window + 15) / 16 + 1 : a.bt_stride;
-  const bool whole = g_q4_whole < 0 ? batch_invariant() || width <= 8 : g_q4_whole != 0;
+  bool whole = g_q4_whole < 0 ? batch_invariant() || width <= 8 : g_q4_whole != 0;
   float* scratch = nullptr;
-  const int rc = stream_scratch(1, (size_t)(q4_chain_floats(warps) + 2 * warps * q4_piece_floats(a.G, D)) * sizeof(float), st, &scratch);
-  if (rc) return rc;
+  // (where there is no memory for pieces, items go to warps whole)
+  if (!whole && stream_scratch(1, (size_t)(q4_chain_floats(warps) + 2 * warps * q4_piece_floats(a.G, D)) * sizeof(float), st, &scratch)) {
+    cudaGetLastError();
+    whole = true;
+  }
   std::lock_guard<std::mutex> together(g_q4_pair);
   B200Q_CUDA(launch_early(kern, dim3(ctas), C::WARPS * 32, C::smem(a.G), st, 1, a, C::stage_bytes(a.G), (int)whole, whole ? 1 : Q4_LEAST_SHARE, scratch));
   count_launch();
