@@ -344,7 +344,7 @@ struct __align__(16) Q4Chain {
 struct Q4Item {
   int seq, head, ctx, lo, page0, pages;
 };
-// scratch: two chains per warp (of the piece at its beginning, of the one at its end), then two pieces per warp, [G][D] outputs, [G] maxima, [G] sums
+// scratch (none for whole items): two chains per warp (of the piece at its beginning, of the one at its end), then two pieces per warp, [G][D] outputs, [G] maxima, [G] sums
 __host__ __device__ inline long long q4_piece_floats(int G, int D) { return ((long long)G * (D + 2) + 3) / 4 * 4; }
 __host__ __device__ inline long long q4_chain_floats(int warps) { return 8LL * warps; }
 
@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(Q4Stream<D>::WARPS * 32, Q4Stream<D>::CTAS) kv
   long long u0 = piece0, u1 = min(u0 + share, units);
   Q4Chain* chains = reinterpret_cast<Q4Chain*>(scratch) + 2 * w_at;
   float* pieces = scratch + q4_chain_floats(n_warps) + 2 * w_at * q4_piece_floats(a.G, D);
-  if (lane < 2) chains[lane] = {0, 0, 0, 0};
+  if (!whole_items && lane < 2) chains[lane] = {0, 0, 0, 0};  // (whole items have no pieces, and no scratch)
   __syncwarp();
   if (u0 >= u1) return;
   // ---- the sequence that has unit u, and its first unit
