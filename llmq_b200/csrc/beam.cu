@@ -2,12 +2,15 @@
 // the K largest of W V, of equal ones those with the lowest w V + v first; and the first W of them that do not end.
 //
 // Two kernels.  The first has a piece of a row per CTA and goes through it once: the sum of its exponentials and its K best logits (a row's
-// order needs no logarithm).  The largest logits of groups of threads give a bound that K of the first tile reach; what reaches it, K or a
-// few more, is ranked by counting, and the K-th best so far is the bound from there on.  The second has a group per CTA: sums to logarithms, best logits to scores, and again a bound (the K-th
-// best of the pieces' first entries), what reaches it, and ranks.
+// order needs no logarithm).  The largest logits of groups of threads give a bound that K of the first tile reach; vectors in which something
+// reaches it are collected, and once they are many their logits are ranked by counting: the K-th best so far is the bound from there on.  The
+// second kernel has a group per CTA: sums to logarithms, best logits to scores, and again a bound (the K-th best of the pieces' first entries),
+// what reaches it, and ranks.
 // Scores that are compared across rows are 64 bits; a row's logarithm comes from sums whose terms are off by some 2^-23 in either direction.
-// Bound: the logits, 2 bytes each, once; next to it the exponentials, four instructions a logit, one of them of the unit that has a quarter
-// of the others' rate.
+// Bound: the logits, 2 bytes each, once; next to it the exponentials (16 a cycle and SM: two thirds of the memory's
+// time) and some nine instructions a logit.  Logits come by asynchronous copies two tiles ahead (in registers a tile ahead 55 us).
+// 48 groups of 8 beams over 256000 tokens, 16 candidates: 52.3 us (the memory's share 30; the first kernel 47, of which an eighth is looking for
+// the 16 best: 41 with one), one group of 4 over 128256: 10.2.
 #include "common.cuh"
 
 namespace b200q {
@@ -17,6 +20,12 @@ constexpr int BEAM_THREADS = 256, BEAM_MOST_K = 64, BEAM_MOST_W = 32, BEAM_FOUND
 __device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// either of two numbers >= that of `bound` (NaN is not)
+__device__ __forceinline__ bool reaches_bf16x2(uint32_t m, uint32_t bound) {
+  int r;
+  asm("{ .reg .pred p, q;\n setp.ge.bf16x2 p|q, %1, %2;\n or.pred p, p, q;\n selp.s32 %0, 1, 0, p; }" : "=r"(r) : "r"(m), "r"(bound));
   return r;
 }
 // unsigned integers of the same order as the numbers (bf16 bits); NaN counts as -infinity
@@ -102,6 +111,11 @@ struct BeamRow {
   }
 };
 
+__device__ __forceinline__ uint4 lds_v4(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
 // the next place in a list in shared memory (few lanes at a time ask for one: no need to ask for all of them together)
 __device__ __forceinline__ int next_place(int* count) {
   int at;
@@ -109,8 +123,9 @@ __device__ __forceinline__ int next_place(int* count) {
   return at;
 }
 
-// A piece of a row, in tiles of TILE vectors; the next tile is on its way while one is looked at.
-constexpr int BEAM_NV = 4, TILE = BEAM_NV * BEAM_THREADS;
+// A piece of a row, in tiles of TILE vectors; the next ones are on their way while one is looked at.  Vectors collected from which on they are
+// ranked: 24 / 48 / 96 cost 384 rows of 256000 logits 52.5 / 52.2 / 57.2 us.
+constexpr int BEAM_NV = 4, TILE = BEAM_NV * BEAM_THREADS, BEAM_MANY = 48, BEAM_RING = 2;
 template <bool kAligned>
 __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* logits, long long V, int K, long long row0, long long rows,
                                                                     int2* entries, double* logs) {
@@ -126,12 +141,42 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
   __shared__ uint4 vectors[BEAM_VECTORS];  // that hold a logit that reaches the bound, and which they are
   __shared__ int vector_at[BEAM_VECTORS], n_vectors, n_found, bound_s;
   __shared__ uint64_t best_s[BEAM_THREADS / 32];
-  uint4 a[BEAM_NV];
+  // Rows of aligned vectors come through a ring of BEAM_RING tiles, every thread's vectors in places of its own (no waiting for others); of
+  // other rows the next tile's are in registers.
+  extern __shared__ uint4 ring[];
+  const uint32_t place = smem_u32(ring + tid);
+  const uint4* source = x.base + v0 + tid;
+  const int whole = (v1 - v0) / TILE;
+  auto ask = [&](int tile, int stage) {
+    const uint32_t to = place + 16 * stage * TILE;
+    if (tile < whole) {
 #pragma unroll
-  for (int u = 0; u < BEAM_NV; ++u) a[u] = v0 + u * BEAM_THREADS + tid < v1 ? x(v0 + u * BEAM_THREADS + tid) : none;
+      for (int u = 0; u < BEAM_NV; ++u)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 16 * u * BEAM_THREADS), "l"(source + u * BEAM_THREADS) : "memory");
+    } else {
+      const int left = v1 - v0 - tile * TILE - tid;
+#pragma unroll
+      for (int u = 0; u < BEAM_NV; ++u)
+        if (u * BEAM_THREADS < left)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 16 * u * BEAM_THREADS), "l"(source + u * BEAM_THREADS) : "memory");
+    }
+    source += TILE;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  uint4 a[BEAM_NV];
+  if constexpr (kAligned) {
+#pragma unroll
+    for (int s = 0; s < BEAM_RING; ++s) ask(s, s);
+    asm volatile("cp.async.wait_group %0;" ::"n"(BEAM_RING - 1) : "memory");
+#pragma unroll
+    for (int u = 0; u < BEAM_NV; ++u) a[u] = v0 + u * BEAM_THREADS + tid < v1 ? lds_v4(place + 16 * u * BEAM_THREADS) : none;
+  } else {
+#pragma unroll
+    for (int u = 0; u < BEAM_NV; ++u) a[u] = v0 + u * BEAM_THREADS + tid < v1 ? x(v0 + u * BEAM_THREADS + tid) : none;
+  }
   if (tid == 0) n_found = n_vectors = 0;
   float bound = -INFINITY;
-  uint32_t top2 = 0xff80ff80u;
+  uint32_t bound2 = 0xff80ff80u;  // twice the same as bf16
   f32x2 sum = 0;
   // the logits of the collected vectors that reach the bound, and the k0 in best: the K best of them into best, in order; the K-th is the new
   // bound.  False: too many to look at
@@ -183,7 +228,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
     uint32_t m = 0xff80ff80u;
 #pragma unroll
     for (int u = 0; u < BEAM_NV; ++u) m = max_bf16x2(m, max_bf16x2(max_bf16x2(a[u].x, a[u].y), max_bf16x2(a[u].z, a[u].w)));
-    const int deep = K <= 16 ? 3 : K <= 32 ? 2 : 1, groups = BEAM_THREADS >> deep;
+    const int deep = K <= 32 ? 2 : 1, groups = BEAM_THREADS >> deep;
     float mine = fmaxf(bf16_lo(m), bf16_hi(m));  // (max of a number and NaN is the number; -infinity was among them)
     for (int o = 1; o < 1 << deep; o <<= 1) mine = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, o));
     if ((tid & ((1 << deep) - 1)) == 0) tops[tid >> deep] = mine;
@@ -197,24 +242,36 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
     }
     __syncthreads();
     bound = __int_as_float(bound_s);
+    bound2 = (uint32_t)bound_s >> 16 | ((uint32_t)bound_s & 0xffff0000u);
   }
-  auto look = [&](const uint4& v, int c) {
-    const uint32_t m = max_bf16x2(max_bf16x2(v.x, v.y), max_bf16x2(v.z, v.w));
-    top2 = max_bf16x2(top2, m);
-    if (fmaxf(bf16_lo(m), bf16_hi(m)) >= bound) {  // (seldom)
-      const int at = next_place(&n_vectors);
-      if (at < BEAM_VECTORS) {
-        vectors[at] = v;
-        vector_at[at] = c;
-      }
+  auto most_of = [](const uint4& v) { return max_bf16x2(max_bf16x2(v.x, v.y), max_bf16x2(v.z, v.w)); };
+  auto collect = [&](const uint4& v, int c) {
+    const int at = next_place(&n_vectors);
+    if (at < BEAM_VECTORS) {
+      vectors[at] = v;
+      vector_at[at] = c;
     }
+  };
+  auto add = [&](const uint4& v) {
     add_exps(sum, v.x);
     add_exps(sum, v.y);
     add_exps(sum, v.z);
     add_exps(sum, v.w);
   };
-  // Tiles that have a whole one behind them, which is asked for vector by vector as soon as this one's has been seen.  Behind tiles 0, 3, 15,
-  // ... only the K best so far matter.
+  auto look = [&](const uint4& v, int c) {
+    if (reaches_bf16x2(most_of(v), bound2)) collect(v, c);
+    add(v);
+  };
+  auto look_at_two = [&](const uint4& v, const uint4& w, int c) {
+    const uint32_t mv = most_of(v), mw = most_of(w);
+    if (reaches_bf16x2(max_bf16x2(mv, mw), bound2)) {  // (seldom)
+      if (reaches_bf16x2(mv, bound2)) collect(v, c);
+      if (reaches_bf16x2(mw, bound2)) collect(w, c + BEAM_THREADS);
+    }
+    add(v);
+    add(w);
+  };
+  // Whole tiles; what comes next is asked for as soon as a place is free.  Behind tiles 0, 1, 3, 7, ... it is looked at whether enough has been found for only the K best so far to matter from there on (the ranks cost the square of it).
   int c = v0 + tid, kept = 0;
   bool overflow = false;
   auto settle = [&]() {
@@ -222,35 +279,57 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
     kept = K;
     overflow |= !fits || bound == -INFINITY;
     bound = overflow ? INFINITY : value_of(best[K - 1]);  // (overflow: whatever is found from here on does not matter)
+    bound2 = __float_as_uint(bound) >> 16 | __float_as_uint(bound);
   };
-  const int whole = max((v1 - v0) / TILE - 1, 0);
-  for (int t = 0, end = 1; t < whole; end *= 4) {
-    for (; t < min(end, whole); ++t, c += TILE)
+  int stage = 0;
+  for (int t = 0, end = 1; t < whole; end *= 2) {
+    for (; t < min(end, whole); ++t) {
+      if constexpr (kAligned) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(BEAM_RING - 1) : "memory");
 #pragma unroll
-      for (int u = 0; u < BEAM_NV; ++u) {
-        look(a[u], c + u * BEAM_THREADS);
-        a[u] = x(c + TILE + u * BEAM_THREADS);
+        for (int u = 0; u < BEAM_NV; ++u) a[u] = lds_v4(place + 16 * (stage * TILE + u * BEAM_THREADS));
+        look_at_two(a[0], a[1], c);
+        look_at_two(a[2], a[3], c + 2 * BEAM_THREADS);
+        ask(t + BEAM_RING, stage);
+        stage = stage + 1 < BEAM_RING ? stage + 1 : 0;
+        c += TILE;
+      } else {
+#pragma unroll
+        for (int u = 0; u < BEAM_NV; u += 2) {
+          look_at_two(a[u], a[u + 1], c);
+#pragma unroll
+          for (int k = u; k < u + 2; ++k, c += BEAM_THREADS)
+            if (c + TILE < v1) a[k] = x(c + TILE);
+        }
       }
-    if (t < whole || v0 + (t + 1) * TILE < v1) settle();
+    }
+    // (the count that a thread sees holds its own vectors, so that the last one to add any sees them all)
+    if (t < whole && __syncthreads_or(*(volatile int*)&n_vectors > BEAM_MANY)) settle();
   }
-  // the last whole tile, which is there already, and what is behind it
+  // what is behind the last whole tile
+  if constexpr (kAligned) asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
-  for (int u = 0; u < BEAM_NV; ++u)
-    if (c + u * BEAM_THREADS < v1) look(a[u], c + u * BEAM_THREADS);
-  for (c += TILE; c < v1; c += BEAM_THREADS) look(x(c), c);
+  for (int u = 0; u < BEAM_NV; ++u, c += BEAM_THREADS)
+    if (c < v1) look(kAligned ? lds_v4(place + 16 * (stage * TILE + u * BEAM_THREADS)) : a[u], c);
   settle();
   const float2 halves = halves_of(sum);
   float mine_sum = halves.x + halves.y;
   // the largest logit: where the exponentials themselves would leave what fp32 holds, or the constant's own error would show, or a thread
   // met NaN, once more by differences to it
-  float top = fmaxf(bf16_lo(top2), bf16_hi(top2));
+  float top = -INFINITY;
+  if (!overflow && v0 < v1) {
+    top = value_of(best[0]);
+  } else {
+    uint32_t m = 0xff80ff80u;
+    for (int c = v0 + tid; c < v1; c += BEAM_THREADS) m = max_bf16x2(m, most_of(x(c)));
+    top = fmaxf(bf16_lo(m), bf16_hi(m));
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  __syncthreads();
-  if ((tid & 31) == 0) tops[tid >> 5] = top;
-  __syncthreads();
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if ((tid & 31) == 0) tops[tid >> 5] = top;
+    __syncthreads();
 #pragma unroll
-  for (int w = 0; w < BEAM_THREADS / 32; ++w) top = fmaxf(top, tops[w]);
+    for (int w = 0; w < BEAM_THREADS / 32; ++w) top = fmaxf(top, tops[w]);
+  }
   const bool far = fabsf(top) > 32.f;
   if (far || mine_sum != mine_sum) {
     mine_sum = 0.f;
@@ -508,8 +587,8 @@ __global__ void __launch_bounds__(MERGE_THREADS) beam_groups_kernel(BeamArgs a) 
 }
 
 // Pieces of a row: the least time of the SM that has most CTAs, each its logits (five CTAs at once are as fast as an SM gets) and 11000 logits'
-// worth beside them, and of the lists that the second kernel has to look at.  384 rows of 256000 logits: 1 / 2 / 3 / 4 / 8 / 16 pieces 73.8 /
-// 62.5 / 58.3 / 62.4 / 67.4 / 81.8 us; 4 rows of 128256: 8 / 24 / 32 / 64 pieces 13.1 / 11.3 / 12.2 / 13.5 us.
+// worth beside them, and of the lists that the second kernel has to look at.  384 rows of 256000 logits: 1 / 2 / 3 / 4 / 6 / 8 pieces 69.0 /
+// 53.7 / 52.3 / 55.1 / 64.7 / 65.6 us; 4 rows of 128256: 8 / 16 / 32 / 48 / 64 pieces 10.4 / 9.9 / 10.1 / 11.1 / 11.9 us.
 static int beam_pieces(long long rows, long long V) {
   int best = 1;
   double least = 1e30;
@@ -563,7 +642,7 @@ int b200q_beam_select(const void* logits, const float* scores, int groups, int b
   for (int64_t r0 = 0; r0 < rows; r0 += 65535) {  // (a grid's second dimension ends there)
     const unsigned n = (unsigned)(rows - r0 < 65535 ? rows - r0 : 65535);
     auto kern = V % 8 ? beam_rows_kernel<false> : beam_rows_kernel<true>;
-    B200Q_CUDA(launch_early(kern, dim3(pieces, n), BEAM_THREADS, 0, st, 1, (const bf16*)logits, (long long)V, K, (long long)r0, (long long)rows, entries, logs));
+    B200Q_CUDA(launch_early(kern, dim3(pieces, n), BEAM_THREADS, V % 8 ? 0 : BEAM_RING * TILE * 16, st, 1, (const bf16*)logits, (long long)V, K, (long long)r0, (long long)rows, entries, logs));
     count_launch();
   }
   const BeamArgs a{scores, stops, entries, logs, cand_scores, next_scores, cand_tokens, cand_rows, next_tokens, next_rows, beams, K, pieces, n_stops,
