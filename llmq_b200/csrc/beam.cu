@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
   const BeamRow<kAligned> x(logits, V, row, rows);
   const int vecs = (int)((V + 7) / 8), per = (vecs + n_pieces - 1) / n_pieces, v0 = min(vecs, piece * per), v1 = min(vecs, v0 + per);
   const uint4 none = make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
-  __shared__ float tops[BEAM_THREADS / 2];
+  __shared__ float tops[BEAM_THREADS];
   __shared__ uint64_t found[BEAM_FOUND], best[BEAM_MOST_K];
   __shared__ double sums[BEAM_THREADS / 32];
   __shared__ uint4 vectors[BEAM_VECTORS];  // that hold a logit that reaches the bound, and which they are
@@ -178,8 +178,8 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
   float bound = -INFINITY;
   uint32_t bound2 = 0xff80ff80u;  // twice the same as bf16
   f32x2 sum = 0;
-  // the logits of the collected vectors that reach the bound, and the k0 in best: the K best of them into best, in order; the K-th is the new
-  // bound.  False: too many to look at
+  // the logits of the collected vectors that reach the bound, and the k0 in best: the K best of them into best, in order.  How many there are;
+  // -1: too many to look at
   auto prune = [&](int k0) {
     __syncthreads();
     const int nv = n_vectors;
@@ -194,8 +194,8 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
       }
     __syncthreads();
     const int n = n_found;
-    if (nv == 0) return true;
-    if (nv > BEAM_VECTORS || n > BEAM_FOUND) return false;
+    if (nv == 0) return k0;
+    if (nv > BEAM_VECTORS || n > BEAM_FOUND) return -1;
     uint64_t key[BEAM_FOUND / BEAM_THREADS + 1];
     int rank[BEAM_FOUND / BEAM_THREADS + 1];
 #pragma unroll
@@ -217,13 +217,14 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
       if (rank[i] < K) best[rank[i]] = key[i];
     if (tid == 0) n_found = n_vectors = 0;
     __syncthreads();
-    return true;
+    return min(k0 + n, K);
   };
   auto value_of = [](uint64_t key) {  // the logit of a key
     const uint32_t o = (uint32_t)(key >> 32), h = (o & 0x8000u) ? o & 0x7fffu : 0xffffu ^ o;
     return __uint_as_float(h << 16);
   };
-  // a bound that K of the first tile reach: the K-th of the largest logits of groups of threads, at least twice as many as are wanted
+  // a bound that K of the first tile reach: the K-th of the largest logits of groups of threads, at least twice as many as are wanted.  Where
+  // fewer are above -infinity, the lowest number there is
   {
     uint32_t m = 0xff80ff80u;
 #pragma unroll
@@ -241,8 +242,8 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
       if (rank == K - 1) bound_s = __float_as_int(y);
     }
     __syncthreads();
-    bound = __int_as_float(bound_s);
-    bound2 = (uint32_t)bound_s >> 16 | ((uint32_t)bound_s & 0xffff0000u);
+    bound = fmaxf(__int_as_float(bound_s), __uint_as_float(0xff7f0000u));
+    bound2 = __float_as_uint(bound) >> 16 | __float_as_uint(bound);
   }
   auto most_of = [](const uint4& v) { return max_bf16x2(max_bf16x2(v.x, v.y), max_bf16x2(v.z, v.w)); };
   auto collect = [&](const uint4& v, int c) {
@@ -275,10 +276,13 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
   int c = v0 + tid, kept = 0;
   bool overflow = false;
   auto settle = [&]() {
-    const bool fits = prune(kept);
-    kept = K;
-    overflow |= !fits || bound == -INFINITY;
-    bound = overflow ? INFINITY : value_of(best[K - 1]);  // (overflow: whatever is found from here on does not matter)
+    const int k = prune(kept);
+    overflow |= k < 0;
+    if (!overflow) kept = k;
+    if (overflow)
+      bound = INFINITY;  // (whatever is found from here on does not matter)
+    else if (kept == K)
+      bound = value_of(best[K - 1]);
     bound2 = __float_as_uint(bound) >> 16 | __float_as_uint(bound);
   };
   int stage = 0;
@@ -317,8 +321,8 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
   // the largest logit: where the exponentials themselves would leave what fp32 holds, or the constant's own error would show, or a thread
   // met NaN, once more by differences to it
   float top = -INFINITY;
-  if (!overflow && v0 < v1) {
-    top = value_of(best[0]);
+  if (!overflow) {
+    if (kept > 0) top = value_of(best[0]);
   } else {
     uint32_t m = 0xff80ff80u;
     for (int c = v0 + tid; c < v1; c += BEAM_THREADS) m = max_bf16x2(m, most_of(x(c)));
@@ -357,11 +361,55 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
   }
   int2* to = entries + out * K;
   auto tell = [&](int rank, uint64_t key) { to[rank] = make_int2(__float_as_int(value_of(key)), (int)(0xffffffffu - (uint32_t)key)); };
-  if (!overflow && v0 < v1) {  // (K and more reach the bound; the keys are all different)
-    if (tid < K) tell(tid, best[tid]);
+  // Too many reached the bound (logits in some order, a mask over the row's first part): tile by tile once more, each with a bound of its own, the
+  // K-th of the threads' largest logits.  384 rows of 256000 logits whose first half is hidden: 189 us (one after the other, as below, 1160).
+  if (overflow) {
+    overflow = false;
+    kept = 0;
+    bound = __uint_as_float(0xff7f0000u);
+    for (int from = v0; from < v1 && !overflow; from += TILE) {
+      __syncthreads();
+      uint32_t m = 0xff80ff80u;
+#pragma unroll
+      for (int u = 0; u < BEAM_NV; ++u) {
+        a[u] = from + u * BEAM_THREADS + tid < v1 ? x(from + u * BEAM_THREADS + tid) : none;
+        m = max_bf16x2(m, most_of(a[u]));
+      }
+      const float mine = fmaxf(bf16_lo(m), bf16_hi(m));
+      tops[tid] = mine;
+      if (tid == 0) n_found = n_vectors = 0;
+      __syncthreads();
+      int rank = 0;
+#pragma unroll 16
+      for (int i = 0; i < BEAM_THREADS; ++i) rank += tops[i] > mine || (tops[i] == mine && i < tid);
+      if (rank == K - 1) bound_s = __float_as_int(mine);
+      __syncthreads();
+      bound = fmaxf(bound, __int_as_float(bound_s));
+      bound2 = __float_as_uint(bound) >> 16 | __float_as_uint(bound);
+#pragma unroll
+      for (int u = 0; u < BEAM_NV; ++u)
+        if (reaches_bf16x2(most_of(a[u]), bound2)) collect(a[u], from + u * BEAM_THREADS + tid);
+      const int k = prune(kept);
+      overflow = k < 0;
+      kept = max(k, 0);
+      if (kept == K) bound = value_of(best[K - 1]);
+    }
+  }
+  if (!overflow) {
+    if (tid < kept) tell(tid, best[tid]);
+    // Fewer than K above -infinity: the first tokens at -infinity follow (NaN counts as that).  They are among the piece's first K.
+    if (kept < K && tid < 32)
+      for (int k0 = 0, at = kept; at < K; k0 += 32) {
+        const long long token = 8LL * v0 + k0 + tid, end = min(8LL * v1, V);
+        const bool low = k0 + tid < K && token < end && !(__bfloat162float(x.x[token]) > -INFINITY);
+        const uint32_t votes = __ballot_sync(0xffffffffu, low || k0 >= K);  // (fewer than K tokens: none)
+        const int place = at + __popc(votes & ((1u << tid) - 1u));
+        if ((votes >> tid & 1u) && place < K) to[place] = make_int2((int)0xff800000u, low ? (int)token : -1);
+        at += __popc(votes);
+      }
     return;
   }
-  // Fewer than K groups with a number above -infinity, or hundreds of equal or ever larger logits: one after the other.
+  // Hundreds of equal or ever larger logits: one after the other.
   uint64_t last = ~0ull;
   for (int k = 0; k < K; ++k) {
     uint64_t most = 0;

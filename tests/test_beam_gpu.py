@@ -64,6 +64,40 @@ def test_select(cuda, V, B, W, K):
     check(lib, cuda, logits, scores, W, K, logits.float().argmax(-1)[:3].tolist())
 
 
+@pytest.mark.parametrize("V", [3001, 50257, 256000])
+@pytest.mark.parametrize("W,K", [(2, 4), (8, 16), (3, 64)])
+def test_few_tokens_allowed(cuda, V, W, K):
+    """rows of which a mask leaves none, one, about K or some hundred tokens, anywhere in them, and rows of which it leaves the second half"""
+    from llmq_b200 import lib
+    g = torch.Generator().manual_seed(V + W)
+    for left in (0, 1, K - 1, K, K + 1, 300):
+        logits = torch.full((2 * W, V), -math.inf)
+        for row in logits:
+            at = torch.randperm(V, generator=g)[:left]
+            row[at] = torch.randn(left, generator=g)
+        check(lib, cuda, logits.to(BF), -torch.rand(2 * W, generator=g), W, K, [])
+    half = torch.randn(2 * W, V, generator=g)
+    half[:, :V // 2] = -math.inf
+    half[-1, V // 2: V // 2 + 40] = math.nan
+    check(lib, cuda, half.to(BF), -torch.rand(2 * W, generator=g), W, K, [])
+
+
+@pytest.mark.parametrize("V", [9000, 50257, 128256])
+@pytest.mark.parametrize("W,K", [(1, 1), (8, 16), (2, 64)])
+def test_logits_in_order(cuda, V, W, K):
+    """rows that rise, fall, rise in steps, and random ones whose largest logits lie side by side"""
+    from llmq_b200 import lib
+    g = torch.Generator().manual_seed(V + K)
+    x = (2.5 * torch.randn(2 * W, V, generator=g)).to(BF)
+    scores = -torch.rand(2 * W, generator=g)
+    check(lib, cuda, x.sort(-1)[0], scores, W, K, [])
+    check(lib, cuda, x.sort(-1, descending=True)[0], scores, W, K, [])
+    steps = torch.arange(V).div(997, rounding_mode="floor").to(BF).expand(2 * W, V).contiguous()
+    check(lib, cuda, steps, scores, W, K, [])
+    x[:, V // 3: V // 3 + 700] = x.float().sort(-1, descending=True)[0][:, :700].to(BF)
+    check(lib, cuda, x, scores, W, K, [])
+
+
 def test_many_groups(cuda):
     from llmq_b200 import lib
     g = torch.Generator().manual_seed(1)
