@@ -660,7 +660,7 @@ int b200q_rope_kvwrite_q4(void* qkv_dev, const void* cos_sin_dev, const int32_t*
 int b200q_kv4_unpack(const void* kv4_layer_dev, const int32_t* pages_dev, int n_pages, void* kv_out_dev, int n_kv, int D,
                      int block_size, void* stream);
 /* b200q_decode_attn_ex over a 4-bit cache (GQA group <= 8).  A sequence of no tokens gives zeros; lengths beyond the table's width count as
- *     its width.  q rows 16-byte aligned, out 8.  Pieces of sequences that several warps share lie in scratch that the stream (a graph: the
+ *     its width, and the entries that a length counts are numbers of pages.  q rows 16-byte aligned, out 8.  Pieces of sequences that several warps share lie in scratch that the stream (a graph: the
  *     graph) keeps, up to 64 MiB, allocated when first needed; where there is no memory for it nothing is shared. */
 int b200q_decode_attn_q4(const void* q_dev, int q_stride, void* out_dev, const void* kv4_layer_dev, const int32_t* block_table_dev,
                          int bt_stride, const int32_t* ctx_lens_dev, int n_seqs, int n_q, int n_kv, int D, int block_size,
@@ -697,8 +697,9 @@ int b200q_beam_select(const void* logits_dev, const float* scores_dev, int group
  *     Free pages go out in the order of the rows; pages that become free by this call are free for later ones.  slots[i] =
  *     page * block_size + place of the next token, -1 where there is none.  Old rows hold nothing any more: refs is kept up.
  *     status[0] = pages that were missing (0: all is well; else nothing has changed, slots are -1), status[1] = rows whose table is
- *     full (slot -1; they hold their parent's pages).  Entries of table_out behind a row's pages stay as they are; it must not
- *     overlap `table`.  n_old, n_new <= 8192, block_size 16. */
+ *     full (slot -1; they hold their parent's pages).  Entries of table_out behind a row's pages, and rows of no parent, stay as they
+ *     are (a step that is enqueued before status has been read needs numbers of pages there, zeros for instance, in case the pool is
+ *     short); it must not overlap `table`.  n_old, n_new <= 8192, block_size 16. */
 int b200q_pages_fork(const int32_t* table_dev, const int32_t* lens_dev, int n_old, const int32_t* parents_dev, int n_new, int bt_stride,
                      int32_t* refs_dev, int num_blocks, int block_size, int32_t* table_out_dev, int32_t* slots_dev, int32_t* pairs_dev,
                      int32_t* status_dev, void* stream);

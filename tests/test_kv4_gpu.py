@@ -256,3 +256,79 @@ def test_captured_and_on_another_stream(cuda):
         torch.cuda.synchronize()
         for name in ("out", "cache", "qkv"):
             assert torch.equal(a[name].view(torch.uint8), b[name].view(torch.uint8)), name
+
+
+@pytest.mark.parametrize("D,n_q,n_kv", [(64, 8, 2), (256, 4, 1)])
+def test_two_calls_at_once(cuda, D, n_q, n_kv):
+    """long contexts, whose pieces lie in scratch: two threads on streams of their own, then two graphs replayed side by side, each time
+    beside the same calls one after the other"""
+    import threading
+    from llmq_b200 import lib
+    sets = [[5000, 33, 9000], [12000, 700]]
+    args = []
+    for k, ctxs in enumerate(sets):
+        cache, table, _ = make_cache(ctxs, n_kv, D, seed=k)
+        qkv = torch.randn(len(ctxs), (n_q + 2 * n_kv) * D, generator=torch.Generator().manual_seed(k)).to(BF)
+        args.append((qkv.to(cuda), cache.to(cuda), table.to(cuda), torch.tensor(ctxs, dtype=torch.int32, device=cuda)))
+
+    def call(k, out, stream=None):
+        q, cache, table, ctx = args[k]
+        lib.decode_attn_q4(q, out, cache, table, ctx, n_q, n_kv, D, BS, D ** -0.5, stream=stream)
+
+    def outs():
+        return [[torch.zeros(len(c), n_q * D, dtype=BF, device=cuda) for _ in range(20)] for c in sets]
+
+    alone = [o[0] for o in outs()]
+    for k in (0, 1):
+        call(k, alone[k])
+        torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in sets], outs()
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=lambda k=k: [call(k, o, streams[k]) for o in got[k]]) for k in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for k in (0, 1):
+        assert all(torch.equal(o, alone[k]) for o in got[k])
+    graphs, got = [torch.cuda.CUDAGraph() for _ in sets], outs()
+    for k in (0, 1):
+        with torch.cuda.graph(graphs[k]):
+            for o in got[k]:
+                call(k, o)
+    for _ in range(2):
+        for k in (0, 1):
+            for o in got[k]:
+                o.zero_()
+        torch.cuda.synchronize()
+        for k in (0, 1):
+            with torch.cuda.stream(streams[k]):
+                graphs[k].replay()
+        torch.cuda.synchronize()
+        for k in (0, 1):
+            assert all(torch.equal(o, alone[k]) for o in got[k])
+
+
+def test_portions_of_one_sequence(cuda):
+    """a prompt whose portions are apart in the step: each sees the keys up to its own tokens, the same as in a step of its own"""
+    from llmq_b200 import lib
+    D, n_q, n_kv = 128, 8, 2
+    cache, table, rows = make_cache([400, 90], n_kv, D, seed=3)
+    portions = [(0, 0, 33), (1, 40, 50), (0, 33, 100), (0, 300, 100)]   # sequence, past, tokens
+    tiles, T = [], 0
+    for s, past, n in portions:
+        tiles += [[s, T + j, min(16, n - j), past + j] for j in range(0, n, 16)]
+        T += n
+    qkv = torch.randn(T, (n_q + 2 * n_kv) * D, generator=torch.Generator().manual_seed(7)).to(BF)
+    out = torch.full((T, n_q * D), float("nan"), dtype=BF, device=cuda)
+    work = torch.full((lib.prefill_attn_q4_workspace(*table.shape, n_kv, D),), 0xFF, dtype=torch.uint8, device=cuda)
+    for window in (0, 20):
+        lib.prefill_attn_q4(qkv.to(cuda), out, cache.to(cuda), table.to(cuda), torch.tensor(tiles, dtype=torch.int32, device=cuda), n_q, n_kv, D, BS,
+                            D ** -0.5, work, window=window)
+        got, at = out.cpu(), 0
+        for s, past, n in portions:
+            q = qkv[at: at + n, : n_q * D].view(n, n_q, D)
+            ref, weight, sz = attention(q, *rows[s], torch.arange(past, past + n), D ** -0.5, 0.0, window)
+            attention_close(got[at: at + n].view(n, n_q, D), ref, weight, sz, D, 2.0 ** -8, f"portion at {past}")
+            at += n
