@@ -10,6 +10,8 @@
 // Bound: fork and compact by latency (chains of a few dependent reads; a cluster of CTAs works on all rows and all pages at once, its
 // barriers between the steps), copies by the pages' bytes.  Results follow from the arguments alone: page numbers are given out in order of
 // rows and pages, counts change by atomic additions of whole numbers.
+// 24 searches of 6 beams of 50 to 900 tokens, 16 layers of 8 heads of 128: fork 10 us, its copies 18 (their bytes 15); of 5 rows 5 and 2.5.
+// 20000 pages moved: 10 us for the plan, 184 for the pages (171).
 #include "layered_common.cuh"
 #include "tcgen05.cuh"
 
@@ -379,10 +381,17 @@ __global__ void __launch_bounds__(PG_THREADS, 1) pages_compact_kernel(CompactArg
   }, [&](int e, int page) { a.table_out[e] = page; });
 }
 
-// a barrier of few warps is shorter: 256 threads where that is a page or an entry or so to each
-static int page_threads(int num_blocks, long long entries) { return num_blocks <= 1024 && entries <= 1024 ? 256 : PG_THREADS; }
-// CTAs of a cluster: one where a thread has a few pages and a few entries
-static int page_ctas(int num_blocks, long long entries) { return num_blocks <= 16384 && entries <= 16384 ? 1 : PG_CTAS; }
+// CTAs and their threads: one where a thread has a few pages and a few entries, a cluster of 8 above that; a barrier of few warps is shorter, so
+// 256 threads where there is about a page and an entry or so to each.  us for fork / compact with 1 x 256, 1 x 1024, 8 x 256, 8 x 1024:
+//   538 pages, 148 entries     5.2 / 4.1     6.0 / 4.8     7.1 / 7.2     8.4 / 8.6
+//   2304 pages, 1184 entries   7.6 / 7.7     7.3 / 6.1     8.1 / 7.4     9.9 / 9.0
+//   3008 pages, 5328 entries   14.6 / 14.8   10.3 / 8.7    9.1 / 8.1     10.6 / 9.1
+//   10432 pages, 9472 entries  23.5 / 31.3   16.3 / 17.7   11.5 / 11.1   11.4 / 10.7
+//   32432 pages, 9472 entries  30.1 / 62.4   18.0 / 36.2   13.0 / 16.0   11.5 / 13.2
+static int page_ctas(int num_blocks, long long entries) { return num_blocks <= 4096 && entries <= 2048 ? 1 : PG_CTAS; }
+static int page_threads(int num_blocks, long long entries, int ctas) {
+  return num_blocks <= 1024 * ctas && entries <= 1024 * ctas ? 256 : PG_THREADS;
+}
 constexpr long long PG_ENTRIES = 0x7fffffff - 8 * PG_CTAS * PG_THREADS;  // of a block table
 
 }  // namespace b200q
@@ -414,7 +423,7 @@ int b200q_pages_fork(const int32_t* table, const int32_t* lens, int n_old, const
   }
   const int ctas = page_ctas(num_blocks, (long long)(n_old > n_new ? n_old : n_new) * bt_stride);
   const ForkArgs a{table, lens, parents, refs, table_out, slots, (int2*)pairs, status, n_old, n_new, bt_stride, num_blocks};
-  B200Q_CUDA(launch_early(pages_fork_kernel, dim3(ctas), page_threads(num_blocks, (long long)(n_old > n_new ? n_old : n_new) * bt_stride), smem, as_stream(stream), ctas, a));
+  B200Q_CUDA(launch_early(pages_fork_kernel, dim3(ctas), page_threads(num_blocks, (long long)(n_old > n_new ? n_old : n_new) * bt_stride, ctas), smem, as_stream(stream), ctas, a));
   count_launch();
   return B200Q_OK;
 }
@@ -460,7 +469,7 @@ int b200q_pages_compact(const int32_t* table, const int32_t* lens, int n_rows, i
   B200Q_CHECK_ARG((reinterpret_cast<uintptr_t>(pairs) & 7) == 0, "pages_compact: pairs must be 8-byte aligned");
   const int ctas = page_ctas(num_blocks, (long long)n_rows * bt_stride);
   const CompactArgs a{table, lens, refs, table_out, refs_out, map, (int2*)pairs, status, bt_stride > 0 ? n_rows : 0, bt_stride, num_blocks};
-  B200Q_CUDA(launch_early(pages_compact_kernel, dim3(ctas), page_threads(num_blocks, (long long)n_rows * bt_stride), 0, as_stream(stream), ctas, a));
+  B200Q_CUDA(launch_early(pages_compact_kernel, dim3(ctas), page_threads(num_blocks, (long long)n_rows * bt_stride, ctas), 0, as_stream(stream), ctas, a));
   count_launch();
   return B200Q_OK;
 }
