@@ -40,10 +40,12 @@ __device__ __forceinline__ void turn_bf8(uint4& x1, uint4& x2, const uint4& c, c
 // Rotation of q and k (pairs i, i + D/2; a bf16 rounding behind every operation, as in elementwise.cu) and the write into 4-bit pages.
 // Items of a token: groups of 16 values of k with those they are paired with (two groups), groups of v, 8 + 8 values of q; a thread to an item,
 // so that no maximum crosses threads; rotated keys exist in registers only.
-// Bound: the rows' bytes (a cached token is 9/16 of a byte per value, a quarter of what the 16-bit write stores).
+// Bound: the rows' bytes (a cached token is 9/16 of a byte per value, a quarter of what the 16-bit write stores).  4608 / 1000 / 7 rows of 32 + 8 + 8
+// heads of 128 that lie in L2: 15.3 / 4.2 / 1.7 us (their bytes from memory 15.6 / 3.4 / 0).  48 registers keep an item's loads together: with 60 (8 blocks of 128 per SM) 16.4 /
+// 4.9 / 1.7, with 32 16.4 / 5.1 / 2.1.  CTAs that go on to the next rows, whose places are known by then: 17.4 to 20.5.
 // ------------------------------------------------------------------------------------------------------------------------
 template <int D>
-__global__ void __launch_bounds__(128, 14) rope_kvwrite_q4_kernel(uint4* qkv, const uint4* cos_sin, const int32_t* positions, const int32_t* slot_mapping,
+__global__ void __launch_bounds__(128, 10) rope_kvwrite_q4_kernel(uint4* qkv, const uint4* cos_sin, const int32_t* positions, const int32_t* slot_mapping,
                                                               uint8_t* kv_layer, int n_q, int n_kv) {
   follow_previous(qkv, cos_sin, positions, slot_mapping, kv_layer);
   constexpr int CPR = D / 8, HALF = CPR / 2;  // 16-byte pieces of a head's row, of half of it
@@ -228,8 +230,8 @@ int b200q_rope_kvwrite_q4(void* qkv, const void* cos_sin, const int32_t* positio
   B200Q_CHECK_ARG(qkv && cos_sin && positions && slot_mapping && kv4_layer, "rope_kvwrite_q4: null argument");
   B200Q_CHECK_ARG(((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(cos_sin) | reinterpret_cast<uintptr_t>(kv4_layer)) & 15) == 0,
                   "rope_kvwrite_q4: qkv, cos_sin and the cache must be 16-byte aligned");
-  // A thread to an item, in blocks of up to 128 (4608 rows of 32 + 8 + 8 heads of 128 and reading them back: 26.7 us, in blocks of 192 27.3, of
-  // 384 31.3; 512 of heads of 64 3.3 / 4.5 / 4.4)
+  // A thread to an item, in blocks of up to 128 (at 32 registers 4608 rows of 32 + 8 + 8 heads of 128 and reading them back: 26.7 us, in blocks of 192
+  // 27.3, of 384 31.3; 512 of heads of 64 3.3 / 4.5 / 4.4)
   const int items = n_kv * (D / 32) + n_kv * (D / 16) + n_q * (D / 16), blocks = (items + 127) / 128;
   const int threads = ((items + blocks - 1) / blocks + 31) / 32 * 32;
   B200Q_KV4_DIMS("rope_kvwrite_q4", D,
