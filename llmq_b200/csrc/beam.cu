@@ -9,8 +9,8 @@
 // Scores that are compared across rows are 64 bits; a row's logarithm comes from sums whose terms are off by some 2^-23 in either direction.
 // Bound: the logits, 2 bytes each, once; next to it the exponentials (16 a cycle and SM: two thirds of the memory's
 // time) and some nine instructions a logit.  Logits come by asynchronous copies two tiles ahead (in registers a tile ahead 55 us).
-// 48 groups of 8 beams over 256000 tokens, 16 candidates: 52.3 us (the memory's share 30; the first kernel 47, of which an eighth is looking for
-// the 16 best: 41 with one), one group of 4 over 128256: 10.2.
+// 48 groups of 8 beams over 256000 tokens, 16 candidates: 51.8 us (the memory's share 30; the first kernel 47, of which an eighth is looking for
+// the 16 best: 41 with one; with 4 or 3 CTAs per SM in place of 5 53.7 and 58.1), one group of 4 over 128256: 10.2.
 #include "common.cuh"
 
 namespace b200q {
@@ -128,8 +128,8 @@ __device__ __forceinline__ int next_place(int* count) {
 constexpr int BEAM_NV = 4, TILE = BEAM_NV * BEAM_THREADS, BEAM_MANY = 48, BEAM_RING = 2;
 template <bool kAligned>
 __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* logits, long long V, int K, long long row0, long long rows,
-                                                                    int2* entries, double* logs) {
-  follow_previous(logits, entries, logs);
+                                                                    int2* entries, double2* piece_sums) {
+  follow_previous(logits, entries, piece_sums);
   const int tid = threadIdx.x, piece = blockIdx.x, n_pieces = gridDim.x;
   const long long row = row0 + blockIdx.y;
   const BeamRow<kAligned> x(logits, V, row, rows);
@@ -356,8 +356,8 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
   if (tid == 0) {
     double s = 0.0;
     for (int w = 0; w < BEAM_THREADS / 32; ++w) s += sums[w];
-    // (-infinity: no logit; +infinity: one is)
-    logs[out] = fabsf(top) == INFINITY ? (double)top : log(s) + (far ? (double)top : 0.0);
+    // s e^base; base +infinity: a logit is, -infinity: there are none
+    piece_sums[out] = make_double2(far ? (double)top : 0.0, s);
   }
   int2* to = entries + out * K;
   auto tell = [&](int rank, uint64_t key) { to[rank] = make_int2(__float_as_int(value_of(key)), (int)(0xffffffffu - (uint32_t)key)); };
@@ -442,7 +442,7 @@ struct BeamArgs {
   const float* scores;
   const int32_t* stops;
   const int2* entries;
-  const double* logs;  // of a piece's sum of exponentials
+  const double2* piece_sums;  // of exponentials: y e^x
   float *cand_scores, *next_scores;
   int32_t *cand_tokens, *cand_rows, *next_tokens, *next_rows;
   int W, K, n_pieces, n_stops;
@@ -456,7 +456,7 @@ __device__ __forceinline__ uint64_t order_double(double v) {
 
 constexpr int MERGE_THREADS = 512, HEADS = 128, MERGE_KEYS = 2048, MERGE_OWN = MERGE_KEYS / MERGE_THREADS;
 __global__ void __launch_bounds__(MERGE_THREADS) beam_groups_kernel(BeamArgs a) {
-  follow_previous(a.scores, a.stops, a.entries, a.logs, a.cand_scores, a.next_scores, a.cand_tokens, a.cand_rows, a.next_tokens, a.next_rows);
+  follow_previous(a.scores, a.stops, a.entries, a.piece_sums, a.cand_scores, a.next_scores, a.cand_tokens, a.cand_rows, a.next_tokens, a.next_rows);
   const int tid = threadIdx.x, W = a.W, K = a.K;
   const long long group = blockIdx.x, row0 = group * W;
   const int lists = W * a.n_pieces, n = lists * K;
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) beam_groups_kernel(BeamArgs a) 
   __shared__ double out_t[BEAM_MOST_K];
   __shared__ int out_token[BEAM_MOST_K], out_row[BEAM_MOST_K];
   const int2* entries = a.entries + row0 * a.n_pieces * K;
-  const double* logs = a.logs + row0 * a.n_pieces;
+  const double2* piece_sums = a.piece_sums + row0 * a.n_pieces;
   const bool held = n <= MERGE_KEYS;  // every thread has its entries, asked for before the rows' logarithms are known
   int2 mine[MERGE_OWN];
 #pragma unroll
@@ -479,13 +479,18 @@ __global__ void __launch_bounds__(MERGE_THREADS) beam_groups_kernel(BeamArgs a) 
   for (int w = tid >> 5; w < W; w += MERGE_THREADS / 32) {
     const int lane = tid & 31;
     const double s = (double)a.scores[row0 + w];
-    double top = -INFINITY;
-    for (int p = lane; p < a.n_pieces; p += 32) top = fmax(top, logs[w * a.n_pieces + p]);
+    // (up to 64 pieces are read once)
+    const double2 none = make_double2(-INFINITY, 0.0);
+    const double2 p0 = lane < a.n_pieces ? piece_sums[w * a.n_pieces + lane] : none,
+                  p1 = lane + 32 < a.n_pieces ? piece_sums[w * a.n_pieces + lane + 32] : none;
+    double top = fmax(p0.x, p1.x);
+    for (int p = lane + 64; p < a.n_pieces; p += 32) top = fmax(top, piece_sums[w * a.n_pieces + p].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
     const bool finite = top > -INFINITY && top < INFINITY;
-    double sum = 0.0;
-    for (int p = lane; p < a.n_pieces && finite; p += 32) sum += exp(logs[w * a.n_pieces + p] - top);
+    auto part = [&](double2 v) { return v.x == top ? v.y : v.x > -INFINITY ? v.y * exp(v.x - top) : 0.0; };  // (mostly the same base: 0)
+    double sum = finite ? part(p0) + part(p1) : 0.0;
+    for (int p = lane + 64; p < a.n_pieces && finite; p += 32) sum += part(piece_sums[w * a.n_pieces + p]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) shift[w] = finite && s > -INFINITY && s < INFINITY ? s - (top + log(sum)) : -INFINITY;
@@ -664,7 +669,7 @@ int64_t b200q_beam_select_workspace(int groups, int beams, int64_t V, int K) {
     return B200Q_EINVAL;
   }
   const int64_t pieces = (int64_t)groups * beams * beam_pieces((int64_t)groups * beams, V);
-  return pieces * (int64_t)(sizeof(double) + K * sizeof(int2));
+  return pieces * (int64_t)(sizeof(double2) + K * sizeof(int2));
 }
 
 int b200q_beam_select(const void* logits, const float* scores, int groups, int beams, int64_t V, const int32_t* stops, int n_stops, int K,
@@ -684,16 +689,16 @@ int b200q_beam_select(const void* logits, const float* scores, int groups, int b
   B200Q_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && (reinterpret_cast<uintptr_t>(logits) & 15) == 0,
                   "beam_select: logits and workspace must be 16-byte aligned");
   const int pieces = beam_pieces(rows, V);
-  double* logs = (double*)workspace;
-  int2* entries = (int2*)(logs + rows * pieces);
+  double2* piece_sums = (double2*)workspace;
+  int2* entries = (int2*)(piece_sums + rows * pieces);
   cudaStream_t st = as_stream(stream);
   for (int64_t r0 = 0; r0 < rows; r0 += 65535) {  // (a grid's second dimension ends there)
     const unsigned n = (unsigned)(rows - r0 < 65535 ? rows - r0 : 65535);
     auto kern = V % 8 ? beam_rows_kernel<false> : beam_rows_kernel<true>;
-    B200Q_CUDA(launch_early(kern, dim3(pieces, n), BEAM_THREADS, V % 8 ? 0 : BEAM_RING * TILE * 16, st, 1, (const bf16*)logits, (long long)V, K, (long long)r0, (long long)rows, entries, logs));
+    B200Q_CUDA(launch_early(kern, dim3(pieces, n), BEAM_THREADS, V % 8 ? 0 : BEAM_RING * TILE * 16, st, 1, (const bf16*)logits, (long long)V, K, (long long)r0, (long long)rows, entries, piece_sums));
     count_launch();
   }
-  const BeamArgs a{scores, stops, entries, logs, cand_scores, next_scores, cand_tokens, cand_rows, next_tokens, next_rows, beams, K, pieces, n_stops,
+  const BeamArgs a{scores, stops, entries, piece_sums, cand_scores, next_scores, cand_tokens, cand_rows, next_tokens, next_rows, beams, K, pieces, n_stops,
                    (long long)V};
   B200Q_CUDA(launch_early(beam_groups_kernel, dim3(groups), MERGE_THREADS, 0, st, 1, a));
   count_launch();
