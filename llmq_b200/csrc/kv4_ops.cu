@@ -99,69 +99,73 @@ __global__ void __launch_bounds__(128, 10) rope_kvwrite_q4_kernel(uint4* qkv, co
 // ------------------------------------------------------------------------------------------------------------------------
 // 4-bit pages as 16-bit ones (the layout of attn.cu: [2][n_kv][16][D], the 16-byte piece c of a row at c ^ (token & 7)).  Exact.
 // ------------------------------------------------------------------------------------------------------------------------
-// One head's page by a warp, through its own place in shared memory (the page's bytes, 16 a lane): then an item is 8 values, 16 bytes out, and a
-// warp's stores are whole rows.
+// Keys or values of one head's page by a warp, through its own place in shared memory (their bytes, 16 a lane): then an item is 8 values, 16 bytes
+// out, and a warp's stores are whole rows.
 template <int D>
-__device__ __forceinline__ void kv4_spread_head(const uint8_t* head, uint4* keys, uint4* values, uint8_t* stage, int lane) {
-  constexpr int CPR = D / 8, PIECES = Kv4<D>::BYTES / 16;
+constexpr int SPREAD_BYTES = Kv4<D>::BYTES / 2;
+template <int D, bool kValue>
+__device__ __forceinline__ void kv4_spread_half(const uint8_t* half, uint4* out, uint8_t* stage, int lane) {
+  constexpr int CPR = D / 8, PIECES = SPREAD_BYTES<D> / 16, FROM = kValue ? SPREAD_BYTES<D> : 0;
   __syncwarp();
   uint4 v[(PIECES + 31) / 32];
 #pragma unroll
   for (int i = 0; i < (PIECES + 31) / 32; ++i)
-    if (i * 32 + lane < PIECES) v[i] = ld_once_v4(head + (i * 32 + lane) * 16);
+    if (i * 32 + lane < PIECES) v[i] = ld_once_v4(half + (i * 32 + lane) * 16);
 #pragma unroll
   for (int i = 0; i < (PIECES + 31) / 32; ++i)
     if (i * 32 + lane < PIECES) st_v4(stage + (i * 32 + lane) * 16, v[i]);
   __syncwarp();
-  auto part = [&](auto is_value) {
-    constexpr bool kValue = decltype(is_value)::value;
-    uint4* out = kValue ? values : keys;
 #pragma unroll 4
-    for (int it = lane; it < 16 * CPR; it += 32) {
-      const int token = it / CPR, c = it % CPR, p = c >> 1, r = kv4_key_row<D>(token);
-      const uint32_t codes = *reinterpret_cast<const uint32_t*>(stage + (kValue ? kv4_value_code<D>(token, p) : kv4_key_code<D>(r, p)) + (c & 1) * 4);
-      const uint32_t b = stage[kValue ? kv4_value_scale<D>(token, p) : kv4_key_scale<D>(r, p)];
-      uint32_t h[4];
-      kv4_halves(codes, h);
-      const float s = kv4_scale_value(b);
-      uint32_t w[4];
+  for (int it = lane; it < 16 * CPR; it += 32) {
+    const int token = it / CPR, c = it % CPR, p = c >> 1, r = kv4_key_row<D>(token);
+    const uint32_t codes = *reinterpret_cast<const uint32_t*>(stage + (kValue ? kv4_value_code<D>(token, p) : kv4_key_code<D>(r, p)) - FROM + (c & 1) * 4);
+    const uint32_t b = stage[(kValue ? kv4_value_scale<D>(token, p) : kv4_key_scale<D>(r, p)) - FROM];
+    uint32_t h[4];
+    kv4_halves(codes, h);
+    const float s = kv4_scale_value(b);
+    uint32_t w[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
-        w[i] = pack_bf16x2(f.x * s, f.y * s);
-      }
-      st_v4(out + token * CPR + (c ^ (token & 7)), make_uint4(w[0], w[1], w[2], w[3]));
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+      w[i] = pack_bf16x2(f.x * s, f.y * s);
     }
-  };
-  part(std::false_type{});
-  part(std::true_type{});
+    st_v4(out + token * CPR + (c ^ (token & 7)), make_uint4(w[0], w[1], w[2], w[3]));
+  }
+}
+// keys (which = 0) or values of head h of page `from` to page `to`
+template <int D>
+__device__ __forceinline__ void kv4_spread_part(const uint8_t* kv4, long long from, uint4* out, long long to, int n_kv, int h, int which, uint8_t* stage, int lane) {
+  const uint8_t* half = kv4 + (from * n_kv + h) * Kv4<D>::BYTES + which * SPREAD_BYTES<D>;
+  uint4* at = out + ((to * 2 + which) * n_kv + h) * (16 * D / 8);
+  if (which)
+    kv4_spread_half<D, true>(half, at, stage, lane);
+  else
+    kv4_spread_half<D, false>(half, at, stage, lane);
 }
 
 constexpr int SPREAD_WARPS = 8;
 template <int D>
 __global__ void __launch_bounds__(SPREAD_WARPS * 32) kv4_unpack_kernel(const uint8_t* kv4, const int32_t* pages, int n_pages, uint4* out, int n_kv) {
   follow_previous(kv4, pages, out);
-  __shared__ __align__(16) uint8_t stage[SPREAD_WARPS][Kv4<D>::BYTES];
+  __shared__ __align__(16) uint8_t stage[SPREAD_WARPS][SPREAD_BYTES<D>];
   const int warp = threadIdx.x >> 5;
-  const long long items = (long long)n_pages * n_kv;
+  const long long items = 2LL * n_pages * n_kv;
   for (long long it = (long long)blockIdx.x * SPREAD_WARPS + warp; it < items; it += (long long)gridDim.x * SPREAD_WARPS) {
-    const long long i = it / n_kv;
-    const int h = (int)(it - i * n_kv);
-    constexpr int ROWS = 16 * D / 8;
-    uint4* keys = out + ((i * 2) * n_kv + h) * ROWS;
-    kv4_spread_head<D>(kv4 + ((long long)pages[i] * n_kv + h) * Kv4<D>::BYTES, keys, keys + (long long)n_kv * ROWS, stage[warp], threadIdx.x & 31);
+    const long long i = it / (2 * n_kv);
+    const int part = (int)(it - i * (2 * n_kv));
+    kv4_spread_part<D>(kv4, pages[i], out, i, n_kv, part >> 1, part & 1, stage[warp], threadIdx.x & 31);
   }
 }
 
 // The pages that a step's portions see, spread out to a workspace in which column c of row r of the block table is page r * bt_stride + c.
-// A warp has one head of one page; what a row needs it finds from the tiles (their first visible and their last key).
+// A warp has the keys or the values of one head of one page; what a row needs it finds from the tiles (their first visible and their last key).
 template <int D>
 __global__ void __launch_bounds__(SPREAD_WARPS * 32) kv4_spread_kernel(const uint8_t* kv4, const int32_t* block_table, int bt_stride, const int4* tiles,
                                                                        int n_tiles, int n_kv, int window, uint4* out, int32_t* table) {
   follow_previous(kv4, block_table, tiles, out, table);
-  __shared__ __align__(16) uint8_t stage[SPREAD_WARPS][Kv4<D>::BYTES];
+  __shared__ __align__(16) uint8_t stage[SPREAD_WARPS][SPREAD_BYTES<D>];
   const int row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int c = (blockIdx.x * SPREAD_WARPS + warp) / n_kv, h = (blockIdx.x * SPREAD_WARPS + warp) % n_kv;
+  const int c = (blockIdx.x * SPREAD_WARPS + warp) / (2 * n_kv), part = (blockIdx.x * SPREAD_WARPS + warp) % (2 * n_kv);
   int lo = 0x7fffffff, hi = 0;
   for (int i = threadIdx.x; i < n_tiles; i += blockDim.x) {
     const int4 t = tiles[i];
@@ -186,10 +190,8 @@ __global__ void __launch_bounds__(SPREAD_WARPS * 32) kv4_spread_kernel(const uin
   // (where a portion follows another of the same row, both are in [lo, hi))
   if (c < s_lo / 16 || c >= min((s_hi + 15) / 16, bt_stride)) return;
   const long long to = (long long)row * bt_stride + c;
-  constexpr int ROWS = 16 * D / 8;
-  uint4* keys = out + ((to * 2) * n_kv + h) * ROWS;
-  kv4_spread_head<D>(kv4 + ((long long)block_table[to] * n_kv + h) * Kv4<D>::BYTES, keys, keys + (long long)n_kv * ROWS, stage[warp], lane);
-  if (h == 0 && lane == 0) table[to] = (int32_t)to;
+  kv4_spread_part<D>(kv4, block_table[to], out, to, n_kv, part >> 1, part & 1, stage[warp], lane);
+  if (part == 0 && lane == 0) table[to] = (int32_t)to;
 }
 
 static inline int64_t spread_pages_bytes(int64_t pages, int n_kv, int D) { return pages * (4LL * n_kv * 16 * D); }
@@ -247,7 +249,7 @@ int b200q_kv4_unpack(const void* kv4_layer, const int32_t* pages, int n_pages, v
   if (n_pages == 0) return B200Q_OK;
   B200Q_CHECK_ARG(kv4_layer && pages && kv_out, "kv4_unpack: null argument");
   B200Q_CHECK_ARG(((reinterpret_cast<uintptr_t>(kv4_layer) | reinterpret_cast<uintptr_t>(kv_out)) & 15) == 0, "kv4_unpack: caches must be 16-byte aligned");
-  const long long items = (long long)n_pages * n_kv, blocks = (items + SPREAD_WARPS - 1) / SPREAD_WARPS;
+  const long long items = 2LL * n_pages * n_kv, blocks = (items + SPREAD_WARPS - 1) / SPREAD_WARPS;
   B200Q_KV4_DIMS("kv4_unpack", D,
                  B200Q_CUDA(launch_early(kv4_unpack_kernel<kD>, dim3((unsigned)(blocks < 1 << 20 ? blocks : 1 << 20)), SPREAD_WARPS * 32, 0, as_stream(stream), 1,
                                          (const uint8_t*)kv4_layer, pages, n_pages, (uint4*)kv_out, n_kv)));
@@ -283,7 +285,7 @@ int b200q_prefill_attn_q4(const void* q, int q_stride, void* out, const void* kv
   const int64_t pages = (int64_t)n_seqs * bt_stride;
   int32_t* table = (int32_t*)((uint8_t*)workspace + spread_pages_bytes(pages, n_kv, D));
   B200Q_KV4_DIMS("prefill_attn_q4", D,
-                 B200Q_CUDA(launch_early(kv4_spread_kernel<kD>, dim3((unsigned)(((int64_t)bt_stride * n_kv + SPREAD_WARPS - 1) / SPREAD_WARPS), n_seqs), SPREAD_WARPS * 32, 0, as_stream(stream),
+                 B200Q_CUDA(launch_early(kv4_spread_kernel<kD>, dim3((unsigned)((2LL * bt_stride * n_kv + SPREAD_WARPS - 1) / SPREAD_WARPS), n_seqs), SPREAD_WARPS * 32, 0, as_stream(stream),
                                          1, (const uint8_t*)kv4_layer, block_table, bt_stride, (const int4*)tiles, n_tiles, n_kv, window,
                                          (uint4*)workspace, table)));
   count_launch();
