@@ -15,6 +15,8 @@
 
 namespace b200q {
 
+bool batch_invariant();
+
 constexpr int BEAM_THREADS = 256, BEAM_MOST_K = 64, BEAM_MOST_W = 32, BEAM_FOUND = 512, BEAM_VECTORS = 256;
 
 __device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
@@ -642,7 +644,9 @@ __global__ void __launch_bounds__(MERGE_THREADS) beam_groups_kernel(BeamArgs a) 
 // Pieces of a row: the least time of the SM that has most CTAs, each its logits (five CTAs at once are as fast as an SM gets) and 11000 logits'
 // worth beside them, and of the lists that the second kernel has to look at.  384 rows of 256000 logits: 1 / 2 / 3 / 4 / 6 / 8 pieces 69.0 /
 // 53.7 / 52.3 / 55.1 / 64.7 / 65.6 us; 4 rows of 128256: 8 / 16 / 32 / 48 / 64 pieces 10.4 / 9.9 / 10.1 / 11.1 / 11.9 us.
+// B200Q_BATCH_INVARIANT=1: as for 64 rows whatever their number, since a row's sum is that of its pieces' sums.
 static int beam_pieces(long long rows, long long V) {
+  if (batch_invariant()) rows = 64;
   int best = 1;
   double least = 1e30;
   for (int p = 1; p <= 256 && (p == 1 || V / p >= 2048); ++p) {

@@ -98,6 +98,23 @@ def test_logits_in_order(cuda, V, W, K):
     check(lib, cuda, x, scores, W, K, [])
 
 
+def test_whatever_the_batch(cuda):
+    """in the batch-invariant mode a group's scores are the same bits alone and beside others"""
+    from llmq_b200 import lib
+    g = torch.Generator().manual_seed(5)
+    W, K, V = 4, 8, 50257
+    logits, scores = (2.5 * torch.randn(90 * W, V, generator=g)).to(BF), -torch.rand(90 * W, generator=g)
+    lib.load().b200q_gemm_set_splitk(1)   # (stands for B200Q_BATCH_INVARIANT)
+    try:
+        many = select(lib, cuda, logits, scores, W, K, [])
+        for b in (0, 57, 89):
+            alone = select(lib, cuda, logits[b * W: (b + 1) * W], scores[b * W: (b + 1) * W], W, K, [])
+            for x, y in zip(many, alone):
+                assert torch.equal(x[0][b], y[0][0]) and torch.equal(x[1][b], y[1][0]) and torch.equal(x[2][b] - b * W, y[2][0])
+    finally:
+        lib.load().b200q_gemm_set_splitk(0)
+
+
 def test_many_groups(cuda):
     from llmq_b200 import lib
     g = torch.Generator().manual_seed(1)
