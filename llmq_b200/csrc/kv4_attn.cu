@@ -721,7 +721,7 @@ static int launch_kv4_stream(const Kv4Args& a, cudaStream_t st) {
   const int ctas = C::CTAS * num_sms(), warps = ctas * C::WARPS;
   // Items of up to 8 pages go to warps whole: adding up pieces costs as much as they do (one sequence of 64 tokens, 8 kv heads, 5.6 us, in
   // pieces 9.5; 2800 of 128 tokens 96.5, in pieces 103.9).
-  const int width = a.window > 0 && (a.window + 15) / 16 + 1 < a.bt_stride ? (a.window + 15) / 16 + 1 : a.bt_stride;
+  const int width = a.window > 0 && a.window / 16 + 2 < a.bt_stride ? a.window / 16 + 2 : a.bt_stride;  // pages of an item at most
   bool whole = g_q4_whole < 0 ? batch_invariant() || width <= 8 : g_q4_whole != 0;
   float* scratch = nullptr;
   // (where there is no memory for pieces, items go to warps whole)

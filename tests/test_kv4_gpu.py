@@ -258,6 +258,23 @@ def test_captured_and_on_another_stream(cuda):
             assert torch.equal(a[name].view(torch.uint8), b[name].view(torch.uint8)), name
 
 
+@pytest.mark.parametrize("window", [-1, 2 ** 31 - 1, 5000, 4999])
+def test_wide_windows(cuda, window):
+    """windows that hide nothing, or one key"""
+    from llmq_b200 import lib
+    D, n_q, n_kv, ctxs = 128, 4, 1, [5000, 3, 0]
+    cache, table, rows = make_cache(ctxs, n_kv, D, seed=8)
+    qkv = torch.randn(3, (n_q + 2 * n_kv) * D, generator=torch.Generator().manual_seed(7)).to(BF)
+    out = torch.full((3, n_q * D), float("nan"), dtype=BF, device=cuda)
+    lib.decode_attn_q4(qkv.to(cuda), out, cache.to(cuda), table.to(cuda), torch.tensor(ctxs, dtype=torch.int32, device=cuda), n_q, n_kv, D, BS, D ** -0.5,
+                       window=window)
+    got = out.cpu()
+    assert (got[2] == 0).all()
+    for i in (0, 1):
+        ref, weight, size = attention(qkv[i: i + 1, : n_q * D].view(1, n_q, D), *rows[i], torch.tensor([ctxs[i] - 1]), D ** -0.5, 0.0, max(window, 0))
+        attention_close(got[i].view(1, n_q, D), ref, weight, size, D, 2.0 ** -11)
+
+
 @pytest.mark.parametrize("D,n_q,n_kv", [(64, 8, 2), (256, 4, 1)])
 def test_two_calls_at_once(cuda, D, n_q, n_kv):
     """long contexts, whose pieces lie in scratch: two threads on streams of their own, then two graphs replayed side by side, each time
