@@ -716,7 +716,8 @@ int b200q_pages_copy(void* kv_dev, const int32_t* pairs_dev, int n_pairs, const 
 int b200q_pages_compact(const int32_t* table_dev, const int32_t* lens_dev, int n_rows, int bt_stride, const int32_t* refs_dev,
                         int num_blocks, int block_size, int32_t* table_out_dev, int32_t* refs_out_dev, int32_t* map_dev,
                         int32_t* pairs_dev, int32_t* status_dev, void* stream);
-/* test hook: b200q_decode_attn_q4 gives a sequence's heads to warps whole (1), or pages evenly (0); -1: as B200Q_BATCH_INVARIANT says */
+/* test hook: b200q_decode_attn_q4 gives a sequence's heads to warps whole (1), pages evenly (0), or heads to clusters (-2, where they are few);
+ *     -1: by size, and as B200Q_BATCH_INVARIANT says */
 int b200q_decode_attn_q4_set_whole(int whole);
 
 /* nonzero once a kernel's bounded wait has run out in this process (its outputs are then missing or wrong); engine steps report

@@ -111,7 +111,8 @@ template <int D>
 struct Q4Query {
   uint32_t b[D / 16][2];
   float c[2];  // c0 times what heads 2 t, 2 t + 1 were divided by
-  __device__ __forceinline__ void load(uint32_t rows, int G, float c0, int lane) {  // [G][D] in shared memory
+  template <typename F>
+  __device__ __forceinline__ void load(F&& values, int G, float c0, int lane) {  // (values i .. i + 7 of the group's [G][D])
     const int g = lane >> 2, t = lane & 3;
     constexpr int PART = D == 256 ? 32 : D / 4, PARTS = D == 256 ? 2 : 1;  // consecutive values
     float x[PARTS][PART];
@@ -120,7 +121,7 @@ struct Q4Query {
     for (int h = 0; h < PARTS; ++h)
 #pragma unroll
       for (int i = 0; i < PART / 8; ++i) {
-        const uint4 v = g < G ? lds_v4(rows + (g * D + h * 128 + t * PART + i * 8) * 2) : make_uint4(0, 0, 0, 0);
+        const uint4 v = g < G ? values(g * D + h * 128 + t * PART + i * 8) : make_uint4(0, 0, 0, 0);
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -574,7 +575,7 @@ __global__ void __launch_bounds__(Q4Stream<D>::WARPS * 32, Q4Stream<D>::CTAS) kv
       __syncwarp();
       const uint32_t at = ring + stage * stage_bytes;
       if (first_turn) {
-        q.load(at + C::TURN, a.G, a.c0, lane);
+        q.load([&](int i) { return lds_v4(at + C::TURN + 2 * i); }, a.G, a.c0, lane);
         st.clear();
       }
       if (page >= inner && page <= outer) {
@@ -704,8 +705,168 @@ __global__ void __launch_bounds__(4 * Q4_JOIN) kv4_join_kernel(const float* scra
   }
 }
 
-int g_q4_whole = -1;  // test hook: 1 / 0 give items to warps whole or not (-1: as B200Q_BATCH_INVARIANT says)
+// ------------------------------------------------------------------------------------------------------------------------
+// Few sequences: a cluster of CTAs to a sequence and head, each warp of it with every n-th page; no lists to make before the first page can be
+// asked for and no second kernel, but whatever the lengths, every sequence gets the same warps.
+// ------------------------------------------------------------------------------------------------------------------------
+constexpr int Q4_MOST_CTAS = 16;
+template <int D>
+struct Q4Cluster {
+  static constexpr int WARPS = 4, STAGES = 3, CTAS = Q4Stream<D>::CTAS, TURN = Q4Cfg<D>::TURN, RING = STAGES * TURN, SMEM = WARPS * RING;
+  static_assert((8 * D + 32) * 4 <= RING, "a warp's outputs, maxima and sums");
+};
+template <int D, bool kCap>
+__global__ void __launch_bounds__(Q4Cluster<D>::WARPS * 32, Q4Cluster<D>::CTAS) kv4_cluster_kernel(Kv4Args a) {
+  follow_previous(a.q, a.out, a.kv, a.block_table, a.ctx_lens);
+  using C = Q4Cluster<D>;
+  constexpr int P = Q4Cfg<D>::PAGES, STAGES = C::STAGES, WARPS = C::WARPS, PIECES = Kv4<D>::BYTES / 16;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int splits = gridDim.x, split = blockIdx.x, seq = blockIdx.y, kvh = blockIdx.z;
+  const uint32_t ring = smem_u32(smem + warp * C::RING);
+  // pages wg, wg + n_warps, ... of those that hold visible keys
+  const int wg = split * WARPS + warp, n_warps = splits * WARPS;
+  const Q4Span f(a, a.ctx_lens[seq]);
+  const int n = f.pages > wg ? (f.pages - wg + n_warps - 1) / n_warps : 0, turns = (n + P - 1) / P;
+  const int32_t* row = a.block_table + (long long)seq * a.bt_stride + f.page0 + wg;
+  const uint8_t* kv = a.kv + (long long)kvh * Kv4<D>::BYTES + lane * 16;
+  const long long page_stride = (long long)a.n_kv * Kv4<D>::BYTES;
+  int ids_at = 0, ids = lane < n ? row[n_warps * lane] : 0;  // numbers of 32 pages
+  auto fetch = [&](int k) {
+    if (k < turns) {
+      const int k0 = k * P, count = min(P, n - k0);
+      if (k0 - ids_at >= 32) {
+        ids_at += 32;
+        ids = ids_at + lane < n ? row[n_warps * (ids_at + lane)] : 0;
+      }
+      const uint8_t* from[P];
+#pragma unroll
+      for (int x = 0; x < P; ++x) from[x] = kv + (long long)__shfl_sync(0xffffffffu, ids, k0 - ids_at + x) * page_stride;
+      const uint32_t to = ring + k % STAGES * C::TURN + lane * 16;
+#pragma unroll
+      for (int i = 0; i < C::TURN / 512; ++i) {
+        const int x0 = 32 * i / PIECES, x1 = (32 * i + 31) / PIECES;  // the pages in which a copy's lanes lie
+        const bool second = x0 != x1 && lane >= x1 * PIECES - 32 * i;
+        const uint8_t* src = second ? from[x1] + 16 * (32 * i - x1 * PIECES) : from[x0] + 16 * (32 * i - x0 * PIECES);
+        if ((second ? x1 : x0) < count) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 512 * i), "l"(src) : "memory");
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int k = 0; k < STAGES; ++k) fetch(k);
+  Q4Query<D> q;
+  const bf16* q_rows = a.q + (long long)seq * a.q_stride + (long long)kvh * a.G * D;
+  q.load([&](int i) { return ld_v4(q_rows + i); }, a.G, a.c0, lane);
+  Q4State<D> st;
+  st.clear();
+  for (int k = 0; k < turns; ++k) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+    __syncwarp();
+    const uint32_t at = ring + k % STAGES * C::TURN;
+    int first[P];
+#pragma unroll
+    for (int x = 0; x < P; ++x) first[x] = (f.page0 + wg + n_warps * (k * P + x)) * 16;
+    if (first[0] < f.lo || first[P - 1] + 16 > f.ctx)
+      q4_turn<D, kCap, true>(at, q, st, a.c1, first, f.lo, f.ctx, lane);
+    else
+      q4_turn<D, kCap, false>(at, q, st, a.c1, nullptr, 0, 0, lane);
+    __syncwarp();
+    fetch(k + STAGES);
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncwarp();
+  // ---- this warp's state into its ring: [head][D] | maxima [8] | sums [8]
+  float* mine = reinterpret_cast<float*>(smem + warp * C::RING);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    st.l[i] += __shfl_xor_sync(0xffffffffu, st.l[i], 4);
+    st.l[i] += __shfl_xor_sync(0xffffffffu, st.l[i], 8);
+    st.l[i] += __shfl_xor_sync(0xffffffffu, st.l[i], 16);
+    const int head = 2 * t + i;
+    if (head < a.G) {
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) *reinterpret_cast<float2*>(mine + head * D + g * (D / 8) + 2 * k) = make_float2(st.o[k][i], st.o[k][2 + i]);
+      if (g == 0) {
+        mine[8 * D + head] = st.m[i];
+        mine[8 * D + 8 + head] = st.l[i];
+      }
+    }
+  }
+  __syncthreads();
+  // ---- one state per CTA, in the first warp's place (an item is two values, which one thread reads and writes)
+  constexpr int RING_F = C::RING / 4;
+  float* all = reinterpret_cast<float*>(smem);
+  bf16* out = a.out + ((long long)seq * a.n_q + (long long)kvh * a.G) * D;
+  auto write = [&](int i, float2 num, float den) {
+    const float inv = den > 0.f ? 1.f / den : den;  // (NaN stays)
+    *reinterpret_cast<uint32_t*>(out + i) = pack_bf16x2(num.x * inv, num.y * inv);
+  };
+  for (int i = threadIdx.x * 2; i < a.G * D; i += WARPS * 64) {
+    const int r = i / D;
+    float M = -INFINITY, den = 0.f;
+    float2 num = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int x = 0; x < WARPS; ++x) M = fmaxf(M, all[x * RING_F + 8 * D + r]);
+#pragma unroll
+    for (int x = 0; x < WARPS; ++x) {
+      const float m = all[x * RING_F + 8 * D + r], l = all[x * RING_F + 8 * D + 8 + r];
+      const float weight = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : q4_ex2(m - M);  // (no maximum and a sum: NaN)
+      const float2 v = *reinterpret_cast<const float2*>(all + x * RING_F + i);
+      num.x += weight * v.x;
+      num.y += weight * v.y;
+      den += weight * l;
+    }
+    if (splits > 1) {
+      *reinterpret_cast<float2*>(all + i) = num;
+      if (i % D == 0) {  // (the first warp's maxima and sums are still read: these go behind them)
+        all[8 * D + 16 + r] = M;
+        all[8 * D + 24 + r] = den;
+      }
+    } else {
+      write(i, num, den);
+    }
+  }
+  if (splits > 1) {
+    cluster_sync_all();
+    const int per = (a.G * D / 2 + splits - 1) / splits * 2;
+    for (int i = split * per + threadIdx.x * 2; i < min((split + 1) * per, a.G * D); i += WARPS * 64) {
+      const int r = i / D;
+      float M = -INFINITY, den = 0.f;
+      float2 num = make_float2(0.f, 0.f);
+      for (int x = 0; x < splits; ++x) M = fmaxf(M, ld_cluster_f32(mapa_shared(all + 8 * D + 16 + r, x)));
+      for (int x = 0; x < splits; ++x) {
+        const float m = ld_cluster_f32(mapa_shared(all + 8 * D + 16 + r, x)), l = ld_cluster_f32(mapa_shared(all + 8 * D + 24 + r, x));
+        const float weight = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : q4_ex2(m - M);
+        const uint32_t from = mapa_shared(all + i, x);
+        num.x += weight * ld_cluster_f32(from);
+        num.y += weight * ld_cluster_f32(from + 4);
+        den += weight * l;
+      }
+      write(i, num, den);
+    }
+    cluster_sync_all();  // nobody leaves while a peer still reads
+  }
+}
+
+int g_q4_whole = -1;  // test hook: 1 / 0 give items to warps whole or not, -2 to clusters (-1: by size, and as B200Q_BATCH_INVARIANT says)
 static std::mutex g_q4_pair;  // no other thread's pieces on the same stream between a stream kernel and its join
+
+// CTAs of a cluster for each of these items of up to `pages` pages, or 0: the kernel above.  Times in us, measured at 1 to 48 sequences of 300 to
+// 16000 tokens, 8 heads: clusters 4 and what a CTA's pages take (16 CTAs to a cluster 2.5 more); the kernel above `start` and `slope` times what all
+// pages take from memory.  us above / with clusters, D = 128: one sequence of 300 tokens 10.2 / 5.5, 16 of 1000 14.5 / 9.2, 16 of 4000 25 / 22.9,
+// 24 of 4000 32.9 / 36.1; D = 256: 6 of 4000 22.8 / 19.1, 8 of 4000 26.3 / 32.2.  Lengths below the table's width: 48 of 200 to 2000 23.8 / 30.2.
+template <int D>
+static int kv4_clusters(long long items, int pages, bool forced) {
+  constexpr double page = D == 64 ? 0.15 : D == 128 ? 0.27 : 0.44, start = D == 64 ? 9.5 : D == 128 ? 10.0 : 14.0,
+                   slope = D == 64 ? 1.5 : D == 128 ? 1.33 : 1.05;
+  const long long places = (long long)num_sms() * Q4Cluster<D>::CTAS;
+  if (items > places) return 0;
+  int n = 1;  // (clusters of 16 leave places that none fits into: where they fill two thirds)
+  while (n < Q4_MOST_CTAS && items * n * 2 <= (n == 8 ? places * 13 / 20 : places) && pages >= 2 * n * Q4Cluster<D>::WARPS * Q4Cfg<D>::PAGES) n *= 2;
+  const double all = (double)items * pages * Kv4<D>::BYTES / 6.45e6;
+  return forced || 4.0 + page * pages / n + (n == 16 ? 2.5 : 0.0) < (pages <= 8 ? 5.5 : start) + slope * all ? n : 0;
+}
 
 template <int D, bool kCap>
 static int launch_kv4_stream(const Kv4Args& a, cudaStream_t st) {
@@ -716,12 +877,20 @@ static int launch_kv4_stream(const Kv4Args& a, cudaStream_t st) {
   B200Q_CUDA(cudaGetDevice(&dev));
   if (dev >= 64 || !ready[dev]) {
     B200Q_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem(8)));
+    B200Q_CUDA(cudaFuncSetAttribute(kv4_cluster_kernel<D, kCap>, cudaFuncAttributeMaxDynamicSharedMemorySize, Q4Cluster<D>::SMEM));
+    B200Q_CUDA(cudaFuncSetAttribute(kv4_cluster_kernel<D, kCap>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     if (dev < 64) ready[dev] = true;
   }
   const int ctas = C::CTAS * num_sms(), warps = ctas * C::WARPS;
   // Items of up to 8 pages go to warps whole: adding up pieces costs as much as they do (one sequence of 64 tokens, 8 kv heads, 5.6 us, in
   // pieces 9.5; 2800 of 128 tokens 96.5, in pieces 103.9).
   const int width = a.window > 0 && a.window / 16 + 2 < a.bt_stride ? a.window / 16 + 2 : a.bt_stride;  // pages of an item at most
+  if (g_q4_whole == -2 || (g_q4_whole == -1 && !batch_invariant()))
+    if (const int n = kv4_clusters<D>((long long)a.n_seqs * a.n_kv, width, g_q4_whole == -2)) {
+      B200Q_CUDA(launch_early(kv4_cluster_kernel<D, kCap>, dim3(n, a.n_seqs, a.n_kv), Q4Cluster<D>::WARPS * 32, Q4Cluster<D>::SMEM, st, n, a));
+      count_launch();
+      return B200Q_OK;
+    }
   bool whole = g_q4_whole < 0 ? batch_invariant() || width <= 8 : g_q4_whole != 0;
   float* scratch = nullptr;
   // (where there is no memory for pieces, items go to warps whole)
@@ -745,7 +914,7 @@ using namespace b200q;
 extern "C" {
 
 int b200q_decode_attn_q4_set_whole(int whole) {
-  B200Q_CHECK_ARG(whole >= -1 && whole <= 1, "decode_attn_q4: whole must be -1..1");
+  B200Q_CHECK_ARG(whole >= -2 && whole <= 1, "decode_attn_q4: whole must be -2..1");
   g_q4_whole = whole;
   bump_tuning_epoch();
   return B200Q_OK;

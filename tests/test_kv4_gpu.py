@@ -349,3 +349,48 @@ def test_portions_of_one_sequence(cuda):
             ref, weight, sz = attention(q, *rows[s], torch.arange(past, past + n), D ** -0.5, 0.0, window)
             attention_close(got[at: at + n].view(n, n_q, D), ref, weight, sz, D, 2.0 ** -8, f"portion at {past}")
             at += n
+
+
+@pytest.mark.parametrize("D,n_q,n_kv", [(64, 8, 2), (64, 7, 1), (128, 8, 8), (128, 8, 1), (128, 6, 2), (256, 8, 2), (256, 8, 1)])
+@pytest.mark.parametrize("ctxs", CASES + [[300, 0, 5000], [7001]], ids=lambda c: f"{len(c)}x{max(c)}")
+@pytest.mark.parametrize("cap,window", [(0.0, 0), (20.0, 100), (0.0, 1), (0.0, 3000)])
+def test_decode_clusters(cuda, D, n_q, n_kv, ctxs, cap, window):
+    """few sequences, a cluster to each head: any number of CTAs and pages, tables wider than the lengths"""
+    from llmq_b200 import lib
+    cache, table, rows = make_cache(ctxs, n_kv, D, seed=len(ctxs) + D)
+    B = len(ctxs)
+    qkv = torch.randn(B, (n_q + 2 * n_kv) * D, generator=torch.Generator().manual_seed(9)).to(BF)
+    wide = torch.cat([table, torch.full((B, 60), 2 ** 30, dtype=torch.int32)], 1).contiguous()   # (numbers that no length counts)
+    for bt in (table, wide):
+        out = torch.full((B + 1, n_q * D), float("nan"), dtype=BF, device=cuda)
+        lib.decode_attn_q4_set_whole(-2)
+        try:
+            lib.decode_attn_q4(qkv.to(cuda), out, cache.to(cuda), bt.to(cuda), torch.tensor(ctxs, dtype=torch.int32, device=cuda), n_q, n_kv, D, BS,
+                               D ** -0.5, softcap=cap, window=window)
+        finally:
+            lib.decode_attn_q4_set_whole(-1)
+        got = out.cpu()
+        assert torch.isnan(got[B].float()).all()
+        for i, c in enumerate(ctxs):
+            if c == 0:
+                assert (got[i] == 0).all()
+                continue
+            ref, weight, size = attention(qkv[i: i + 1, : n_q * D].view(1, n_q, D), *rows[i], torch.tensor([c - 1]), D ** -0.5, cap, window)
+            attention_close(got[i].view(1, n_q, D), ref, weight, size, D, 2.0 ** -11, f"ctx {c}")
+
+
+@pytest.mark.parametrize("way", [-2, 0, 1])
+def test_ways_of_sharing(cuda, way):
+    """sizes and growth of scores, NaN, far pages and two calls at once, whichever way the work is shared"""
+    from llmq_b200 import lib
+    lib.decode_attn_q4_set_whole(way)
+    try:
+        test_decode_sizes_of_values(cuda, 128, 8, 2, 1e4, 1.0, 1e-5)
+        test_decode_sizes_of_values(cuda, 256, 2, 1, 1e-6, 30.0, 1e4)
+        for D in (64, 128, 256):
+            test_decode_growing_scores(cuda, D)
+        test_decode_far_pages_and_many_rows(cuda)
+        test_two_calls_at_once(cuda, 64, 8, 2)
+        test_wide_windows(cuda, 4999)
+    finally:
+        lib.decode_attn_q4_set_whole(-1)
