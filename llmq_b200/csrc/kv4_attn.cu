@@ -16,6 +16,7 @@
 // Queries are divided by the power of two in their largest magnitude before they become fp16, which costs nothing that fp32 sums would keep.
 // 700 sequences of 33 to 1000 tokens, 32 / 8 heads of 128: 94.9 us, 4.5 TB/s (the memory's share 66 us); 22 of 16000: 84, its copies alone 70 and
 // its arithmetic alone 75; 3 of 9000 to 16000, heads of 64: 16.3 (3.4), of which the join is 3; one of 8000 13.4.
+#include <algorithm>
 #include <mutex>
 #include <type_traits>
 
@@ -853,7 +854,7 @@ int g_q4_whole = -1;  // test hook: 1 / 0 give items to warps whole or not, -2 t
 static std::mutex g_q4_pair;  // no other thread's pieces on the same stream between a stream kernel and its join
 
 // CTAs of a cluster for each of these items of up to `pages` pages, or 0: the kernel above.  Times in us, measured at 1 to 48 sequences of 300 to
-// 16000 tokens, 8 heads: clusters 4 and what a CTA's pages take (16 CTAs to a cluster 2.5 more); the kernel above `start` and `slope` times what all
+// 16000 tokens, 8 heads: clusters 4 and what a CTA's pages take (beside three others on an SM; alone half; 16 CTAs to a cluster 2.5 more); the kernel above `start` and `slope` times what all
 // pages take from memory.  us above / with clusters, D = 128: one sequence of 300 tokens 10.2 / 5.5, 16 of 1000 14.5 / 9.2, 16 of 4000 25 / 22.9,
 // 24 of 4000 32.9 / 36.1; D = 256: 6 of 4000 22.8 / 19.1, 8 of 4000 26.3 / 32.2.  Lengths below the table's width: 48 of 200 to 2000 23.8 / 30.2.
 template <int D>
@@ -864,8 +865,9 @@ static int kv4_clusters(long long items, int pages, bool forced) {
   if (items > places) return 0;
   int n = 1;  // (clusters of 16 leave places that none fits into: where they fill two thirds)
   while (n < Q4_MOST_CTAS && items * n * 2 <= (n == 8 ? places * 13 / 20 : places) && pages >= 2 * n * Q4Cluster<D>::WARPS * Q4Cfg<D>::PAGES) n *= 2;
-  const double all = (double)items * pages * Kv4<D>::BYTES / 6.45e6;
-  return forced || 4.0 + page * pages / n + (n == 16 ? 2.5 : 0.0) < (pages <= 8 ? 5.5 : start) + slope * all ? n : 0;
+  const double all = (double)items * pages * Kv4<D>::BYTES / 6.45e6, per_sm = (double)(items * n) / num_sms(),
+               full = std::min(1.0, D == 256 ? 0.5 + 0.2 * per_sm : 0.3 + 0.25 * per_sm);
+  return forced || 4.0 + full * page * pages / n + (n == 16 ? 2.5 : 0.0) < (pages <= 8 ? 5.5 : start) + slope * all ? n : 0;
 }
 
 template <int D, bool kCap>
