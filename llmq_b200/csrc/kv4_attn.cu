@@ -853,21 +853,25 @@ __global__ void __launch_bounds__(Q4Cluster<D>::WARPS * 32, Q4Cluster<D>::CTAS) 
 int g_q4_whole = -1;  // test hook: 1 / 0 give items to warps whole or not, -2 to clusters (-1: by size, and as B200Q_BATCH_INVARIANT says)
 static std::mutex g_q4_pair;  // no other thread's pieces on the same stream between a stream kernel and its join
 
-// CTAs of a cluster for each of these items of up to `pages` pages, or 0: the kernel above.  Times in us, measured at 1 to 48 sequences of 300 to
-// 16000 tokens, 8 heads: clusters 4 and what a CTA's pages take (beside three others on an SM; alone half; 16 CTAs to a cluster 2.5 more); the kernel above `start` and `slope` times what all
-// pages take from memory.  us above / with clusters, D = 128: one sequence of 300 tokens 10.2 / 5.5, 16 of 1000 14.5 / 9.2, 16 of 4000 25 / 22.9,
-// 24 of 4000 32.9 / 36.1; D = 256: 6 of 4000 22.8 / 19.1, 8 of 4000 26.3 / 32.2.  Lengths below the table's width: 48 of 200 to 2000 23.8 / 30.2.
+// CTAs of a cluster for each of these items of up to `pages` pages, or 0: the kernel above.  Times in us, fitted to 1 to 450 sequences of 16 to 16000
+// tokens, 8 heads.  Clusters: 4 and what a CTA's pages take (beside three others on an SM; alone half; 16 CTAs to a cluster 2.5 more), or several
+// rounds of CTAs; the kernel above: `start`, or where items are whole what the pages of one take a warp, and `slope` times what all pages take from
+// memory.  us above / with clusters, D = 128: one sequence of 64 tokens 5.5 / 3.1, of 300 10.2 / 5.1, 16 of 1000 14.5 / 9.2, 16 of 4000 25 / 22.9, 24 of
+// 4000 32.9 / 36.1, 150 of 300 23.3 / 20.2, 250 of 128 13.8 / 16.2; D = 256: 6 of 4000 22.8 / 19.1, 8 of 4000 26.3 / 32.2.  Lengths below the table's width:
+// 48 of 200 to 2000 23.8 / 30.2, 700 of 33 to 1000 95 / 105.
 template <int D>
 static int kv4_clusters(long long items, int pages, bool forced) {
   constexpr double page = D == 64 ? 0.15 : D == 128 ? 0.27 : 0.44, start = D == 64 ? 9.5 : D == 128 ? 10.0 : 14.0,
                    slope = D == 64 ? 1.5 : D == 128 ? 1.33 : 1.05;
   const long long places = (long long)num_sms() * Q4Cluster<D>::CTAS;
-  if (items > places) return 0;
+  if (items > 8 * places) return 0;
   int n = 1;  // (clusters of 16 leave places that none fits into: where they fill two thirds)
   while (n < Q4_MOST_CTAS && items * n * 2 <= (n == 8 ? places * 13 / 20 : places) && pages >= 2 * n * Q4Cluster<D>::WARPS * Q4Cfg<D>::PAGES) n *= 2;
   const double all = (double)items * pages * Kv4<D>::BYTES / 6.45e6, per_sm = (double)(items * n) / num_sms(),
-               full = std::min(1.0, D == 256 ? 0.5 + 0.2 * per_sm : 0.3 + 0.25 * per_sm);
-  return forced || 4.0 + full * page * pages / n + (n == 16 ? 2.5 : 0.0) < (pages <= 8 ? 5.5 : start) + slope * all ? n : 0;
+               full = std::min(1.0, D == 256 ? 0.5 + 0.2 * per_sm : 0.3 + 0.25 * per_sm), rounds = (double)items / places,
+               clusters = rounds <= 1.0 ? 4.0 + full * page * pages / n + (n == 16 ? 2.5 : 0.0) : 3.0 + rounds * (2.8 + page * pages),
+               above = pages <= 8 ? 4.5 + 2.0 * page * pages + 1.33 * all : start + slope * all;
+  return forced || clusters < above ? n : 0;
 }
 
 template <int D, bool kCap>
