@@ -14,8 +14,9 @@
 //     Probabilities are fp16 with 2^8 for the maximum's place (up to 2^12), so that a probability of 2^-32 of the largest still counts.
 //   * A warp has its own pages on their way, by asynchronous copies; nobody waits for another warp.
 // Queries are divided by the power of two in their largest magnitude before they become fp16, which costs nothing that fp32 sums would keep.
+// Many sequences are streamed through by all warps (kv4_stream_kernel), few get a cluster of CTAs for each head (kv4_cluster_kernel).
 // 700 sequences of 33 to 1000 tokens, 32 / 8 heads of 128: 94.9 us, 4.5 TB/s (the memory's share 66 us); 22 of 16000: 84, its copies alone 70 and
-// its arithmetic alone 75; 3 of 9000 to 16000, heads of 64: 16.3 (3.4), of which the join is 3; one of 8000 13.4.
+// its arithmetic alone 75; 16 of 1000 9.2; 3 of 9000 to 16000, heads of 64: 13.4 (3.4).
 #include <algorithm>
 #include <mutex>
 #include <type_traits>
