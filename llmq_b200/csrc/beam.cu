@@ -6,7 +6,8 @@
 // reaches it are collected, and once they are many their logits are ranked by counting: the K-th best so far is the bound from there on.  The
 // second kernel has a group per CTA: sums to logarithms, best logits to scores, and again a bound (the K-th best of the pieces' first entries),
 // what reaches it, and ranks.
-// Scores that are compared across rows are 64 bits; a row's logarithm comes from sums whose terms are off by some 2^-23 in either direction.
+// Scores that are compared across rows are 64 bits; a row's logarithm comes from sums whose terms are off by 2^-22 (the exponential) and 1.5 x 2^-24
+// (its exponent's rounding) at most, whatever the logits' size.
 // Bound: the logits, 2 bytes each, once; next to it the exponentials (16 a cycle and SM: two thirds of the memory's
 // time) and some nine instructions a logit.  Logits come by asynchronous copies two tiles ahead (in registers a tile ahead 55 us).
 // 48 groups of 8 beams over 256000 tokens, 16 candidates: 51.8 us (the memory's share 30; the first kernel 47, of which an eighth is looking for
@@ -47,9 +48,9 @@ __device__ __forceinline__ float2 halves_of(f32x2 v) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
   return r;
 }
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
   f32x2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
 __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
@@ -57,16 +58,23 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// sum += e^w of two logits.  The exponent's rounding, 2^-24 of it, and what the fp32 constant is off by follow from the logit alone and are the
-// same for the rows that are compared.
-__device__ __forceinline__ void add_exps(f32x2& sum, uint32_t w) {
-  constexpr float L = 1.44269504088896341f;
-  const float2 h = halves_of(mul2(pair_of(bf16_lo(w), bf16_hi(w)), pair_of(L, L)));
-  float x, y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x) : "f"(h.x));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(h.y));
-  sum = add2(sum, pair_of(x, y));
+// Sums of a row are those of 2^(L x - c), L the fp32 number next to log2(e) and c a whole number near L times the largest logit so far: L x - c is
+// rounded once, so that it is off by 2^-24 of itself, not of x, and by more than 1.5 x 2^-24 only where the term is small beside the largest.  What L is
+// off by makes e^x of 2^(L x) by a factor e^(BEAM_LOW x), for which that of the largest logit stands.
+constexpr float BEAM_L = 1.44269504088896341f;
+constexpr double BEAM_LOW = (1.44269504088896340736 - 1.44269502162933349609) * 0.69314718055994530942;
+__device__ __forceinline__ float beam_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
+// sum += 2^(L w + minus_c) of two logits
+__device__ __forceinline__ void add_exps(f32x2& sum, uint32_t w, float minus_c) {
+  const float2 h = halves_of(fma2(pair_of(bf16_lo(w), bf16_hi(w)), pair_of(BEAM_L, BEAM_L), pair_of(minus_c, minus_c)));
+  sum = add2(sum, pair_of(beam_ex2(h.x), beam_ex2(h.y)));
+}
+// 2^e of a whole number e (0 below the smallest)
+__device__ __forceinline__ float power_of_two(float e) { return e < -126.f ? 0.f : __int_as_float((127 + (int)e) << 23); }
 
 // logits 8 i .. 8 i + 7 of a row, those behind its end as -infinity.  Rows of a V that is no multiple of 8 begin anywhere: they are cut at the
 // same places all the same, so that equal rows give equal sums, and a vector is put together from the two aligned ones that it lies in.
@@ -141,7 +149,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
   __shared__ uint64_t found[BEAM_FOUND], best[BEAM_MOST_K];
   __shared__ double sums[BEAM_THREADS / 32];
   __shared__ uint4 vectors[BEAM_VECTORS];  // that hold a logit that reaches the bound, and which they are
-  __shared__ int vector_at[BEAM_VECTORS], n_vectors, n_found, bound_s;
+  __shared__ int vector_at[BEAM_VECTORS], n_vectors, n_found, bound_s, top_s;
   __shared__ uint64_t best_s[BEAM_THREADS / 32];
   // Rows of aligned vectors come through a ring of BEAM_RING tiles, every thread's vectors in places of its own (no waiting for others); of
   // other rows the next tile's are in registers.
@@ -242,11 +250,21 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
 #pragma unroll 16
       for (int i = 0; i < groups; ++i) rank += tops[i] > y || (tops[i] == y && i < tid);
       if (rank == K - 1) bound_s = __float_as_int(y);
+      if (rank == 0) top_s = __float_as_int(y);
     }
     __syncthreads();
     bound = fmaxf(__int_as_float(bound_s), __uint_as_float(0xff7f0000u));
     bound2 = __float_as_uint(bound) >> 16 | __float_as_uint(bound);
   }
+  // minus c of this thread's sum.  No logit above -infinity so far: one comes to `raise` before it is added, as it reaches the bound
+  float minus_c = __int_as_float(top_s) > -INFINITY ? -rintf(__int_as_float(top_s) * BEAM_L) : 3e38f;
+  auto raise = [&](float to) {
+    if (!(to > 1.f - minus_c)) return;
+    const float c = rintf(to), down = power_of_two(-minus_c - c);
+    const float2 h = halves_of(sum);
+    sum = pair_of(h.x * down, h.y * down);
+    minus_c = -c;
+  };
   auto most_of = [](const uint4& v) { return max_bf16x2(max_bf16x2(v.x, v.y), max_bf16x2(v.z, v.w)); };
   auto collect = [&](const uint4& v, int c) {
     const int at = next_place(&n_vectors);
@@ -256,20 +274,25 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
     }
   };
   auto add = [&](const uint4& v) {
-    add_exps(sum, v.x);
-    add_exps(sum, v.y);
-    add_exps(sum, v.z);
-    add_exps(sum, v.w);
+    add_exps(sum, v.x, minus_c);
+    add_exps(sum, v.y, minus_c);
+    add_exps(sum, v.z, minus_c);
+    add_exps(sum, v.w, minus_c);
   };
   auto look = [&](const uint4& v, int c) {
-    if (reaches_bf16x2(most_of(v), bound2)) collect(v, c);
+    const uint32_t m = most_of(v);
+    if (reaches_bf16x2(m, bound2)) {
+      collect(v, c);
+      raise(fmaxf(bf16_lo(m), bf16_hi(m)) * BEAM_L);
+    }
     add(v);
   };
   auto look_at_two = [&](const uint4& v, const uint4& w, int c) {
-    const uint32_t mv = most_of(v), mw = most_of(w);
-    if (reaches_bf16x2(max_bf16x2(mv, mw), bound2)) {  // (seldom)
+    const uint32_t mv = most_of(v), mw = most_of(w), m = max_bf16x2(mv, mw);
+    if (reaches_bf16x2(m, bound2)) {  // (seldom)
       if (reaches_bf16x2(mv, bound2)) collect(v, c);
       if (reaches_bf16x2(mw, bound2)) collect(w, c + BEAM_THREADS);
+      raise(fmaxf(bf16_lo(m), bf16_hi(m)) * BEAM_L);
     }
     add(v);
     add(w);
@@ -281,10 +304,11 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
     const int k = prune(kept);
     overflow |= k < 0;
     if (!overflow) kept = k;
-    if (overflow)
-      bound = INFINITY;  // (whatever is found from here on does not matter)
+    if (overflow)  // (whatever is found from here on does not matter, but for logits that c has to follow)
+      bound = __uint_as_float(__float_as_uint((1.f - minus_c) * (1.f / BEAM_L)) & 0xffff0000u);
     else if (kept == K)
       bound = value_of(best[K - 1]);
+    raise(bound * BEAM_L);  // (logits below the bound are not looked at: c is not below it)
     bound2 = __float_as_uint(bound) >> 16 | __float_as_uint(bound);
   };
   int stage = 0;
@@ -320,8 +344,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
   settle();
   const float2 halves = halves_of(sum);
   float mine_sum = halves.x + halves.y;
-  // the largest logit: where the exponentials themselves would leave what fp32 holds, or the constant's own error would show, or a thread
-  // met NaN, once more by differences to it
+  // the largest logit: where the sum would leave what 64 bits hold once more by differences to it; where a thread met NaN once more without
   float top = -INFINITY;
   if (!overflow) {
     if (kept > 0) top = value_of(best[0]);
@@ -336,7 +359,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
 #pragma unroll
     for (int w = 0; w < BEAM_THREADS / 32; ++w) top = fmaxf(top, tops[w]);
   }
-  const bool far = fabsf(top) > 32.f;
+  const bool far = fabsf(top) > 600.f;
   if (far || mine_sum != mine_sum) {
     mine_sum = 0.f;
     for (int c = v0 + tid; c < v1; c += BEAM_THREADS) {
@@ -345,11 +368,13 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const float y = k & 1 ? bf16_hi(w[k >> 1]) : bf16_lo(w[k >> 1]);
-        if (y == y) mine_sum += far ? (y == top ? 1.f : expf(y - top)) : expf(y);
+        if (y == y) mine_sum += far ? (y == top ? 1.f : expf(y - top)) : beam_ex2(fmaf(y, BEAM_L, minus_c));
       }
     }
   }
-  double d = (double)mine_sum;
+  // (far below the largest logit, if there is one: 0)
+  const double unit = far ? 1.0 : minus_c > 1000.f ? 0.0 : __hiloint2double((1023 - (int)minus_c) << 20, 0);
+  double d = (double)mine_sum * unit;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
   if ((tid & 31) == 0) sums[tid >> 5] = d;
@@ -358,6 +383,8 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
   if (tid == 0) {
     double s = 0.0;
     for (int w = 0; w < BEAM_THREADS / 32; ++w) s += sums[w];
+    const double low = (double)top * BEAM_LOW;  // (up to 8e-6)
+    if (!far) s *= 1.0 + low * (1.0 + 0.5 * low);
     // s e^base; base +infinity: a logit is, -infinity: there are none
     piece_sums[out] = make_double2(far ? (double)top : 0.0, s);
   }
@@ -463,6 +490,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) beam_groups_kernel(BeamArgs a) 
   const long long group = blockIdx.x, row0 = group * W;
   const int lists = W * a.n_pieces, n = lists * K;
   __shared__ double shift[BEAM_MOST_W];  // score - log of the sum; -infinity: the row has no candidates
+  __shared__ float score[BEAM_MOST_W];
   __shared__ uint64_t bound_s;
   __shared__ int n_found;
   constexpr int FOUND = 1024;
@@ -495,6 +523,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) beam_groups_kernel(BeamArgs a) 
     for (int p = lane + 64; p < a.n_pieces && finite; p += 32) sum += part(piece_sums[w * a.n_pieces + p]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) score[w] = a.scores[row0 + w];
     if (lane == 0) shift[w] = finite && s > -INFINITY && s < INFINITY ? s - (top + log(sum)) : -INFINITY;
   }
   if (tid == 0) {
@@ -509,7 +538,8 @@ __global__ void __launch_bounds__(MERGE_THREADS) beam_groups_kernel(BeamArgs a) 
     token = e.y;
     if (shift[w] == -INFINITY) token = list % a.n_pieces == 0 ? i % K : -1;
     const float x = __int_as_float(e.x);
-    return shift[w] == -INFINITY || !(x > -INFINITY) ? -INFINITY : shift[w] + (double)x;
+    // (no token is more than certain)
+    return shift[w] == -INFINITY || !(x > -INFINITY) ? -INFINITY : fmin(shift[w] + (double)x, (double)score[w]);
   };
   auto entry = [&](int i, int& w, int& token) { return score_of(entries[i], i, w, token); };
   auto key_of = [&](int2 e, int i) -> uint64_t {

@@ -115,6 +115,33 @@ def test_whatever_the_batch(cuda):
         lib.load().b200q_gemm_set_splitk(0)
 
 
+# A row's logarithm: terms off by at most 2^-22 (the exponential) and 1.5 x 2^-24 (the rounding of its exponent, which is taken relative to the
+# row's own largest logits), five additions in fp32 on a term's way into a sum of 64 bits: (4 + 1.5 + 5) 2^-24, and a result rounded to fp32.
+LOG_SUM = 10.5 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("V", [64, 3001, 128256])
+def test_one_logit(cuda, V):
+    """rows of which a mask leaves one token, and rows whose largest logit has all but 2^-20 of the sum: the token's probability is 1 within what
+    a row's logarithm may be off by, whatever the logit's size, and never above 1"""
+    from llmq_b200 import lib
+    sizes = [15.3125, 23.0, 30.625, 31.875, -15.3125, -30.625, -31.5, 0.0, 100.0, -100.0, 599.0, -640.0, 1e4, -1e4, 1e30, -1e30]
+    for rest in (-math.inf, -30.0):
+        x = torch.full((len(sizes), V), -math.inf, dtype=torch.float64)
+        for i, size in enumerate(sizes):
+            if rest > -math.inf and abs(size) < 1000:
+                x[i] = size + rest
+            x[i, V * i // len(sizes)] = size
+        x, scores = x.to(BF), -torch.rand(len(sizes), generator=torch.Generator().manual_seed(V))
+        cand, _ = select(lib, cuda, x, scores, 1, 1, [])
+        want, _ = select_rules(x, scores, 1, 1, [])
+        assert cand[1].tolist() == want[1]
+        ref = torch.tensor(want[0], dtype=torch.float64).flatten()
+        got = cand[0].double().flatten()
+        assert ((got - ref).abs() <= LOG_SUM + 2.0 ** -24 * ref.abs()).all(), (got - ref) * 2 ** 24
+        assert (got <= scores.double()).all()
+
+
 def test_many_groups(cuda):
     from llmq_b200 import lib
     g = torch.Generator().manual_seed(1)
