@@ -7,7 +7,7 @@
 // second kernel has a group per CTA: sums to logarithms, best logits to scores, and again a bound (the K-th best of the pieces' first entries),
 // what reaches it, and ranks.
 // Scores that are compared across rows are 64 bits; a row's logarithm comes from sums whose terms are off by 2^-22 (the exponential) and 1.5 x 2^-24
-// (its exponent's rounding) at most, whatever the logits' size.
+// (its exponent's rounding) at most, whatever the logits' size, and go through five additions in fp32 before those in 64 bits.
 // Bound: the logits, 2 bytes each, once; next to it the exponentials (16 a cycle and SM: two thirds of the memory's
 // time) and some nine instructions a logit.  Logits come by asynchronous copies two tiles ahead (in registers a tile ahead 55 us).
 // 48 groups of 8 beams over 256000 tokens, 16 candidates: 51.8 us (the memory's share 30; the first kernel 47, of which an eighth is looking for
@@ -68,10 +68,13 @@ __device__ __forceinline__ float beam_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// sum += 2^(L w + minus_c) of two logits
-__device__ __forceinline__ void add_exps(f32x2& sum, uint32_t w, float minus_c) {
+// 2^(L w + minus_c) of two logits, and of eight (a pair of sums)
+__device__ __forceinline__ f32x2 beam_exps(uint32_t w, float minus_c) {
   const float2 h = halves_of(fma2(pair_of(bf16_lo(w), bf16_hi(w)), pair_of(BEAM_L, BEAM_L), pair_of(minus_c, minus_c)));
-  sum = add2(sum, pair_of(beam_ex2(h.x), beam_ex2(h.y)));
+  return pair_of(beam_ex2(h.x), beam_ex2(h.y));
+}
+__device__ __forceinline__ f32x2 beam_exps(const uint4& v, float minus_c) {
+  return add2(add2(beam_exps(v.x, minus_c), beam_exps(v.y, minus_c)), add2(beam_exps(v.z, minus_c), beam_exps(v.w, minus_c)));
 }
 // 2^e of a whole number e (0 below the smallest)
 __device__ __forceinline__ float power_of_two(float e) { return e < -126.f ? 0.f : __int_as_float((127 + (int)e) << 23); }
@@ -187,7 +190,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
   if (tid == 0) n_found = n_vectors = 0;
   float bound = -INFINITY;
   uint32_t bound2 = 0xff80ff80u;  // twice the same as bf16
-  f32x2 sum = 0;
+  double sum = 0.0;  // (an fp32 sum swallows the small terms behind a large one: only a tile's meet there)
   // the logits of the collected vectors that reach the bound, and the k0 in best: the K best of them into best, in order.  How many there are;
   // -1: too many to look at
   auto prune = [&](int k0) {
@@ -261,8 +264,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
   auto raise = [&](float to) {
     if (!(to > 1.f - minus_c)) return;
     const float c = rintf(to), down = power_of_two(-minus_c - c);
-    const float2 h = halves_of(sum);
-    sum = pair_of(h.x * down, h.y * down);
+    sum *= (double)down;
     minus_c = -c;
   };
   auto most_of = [](const uint4& v) { return max_bf16x2(max_bf16x2(v.x, v.y), max_bf16x2(v.z, v.w)); };
@@ -273,11 +275,9 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
       vector_at[at] = c;
     }
   };
-  auto add = [&](const uint4& v) {
-    add_exps(sum, v.x, minus_c);
-    add_exps(sum, v.y, minus_c);
-    add_exps(sum, v.z, minus_c);
-    add_exps(sum, v.w, minus_c);
+  auto add = [&](f32x2 exps) {
+    const float2 h = halves_of(exps);
+    sum += (double)(h.x + h.y);
   };
   auto look = [&](const uint4& v, int c) {
     const uint32_t m = most_of(v);
@@ -285,20 +285,24 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
       collect(v, c);
       raise(fmaxf(bf16_lo(m), bf16_hi(m)) * BEAM_L);
     }
-    add(v);
+    add(beam_exps(v, minus_c));
   };
-  auto look_at_two = [&](const uint4& v, const uint4& w, int c) {
-    const uint32_t mv = most_of(v), mw = most_of(w), m = max_bf16x2(mv, mw);
-    if (reaches_bf16x2(m, bound2)) {  // (seldom)
-      if (reaches_bf16x2(mv, bound2)) collect(v, c);
-      if (reaches_bf16x2(mw, bound2)) collect(w, c + BEAM_THREADS);
-      raise(fmaxf(bf16_lo(m), bf16_hi(m)) * BEAM_L);
+  int c = v0 + tid;
+  auto look_at_tile = [&]() {
+    uint32_t m[BEAM_NV];
+#pragma unroll
+    for (int u = 0; u < BEAM_NV; ++u) m[u] = most_of(a[u]);
+    const uint32_t top = max_bf16x2(max_bf16x2(m[0], m[1]), max_bf16x2(m[2], m[3]));
+    if (reaches_bf16x2(top, bound2)) {  // (seldom)
+#pragma unroll
+      for (int u = 0; u < BEAM_NV; ++u)
+        if (reaches_bf16x2(m[u], bound2)) collect(a[u], c + u * BEAM_THREADS);
+      raise(fmaxf(bf16_lo(top), bf16_hi(top)) * BEAM_L);
     }
-    add(v);
-    add(w);
+    add(add2(add2(beam_exps(a[0], minus_c), beam_exps(a[1], minus_c)), add2(beam_exps(a[2], minus_c), beam_exps(a[3], minus_c))));
   };
   // Whole tiles; what comes next is asked for as soon as a place is free.  Behind tiles 0, 1, 3, 7, ... it is looked at whether enough has been found for only the K best so far to matter from there on (the ranks cost the square of it).
-  int c = v0 + tid, kept = 0;
+  int kept = 0;
   bool overflow = false;
   auto settle = [&]() {
     const int k = prune(kept);
@@ -318,19 +322,15 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
         asm volatile("cp.async.wait_group %0;" ::"n"(BEAM_RING - 1) : "memory");
 #pragma unroll
         for (int u = 0; u < BEAM_NV; ++u) a[u] = lds_v4(place + 16 * (stage * TILE + u * BEAM_THREADS));
-        look_at_two(a[0], a[1], c);
-        look_at_two(a[2], a[3], c + 2 * BEAM_THREADS);
+        look_at_tile();
         ask(t + BEAM_RING, stage);
         stage = stage + 1 < BEAM_RING ? stage + 1 : 0;
         c += TILE;
       } else {
+        look_at_tile();
 #pragma unroll
-        for (int u = 0; u < BEAM_NV; u += 2) {
-          look_at_two(a[u], a[u + 1], c);
-#pragma unroll
-          for (int k = u; k < u + 2; ++k, c += BEAM_THREADS)
-            if (c + TILE < v1) a[k] = x(c + TILE);
-        }
+        for (int u = 0; u < BEAM_NV; ++u, c += BEAM_THREADS)
+          if (c + TILE < v1) a[u] = x(c + TILE);
       }
     }
     // (the count that a thread sees holds its own vectors, so that the last one to add any sees them all)
@@ -342,8 +342,6 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
   for (int u = 0; u < BEAM_NV; ++u, c += BEAM_THREADS)
     if (c < v1) look(kAligned ? lds_v4(place + 16 * (stage * TILE + u * BEAM_THREADS)) : a[u], c);
   settle();
-  const float2 halves = halves_of(sum);
-  float mine_sum = halves.x + halves.y;
   // the largest logit: where the sum would leave what 64 bits hold once more by differences to it; where a thread met NaN once more without
   float top = -INFINITY;
   if (!overflow) {
@@ -360,21 +358,23 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
     for (int w = 0; w < BEAM_THREADS / 32; ++w) top = fmaxf(top, tops[w]);
   }
   const bool far = fabsf(top) > 600.f;
-  if (far || mine_sum != mine_sum) {
-    mine_sum = 0.f;
+  if (far || sum != sum) {
+    sum = 0.0;
     for (int c = v0 + tid; c < v1; c += BEAM_THREADS) {
       const uint4 v = x(c);
       const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      float part[2] = {0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const float y = k & 1 ? bf16_hi(w[k >> 1]) : bf16_lo(w[k >> 1]);
-        if (y == y) mine_sum += far ? (y == top ? 1.f : expf(y - top)) : beam_ex2(fmaf(y, BEAM_L, minus_c));
+        if (y == y) part[k & 1] += far ? (y == top ? 1.f : expf(y - top)) : beam_ex2(fmaf(y, BEAM_L, minus_c));
       }
+      sum += (double)(part[0] + part[1]);
     }
   }
   // (far below the largest logit, if there is one: 0)
   const double unit = far ? 1.0 : minus_c > 1000.f ? 0.0 : __hiloint2double((1023 - (int)minus_c) << 20, 0);
-  double d = (double)mine_sum * unit;
+  double d = sum * unit;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
   if ((tid & 31) == 0) sums[tid >> 5] = d;

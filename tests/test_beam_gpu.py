@@ -142,6 +142,21 @@ def test_one_logit(cuda, V):
         assert (got <= scores.double()).all()
 
 
+@pytest.mark.parametrize("V,R", [(128256, 740), (50257, 740), (256000, 384), (256000, 4)])
+def test_peak_over_a_flat_tail(cuda, V, R):
+    """rows of one large logit, wherever it is, and a tail whose terms lie below half of its last place each: they count"""
+    from llmq_b200 import lib
+    tail, peak = -2.875, 14.0
+    x = torch.full((R, V), tail, dtype=BF)
+    at = [(0, V - 1, V // 2, 1, 8, 4096, V // 3, 7919)[i % 8] + 2 * (i // 8) * (-1 if i % 8 in (1, 2) else 1) for i in range(R)]
+    x[torch.arange(R), torch.tensor(at)] = peak
+    scores = torch.zeros(R)
+    cand, _ = select(lib, cuda, x, scores, 1, 1, [])
+    ref = -math.log1p((V - 1) * math.exp(tail - peak))
+    assert cand[1].flatten().tolist() == at
+    assert ((cand[0].double() - ref).abs() <= LOG_SUM + 2.0 ** -24 * abs(ref)).all(), (cand[0].double() - ref).abs().max() * 2 ** 24
+
+
 def test_many_groups(cuda):
     from llmq_b200 import lib
     g = torch.Generator().manual_seed(1)
