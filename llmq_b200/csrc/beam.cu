@@ -31,9 +31,10 @@ __device__ __forceinline__ bool reaches_bf16x2(uint32_t m, uint32_t bound) {
   asm("{ .reg .pred p, q;\n setp.ge.bf16x2 p|q, %1, %2;\n or.pred p, p, q;\n selp.s32 %0, 1, 0, p; }" : "=r"(r) : "r"(m), "r"(bound));
   return r;
 }
-// unsigned integers of the same order as the numbers (bf16 bits); NaN counts as -infinity
+// unsigned integers of the same order as the numbers (bf16 bits); NaN counts as -infinity, -0 as 0
 __device__ __forceinline__ uint32_t beam_order(uint32_t h) {
   if ((h & 0x7fffu) > 0x7f80u) h = 0xff80u;
+  if (h == 0x8000u) h = 0u;
   return (h & 0x8000u) ? 0xffffu ^ h : h | 0x8000u;
 }
 // two numbers at once, as neighbouring registers (one issue slot)
@@ -477,9 +478,9 @@ struct BeamArgs {
   int W, K, n_pieces, n_stops;
   long long V;
 };
-// unsigned 64-bit integers of the same order as the numbers
+// unsigned 64-bit integers of the same order as the numbers (-0 is 0)
 __device__ __forceinline__ uint64_t order_double(double v) {
-  const uint64_t b = (uint64_t)__double_as_longlong(v);
+  const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);
   return b >> 63 ? ~b : b | 0x8000000000000000ull;
 }
 

@@ -198,6 +198,25 @@ def test_equal_and_hidden_logits(cuda, V, W, K):
     check(lib, cuda, close, torch.full((R,), -1.25), W, K, [])
 
 
+@pytest.mark.parametrize("V", [64, 3001, 40001])
+@pytest.mark.parametrize("W,K", [(1, 4), (4, 8), (3, 64)])
+def test_zeros_of_either_sign(cuda, V, W, K):
+    """a logit or a score of -0 is as large as one of 0: the lower row and token first"""
+    from llmq_b200 import lib
+    g = torch.Generator().manual_seed(V)
+    R = 2 * W
+    zeros = torch.where(torch.rand(R, V, generator=g) < 0.5, -0.0, 0.0)
+    scores = -torch.rand(R, generator=g)
+    check(lib, cuda, zeros.to(BF), scores, W, K, [])                       # all equal
+    few = torch.where(torch.rand(R, V, generator=g) < 40 / V, zeros, torch.tensor(-5.0))
+    check(lib, cuda, few.to(BF), scores, W, K, [])
+    few[:, V // 2] = 1.0
+    check(lib, cuda, few.to(BF), scores, W, K, [])
+    one = torch.full((R, V), -math.inf)                                    # certain tokens: scores of -0 and 0
+    one[torch.arange(R), torch.arange(R) * 7 % V] = torch.where(torch.arange(R) % 2 == 0, -0.0, 0.0)
+    check(lib, cuda, one.to(BF), torch.where(torch.arange(R) % 2 == 0, -0.0, 0.0), W, K, [])
+
+
 @pytest.mark.parametrize("D,n_q,n_kv", [(64, 4, 2), (128, 8, 2), (256, 4, 1)])
 def test_search(cuda, D, n_q, n_kv):
     """A model of one layer whose queries, keys and values are rows of a table and whose logits are its attention's outputs times another:
