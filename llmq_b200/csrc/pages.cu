@@ -52,6 +52,12 @@ __device__ __forceinline__ int block_prefix(int v, int* total, int* scratch /* 3
   return before;
 }
 
+// pages of a row of len tokens (lengths beyond the table's width count as its width; len + 15 may pass 2^31)
+__device__ __forceinline__ int pages_held(int len, int stride) {
+  const int n = max(len, 0);
+  return min(n / PG_BLOCK + (n % PG_BLOCK != 0), stride);
+}
+
 // the share of [0, n) of this CTA of the cluster, cut at multiples of 4 (refs is read four at a time)
 struct PageShare {
   int from, to;
@@ -268,7 +274,7 @@ __global__ void __launch_bounds__(256) pages_free_kernel(const int32_t* table, c
   const int lane = threadIdx.x & 31;
   for (int r = blockIdx.x * 8 + (threadIdx.x >> 5); r < n; r += gridDim.x * 8) {
     if (ends && ends[r] == 0) continue;
-    const int pages = min((max(lens[r], 0) + PG_BLOCK - 1) / PG_BLOCK, stride);
+    const int pages = pages_held(lens[r], stride);
     for (int c = lane; c < pages; c += 32) {
       const int p = table[(long long)r * stride + c];
       if (p >= 0 && p < num_blocks) atomicAdd(refs + p, -1);
@@ -375,7 +381,7 @@ __global__ void __launch_bounds__(PG_THREADS, 1) pages_compact_kernel(CompactArg
   }
   rows_sync();
   for_entries(a.n_rows * a.stride, a.stride, at, threads, [&](int r, int c) {
-    if (c >= min((max(a.lens[r], 0) + PG_BLOCK - 1) / PG_BLOCK, a.stride)) return NO_ENTRY;
+    if (c >= pages_held(a.lens[r], a.stride)) return NO_ENTRY;
     const int p = a.table[r * a.stride + c];
     return p >= 0 && p < a.num_blocks ? a.map[p] : -1;
   }, [&](int e, int page) { a.table_out[e] = page; });

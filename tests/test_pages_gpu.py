@@ -211,6 +211,37 @@ def test_compact(cuda, blocks, live, in_place):
     assert page_map.cpu().tolist() == where and r_out.cpu().tolist() == counts and t_out.cpu().tolist() == want
 
 
+@pytest.mark.parametrize("n", [2 ** 31 - 1, 2 ** 31 - 15, 2 ** 31 - 16, 7 * BS + 1])
+def test_lengths_beyond_the_table(cuda, n):
+    """they count as the table's width, up to the largest there are"""
+    from llmq_b200 import lib
+    stride, rows, blocks = 7, 3, 60
+    table = [[20 + 7 * r + c - r * (c == 0) for c in range(stride)] for r in range(rows)]   # (the rows' first pages: 20, 26, 32)
+    refs = [0] * blocks
+    for row in table:
+        for q in row:
+            refs[q] += 1
+    used = [q for q in range(blocks) if refs[q]]
+    where = {q: i for i, q in enumerate([q for q in used if q < len(used)])}
+    free = [q for q in range(len(used)) if refs[q] == 0]
+    where = {q: q for q in used if q < len(used)} | dict(zip([q for q in used if q >= len(used)], free))
+    t, r, lens = ints(table, cuda), ints(refs, cuda), ints([n, 0, n], cuda)
+    t_out, r_out, page_map = t.clone(), torch.zeros_like(r), torch.zeros_like(r)
+    pairs, status = torch.zeros(blocks // 2 + 1, 2, dtype=torch.int32, device=cuda), ints([0, 0], cuda)
+    lib.pages_compact(t, lens, r, t_out, r_out, page_map, pairs, status)
+    assert t_out.cpu().tolist() == [[where[q] for q in table[0]], table[1], [where[q] for q in table[2]]]
+    lib.pages_free(t, lens, r)
+    want = list(refs)
+    for q in table[0] + table[2]:
+        want[q] -= 1
+    assert r.cpu().tolist() == want
+    out = [[-3] * stride for _ in range(rows)]
+    f = fork(lib, cuda, table, [n, 5, n], [0, 2, 0], refs, stride, out)
+    w = fork_rules(table, [n, 5, n], [0, 2, 0], refs, out)
+    for name, x in zip(("out", "refs", "slots", "pairs", "status"), w):
+        assert f[name].cpu().tolist() == x, name
+
+
 def test_unaligned_counts(cuda):
     """counts that do not begin on a 16-byte boundary"""
     from llmq_b200 import lib
