@@ -726,6 +726,7 @@ __global__ void __launch_bounds__((PfCfg<D>::MAX_G + 1) * 32)
   if (long_keys > 0 && portion_keys(tiles, n_tiles, blockIdx.x, lane) >= long_keys) return;
   const int4 tile = tiles[blockIdx.x];
   const int bt_row = tile.x, row0 = tile.y, n_rows = tile.z, pos0 = tile.w;
+  if (n_rows <= 0) return;             // (a padded list of tiles: entries of the block table that nobody sees need not be page numbers)
   const int total_kv = pos0 + n_rows;  // keys 0 .. pos0+n_rows-1 are visible to this tile
   const int n_pages = (total_kv + BS - 1) / BS;
   // sliding window: row i (position pos0+i) sees keys j > pos0+i-window; the tile starts at the

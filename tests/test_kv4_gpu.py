@@ -211,6 +211,39 @@ def test_prompts(cuda, D, n_q, n_kv, portions, cap, window):
     assert lib.load().b200q_wait_failures() == 0
 
 
+@pytest.mark.parametrize("route", [-1, 0, 1, 2])
+@pytest.mark.parametrize("D,n_q,n_kv", [(64, 8, 2), (128, 8, 1), (256, 8, 2)])
+@pytest.mark.parametrize("window", [0, 50])
+def test_padded_lists_of_tiles(cuda, D, n_q, n_kv, window, route):
+    """tiles of no rows between the others and behind them, at positions whose pages nobody sees: as if they were not there"""
+    from llmq_b200 import lib
+    portions = [(5, 11), (333, 0), (170, 100)]
+    cache, table, rows = make_cache([n + past for n, past in portions], n_kv, D, seed=D)
+    table = torch.cat([table, torch.zeros(2, table.shape[1], dtype=torch.int32)]).contiguous()   # (two rows of no portion)
+    tiles, T = tiles_of(portions)
+    padded = []
+    for i, t in enumerate(tiles.tolist()):
+        padded += [[4, t[1], 0, 300], [t[0], t[1], 0, t[3]], t][i % 3:]
+    padded += [[3, T, 0, 37], [0, T, 0, 300], [2, T, 0, 271], [1, 0, -1, 20]] * 3
+    qkv = torch.randn(T, (n_q + 2 * n_kv) * D, generator=torch.Generator().manual_seed(7)).to(BF)
+    out = torch.full((T + 1, n_q * D), float("nan"), dtype=BF, device=cuda)
+    work = torch.full((lib.prefill_attn_q4_workspace(*table.shape, n_kv, D),), 0xFF, dtype=torch.uint8, device=cuda)
+    lib.check(lib.load().b200q_prefill_attn_set_route(route))
+    try:
+        lib.prefill_attn_q4(qkv.to(cuda), out, cache.to(cuda), table.to(cuda), torch.tensor(padded, dtype=torch.int32, device=cuda), n_q, n_kv, D, BS,
+                            D ** -0.5, work, window=window)
+    finally:
+        lib.check(lib.load().b200q_prefill_attn_set_route(-1))
+    got, at = out.cpu(), 0
+    assert torch.isnan(got[T].float()).all()
+    for i, (n, past) in enumerate(portions):
+        q = qkv[at: at + n, : n_q * D].view(n, n_q, D)
+        ref, weight, sz = attention(q, *rows[i], torch.arange(past, past + n), D ** -0.5, 0.0, window)
+        attention_close(got[at: at + n].view(n, n_q, D), ref, weight, sz, D, 2.0 ** -8, f"portion {i}")
+        at += n
+    assert lib.load().b200q_wait_failures() == 0
+
+
 def test_captured_and_on_another_stream(cuda):
     """a write and the attention behind it, captured once and replayed over other inputs, beside the same on a stream of its own"""
     from llmq_b200 import lib
