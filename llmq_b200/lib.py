@@ -645,6 +645,13 @@ def _bytes(n):
     return int(n)
 
 
+def _kv4(t, n_kv, D, dev):
+    """data_ptr of a layer of the 4-bit cache: whole pages of n_kv heads"""
+    page = 18 * n_kv * D
+    _want(page <= 0 or t.numel() * t.element_size() % page == 0, f"kv4_layer: not a whole number of pages of {n_kv} heads of {D}")
+    return _arg(t, None, "kv4_layer", dev)
+
+
 def kv4_page_bytes(n_kv, D):
     """bytes of a page of the 4-bit cache (16 tokens, all heads of a layer)"""
     return _bytes(load().b200q_kv4_page_bytes(n_kv, D))
@@ -656,7 +663,7 @@ def rope_kvwrite_q4(qkv, cos_sin, positions, slot_mapping, kv4_layer, n_q, n_kv,
     _want(width == (n_q + 2 * n_kv) * D and positions.numel() == T and slot_mapping.numel() == T and cos_sin.shape[1] == D,
           "rope_kvwrite_q4: rows of qkv, cos_sin, positions or slots do not fit the heads")
     check(load().b200q_rope_kvwrite_q4(_arg(qkv, "h", "qkv", dev), _arg(cos_sin, "h", "cos_sin", dev), _arg(positions, "i", "positions", dev),
-                                       _arg(slot_mapping, "i", "slot_mapping", dev), _arg(kv4_layer, None, "kv4_layer", dev), T, n_q, n_kv, D,
+                                       _arg(slot_mapping, "i", "slot_mapping", dev), _kv4(kv4_layer, n_kv, D, dev), T, n_q, n_kv, D,
                                        block_size, s))
 
 
@@ -664,7 +671,7 @@ def kv4_unpack(kv4_layer, pages, kv_out, n_kv, D, block_size, stream=None):
     """pages of the 4-bit cache as pages of the 16-bit one: kv_out[i] = page pages[i]"""
     n, (s, dev) = pages.numel(), _here(stream)
     _want(kv_out.numel() >= n * 2 * n_kv * block_size * D, "kv4_unpack: kv_out is too small")
-    check(load().b200q_kv4_unpack(_arg(kv4_layer, None, "kv4_layer", dev), _arg(pages, "i", "pages", dev), n, _arg(kv_out, "h", "kv_out", dev), n_kv, D,
+    check(load().b200q_kv4_unpack(_kv4(kv4_layer, n_kv, D, dev), _arg(pages, "i", "pages", dev), n, _arg(kv_out, "h", "kv_out", dev), n_kv, D,
                                   block_size, s))
 
 
@@ -672,7 +679,7 @@ def decode_attn_q4(qkv, out, kv4_layer, block_table, ctx_lens, n_q, n_kv, D, blo
     """decode_attn over a layer of the 4-bit cache"""
     n, (rows, width), (table, columns), (s, dev) = ctx_lens.numel(), qkv.shape, block_table.shape, _here(stream)
     _want(rows >= n and width >= n_q * D and table >= n and out.numel() >= n * n_q * D, "decode_attn_q4: rows of qkv, out or the block table are missing")
-    check(load().b200q_decode_attn_q4(_arg(qkv, "h", "qkv", dev), width, _arg(out, "h", "out", dev), _arg(kv4_layer, None, "kv4_layer", dev),
+    check(load().b200q_decode_attn_q4(_arg(qkv, "h", "qkv", dev), width, _arg(out, "h", "out", dev), _kv4(kv4_layer, n_kv, D, dev),
                                       _arg(block_table, "i", "block_table", dev), columns, _arg(ctx_lens, "i", "ctx_lens", dev), n, n_q, n_kv, D,
                                       block_size, scale, softcap, window, s))
 
@@ -688,10 +695,10 @@ def prefill_attn_q4_workspace(n_seqs, bt_stride, n_kv, D):
 
 def prefill_attn_q4(qkv, out, kv4_layer, block_table, tiles, n_q, n_kv, D, block_size, scale, workspace, stream=None, softcap: float = 0.0,
                     window: int = 0):
-    """prefill_attn over a layer of the 4-bit cache; workspace: a tensor of prefill_attn_q4_workspace(*block_table.shape, n_kv, D) bytes"""
+    """prefill_attn over a layer of the 4-bit cache; out has as many rows as qkv at least; workspace: a tensor of prefill_attn_q4_workspace(*block_table.shape, n_kv, D) bytes"""
     (rows, width), (table, columns), (n_tiles, four), (s, dev) = qkv.shape, block_table.shape, tiles.shape, _here(stream)
-    _want(width >= n_q * D and four == 4, "prefill_attn_q4: rows of qkv or tiles do not fit")
-    check(load().b200q_prefill_attn_q4(_arg(qkv, "h", "qkv", dev), width, _arg(out, "h", "out", dev), _arg(kv4_layer, None, "kv4_layer", dev),
+    _want(width >= n_q * D and four == 4 and out.numel() >= rows * n_q * D, "prefill_attn_q4: rows of qkv, out or tiles do not fit")
+    check(load().b200q_prefill_attn_q4(_arg(qkv, "h", "qkv", dev), width, _arg(out, "h", "out", dev), _kv4(kv4_layer, n_kv, D, dev),
                                        _arg(block_table, "i", "block_table", dev), columns, table, _arg(tiles, "i", "tiles", dev), n_tiles, n_q, n_kv, D,
                                        block_size, scale, softcap, window, _arg(workspace, None, "workspace", dev),
                                        workspace.numel() * workspace.element_size(), s))

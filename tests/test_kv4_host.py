@@ -112,3 +112,51 @@ def test_tensors_are_looked_at():
         lib._arg(torch.zeros(3, dtype=torch.int64), "i", "x")
     with pytest.raises(ValueError, match="CUDA"):
         lib._arg(torch.zeros(3, dtype=torch.int32), "i", "x")
+
+
+def test_caches_and_outputs_are_looked_at(monkeypatch):
+    """a cache that is no whole number of pages, and outputs with fewer rows than there are queries, before anything is called"""
+    import torch
+
+    from llmq_b200 import lib
+    called = []
+
+    class Calls:
+        def __getattr__(self, name):
+            return lambda *a: called.append(name) or 0
+    monkeypatch.setattr(lib, "load", Calls)
+    monkeypatch.setattr(lib, "_here", lambda stream: (0, -1))   # (tensors of the CPU are on device -1)
+    n_q, n_kv, D, T = 4, 2, 64, 5
+    bf = dict(dtype=torch.bfloat16)
+    i32 = dict(dtype=torch.int32)
+    page = 18 * n_kv * D
+    qkv, cos_sin, rows = torch.zeros(T, (n_q + 2 * n_kv) * D, **bf), torch.zeros(9, D, **bf), torch.zeros(T, **i32)
+    table, tiles, work = torch.zeros(T, 3, **i32), torch.zeros(2, 4, **i32), torch.zeros(8, dtype=torch.uint8)
+    back = torch.zeros(T, 2 * n_kv * 16 * D, **bf)
+
+    def write(kv):
+        lib.rope_kvwrite_q4(qkv, cos_sin, rows, rows, kv, n_q, n_kv, D, 16)
+
+    def unpack(kv):
+        lib.kv4_unpack(kv, rows, back, n_kv, D, 16)
+
+    def decode(kv, n=T):
+        lib.decode_attn_q4(qkv, torch.zeros(n, n_q * D, **bf), kv, table, rows, n_q, n_kv, D, 16, 1.0)
+
+    def prompts(kv, n=T):
+        lib.prefill_attn_q4(qkv, torch.zeros(n, n_q * D, **bf), kv, table, tiles, n_q, n_kv, D, 16, 1.0, work)
+
+    for call in (write, unpack, decode, prompts):
+        for size in (page + 16, 3 * page - 1, 18 * D):
+            with pytest.raises(ValueError, match="whole number of pages"):
+                call(torch.zeros(size, dtype=torch.uint8))
+    for call in (decode, prompts):
+        with pytest.raises(ValueError, match="out"):
+            call(torch.zeros(page, dtype=torch.uint8), T - 1)
+    assert not called
+    for call in (write, unpack, decode, prompts):
+        for kv in (torch.zeros(3, n_kv, 18 * D, dtype=torch.uint8), torch.zeros(page // 4, **i32), torch.zeros(0, dtype=torch.uint8)):
+            call(kv)
+    decode(torch.zeros(page, dtype=torch.uint8), T + 1)
+    prompts(torch.zeros(page, dtype=torch.uint8), T + 1)
+    assert len(called) == 14
