@@ -660,8 +660,9 @@ int b200q_rope_kvwrite_q4(void* qkv_dev, const void* cos_sin_dev, const int32_t*
 int b200q_kv4_unpack(const void* kv4_layer_dev, const int32_t* pages_dev, int n_pages, void* kv_out_dev, int n_kv, int D,
                      int block_size, void* stream);
 /* b200q_decode_attn_ex over a 4-bit cache (GQA group <= 8).  A sequence of no tokens gives zeros; lengths beyond the table's width count as
- *     its width, and the entries that a length counts are numbers of pages.  q rows 16-byte aligned, out 8.  Pieces of sequences that several warps share lie in scratch that the stream (a graph: the
- *     graph) keeps, up to 64 MiB, allocated when first needed; where there is no memory for it nothing is shared. */
+ *     its width, and the entries that a length counts are numbers of pages.  Tables of up to 2^32 pages of a head, 2^31 of a sequence's heads
+ *     and 2^40 in all.  q rows 16-byte aligned, out 8.  Pieces of sequences that several warps share lie in scratch that the stream (a graph:
+ *     the graph) keeps, up to 64 MiB, allocated when first needed; where there is no memory for it nothing is shared. */
 int b200q_decode_attn_q4(const void* q_dev, int q_stride, void* out_dev, const void* kv4_layer_dev, const int32_t* block_table_dev,
                          int bt_stride, const int32_t* ctx_lens_dev, int n_seqs, int n_q, int n_kv, int D, int block_size,
                          float scale, float softcap, int window, void* stream);

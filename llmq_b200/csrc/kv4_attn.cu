@@ -935,6 +935,11 @@ int b200q_decode_attn_q4(const void* q, int q_stride, void* out, const void* kv4
   B200Q_CHECK_ARG(block_size == 16 && (D == 64 || D == 128 || D == 256), "decode_attn_q4: unsupported D=%d block_size=%d (D in {64,128,256}, block 16)",
                   D, block_size);
   B200Q_CHECK_ARG(bt_stride >= 0 && bt_stride <= (1 << 26), "decode_attn_q4: bad bt_stride=%d", bt_stride);
+  // (what the kernel counts in 32 bits: units of a head, of a sequence, of a warp's piece)
+  const long long units = bt_stride + Q4_BEGIN;
+  B200Q_CHECK_ARG(units * n_seqs < 1ll << 32 && units * n_kv < 1ll << 31 && units * n_seqs < (1ll << 40) / n_kv,
+                  "decode_attn_q4: too much at once: n_seqs=%d bt_stride=%d n_kv=%d (2^32 pages of a head, 2^31 of a sequence, 2^40 in all)", n_seqs,
+                  bt_stride, n_kv);
   if (n_seqs == 0) return B200Q_OK;
   B200Q_CHECK_ARG(q && out && kv4_layer && block_table && ctx_lens, "decode_attn_q4: null argument");
   B200Q_CHECK_ARG(q_stride % 8 == 0 && q_stride >= n_q * D && ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(kv4_layer)) & 15) == 0,

@@ -49,6 +49,13 @@ def test_decode(change, word):
     assert lib.load().b200q_decode_attn_q4_set_whole(2) == -1
 
 
+@pytest.mark.parametrize("n,bt,n_kv", [(64, 1 << 26, 2), (4, 1 << 26, 32), (4000, 1 << 20, 512), ((1 << 31) - 1, 1, 2)])
+def test_decode_of_too_many_pages(n, bt, n_kv):
+    """tables beyond what the kernel's own counts hold"""
+    from llmq_b200 import lib
+    refused(lib.load().b200q_decode_attn_q4(P, 128 * n_kv, P, P, P, bt, P, n, n_kv, n_kv, 128, 16, 1.0, 0.0, 0, 0), "too much at once")
+
+
 @pytest.mark.parametrize("change,word", [(dict(D=256, n_q=16), "GQA"), (dict(n_q=18), "GQA"), (dict(bytes=100), "too small"), (dict(work=P + 128), "aligned"),
                                          (dict(rows=70000), "table"), (dict(work=0), "null"), (dict(block=1), "block_size=1")])
 def test_prompts(change, word):
