@@ -776,7 +776,7 @@ int num_sms() {
 // captured on.  Nothing here waits for the device or frees: either would end other threads' captures.  A stream's buffer stays with its
 // handle (which comes back for another stream only once the work of the one before is done), a graph's comes back with the last of the
 // graph and its executables and serves whoever asks next.  Sizes go by powers of two from 1 MiB, so that streams hold twice what their
-// largest product needs at most.
+// largest product needs at most.  cudaStreamPerThread is a stream of its own for each thread that names it, and has a buffer for each.
 struct ModelScratch {
   void* p = nullptr;
   size_t bytes = 0;
@@ -791,12 +791,19 @@ struct SplitBuffer {
   size_t bytes = 0;
   int device = 0;
   cudaStream_t stream = nullptr;
+  unsigned thread = 0;             // of cudaStreamPerThread: whose it is
   unsigned long long capture = 0;  // of the graph that owns it; 0: the stream does
   int kind = 0;                    // 0: parts of split products, 1: pieces of attention (which parts may have to outlive)
   std::atomic<bool> free{false};   // the graph is gone
 };
 std::mutex g_split_mu;
 std::vector<SplitBuffer*> g_split;  // (entries stay: a graph's callback names its own)
+// a number of the calling thread's own, never given again
+unsigned this_thread() {
+  static std::atomic<unsigned> threads{0};
+  static thread_local const unsigned mine = ++threads;
+  return mine;
+}
 }  // namespace
 
 int stream_scratch(int kind, size_t need, cudaStream_t st, float** out) {
@@ -813,13 +820,14 @@ int stream_scratch(int kind, size_t need, cudaStream_t st, float** out) {
     cudaGetLastError();  // (a product that cannot run here fails at its launch)
     capture = 0;
   }
+  const unsigned thread = st == cudaStreamPerThread ? this_thread() : 0;
   std::lock_guard<std::mutex> lock(g_split_mu);
   SplitBuffer *own = nullptr, *spare = nullptr;
   for (SplitBuffer* b : g_split) {
     if (b->device != device || b->bytes < need || b->kind != kind) continue;
     if (b->free.load()) {
       if (!spare || b->bytes < spare->bytes) spare = b;
-    } else if (b->stream == st && b->capture == capture && (!own || b->bytes > own->bytes)) {
+    } else if (b->stream == st && b->thread == thread && b->capture == capture && (!own || b->bytes > own->bytes)) {
       own = b;
     }
   }
@@ -850,6 +858,7 @@ int stream_scratch(int kind, size_t need, cudaStream_t st, float** out) {
       B200Q_CUDA(cudaGraphRetainUserObject(graph, held, 1, cudaGraphUserObjectMove));
     }
     own->stream = st;
+    own->thread = thread;
     own->capture = capture;
     own->free.store(false);
   }

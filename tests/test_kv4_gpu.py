@@ -427,3 +427,47 @@ def test_ways_of_sharing(cuda, way):
         test_wide_windows(cuda, 4999)
     finally:
         lib.decode_attn_q4_set_whole(-1)
+
+
+@pytest.mark.parametrize("what", ["attention", "products"])
+def test_each_threads_own_stream(cuda, what):
+    """cudaStreamPerThread is one handle and a stream for each thread: pieces and parts of two threads do not meet"""
+    import threading
+    from types import SimpleNamespace
+    from llmq_b200 import lib
+    own = SimpleNamespace(cuda_stream=2)   # (the handle)
+    g = torch.Generator().manual_seed(2)
+    if what == "attention":
+        D, n_q, n_kv, args = 64, 8, 2, []
+        for k, ctxs in enumerate([[5000, 33, 9000], [12000, 700]]):
+            cache, table, _ = make_cache(ctxs, n_kv, D, seed=k)
+            qkv = torch.randn(len(ctxs), (n_q + 2 * n_kv) * D, generator=g).to(BF)
+            args.append((qkv.to(cuda), cache.to(cuda), table.to(cuda), torch.tensor(ctxs, dtype=torch.int32, device=cuda)))
+        shape = [(len(a[0]), n_q * D) for a in args]
+
+        def call(k, out, stream=None):
+            q, cache, table, ctx = args[k]
+            lib.decode_attn_q4(q, out, cache, table, ctx, n_q, n_kv, D, BS, D ** -0.5, stream=stream)
+    else:
+        args = [(torch.randn(256, 8192, generator=g).to(BF).to(cuda), torch.randn(512, 8192, generator=g).to(BF).to(cuda)) for _ in range(2)]
+        assert lib.gemm_bf16_splitk(*args[0])[1] > 1
+        shape = [(256, 512)] * 2
+
+        def call(k, out, stream=None):
+            lib.gemm_bf16(*args[k], out, stream=stream)
+    alone, got = ([[torch.zeros(*s, dtype=BF, device=cuda) for _ in range(n)] for s in shape] for n in (1, 20))
+    lib.decode_attn_q4_set_whole(0)
+    try:
+        for k in (0, 1):
+            call(k, alone[k][0])
+            torch.cuda.synchronize()
+        threads = [threading.Thread(target=lambda k=k: [call(k, o, own) for o in got[k]]) for k in (0, 1)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+    finally:
+        lib.decode_attn_q4_set_whole(-1)
+    for k in (0, 1):
+        assert all(torch.equal(o, alone[k][0]) for o in got[k])
