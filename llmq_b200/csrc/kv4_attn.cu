@@ -941,7 +941,8 @@ int b200q_decode_attn_q4(const void* q, int q_stride, void* out, const void* kv4
                   "decode_attn_q4: too much at once: n_seqs=%d bt_stride=%d n_kv=%d (2^32 pages of a head, 2^31 of a sequence, 2^40 in all)", n_seqs,
                   bt_stride, n_kv);
   if (n_seqs == 0) return B200Q_OK;
-  B200Q_CHECK_ARG(q && out && kv4_layer && block_table && ctx_lens, "decode_attn_q4: null argument");
+  // (a table of no columns need not exist)
+  B200Q_CHECK_ARG(q && out && ctx_lens && (bt_stride == 0 || (kv4_layer && block_table)), "decode_attn_q4: null argument");
   B200Q_CHECK_ARG(q_stride % 8 == 0 && q_stride >= n_q * D && ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(kv4_layer)) & 15) == 0,
                   "decode_attn_q4: q (rows of q_stride=%d, a multiple of 8) and the cache must be 16-byte aligned", q_stride);
   B200Q_CHECK_ARG((reinterpret_cast<uintptr_t>(out) & 7) == 0, "decode_attn_q4: out must be 8-byte aligned");

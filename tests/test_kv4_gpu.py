@@ -471,3 +471,20 @@ def test_each_threads_own_stream(cuda, what):
         lib.decode_attn_q4_set_whole(-1)
     for k in (0, 1):
         assert all(torch.equal(o, alone[k][0]) for o in got[k])
+
+
+@pytest.mark.parametrize("D", [64, 256])
+@pytest.mark.parametrize("way", [-1, -2, 0, 1])
+def test_table_of_no_columns(cuda, D, way):
+    """sequences of no tokens, and of any by a table that holds none: zeros"""
+    from llmq_b200 import lib
+    n_q, n_kv, B = 4, 2, 3
+    qkv = torch.randn(B, (n_q + 2 * n_kv) * D, generator=torch.Generator().manual_seed(7)).to(BF).to(cuda)
+    out = torch.full((B + 1, n_q * D), float("nan"), dtype=BF, device=cuda)
+    cache, table = torch.zeros(0, n_kv, 18 * D, dtype=torch.uint8, device=cuda), torch.zeros(B, 0, dtype=torch.int32, device=cuda)
+    lib.decode_attn_q4_set_whole(way)
+    try:
+        lib.decode_attn_q4(qkv, out, cache, table, torch.tensor([0, 5, 0], dtype=torch.int32, device=cuda), n_q, n_kv, D, BS, D ** -0.5)
+    finally:
+        lib.decode_attn_q4_set_whole(-1)
+    assert (out[:B] == 0).all() and torch.isnan(out[B].float()).all()
