@@ -718,7 +718,7 @@ int b200q_pages_compact(const int32_t* table_dev, const int32_t* lens_dev, int n
                         int num_blocks, int block_size, int32_t* table_out_dev, int32_t* refs_out_dev, int32_t* map_dev,
                         int32_t* pairs_dev, int32_t* status_dev, void* stream);
 /* test hook: b200q_decode_attn_q4 gives a sequence's heads to warps whole (1), pages evenly (0), or heads to clusters (-2, where they are few);
- *     -1: by size, and as B200Q_BATCH_INVARIANT says */
+ *     -3: as 0, where there is no memory for the pieces; -1: by size, and as B200Q_BATCH_INVARIANT says */
 int b200q_decode_attn_q4_set_whole(int whole);
 
 /* nonzero once a kernel's bounded wait has run out in this process (its outputs are then missing or wrong); engine steps report

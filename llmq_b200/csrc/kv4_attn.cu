@@ -851,7 +851,9 @@ __global__ void __launch_bounds__(Q4Cluster<D>::WARPS * 32, Q4Cluster<D>::CTAS) 
   }
 }
 
-int g_q4_whole = -1;  // test hook: 1 / 0 give items to warps whole or not, -2 to clusters (-1: by size, and as B200Q_BATCH_INVARIANT says)
+// test hook: 1 / 0 give items to warps whole or not, -2 to clusters, -3 as 0 but that the pieces ask for more memory than any GPU has (-1: by size,
+// and as B200Q_BATCH_INVARIANT says)
+int g_q4_whole = -1;
 static std::mutex g_q4_pair;  // no other thread's pieces on the same stream between a stream kernel and its join
 
 // CTAs of a cluster for each of these items of up to `pages` pages, or 0: the kernel above.  Times in us, fitted to 1 to 450 sequences of 16 to 16000
@@ -898,10 +900,11 @@ static int launch_kv4_stream(const Kv4Args& a, cudaStream_t st) {
       count_launch();
       return B200Q_OK;
     }
-  bool whole = g_q4_whole < 0 ? batch_invariant() || width <= 8 : g_q4_whole != 0;
+  bool whole = g_q4_whole == -1 || g_q4_whole == -2 ? batch_invariant() || width <= 8 : g_q4_whole == 1;
   float* scratch = nullptr;
   // (where there is no memory for pieces, items go to warps whole)
-  if (!whole && stream_scratch(1, (size_t)(q4_chain_floats(warps) + 2 * warps * q4_piece_floats(a.G, D)) * sizeof(float), st, &scratch)) {
+  const size_t bytes = g_q4_whole == -3 ? (size_t)1 << 60 : (size_t)(q4_chain_floats(warps) + 2 * warps * q4_piece_floats(a.G, D)) * sizeof(float);
+  if (!whole && stream_scratch(1, bytes, st, &scratch)) {
     cudaGetLastError();
     whole = true;
   }
@@ -921,7 +924,7 @@ using namespace b200q;
 extern "C" {
 
 int b200q_decode_attn_q4_set_whole(int whole) {
-  B200Q_CHECK_ARG(whole >= -2 && whole <= 1, "decode_attn_q4: whole must be -2..1");
+  B200Q_CHECK_ARG(whole >= -3 && whole <= 1, "decode_attn_q4: whole must be -3..1");
   g_q4_whole = whole;
   bump_tuning_epoch();
   return B200Q_OK;

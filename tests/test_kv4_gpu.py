@@ -473,6 +473,102 @@ def test_each_threads_own_stream(cuda, what):
         assert all(torch.equal(o, alone[k][0]) for o in got[k])
 
 
+@pytest.mark.parametrize("D,n_q,n_kv", [(64, 8, 2), (128, 8, 1), (256, 4, 1)])
+def test_without_memory_for_pieces(cuda, D, n_q, n_kv):
+    """items go to warps whole where scratch is refused, in a call and in a capture, and are shared again in the next call"""
+    from llmq_b200 import lib
+    ctxs = [5000, 33, 0, 900]
+    cache, table, rows = make_cache(ctxs, n_kv, D, seed=D)
+    qkv = torch.randn(len(ctxs), (n_q + 2 * n_kv) * D, generator=torch.Generator().manual_seed(7)).to(BF)
+    args = (cache.to(cuda), table.to(cuda), torch.tensor(ctxs, dtype=torch.int32, device=cuda), n_q, n_kv, D, BS, D ** -0.5)
+    q = qkv.to(cuda)
+    outs = [torch.full((len(ctxs), n_q * D), float("nan"), dtype=BF, device=cuda) for _ in range(4)]
+    graph = torch.cuda.CUDAGraph()
+    try:
+        for way, out in ((1, outs[0]), (-3, outs[1]), (0, outs[2])):
+            lib.decode_attn_q4_set_whole(way)
+            lib.decode_attn_q4(q, out, *args)
+        lib.decode_attn_q4_set_whole(-3)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            lib.decode_attn_q4(q, outs[3], *args)
+        graph.replay()
+        torch.cuda.synchronize()
+    finally:
+        lib.decode_attn_q4_set_whole(-1)
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[3])
+    for i, c in enumerate(ctxs):
+        if c == 0:
+            assert all((o[i] == 0).all() for o in outs)
+            continue
+        ref, weight, size = attention(qkv[i: i + 1, : n_q * D].view(1, n_q, D), *rows[i], torch.tensor([c - 1]), D ** -0.5)
+        for o in outs:
+            attention_close(o[i].view(1, n_q, D), ref, weight, size, D, 2.0 ** -11, f"ctx {c}")
+
+
+@pytest.mark.parametrize("D,n_q,n_kv", [(64, 8, 2), (256, 4, 1)])
+def test_pieces_of_calls_at_once(cuda, D, n_q, n_kv):
+    """calls whose pieces lie in scratch: on streams of their own and in graphs, then from two threads on one stream"""
+    import threading
+    from llmq_b200 import lib
+    lib.decode_attn_q4_set_whole(0)
+    try:
+        test_two_calls_at_once(cuda, D, n_q, n_kv)
+        args = []
+        for k, ctxs in enumerate([[5000, 33, 9000], [12000, 700]]):
+            cache, table, _ = make_cache(ctxs, n_kv, D, seed=k)
+            qkv = torch.randn(len(ctxs), (n_q + 2 * n_kv) * D, generator=torch.Generator().manual_seed(k)).to(BF)
+            args.append((qkv.to(cuda), cache.to(cuda), table.to(cuda), torch.tensor(ctxs, dtype=torch.int32, device=cuda)))
+        stream = torch.cuda.Stream()
+
+        def call(k, out):
+            q, cache, table, ctx = args[k]
+            lib.decode_attn_q4(q, out, cache, table, ctx, n_q, n_kv, D, BS, D ** -0.5, stream=stream)
+
+        alone, got = ([[torch.zeros(len(a[0]), n_q * D, dtype=BF, device=cuda) for _ in range(n)] for a in args] for n in (1, 40))
+        torch.cuda.synchronize()
+        for k in (0, 1):
+            call(k, alone[k][0])
+            torch.cuda.synchronize()
+        threads = [threading.Thread(target=lambda k=k: [call(k, o) for o in got[k]]) for k in (0, 1)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        for k in (0, 1):
+            assert all(torch.equal(o, alone[k][0]) for o in got[k])
+    finally:
+        lib.decode_attn_q4_set_whole(-1)
+
+
+@pytest.mark.parametrize("D,n_q,n_kv", [(64, 8, 2), (256, 4, 1)])
+@pytest.mark.parametrize("window", [0, 40])
+def test_prompts_of_few_rows_of_a_large_table(cuda, D, n_q, n_kv, window):
+    """an engine's table: a row for every slot and columns up to the model's length, of which the step's portions see a few; the others hold
+    whatever they do"""
+    from llmq_b200 import lib
+    portions, at_rows = [(5, 11), (133, 0), (70, 900)], [63, 5, 40]
+    cache, small, rows = make_cache([n + past for n, past in portions], n_kv, D, seed=D)
+    table = torch.full((64, 512), 2 ** 30, dtype=torch.int32)
+    for i, r in enumerate(at_rows):
+        held_pages = (sum(portions[i]) + 15) // 16
+        table[r, :held_pages] = small[i, :held_pages]
+    tiles, T = tiles_of(portions)
+    tiles[:, 0] = torch.tensor(at_rows, dtype=torch.int32)[tiles[:, 0].long()]
+    qkv = torch.randn(T, (n_q + 2 * n_kv) * D, generator=torch.Generator().manual_seed(7)).to(BF)
+    out = torch.full((T, n_q * D), float("nan"), dtype=BF, device=cuda)
+    work = torch.full((lib.prefill_attn_q4_workspace(*table.shape, n_kv, D),), 0xFF, dtype=torch.uint8, device=cuda)
+    lib.prefill_attn_q4(qkv.to(cuda), out, cache.to(cuda), table.to(cuda), tiles.to(cuda), n_q, n_kv, D, BS, D ** -0.5, work, window=window)
+    got, at = out.cpu(), 0
+    for i, (n, past) in enumerate(portions):
+        q = qkv[at: at + n, : n_q * D].view(n, n_q, D)
+        ref, weight, sz = attention(q, *rows[i], torch.arange(past, past + n), D ** -0.5, 0.0, window)
+        attention_close(got[at: at + n].view(n, n_q, D), ref, weight, sz, D, 2.0 ** -8, f"portion {i}")
+        at += n
+    assert lib.load().b200q_wait_failures() == 0
+
+
 @pytest.mark.parametrize("D", [64, 256])
 @pytest.mark.parametrize("way", [-1, -2, 0, 1])
 def test_table_of_no_columns(cuda, D, way):
