@@ -169,12 +169,6 @@ __device__ __forceinline__ void scale_ot(float (&o)[D / 16][4], float h0, float 
   }
 }
 
-__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
-  uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
-  return r;
-}
-
 // zero rows [n_valid, BS) of a V page in shared memory (whole warp), so that masked
 // probabilities (exactly 0) never meet stale NaN/Inf bit patterns in the PV mma.
 template <int D, int BS>

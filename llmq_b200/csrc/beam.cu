@@ -37,28 +37,6 @@ __device__ __forceinline__ uint32_t beam_order(uint32_t h) {
   if (h == 0x8000u) h = 0u;
   return (h & 0x8000u) ? 0xffffu ^ h : h | 0x8000u;
 }
-// two numbers at once, as neighbouring registers (one issue slot)
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pair_of(float lo, float hi) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ float2 halves_of(f32x2 v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 // Sums of a row are those of 2^(L x - c), L the fp32 number next to log2(e) and c a whole number near L times the largest logit so far: L x - c is
 // rounded once, so that it is off by 2^-24 of itself, not of x, and by more than 1.5 x 2^-24 only where the term is small beside the largest.  What L is
 // off by makes e^x of 2^(L x) by a factor e^(BEAM_LOW x), for which that of the largest logit stands.
@@ -125,11 +103,6 @@ struct BeamRow {
   }
 };
 
-__device__ __forceinline__ uint4 lds_v4(uint32_t at) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
-  return v;
-}
 // the next place in a list in shared memory (few lanes at a time ask for one: no need to ask for all of them together)
 __device__ __forceinline__ int next_place(int* count) {
   int at;

@@ -41,11 +41,6 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-__device__ __forceinline__ uint32_t transposed8x8(uint32_t v) {
-  uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
-  return r;
-}
 __device__ __forceinline__ float q4_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -87,11 +82,6 @@ struct Q4State {
   }
 };
 
-__device__ __forceinline__ uint4 lds_v4(uint32_t at) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
-  return v;
-}
 __device__ __forceinline__ uint2 lds_v2(uint32_t at) {
   uint2 v;
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
@@ -310,7 +300,7 @@ __device__ __forceinline__ void q4_turn(uint32_t at, const Q4Query<D>& q, Q4Stat
   }
 #pragma unroll
   for (int x = 0; x < P; ++x) {
-    const uint32_t p0 = transposed8x8(pack_half2(s[x][0], s[x][1])), p1 = transposed8x8(pack_half2(s[x][2], s[x][3]));
+    const uint32_t p0 = movmatrix_trans(pack_half2(s[x][0], s[x][1])), p1 = movmatrix_trans(pack_half2(s[x][2], s[x][3]));
     uint32_t keep = 0;
     if (kEdge) {
 #pragma unroll
