@@ -668,7 +668,8 @@ int b200q_decode_attn_q4(const void* q_dev, int q_stride, void* out_dev, const v
                          float scale, float softcap, int window, void* stream);
 /* b200q_prefill_attn_seqs over a 4-bit cache.  The workspace (256-byte aligned, of b200q_prefill_attn_q4_workspace bytes for the
  *     block table's n_seqs rows of bt_stride entries) holds the pages that the portions see as 16-bit ones; what is in it need not
- *     be kept between calls.  GQA group <= 8, at D = 256 <= 4. */
+ *     be kept between calls.  Its size and a part of the work follow the table's, not what the portions see: hand over the rows and columns
+ *     that the step's portions have.  GQA group <= 8, at D = 256 <= 4. */
 int64_t b200q_prefill_attn_q4_workspace(int n_seqs, int bt_stride, int n_kv, int D);
 int b200q_prefill_attn_q4(const void* q_dev, int q_stride, void* out_dev, const void* kv4_layer_dev, const int32_t* block_table_dev,
                           int bt_stride, int n_seqs, const int32_t* tiles_dev, int n_tiles, int n_q, int n_kv, int D, int block_size,
@@ -681,7 +682,9 @@ int b200q_prefill_attn_q4(const void* q_dev, int q_stride, void* out_dev, const 
  *     logits[r, v] of a group's rows the K largest, best first, of equal ones the lowest row, then the lowest token.  cand_* [groups, K]:
  *     the value (fp32; compared in 64 bits), v, r.  next_* [groups, beams]: the first `beams` of them whose token is none of
  *     stops[n_stops]; where there are fewer, value -infinity, token 0, the group's first row.  A row whose score is not finite, or
- *     whose logits are all -infinity or one +infinity, counts as -infinity throughout; a NaN logit as -infinity.
+ *     whose logits are all -infinity or one +infinity, counts as -infinity throughout; a NaN logit as -infinity, -0 as 0.  Within a row the
+ *     order is exact.  A row's logarithm is off by 10.5 x 2^-24 at most, so that candidates of different rows that are nearer to each other
+ *     than twice that may change places; equal rows give equal bits, and no value is above its row's score.
  *     next_scores may be scores.  logits and workspace are 16-byte aligned; the workspace need not be kept between calls. */
 int64_t b200q_beam_select_workspace(int groups, int beams, int64_t V, int K);
 int b200q_beam_select(const void* logits_dev, const float* scores_dev, int groups, int beams, int64_t V, const int32_t* stops_dev,

@@ -9,9 +9,9 @@
 // Scores that are compared across rows are 64 bits; a row's logarithm comes from sums whose terms are off by 2^-22 (the exponential) and 1.5 x 2^-24
 // (its exponent's rounding) at most, whatever the logits' size, and go through five additions in fp32 before those in 64 bits.
 // Bound: the logits, 2 bytes each, once; next to it the exponentials (16 a cycle and SM: two thirds of the memory's
-// time) and some nine instructions a logit.  Logits come by asynchronous copies two tiles ahead (in registers a tile ahead 55 us).
-// 48 groups of 8 beams over 256000 tokens, 16 candidates: 51.8 us (the memory's share 30; the first kernel 47, of which an eighth is looking for
-// the 16 best: 41 with one; with 4 or 3 CTAs per SM in place of 5 53.7 and 58.1), one group of 4 over 128256: 10.2.
+// time) and some nine instructions a logit.  Logits come by asynchronous copies two tiles ahead (in registers a tile ahead 2.7 us more).
+// 48 groups of 8 beams over 256000 tokens, 16 candidates: 54.4 us (the memory's share 30; 46.5 for one candidate of each row, so that looking for
+// the 16 best and the second kernel's ranks are 8; with 4 or 3 CTAs per SM in place of 5 55.3 and 60.0), one group of 4 over 128256: 10.4.
 #include "common.cuh"
 
 namespace b200q {
@@ -111,7 +111,7 @@ __device__ __forceinline__ int next_place(int* count) {
 }
 
 // A piece of a row, in tiles of TILE vectors; the next ones are on their way while one is looked at.  Vectors collected from which on they are
-// ranked: 24 / 48 / 96 cost 384 rows of 256000 logits 52.5 / 52.2 / 57.2 us.
+// ranked: 24 / 48 / 96 cost 384 rows of 256000 logits 54.9 / 54.4 / 60.0 us.
 constexpr int BEAM_NV = 4, TILE = BEAM_NV * BEAM_THREADS, BEAM_MANY = 48, BEAM_RING = 2;
 template <bool kAligned>
 __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* logits, long long V, int K, long long row0, long long rows,
@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
   int2* to = entries + out * K;
   auto tell = [&](int rank, uint64_t key) { to[rank] = make_int2(__float_as_int(value_of(key)), (int)(0xffffffffu - (uint32_t)key)); };
   // Too many reached the bound (logits in some order, a mask over the row's first part): tile by tile once more, each with a bound of its own, the
-  // K-th of the threads' largest logits.  384 rows of 256000 logits whose first half is hidden: 189 us (one after the other, as below, 1160).
+  // K-th of the threads' largest logits.  384 rows of 256000 logits whose first half is hidden: 178 us (one after the other, as below, 1160).
   if (overflow) {
     overflow = false;
     kept = 0;
@@ -646,8 +646,8 @@ __global__ void __launch_bounds__(MERGE_THREADS) beam_groups_kernel(BeamArgs a) 
 }
 
 // Pieces of a row: the least time of the SM that has most CTAs, each its logits (five CTAs at once are as fast as an SM gets) and 11000 logits'
-// worth beside them, and of the lists that the second kernel has to look at.  384 rows of 256000 logits: 1 / 2 / 3 / 4 / 6 / 8 pieces 69.0 /
-// 53.7 / 52.3 / 55.1 / 64.7 / 65.6 us; 4 rows of 128256: 8 / 16 / 32 / 48 / 64 pieces 10.4 / 9.9 / 10.1 / 11.1 / 11.9 us.
+// worth beside them, and of the lists that the second kernel has to look at.  384 rows of 256000 logits: 1 / 2 / 3 / 4 / 6 / 8 pieces 71.3 /
+// 56.2 / 54.6 / 57.8 / 64.6 / 67.2 us; 4 rows of 128256: 8 / 16 / 32 / 48 / 64 pieces 11.1 / 10.5 / 10.5 / 11.4 / 12.4 us.
 // B200Q_BATCH_INVARIANT=1: as for 64 rows whatever their number, since a row's sum is that of its pieces' sums.
 static int beam_pieces(long long rows, long long V) {
   if (batch_invariant()) rows = 64;

@@ -15,8 +15,8 @@
 //   * A warp has its own pages on their way, by asynchronous copies; nobody waits for another warp.
 // Queries are divided by the power of two in their largest magnitude before they become fp16, which costs nothing that fp32 sums would keep.
 // Many sequences are streamed through by all warps (kv4_stream_kernel), few get a cluster of CTAs for each head (kv4_cluster_kernel).
-// 700 sequences of 33 to 1000 tokens, 32 / 8 heads of 128: 94.9 us, 4.5 TB/s (the memory's share 66 us); 22 of 16000: 84, its copies alone 70 and
-// its arithmetic alone 75; 16 of 1000 9.2; 3 of 9000 to 16000, heads of 64: 13.4 (3.4).
+// 700 sequences of 33 to 1000 tokens, 32 / 8 heads of 128: 95.1 us, 4.5 TB/s (the memory's share 66 us); 22 of 16000: 84, its copies alone 70 and
+// its arithmetic alone 75; 16 of 1000 9.6; 3 of 9000 to 16000, heads of 64: 13.5 (3.4); 64 of 100 to 1500, 16 / 8 heads of 256, cap: 33.9 (17.5).
 #include <algorithm>
 #include <mutex>
 #include <type_traits>
@@ -849,8 +849,8 @@ static std::mutex g_q4_pair;  // no other thread's pieces on the same stream bet
 // CTAs of a cluster for each of these items of up to `pages` pages, or 0: the kernel above.  Times in us, fitted to 1 to 450 sequences of 16 to 16000
 // tokens, 8 heads.  Clusters: 4 and what a CTA's pages take (beside three others on an SM; alone half; 16 CTAs to a cluster 2.5 more), or several
 // rounds of CTAs; the kernel above: `start`, or where items are whole what the pages of one take a warp, and `slope` times what all pages take from
-// memory.  us above / with clusters, D = 128: one sequence of 64 tokens 5.5 / 3.1, of 300 10.2 / 5.1, 16 of 1000 14.5 / 9.2, 16 of 4000 25 / 22.9, 24 of
-// 4000 32.9 / 36.1, 150 of 300 23.3 / 20.2, 250 of 128 13.8 / 16.2; D = 256: 6 of 4000 22.8 / 19.1, 8 of 4000 26.3 / 32.2.  Lengths below the table's width:
+// memory.  us above / with clusters, D = 128: one sequence of 64 tokens 5.9 / 3.4, of 300 10.8 / 5.6, 16 of 1000 15.1 / 9.6, 16 of 4000 24.4 / 20.5, 24 of
+// 4000 33.9 / 34.5, 150 of 300 22.5 / 18.1, 250 of 128 14.1 / 15.8; D = 256: 6 of 4000 22.0 / 17.1, 8 of 4000 25.4 / 26.6.  Lengths below the table's width:
 // 48 of 200 to 2000 23.8 / 30.2, 700 of 33 to 1000 95 / 105.
 template <int D>
 static int kv4_clusters(long long items, int pages, bool forced) {
