@@ -282,11 +282,13 @@ __global__ void __launch_bounds__(BEAM_THREADS, 5) beam_rows_kernel(const bf16* 
     const int k = prune(kept);
     overflow |= k < 0;
     if (!overflow) kept = k;
-    if (overflow)  // (whatever is found from here on does not matter, but for logits that c has to follow)
-      bound = __uint_as_float(__float_as_uint((1.f - minus_c) * (1.f / BEAM_L)) & 0xffff0000u);
-    else if (kept == K)
-      bound = value_of(best[K - 1]);
-    raise(bound * BEAM_L);  // (logits below the bound are not looked at: c is not below it)
+    if (overflow) {  // (whatever is found from here on does not matter, but for logits that c has to follow: the bf16 number below c's reach)
+      const uint32_t b = __float_as_uint((1.f - minus_c) * (1.f / BEAM_L));
+      bound = __uint_as_float((b + (b >> 31 ? 0xffffu : 0u)) & 0xffff0000u);
+    } else {
+      if (kept == K) bound = value_of(best[K - 1]);
+      raise(bound * BEAM_L);  // (logits below the bound are not looked at: c is not below it)
+    }
     bound2 = __float_as_uint(bound) >> 16 | __float_as_uint(bound);
   };
   int stage = 0;

@@ -157,6 +157,26 @@ def test_peak_over_a_flat_tail(cuda, V, R):
     assert ((cand[0].double() - ref).abs() <= LOG_SUM + 2.0 ** -24 * abs(ref)).all(), (cand[0].double() - ref).abs().max() * 2 ** 24
 
 
+@pytest.mark.parametrize("V,R", [(128256, 740), (256000, 384), (50257, 300)])
+def test_sums_of_rows_with_too_many_near_the_bound(cuda, V, R):
+    """rows of hundreds of equal largest logits, of any size, with and without larger ones behind them"""
+    from llmq_b200 import lib
+    sizes = [-500.0, -556.0, -598.0, -37.0, -3.0, 0.0, 5.0, 41.0, 300.0, 556.0]
+    x = torch.empty(R, V, dtype=BF)
+    ref = []
+    for i in range(R):
+        size, more = sizes[i % 10], (0.0, 1.0, 4.0, 12.0)[i // 10 % 4]
+        x[i] = size
+        at = V - 1 - 97 * (i % 5)
+        x[i, at] = size + more
+        y = float(x[i, at]) - float(x[i, 0])   # (sizes are rounded to bf16)
+        ref.append(-math.log1p((V - 1) * math.exp(-y)))
+    cand, _ = select(lib, cuda, x, torch.zeros(R), 1, 1, [])
+    ref = torch.tensor(ref, dtype=torch.float64)
+    e = (cand[0].flatten().double() - ref).abs()
+    assert (e <= LOG_SUM + 2.0 ** -24 * ref.abs()).all(), (e * 2 ** 24).max()
+
+
 def test_many_groups(cuda):
     from llmq_b200 import lib
     g = torch.Generator().manual_seed(1)
