@@ -724,6 +724,44 @@ int b200q_pages_compact(const int32_t* table_dev, const int32_t* lens_dev, int n
  *     -3: as 0, where there is no memory for the pieces; -1: by size, and as B200Q_BATCH_INVARIANT says */
 int b200q_decode_attn_q4_set_whole(int whole);
 
+/* ---- linear layers in 8 bits (fp8_ops.cu, gemm_fp8.cu; conversions: fp8.cuh) --------------------------------------------------
+ * A value is an e4m3 code times an fp32 scale.  Activations: codes [T, K], scales [ceil(K / 128)][ld]: element (t, k) is
+ * codes[t, k] * scales[k / 128][t]; ld >= T, for products a multiple of 4.  Weights: codes [N, K], scales [ceil(N / 128)]
+ * [ceil(K / 128)], one for a square of 128 x 128.  K is a multiple of 16.  A scale is a 448th of its block's largest magnitude (2^-100 at
+ * least), codes are rounded to nearest (even).  A block with a NaN or an infinity reads back as NaN throughout.  Matrices are
+ * 16-byte aligned; scales behind the last row are neither written nor do they count.  The activations' scales of products are 16-byte aligned too. */
+
+/* b200q_rmsnorm / b200q_add_rmsnorm with an output in 8 bits: residual <- x + residual (rounded to its type; NULL: x alone), y = that
+ *     / sqrt(mean of its squares + eps) * w, not rounded before it is quantised.  dtype: of x, residual and w.  x is not written; H <= 16384. */
+int b200q_rmsnorm_fp8(const void* x_dev, void* residual_dev, const void* w_dev, void* y_dev, float* scales_dev, int ld_scales, int T, int H,
+                      float eps, int dtype, void* stream);
+/* rows of x (ld_x elements apart, a multiple of 8) in 8 bits; rows != NULL: row i of y is row rows[i] of x (tokens sorted by expert: perm_tok
+ *     of b200q_moe_route) */
+int b200q_quantize_fp8(const void* x_dev, int64_t ld_x, const int32_t* rows_dev, void* y_dev, float* scales_dev, int ld_scales, int T, int K,
+                       int dtype, void* stream);
+/* weights [groups][N, K] in 8 bits */
+int b200q_quantize_fp8_weight(const void* w_dev, void* q_dev, float* scales_dev, int groups, int N, int K, int dtype, void* stream);
+/* C[M,N] = A[M,K] * W[N,K]^T of values in 8 bits, fp32 sums, C bf16 or (out_f32) fp32; N % 8 == 0.  Waits are bounded
+ *     (b200q_wait_failures), for the products below too.  No scratch. */
+int b200q_gemm_fp8(const void* A_dev, const float* a_scales_dev, int ld_a_scales, const void* W_dev, const float* w_scales_dev, void* C_dev,
+                   int M, int N, int K, int out_f32, void* stream);
+/* the same with a gated unit, whose values leave in 8 bits: Y [M, N/2] = act(gate) * up, act 0 = SiLU, 1 = tanh GELU; rows of W in turns of
+ *     128 as for b200q_gemm_swiglu_bf16 (N % 256 == 0).  Sums are not rounded before the unit, nor its values before they are quantised. */
+int b200q_gemm_gated_fp8(const void* A_dev, const float* a_scales_dev, int ld_a_scales, const void* W_dev, const float* w_scales_dev, void* Y_dev,
+                         float* y_scales_dev, int ld_y_scales, int M, int N, int K, int act, void* stream);
+/* both by expert: the rows of A and of the output are sorted by group, W is [groups][N, K] (scales [groups][ceil(N/128)][ceil(K/128)]);
+ *     tab, n_mt: the tiles of up to 128 rows that b200q_moe_route wrote (n_mt of them, at most max_mtiles; 16-byte aligned): entry {group, first
+ *     row, end of the group's rows, 0} is rows first .. min(first + 128, end) - 1, which lie in 0 .. a_rows - 1, in no other entry too.
+ *     Rows of no entry stay as they are. */
+int b200q_gemm_grouped_fp8(const void* A_dev, int a_rows, const float* a_scales_dev, int ld_a_scales, const void* W_dev, const float* w_scales_dev,
+                           int groups, void* C_dev, int N, int K, const void* tab_dev, const int32_t* n_mt_dev, int max_mtiles, int out_f32,
+                           void* stream);
+int b200q_gemm_grouped_gated_fp8(const void* A_dev, int a_rows, const float* a_scales_dev, int ld_a_scales, const void* W_dev,
+                                 const float* w_scales_dev, int groups, void* Y_dev, float* y_scales_dev, int ld_y_scales, int N, int K,
+                                 const void* tab_dev, const int32_t* n_mt_dev, int max_mtiles, int act, void* stream);
+/* test hook: 0 = by size, 1 = small tiles, 2 = large tiles of one CTA, 3 = of a pair (dense products) */
+int b200q_gemm_fp8_set_mode(int mode);
+
 /* nonzero once a kernel's bounded wait has run out in this process (its outputs are then missing or wrong); engine steps report
  * it as B200Q_ECUDA.  Calls return before their kernels run: who calls b200q_gemm_* (up to 128 rows), b200q_prefill_attn* or the
  * layered attention directly asks here once the stream has been waited for. */

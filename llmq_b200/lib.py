@@ -317,6 +317,14 @@ SIGNATURES = {
     "b200q_prefill_attn_q4": (_i, [_vp, _i, _vp, _vp, _vp, _i, _i, _vp, _i, _i, _i, _i, _i, _f, _f, _i, _vp, _i64, _vp]),
     "b200q_beam_select_workspace": (_i64, [_i, _i, _i64, _i]),
     "b200q_beam_select": (_i, [_vp, _vp, _i, _i, _i64, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "b200q_rmsnorm_fp8": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _i, _vp]),
+    "b200q_quantize_fp8": (_i, [_vp, _i64, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "b200q_quantize_fp8_weight": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "b200q_gemm_fp8": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "b200q_gemm_gated_fp8": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
+    "b200q_gemm_grouped_fp8": (_i, [_vp, _i, _vp, _i, _vp, _vp, _i, _vp, _i, _i, _vp, _vp, _i, _i, _vp]),
+    "b200q_gemm_grouped_gated_fp8": (_i, [_vp, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _vp, _vp, _i, _i, _vp]),
+    "b200q_gemm_fp8_set_mode": (_i, [_i]),
     "b200q_pages_fork": (_i, [_vp, _vp, _i, _vp, _i, _i, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp]),
     "b200q_pages_free": (_i, [_vp, _vp, _vp, _i, _i, _vp, _i, _i, _vp]),
     "b200q_pages_copy": (_i, [_vp, _vp, _i, _vp, _i64, _i, _i64, _i, _vp]),
@@ -607,7 +615,7 @@ _TORCH = {}
 def _types():
     import torch
 
-    _TORCH.update(i=torch.int32, f=torch.float32, h=torch.bfloat16)
+    _TORCH.update(i=torch.int32, f=torch.float32, h=torch.bfloat16, e=torch.float8_e4m3fn)
     return _TORCH
 
 
@@ -620,7 +628,7 @@ def _refuse(t, kind, what, dev):
 
 
 def _arg(t, kind, what, dev=0):
-    """data_ptr of a contiguous tensor of this type ("i", "f", "h": int32, fp32, bf16; None: any) on device dev, the current one"""
+    """data_ptr of a contiguous tensor of this type ("i", "f", "h", "e": int32, fp32, bf16, e4m3; None: any) on device dev, the current one"""
     if t.get_device() != dev or not t.is_contiguous() or (kind and t.dtype is not (_TORCH or _types())[kind]):
         _refuse(t, kind, what, dev)
     return t.data_ptr()
@@ -760,3 +768,109 @@ def pages_compact(table, lens, refs, table_out, refs_out, page_map, pairs, statu
     check(load().b200q_pages_compact(_arg(table, "i", "table", dev), _arg(lens, "i", "lens", dev), rows, columns, _arg(refs, "i", "refs", dev), n,
                                      block_size, _arg(table_out, "i", "table_out", dev), _arg(refs_out, "i", "refs_out", dev),
                                      _arg(page_map, "i", "page_map", dev), _arg(pairs, "i", "pairs", dev), _arg(status, "i", "status", dev), s))
+
+
+# ---- linear layers in 8 bits (include/b200q.h: layout of codes and scales, what each computes) ------------------------------
+# Codes are float8_e4m3fn tensors.  Scales of rows: fp32 [ceil(K / 128), ld], ld >= rows (fp8_row_scales makes one); of weights: fp32
+# [ceil(N / 128), ceil(K / 128)], with as many leading dimensions as the weights have.
+ACTS = {"silu": 0, "gelu": 1}
+
+
+def fp8_row_scales(rows, K, device="cuda"):
+    """room for the scales of `rows` rows of K values"""
+    import torch
+
+    return torch.empty((K + 127) // 128, (rows + 3) // 4 * 4, dtype=torch.float32, device=device)
+
+
+def _row_scales(t, rows, K, what, dev):
+    """(data_ptr, ld) of scales of rows"""
+    blocks, ld = t.shape
+    _want(blocks == (K + 127) // 128 and ld >= rows, f"{what}: [{(K + 127) // 128}, {rows} or more] is wanted, not {tuple(t.shape)}")
+    return _arg(t, "f", what, dev), ld
+
+
+def _weight_scales(t, w, dev):
+    N, K = w.shape[-2:]
+    _want(t.shape == (*w.shape[:-2], (N + 127) // 128, (K + 127) // 128), f"w_scales: {tuple(t.shape)} does not fit {tuple(w.shape)}")
+    return _arg(t, "f", "w_scales", dev)
+
+
+def _float(t, what):
+    """dtype code of a bf16 or fp32 tensor"""
+    kinds = _TORCH or _types()
+    if t.dtype is kinds["h"]:
+        return "h", DTYPE_BF16
+    _want(t.dtype is kinds["f"], f"{what}: {t.dtype}, neither bfloat16 nor float32")
+    return "f", DTYPE_F32
+
+
+def rmsnorm_fp8(x, w, y, scales, eps, residual=None, stream=None):
+    """residual <- x + residual (None: x alone); y, scales = that, RMS-normed and times w, in 8 bits.  x is not written."""
+    (T, H), (s, dev), (kind, dtype) = x.shape, _here(stream), _float(x, "x")
+    _want(w.numel() == H and y.shape == x.shape and (residual is None or residual.shape == x.shape), "rmsnorm_fp8: w, y or residual do not fit x")
+    ps, ld = _row_scales(scales, T, H, "scales", dev)
+    check(load().b200q_rmsnorm_fp8(_arg(x, kind, "x", dev), 0 if residual is None else _arg(residual, kind, "residual", dev), _arg(w, kind, "w", dev),
+                                   _arg(y, "e", "y", dev), ps, ld, T, H, eps, dtype, s))
+
+
+def quantize_fp8(x, y, scales, rows=None, stream=None):
+    """y, scales = the rows of x (of x[rows]) in 8 bits; x may be a slice of wider rows"""
+    (n, K), (T, Ky), (s, dev), (kind, dtype) = x.shape, y.shape, _here(stream), _float(x, "x")
+    _want(K == Ky and (T <= n if rows is None else rows.numel() == T), "quantize_fp8: y or rows do not fit x")
+    _want(x.get_device() == dev and (x.stride(1) == 1 or K == 1), f"x: rows on device {dev}, the current one, are wanted")
+    ps, ld = _row_scales(scales, T, K, "scales", dev)
+    ld_x = x.stride(0) if n > 1 else (K + 7) // 8 * 8
+    check(load().b200q_quantize_fp8(x.data_ptr(), ld_x, 0 if rows is None else _arg(rows, "i", "rows", dev), _arg(y, "e", "y", dev), ps, ld, T, K,
+                                    dtype, s))
+
+
+def quantize_fp8_weight(w, q, scales, stream=None):
+    """q, scales = weights [N, K] or [groups, N, K] in 8 bits"""
+    (s, dev), (kind, dtype) = _here(stream), _float(w, "w")
+    _want(w.dim() in (2, 3) and q.shape == w.shape, "quantize_fp8_weight: w is [N, K] or [groups, N, K], q of its shape")
+    N, K = w.shape[-2:]
+    check(load().b200q_quantize_fp8_weight(_arg(w, kind, "w", dev), _arg(q, "e", "q", dev), _weight_scales(scales, w, dev),
+                                           w.shape[0] if w.dim() == 3 else 1, N, K, dtype, s))
+
+
+def gemm_fp8(a, a_scales, w, w_scales, c, stream=None):
+    """c [M, N] (bf16 or fp32) = a [M, K] * w [N, K]^T, both in 8 bits"""
+    (M, K), (N, Kw), (s, dev), (kind, dtype) = a.shape, w.shape, _here(stream), _float(c, "c")
+    _want(K == Kw and c.shape == (M, N), "gemm_fp8: shapes do not fit")
+    ps, ld = _row_scales(a_scales, M, K, "a_scales", dev)
+    check(load().b200q_gemm_fp8(_arg(a, "e", "a", dev), ps, ld, _arg(w, "e", "w", dev), _weight_scales(w_scales, w, dev), _arg(c, kind, "c", dev), M, N,
+                                K, dtype, s))
+
+
+def gemm_gated_fp8(a, a_scales, w, w_scales, y, y_scales, act="silu", stream=None):
+    """y [M, N / 2], y_scales = act(gate) * up of a * w^T in 8 bits; rows of w: gate and up in turns of 128"""
+    (M, K), (N, Kw), (s, dev) = a.shape, w.shape, _here(stream)
+    _want(K == Kw and y.shape == (M, N // 2), "gemm_gated_fp8: shapes do not fit")
+    (ps, ld), (py, ldy) = _row_scales(a_scales, M, K, "a_scales", dev), _row_scales(y_scales, M, N // 2, "y_scales", dev)
+    check(load().b200q_gemm_gated_fp8(_arg(a, "e", "a", dev), ps, ld, _arg(w, "e", "w", dev), _weight_scales(w_scales, w, dev), _arg(y, "e", "y", dev), py,
+                                      ldy, M, N, K, ACTS[act], s))
+
+
+def gemm_grouped_fp8(a, a_scales, w, w_scales, c, tile_tab, n_tiles, stream=None):
+    """c [rows, N] (bf16 or fp32): row r of a, which is sorted by expert, times the w [E, N, K] of its expert; tile_tab, n_tiles: moe_route's"""
+    (M, K), (E, N, Kw), (mt, four), (s, dev), (kind, dtype) = a.shape, w.shape, tile_tab.shape, _here(stream), _float(c, "c")
+    _want(K == Kw and c.shape == (M, N) and four == 4 and n_tiles.numel() >= 1, "gemm_grouped_fp8: shapes do not fit")
+    ps, ld = _row_scales(a_scales, M, K, "a_scales", dev)
+    check(load().b200q_gemm_grouped_fp8(_arg(a, "e", "a", dev), M, ps, ld, _arg(w, "e", "w", dev), _weight_scales(w_scales, w, dev), E,
+                                        _arg(c, kind, "c", dev), N, K, _arg(tile_tab, "i", "tile_tab", dev), _arg(n_tiles, "i", "n_tiles", dev), mt,
+                                        dtype, s))
+
+
+def gemm_grouped_gated_fp8(a, a_scales, w, w_scales, y, y_scales, tile_tab, n_tiles, act="silu", stream=None):
+    """gemm_gated_fp8 by expert, arguments as of gemm_grouped_fp8"""
+    (M, K), (E, N, Kw), (mt, four), (s, dev) = a.shape, w.shape, tile_tab.shape, _here(stream)
+    _want(K == Kw and y.shape == (M, N // 2) and four == 4 and n_tiles.numel() >= 1, "gemm_grouped_gated_fp8: shapes do not fit")
+    (ps, ld), (py, ldy) = _row_scales(a_scales, M, K, "a_scales", dev), _row_scales(y_scales, M, N // 2, "y_scales", dev)
+    check(load().b200q_gemm_grouped_gated_fp8(_arg(a, "e", "a", dev), M, ps, ld, _arg(w, "e", "w", dev), _weight_scales(w_scales, w, dev), E,
+                                              _arg(y, "e", "y", dev), py, ldy, N, K, _arg(tile_tab, "i", "tile_tab", dev),
+                                              _arg(n_tiles, "i", "n_tiles", dev), mt, ACTS[act], s))
+
+
+def gemm_fp8_set_mode(mode: int):
+    check(load().b200q_gemm_fp8_set_mode(mode))
