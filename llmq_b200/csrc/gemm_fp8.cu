@@ -114,10 +114,14 @@ __device__ __noinline__ void f8_let_copies_end() {
 constexpr int FL_THREADS = 384, FL_BN = 256, FL_PATCH = 4096;
 // registers: 384 threads begin with 168; four warps give back 128 each and eight take 64 more (40 x 128 + 232 x 256 = 168 x 384)
 constexpr int FL_REGS_FEW = 40, FL_REGS_MANY = 232;
-template <bool PAIR>
+// The products of a block are two to 128 columns, whose accumulators are filled and emptied on their own: a half's next product waits for four
+// warps and not for eight, and the tensor core has the other half's to do meanwhile.  Rows of W come in boxes, so that the columns of a half
+// are 128 neighbours, or (gated) 64 gates and the 64 that they gate; of a pair each CTA has 64 of them.
+template <bool PAIR, bool GATED>
 struct LargeCfg {
   static constexpr int STAGE = F8_STAGE_W + (PAIR ? F8_STAGE_W : 2 * F8_STAGE_W);  // 128 rows of A, 256 (the pair: 128) of W
   static constexpr int STAGES = PAIR ? 6 : 4;
+  static constexpr int BOX = PAIR || GATED ? 64 : 256, BOXES = (PAIR ? 128 : 256) / BOX;  // rows of W, boxes of a stage
   static constexpr int SMEM = STAGES * STAGE + 8 * FL_PATCH + 1024;
 };
 
@@ -131,12 +135,12 @@ template <bool PAIR, bool GATED, bool GROUPED>
 __global__ void __launch_bounds__(FL_THREADS, 1)
     gemm_fp8_large_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
                           const __grid_constant__ CUtensorMap tmap_c, const __grid_constant__ Fp8Args a) {
-  using Cfg = LargeCfg<PAIR>;
+  using Cfg = LargeCfg<PAIR, GATED>;
   constexpr int STAGES = Cfg::STAGES, BM = PAIR ? 256 : 128;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* patches = smem + STAGES * Cfg::STAGE;
-  __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2];
+  __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], acc_full[2][2], acc_empty[2][2];  // of accumulators: [half of the columns][turn]
   __shared__ uint32_t tmem_slot;
   __shared__ int dead;
   __shared__ uint32_t most[2][128];  // gated: the largest of a half row's 64 values
@@ -144,6 +148,8 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
   const int rank = PAIR ? (int)cluster_ctarank() : 0;
   const int unit = PAIR ? blockIdx.x >> 1 : blockIdx.x, units = PAIR ? gridDim.x >> 1 : gridDim.x;
   const int n_tiles = (a.N + FL_BN - 1) / FL_BN, blocks = a.blocks;
+  // the i-th box of a stage begins so many rows of W behind the tile's first
+  auto w_box = [&](int i) { return PAIR ? (GATED ? rank * 128 + i * 64 : i * 128 + rank * 64) : GATED ? (i & 1) * 128 + (i >> 1) * 64 : 0; };
 
   if (warp == 0 && lane == 0) {
     dead = 0;
@@ -151,11 +157,11 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
     tma_prefetch_desc(&tmap_w);
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(full + s, PAIR ? 2 : 1);
-      mbar_init(empty + s, 1);
+      mbar_init(empty + s, 2);  // both halves' products
     }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(acc_full + s, 1);
-      mbar_init(acc_empty + s, PAIR ? 16 : 8);  // (the leader's) the warps that promote
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(acc_full[s >> 1] + (s & 1), 1);
+      mbar_init(acc_empty[s >> 1] + (s & 1), PAIR ? 8 : 4);  // (the leader's) the warps that promote
     }
     mbar_fence_init();
   }
@@ -173,8 +179,9 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
   if (!GROUPED && warp == 0 && lane == 0) {  // the first weights into L2 while the kernel before this one ends
-    const int m_tiles = (a.M + BM - 1) / BM, row = unit / m_tiles * FL_BN + rank * 128;
-    for (int b = 0; b < min(STAGES, blocks); ++b) tma_prefetch_2d(&tmap_w, b * 64, row);
+    const int m_tiles = (a.M + BM - 1) / BM, n0 = unit / m_tiles * FL_BN;
+    for (int b = 0; b < min(STAGES, blocks); ++b)
+      for (int i = 0; i < Cfg::BOXES; ++i) tma_prefetch_2d(&tmap_w, b * 64, n0 + w_box(i));
   }
   __syncwarp();
   const float *as = a.as, *ws = a.ws;
@@ -208,18 +215,20 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
         for (int tile = unit; tile < num_tiles; tile += units) {
           int g, row0, row_end, n0;
           tile_of(tile, g, row0, row_end, n0);
-          const int wrow = g * a.N + n0 + rank * 128;
+          const int wrow = g * a.N + n0;
           for (int b = 0; b < blocks; ++b) {
             uint8_t* to = smem + stage * Cfg::STAGE;
             f8_wait(empty + stage, phase ^ 1u, &dead, a.failed);
             if constexpr (PAIR) {
               const uint32_t bar = mapa_shared(full + stage, 0);
               f8_expect_tx(bar, Cfg::STAGE);
-              f8_load_2sm(to + F8_STAGE_W, &tmap_w, b * 64, wrow, bar);
+#pragma unroll
+              for (int i = 0; i < Cfg::BOXES; ++i) f8_load_2sm(to + F8_STAGE_W + i * Cfg::BOX * 128, &tmap_w, b * 64, wrow + w_box(i), bar);
               f8_load_2sm(to, &tmap_a, b * 64, row0, bar);
             } else {
               mbar_expect_tx(full + stage, Cfg::STAGE);
-              tma_load_2d(to + F8_STAGE_W, &tmap_w, b * 64, wrow, full + stage);
+#pragma unroll
+              for (int i = 0; i < Cfg::BOXES; ++i) tma_load_2d(to + F8_STAGE_W + i * Cfg::BOX * 128, &tmap_w, b * 64, wrow + w_box(i), full + stage);
               tma_load_2d(to, &tmap_a, b * 64, row0, full + stage);
             }
             if (++stage == STAGES) {
@@ -231,19 +240,20 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
         }
       }
       __syncwarp();
-    } else if (warp == 1 && rank == 0) {
-      constexpr uint32_t idesc = fp8_idesc(BM, FL_BN);
+    } else if (warp < 3 && rank == 0) {  // a warp to the products of each half
+      const int h = warp - 1;
+      constexpr uint32_t idesc = fp8_idesc(BM, 128);
       const uint32_t ring = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
-      bool on = true;
-      for (int tile = unit; on && tile < num_tiles; tile += units)
-        for (int b = 0; b < blocks; ++b) {
-          if (!(on = mbar_wait_warp(acc_empty + acc, acc_phase ^ 1u, &dead, a.failed, WAIT_CYCLES))) break;
-          if (!(on = mbar_wait_warp(full + stage, phase, &dead, a.failed, WAIT_CYCLES))) break;
-          tc_fence_after();
-          if (elect_one()) {
-            const uint32_t sa = ring + (uint32_t)(stage * Cfg::STAGE), sw = sa + F8_STAGE_W, d = tmem + (uint32_t)(acc * FL_BN);
+      if (elect_one())
+        for (int tile = unit; tile < num_tiles; tile += units) {
+          for (int b = 0; b < blocks; ++b) {
+            f8_wait(full + stage, phase, &dead, a.failed);
+            f8_wait(acc_empty[h] + acc, acc_phase ^ 1u, &dead, a.failed);
+            tc_fence_after();
+            const uint32_t sa = ring + (uint32_t)(stage * Cfg::STAGE), sw = sa + F8_STAGE_W + h * (PAIR ? 64 : 128) * 128;
+            const uint32_t d = tmem + (uint32_t)(acc * FL_BN + h * 128);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               if constexpr (PAIR)
@@ -252,20 +262,20 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
                 umma_fp8(d, make_smem_desc(sa + k * 32), make_smem_desc(sw + k * 32), idesc, k > 0);
             }
             if constexpr (PAIR) {
+              f8_commit_2sm(acc_full[h] + acc);
               f8_commit_2sm(empty + stage);
-              f8_commit_2sm(acc_full + acc);
             } else {
+              umma_commit(acc_full[h] + acc);
               umma_commit(empty + stage);
-              umma_commit(acc_full + acc);
             }
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
+            acc ^= 1;
+            if (acc == 0) acc_phase ^= 1u;
           }
-          __syncwarp();
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1u;
-          }
-          acc ^= 1;
-          if (acc == 0) acc_phase ^= 1u;
+          if (*(volatile int*)&dead) break;
         }
       __syncwarp();
     }
@@ -273,11 +283,10 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(FL_REGS_MANY));
     // rows quarter * 32 + lane; columns: plain half * 128 + 0 .. 127, gated half * 64 + 0 .. 63 of the gates and of what they gate
     const int quarter = warp & 3, half = (warp - 4) >> 2;
-    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * (GATED ? 64 : 128));
-    auto column = [&](int c) { return (uint32_t)(GATED ? (c >> 1) * 128 + (c & 1) * 32 : c * 32); };  // of the c-th of four times 32
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
     uint8_t* const patch = patches + (warp - 4) * FL_PATCH;
     const uint32_t patch_s = smem_u32(patch);
-    const uint32_t empty0 = PAIR ? mapa_shared(acc_empty, 0) : smem_u32(acc_empty);
+    const uint32_t empty0 = PAIR ? mapa_shared(acc_empty[half], 0) : smem_u32(acc_empty[half]);
     int acc = 0, parity = 0;
     uint32_t acc_phase = 0;
     for (int tile = unit; tile < num_tiles; tile += units) {
@@ -297,7 +306,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
 #pragma unroll
         for (int j = 0; j < 16; ++j) sum[c][j] = 0ull;
       uint32_t v[2][32];
-      f8_wait(acc_full + acc, acc_phase, &dead, a.failed);
+      f8_wait(acc_full[half] + acc, acc_phase, &dead, a.failed);
       __syncwarp();
       tc_fence_after();
       tmem_ld32(lanes + (uint32_t)(acc * FL_BN), v[0]);
@@ -325,7 +334,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
             for (int c = 0; c < 4; ++c) {
               tmem_ld_wait_for(v[c & 1]);
               if (c < 3) {
-                tmem_ld32(from + column(c + 1), v[(c + 1) & 1]);
+                tmem_ld32(from + (uint32_t)(c * 32 + 32), v[(c + 1) & 1]);
               } else {  // the accumulator is free; the next one's first columns while the last of this are added
                 tc_fence_before();
                 __syncwarp();
@@ -333,7 +342,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
                 acc ^= 1;
                 if (acc == 0) acc_phase ^= 1u;
                 if (b0 + i + 1 < blocks) {
-                  f8_wait(acc_full + acc, acc_phase, &dead, a.failed);
+                  f8_wait(acc_full[half] + acc, acc_phase, &dead, a.failed);
                   __syncwarp();
                   tc_fence_after();
                   tmem_ld32(lanes + (uint32_t)(acc * FL_BN), v[0]);
@@ -361,7 +370,8 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
         most[half][quarter * 32 + lane] = m;
         // (two warps share a quarter's rows, and a patch of 32 rows x 128 codes for each parity of the tile)
         uint8_t* const out = patches + (2 * quarter + parity) * FL_PATCH;
-        if (!GROUPED && half == 0 && lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        const bool copies = !GROUPED && half == 0 && lane == 0;
+        if (copies) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
         asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
         const float scale = fp8_scale(max(m, most[half ^ 1][quarter * 32 + lane])), by = 1.f / scale;
         if (half == 0 && live) a.ys[(long long)(n0 / 256) * a.ld_ys + row] = scale;
@@ -375,15 +385,13 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
           }
           st_v4(out + lane * 128 + (((half * 4 + j) ^ (lane & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
         }
-        if constexpr (!GROUPED) {
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
-          if (half == 0 && lane == 0 && row0 + quarter * 32 < a.M) {
-            f8_store(&tmap_c, n0 / 4, row0 + quarter * 32, smem_u32(out));
-            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-          }
-        } else {
-          asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+        if constexpr (!GROUPED) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+        if (copies) {  // (rows that do not exist leave an empty group, as the wait counts turns)
+          if (row0 + quarter * 32 < a.M) f8_store(&tmap_c, n0 / 4, row0 + quarter * 32, smem_u32(out));
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+        if constexpr (GROUPED) {
           uint8_t* to = (uint8_t*)a.C + (long long)(row0 + quarter * 32) * (a.N / 2) + n0 / 2;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -737,7 +745,7 @@ static int clusters_that_fit(K kern, int cluster, int threads, int smem) {
 
 template <bool PAIR, bool GATED, bool GROUPED>
 static int launch_large(const void* A, long long a_rows, const void* W, long long w_rows, Fp8Args a, cudaStream_t st) {
-  using Cfg = LargeCfg<PAIR>;
+  using Cfg = LargeCfg<PAIR, GATED>;
   auto kern = gemm_fp8_large_kernel<PAIR, GATED, GROUPED>;
   static uint64_t seen[2];
   int rc = once_per_device(seen, [&]() -> int {
@@ -747,7 +755,7 @@ static int launch_large(const void* A, long long a_rows, const void* W, long lon
   CUtensorMap ta, tw, tc = {};
   // (two codes are one element of the maps; a box is 128 codes wide)
   if (!rc) rc = get_tmap(A, a_rows, a.K / 2, 128, &ta);
-  if (!rc) rc = get_tmap(W, w_rows, a.K / 2, PAIR ? 128 : 256, &tw);
+  if (!rc) rc = get_tmap(W, w_rows, a.K / 2, Cfg::BOX, &tw);
   if (!rc && !GROUPED && GATED) rc = get_tmap(a.C, a.M, a.N / 4, 32, &tc);
   if (!rc && !GROUPED && !GATED && !a.out_f32) rc = get_tmap(a.C, a.M, a.N, 32, &tc);
   if (rc) return rc;
