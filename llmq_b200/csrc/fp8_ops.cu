@@ -1,111 +1,108 @@
 // fp8_ops.cu — rows and weights in 8 bits (format: fp8.cuh): RMS norm with the residual's addition, rows as they are or gathered, weights.
-// All three are bound by memory: every value is read once and leaves as one byte; what they compute between is some ten instructions a value.
+// All three are bound by memory: every value is read once and leaves as one byte.  Next to that bound are their instructions, so that eight lanes
+// have a block of 128 (two pieces of eight values each: three exchanges for the largest), pairs of bf16 are added and compared at once, and the
+// norm's factor is multiplied in together with the scale's reciprocal.
 #include "fp8.cuh"
 
 namespace b200q {
 
 constexpr int F8_MAX_H = 16384;
 
-// r <- x + r;  y = r / sqrt(mean(r^2) + eps) * w in 8 bits.  A block to a row, CH pieces of eight values to a thread, held in registers between
-// the sum and the product; sixteen lanes are a block of 128 values, whose largest magnitude crosses them in four exchanges.
+// r <- x + r;  y = r / sqrt(mean(r^2) + eps) * w in 8 bits.  A CTA to a row, CH blocks of 128 values to eight lanes, held in registers between the
+// sum of squares and the products with w, whose largest magnitude is known before the norm's factor is.
 template <typename T, int CH>
 __global__ void __launch_bounds__(256)
     rmsnorm_fp8_kernel(const T* __restrict__ x, T* __restrict__ residual, const T* __restrict__ w, uint2* __restrict__ y,
                        float* __restrict__ scales, int ld_scales, int H, float inv_h, float eps) {
   follow_previous(x, residual, w, y, scales);
   const long long row = blockIdx.x;
-  const int threads = blockDim.x, chunks = H / 8;
-  Eight<T> v[CH], weight[CH];
+  const int groups = blockDim.x / 8, lane = threadIdx.x & 7;
+  auto place = [&](int j, int p) { return (j * groups + (int)(threadIdx.x >> 3)) * FP8_BLOCK + p * 64 + lane * 8; };
+  Eight<T> v[CH][2], u[CH][2];
+#pragma unroll
+  for (int j = 0; j < CH; ++j)
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      v[j][p].zero();
+      u[j][p].zero();
+      if (place(j, p) < H) {
+        v[j][p].load(x + row * H + place(j, p));
+        if (residual) u[j][p].load(residual + row * H + place(j, p));
+      }
+    }
   float ss = 0.f;
 #pragma unroll
-  for (int j = 0; j < CH; ++j) {
-    const int c = threadIdx.x + j * threads;
-    if (c < chunks) v[j].load(x + row * H + c * 8);
-  }
-  if (residual) {
+  for (int j = 0; j < CH; ++j)
 #pragma unroll
-    for (int j = 0; j < CH; ++j) {
-      const int c = threadIdx.x + j * threads;
-      if (c < chunks) weight[j].load(residual + row * H + c * 8);
-    }
-  }
+    for (int p = 0; p < 2; ++p)
+      if (place(j, p) < H) {
+        if (residual) {  // (the residual stream is held in its own type: the sum is rounded before it is normalised)
+          v[j][p].add(u[j][p]);
+          v[j][p].store(residual + row * H + place(j, p));
+        }
 #pragma unroll
-  for (int j = 0; j < CH; ++j) {
-    const int c = threadIdx.x + j * threads;
-    if (c < chunks) {
-      float f[8];
-      v[j].get(f);
-      if (residual) {
-        float r[8];
-        weight[j].get(r);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] += r[i];
-        v[j].set(f);  // (the residual stream is held in its own type: the sum is rounded before it is normalised)
-        v[j].store(residual + row * H + c * 8);
-        v[j].get(f);
+        for (int i = 0; i < 8; ++i) ss += v[j][p].get(i) * v[j][p].get(i);
+        u[j][p].load(w + place(j, p));
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ss += f[i] * f[i];
-      weight[j].load(w + c * 8);
-    }
-  }
   __shared__ float red[8];
   ss = warp_sum(ss);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = ss;
   __syncthreads();
   float total = 0.f;
-  for (int i = 0; i < threads / 32; ++i) total += red[i];
+  for (int i = 0; i < (int)blockDim.x / 32; ++i) total += red[i];
   const float inv = rsqrtf(total * inv_h + eps);
 #pragma unroll
   for (int j = 0; j < CH; ++j) {
-    const int c = threadIdx.x + j * threads;
-    if (j * threads >= chunks) break;  // (a whole warp takes part in the exchanges)
-    float f[8] = {};
-    if (c < chunks) {
-      float g[8];
-      v[j].get(f);
-      weight[j].get(g);
+    Eight<float> n[2];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = f[i] * inv * g[i];
-    }
-    uint32_t m = largest_of(f);
+    for (int p = 0; p < 2; ++p)
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float scale = fp8_scale(m);
-    if (c < chunks) {
-      y[row * chunks + c] = fp8_eight(f, 1.f / scale);
-      if (c % 16 == 0) scales[(long long)(c / 16) * ld_scales + row] = scale;
-    }
+      for (int i = 0; i < 8; ++i) n[p].w[i] = v[j][p].get(i) * u[j][p].get(i);
+    const float scale = fp8_scale(max_of_8_lanes(max_or_nan(n[0].largest(), n[1].largest())) * inv), by = fp8_inverse(scale) * inv;
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+      if (place(j, p) < H) y[(row * H + place(j, p)) >> 3] = fp8_eight(n[p], by);
+    if (lane == 0 && place(j, 0) < H) scales[(long long)(place(j, 0) / FP8_BLOCK) * ld_scales + row] = scale;
   }
 }
 
-// y[i] = row rows[i] (NULL: i) of x in 8 bits.  Sixteen lanes to a block of 128 values.
-template <typename T>
+// y[i] = row rows[i] (NULL: i) of x in 8 bits.  Eight lanes to a block of 128 values, U blocks to each, whose reads are under way together.
+template <typename T, int U>
 __global__ void __launch_bounds__(256)
     quantize_fp8_kernel(const T* __restrict__ x, long long ld_x, const int32_t* __restrict__ rows, uint2* __restrict__ y,
-                        float* __restrict__ scales, int ld_scales, int K, int blocks, long long total) {
+                        float* __restrict__ scales, int ld_scales, int K, uint32_t blocks, uint32_t total) {
   follow_previous(x, rows, y, scales);
-  const long long item = ((long long)blockIdx.x * 256 + threadIdx.x) >> 4;
-  const int at = (threadIdx.x & 15) * 8;
-  const long long row = item / blocks;
-  const int block = (int)(item - row * blocks), k = block * FP8_BLOCK + at;
-  const bool live = item < total && k < K;
-  Eight<T> v;
-  v.zero();
-  if (live) v.load(x + (rows ? (long long)rows[row] : row) * ld_x + k);
-  float f[8];
-  v.get(f);
-  uint32_t m = largest_of(f);
+  const int lane = threadIdx.x & 7;
+  uint32_t row[U], block[U];
+  long long from[U];
+  Eight<T> v[U][2];
+  auto live = [&](int u, int p) { return row[u] != ~0u && (int)block[u] * FP8_BLOCK + p * 64 + lane * 8 < K; };
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float scale = fp8_scale(m);
-  if (live) {
-    y[(row * K + k) >> 3] = fp8_eight(f, 1.f / scale);
-    if (at == 0) scales[(long long)block * ld_scales + row] = scale;
+  for (int u = 0; u < U; ++u) {
+    const uint32_t item = (blockIdx.x * U + u) * 32 + (threadIdx.x >> 3);
+    const uint32_t r = item / blocks;
+    block[u] = item - r * blocks;
+    row[u] = item < total ? r : ~0u;
+    from[u] = item < total && rows ? rows[r] : r;
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      v[u][p].zero();
+      if (live(u, p)) v[u][p].load(x + from[u] * ld_x + block[u] * FP8_BLOCK + p * 64 + lane * 8);
+    }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const float scale = fp8_scale(max_of_8_lanes(max_or_nan(v[u][0].largest(), v[u][1].largest()))), by = fp8_inverse(scale);
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+      if (live(u, p)) y[((long long)row[u] * K + block[u] * FP8_BLOCK + p * 64 + lane * 8) >> 3] = fp8_eight(v[u][p], by);
+    if (lane == 0 && live(u, 0)) scales[(long long)block[u] * ld_scales + row[u]] = scale;
   }
 }
 
-// A square of 128 x 128 weights to a block: eight rows x eight columns to a thread, held in registers between the largest and the codes.
+// A square of 128 x 128 weights to a CTA: eight rows x eight columns to a thread, held in registers between the largest and the codes.
 template <typename T>
 __global__ void __launch_bounds__(256)
     quantize_fp8_weight_kernel(const T* __restrict__ w, uint2* __restrict__ q, float* __restrict__ scales, int N, int K) {
@@ -118,27 +115,20 @@ __global__ void __launch_bounds__(256)
     v[i].zero();
     if (k < K && n0 + 16 * i < N) v[i].load(w + (first + n0 + 16 * i) * K + k);
   }
-  uint32_t m = 0;
+  float m = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float f[8];
-    v[i].get(f);
-    m = max(m, largest_of(f));
-  }
-  m = __reduce_max_sync(0xffffffffu, m);
+  for (int i = 0; i < 8; ++i) m = max_or_nan(m, v[i].largest());
+  const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(m));  // (no sign: NaN is the largest as a whole number too)
   __shared__ uint32_t red[8];
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = most;
   __syncthreads();
+  uint32_t all = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, red[i]);
-  const float scale = fp8_scale(m), by = 1.f / scale;
+  for (int i = 0; i < 8; ++i) all = max(all, red[i]);
+  const float scale = fp8_scale(__uint_as_float(all)), by = fp8_inverse(scale);
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    if (k < K && n0 + 16 * i < N) {
-      float f[8];
-      v[i].get(f);
-      q[((first + n0 + 16 * i) * K + k) >> 3] = fp8_eight(f, by);
-    }
+    if (k < K && n0 + 16 * i < N) q[((first + n0 + 16 * i) * K + k) >> 3] = fp8_eight(v[i], by);
   if (threadIdx.x == 0) scales[((long long)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x] = scale;
 }
 
@@ -159,7 +149,7 @@ int b200q_rmsnorm_fp8(const void* x, void* residual, const void* w, void* y, flo
   if (T_ == 0) return B200Q_OK;
   B200Q_CHECK_ARG(x && w && y && scales, "rmsnorm_fp8: null argument");
   B200Q_CHECK_ARG(aligned16(x, residual, w, y), "rmsnorm_fp8: x, residual, w and y must be 16-byte aligned");
-  const int chunks = H / 8, threads = chunks < 256 ? (chunks + 31) / 32 * 32 : 256, each = (chunks + threads - 1) / threads;
+  const int blocks = (H + FP8_BLOCK - 1) / FP8_BLOCK, threads = blocks < 32 ? (blocks * 8 + 31) / 32 * 32 : 256, each = (blocks + threads / 8 - 1) / (threads / 8);
   auto launch = [&](auto type, auto ch) -> int {
     using T = decltype(type);
     B200Q_CUDA(launch_early(rmsnorm_fp8_kernel<T, decltype(ch)::value>, T_, threads, 0, as_stream(stream), 1, (const T*)x, (T*)residual, (const T*)w,
@@ -170,8 +160,7 @@ int b200q_rmsnorm_fp8(const void* x, void* residual, const void* w, void* y, flo
   auto pieces = [&](auto type) -> int {
     return each <= 1   ? launch(type, std::integral_constant<int, 1>{})
            : each <= 2 ? launch(type, std::integral_constant<int, 2>{})
-           : each <= 4 ? launch(type, std::integral_constant<int, 4>{})
-                       : launch(type, std::integral_constant<int, 8>{});
+                       : launch(type, std::integral_constant<int, 4>{});
   };
   return dtype == B200Q_DTYPE_F32 ? pieces(float{}) : pieces(bf16{});
 }
@@ -184,16 +173,20 @@ int b200q_quantize_fp8(const void* x, int64_t ld_x, const int32_t* rows, void* y
   B200Q_CHECK_ARG(x && y && scales, "quantize_fp8: null argument");
   B200Q_CHECK_ARG(aligned16(x, y), "quantize_fp8: x and y must be 16-byte aligned");
   const int blocks = (K + FP8_BLOCK - 1) / FP8_BLOCK;
-  const long long total = (long long)T_ * blocks, grid = (total + 15) / 16;
-  B200Q_CHECK_ARG(grid < (1ll << 31), "quantize_fp8: too much at once (T=%d K=%d)", T_, K);
-  auto launch = [&](auto type) -> int {
+  const long long total = (long long)T_ * blocks;
+  B200Q_CHECK_ARG(total < (1ll << 31), "quantize_fp8: too much at once (T=%d K=%d)", T_, K);
+  auto launch = [&](auto type, auto each) -> int {
     using T = decltype(type);
-    B200Q_CUDA(launch_early(quantize_fp8_kernel<T>, dim3((unsigned)grid), 256, 0, as_stream(stream), 1, (const T*)x, (long long)ld_x, rows, (uint2*)y, scales,
-                            ld_scales, K, blocks, total));
+    constexpr int U = decltype(each)::value;
+    B200Q_CUDA(launch_early(quantize_fp8_kernel<T, U>, dim3((unsigned)((total + 32 * U - 1) / (32 * U))), 256, 0, as_stream(stream), 1, (const T*)x,
+                            (long long)ld_x, rows, (uint2*)y, scales, ld_scales, K, (uint32_t)blocks, (uint32_t)total));
     count_launch();
     return B200Q_OK;
   };
-  return dtype == B200Q_DTYPE_F32 ? launch(float{}) : launch(bf16{});
+  auto pieces = [&](auto type) -> int {
+    return total <= 32 * 8 * 148 ? launch(type, std::integral_constant<int, 1>{}) : launch(type, std::integral_constant<int, 2>{});
+  };
+  return dtype == B200Q_DTYPE_F32 ? pieces(float{}) : pieces(bf16{});
 }
 
 int b200q_quantize_fp8_weight(const void* w, void* q, float* scales, int groups, int N, int K, int dtype, void* stream) {

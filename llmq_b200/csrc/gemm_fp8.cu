@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
   __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], acc_full[2][2], acc_empty[2][2];  // of accumulators: [half of the columns][turn]
   __shared__ uint32_t tmem_slot;
   __shared__ int dead;
-  __shared__ uint32_t most[2][128];  // gated: the largest of a half row's 64 values
+  __shared__ float most[2][128];  // gated: the largest of a half row's 64 values
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = PAIR ? (int)cluster_ctarank() : 0;
   const int unit = PAIR ? blockIdx.x >> 1 : blockIdx.x, units = PAIR ? gridDim.x >> 1 : gridDim.x;
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
       // ---- the sums leave ----
       if constexpr (GATED) {
         float y[64];
-        uint32_t m = 0;
+        float m = 0.f;
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -366,14 +366,14 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
             y[c * 32 + 2 * j + 1] = fp8_unit(gate.y, up.y, a.gelu);
           }
 #pragma unroll
-        for (int j = 0; j < 64; ++j) m = max(m, abs_bits(y[j]));
+        for (int j = 0; j < 64; ++j) m = max_or_nan(m, fabsf(y[j]));
         most[half][quarter * 32 + lane] = m;
         // (two warps share a quarter's rows, and a patch of 32 rows x 128 codes for each parity of the tile)
         uint8_t* const out = patches + (2 * quarter + parity) * FL_PATCH;
         const bool copies = !GROUPED && half == 0 && lane == 0;
         if (copies) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
         asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
-        const float scale = fp8_scale(max(m, most[half ^ 1][quarter * 32 + lane])), by = 1.f / scale;
+        const float scale = fp8_scale(max_or_nan(m, most[half ^ 1][quarter * 32 + lane])), by = fp8_inverse(scale);
         if (half == 0 && live) a.ys[(long long)(n0 / 256) * a.ld_ys + row] = scale;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -689,8 +689,8 @@ __global__ void __launch_bounds__(GATED ? 320 : 192, small_resident<GATED>(MOST)
       x.y = fp8_unit(x.y, u.y, a.gelu);
       x.z = fp8_unit(x.z, u.z, a.gelu);
       x.w = fp8_unit(x.w, u.w, a.gelu);
-      const uint32_t m = __reduce_max_sync(0xffffffffu, max(max(abs_bits(x.x), abs_bits(x.y)), max(abs_bits(x.z), abs_bits(x.w))));
-      const float scale = fp8_scale(m), by = 1.f / scale;
+      const float m = max_or_nan(max_or_nan(fabsf(x.x), fabsf(x.y)), max_or_nan(fabsf(x.z), fabsf(x.w)));
+      const float scale = fp8_scale(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)))), by = fp8_inverse(scale);
       *reinterpret_cast<uint32_t*>((uint8_t*)a.C + row * (a.N / 2) + n0 / 2 + lane * 4) = fp8_four(x.x * by, x.y * by, x.z * by, x.w * by);
       if (lane == 0) a.ys[(long long)blockIdx.y * a.ld_ys + row] = scale;
     } else if (n0 + lane * 4 < a.N) {

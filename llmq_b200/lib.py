@@ -786,22 +786,25 @@ def fp8_row_scales(rows, K, device="cuda"):
 def _row_scales(t, rows, K, what, dev):
     """(data_ptr, ld) of scales of rows"""
     blocks, ld = t.shape
-    _want(blocks == (K + 127) // 128 and ld >= rows, f"{what}: [{(K + 127) // 128}, {rows} or more] is wanted, not {tuple(t.shape)}")
+    if blocks != (K + 127) >> 7 or ld < rows:
+        raise ValueError(f"{what}: [{(K + 127) // 128}, {rows} or more] is wanted, not {tuple(t.shape)}")
     return _arg(t, "f", what, dev), ld
 
 
 def _weight_scales(t, w, dev):
-    N, K = w.shape[-2:]
-    _want(t.shape == (*w.shape[:-2], (N + 127) // 128, (K + 127) // 128), f"w_scales: {tuple(t.shape)} does not fit {tuple(w.shape)}")
+    *groups, N, K = w.shape
+    if t.shape != (*groups, (N + 127) >> 7, (K + 127) >> 7):
+        raise ValueError(f"w_scales: {tuple(t.shape)} does not fit {tuple(w.shape)}")
     return _arg(t, "f", "w_scales", dev)
 
 
 def _float(t, what):
     """dtype code of a bf16 or fp32 tensor"""
-    kinds = _TORCH or _types()
-    if t.dtype is kinds["h"]:
+    kinds, have = _TORCH or _types(), t.dtype
+    if have is kinds["h"]:
         return "h", DTYPE_BF16
-    _want(t.dtype is kinds["f"], f"{what}: {t.dtype}, neither bfloat16 nor float32")
+    if have is not kinds["f"]:
+        raise ValueError(f"{what}: {have}, neither bfloat16 nor float32")
     return "f", DTYPE_F32
 
 
@@ -818,7 +821,8 @@ def quantize_fp8(x, y, scales, rows=None, stream=None):
     """y, scales = the rows of x (of x[rows]) in 8 bits; x may be a slice of wider rows"""
     (n, K), (T, Ky), (s, dev), (kind, dtype) = x.shape, y.shape, _here(stream), _float(x, "x")
     _want(K == Ky and (T <= n if rows is None else rows.numel() == T), "quantize_fp8: y or rows do not fit x")
-    _want(x.get_device() == dev and (x.stride(1) == 1 or K == 1), f"x: rows on device {dev}, the current one, are wanted")
+    if x.get_device() != dev or x.stride(1) != 1:
+        raise ValueError(f"x: rows on device {dev}, the current one, are wanted")
     ps, ld = _row_scales(scales, T, K, "scales", dev)
     ld_x = x.stride(0) if n > 1 else (K + 7) // 8 * 8
     check(load().b200q_quantize_fp8(x.data_ptr(), ld_x, 0 if rows is None else _arg(rows, "i", "rows", dev), _arg(y, "e", "y", dev), ps, ld, T, K,
