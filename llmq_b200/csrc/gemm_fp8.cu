@@ -29,9 +29,9 @@ struct Fp8Args {
   const int4* tab;   // [*n_mt] {group, first row, end of its rows, 0}, or NULL: the rows are one group
   const int32_t* n_mt;
   int* failed;
-  int ld_as, ld_ys, M, N, K, blocks, n_blocks, max_mt, groups, out_f32, gelu;
+  int ld_as, ld_ys, M, N, K, blocks, n_blocks, max_mt, groups, out_f32, gelu, a_bytes;
   // small tiles
-  int rows, box_rows, stages, cols, splits;
+  int rows, box_rows, stages, accs, cols, splits;
 };
 
 __device__ __forceinline__ void umma_fp8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
@@ -82,6 +82,12 @@ __device__ __forceinline__ void f8_commit_2sm(uint64_t* bar) {
                "h"((uint16_t)3)
                : "memory");
 }
+// the last barrier of a cluster: what the others have read of this CTA's memory they have used, and nothing else is handed over (an arrival that
+// releases waits for the outputs' stores)
+__device__ __forceinline__ void f8_leave_cluster() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+}
 // the unit of a gate and what it gates, fp32 from the sums on: g sigmoid(g) u, or tanh GELU, 0.5 g (1 + tanh t) = g sigmoid(2 t)
 __device__ __forceinline__ float fp8_unit(float g, float u, int gelu) {
   const float t = gelu ? 1.5957691216057308f * (g + 0.044715f * (g * g * g)) : g;
@@ -111,32 +117,36 @@ __device__ __noinline__ void f8_let_copies_end() {
 }
 
 // ---- large ---------------------------------------------------------------------------------------------------------------------
-constexpr int FL_THREADS = 384, FL_BN = 256, FL_PATCH = 4096;
+constexpr int FL_THREADS = 384, FL_PATCH = 4096, FL_MAX_SPLITS = 8;
 // registers: 384 threads begin with 168; four warps give back 128 each and eight take 64 more (40 x 128 + 232 x 256 = 168 x 384)
 constexpr int FL_REGS_FEW = 40, FL_REGS_MANY = 232;
-// The products of a block are two to 128 columns, whose accumulators are filled and emptied on their own: a half's next product waits for four
-// warps and not for eight, and the tensor core has the other half's to do meanwhile.  Rows of W come in boxes, so that the columns of a half
-// are 128 neighbours, or (gated) 64 gates and the 64 that they gate; of a pair each CTA has 64 of them.
-template <bool PAIR, bool GATED>
+// A tile has 64 CH columns.  The products of a block are two, to a half of them each, whose accumulators are filled and emptied on their own: a
+// half's next product waits for four warps and not for eight, and the tensor core has the other half's to do meanwhile.  Rows of W come in boxes,
+// so that the columns of a half are neighbours, or (gated) 64 gates and the 64 that they gate; of a pair each CTA has half of them.
+template <bool PAIR, int CH, bool GATED>
 struct LargeCfg {
-  static constexpr int STAGE = F8_STAGE_W + (PAIR ? F8_STAGE_W : 2 * F8_STAGE_W);  // 128 rows of A, 256 (the pair: 128) of W
-  static constexpr int STAGES = PAIR ? 6 : 4;
-  static constexpr int BOX = PAIR || GATED ? 64 : 256, BOXES = (PAIR ? 128 : 256) / BOX;  // rows of W, boxes of a stage
+  static constexpr int BN = 64 * CH, W_ROWS = PAIR ? BN / 2 : BN;                // columns of a tile; rows of W that a CTA fetches
+  static constexpr int STAGE = F8_STAGE_W + W_ROWS * FP8_BLOCK;                  // behind 128 rows of A
+  static constexpr int STAGES = 196608 / STAGE < 8 ? 196608 / STAGE : 8;
+  static constexpr int BOX = PAIR ? 16 * CH : GATED ? 64 : BN, BOXES = W_ROWS / BOX;
   static constexpr int SMEM = STAGES * STAGE + 8 * FL_PATCH + 1024;
 };
 
-// 64 sums to a thread (its row, columns in turn) += scale * 32 of them that have come from tensor memory
+// 32 of a thread's sums (its row, columns in turn) += scale * what has come from tensor memory
 __device__ __forceinline__ void promote(f32x2* acc, const uint32_t (&v)[32], f32x2 scale) {
 #pragma unroll
   for (int j = 0; j < 16; ++j) acc[j] = fma2(pair_of(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), scale, acc[j]);
 }
 
-template <bool PAIR, bool GATED, bool GROUPED>
+// SPLIT: a cluster to a tile, a part of the reduction to each of its CTAs, whose sums meet in distributed shared memory in the order of the parts
+template <bool PAIR, int CH, bool GATED, bool GROUPED, bool SPLIT>
 __global__ void __launch_bounds__(FL_THREADS, 1)
     gemm_fp8_large_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
                           const __grid_constant__ CUtensorMap tmap_c, const __grid_constant__ Fp8Args a) {
-  using Cfg = LargeCfg<PAIR, GATED>;
-  constexpr int STAGES = Cfg::STAGES, BM = PAIR ? 256 : 128;
+  using Cfg = LargeCfg<PAIR, CH, GATED>;
+  static_assert(!GATED || CH == 4, "a gated tile has 128 gates");
+  static_assert(!SPLIT || !(PAIR || GROUPED || GATED), "parts of dense products of single CTAs");
+  constexpr int STAGES = Cfg::STAGES, BM = PAIR ? 256 : 128, BN = Cfg::BN;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* patches = smem + STAGES * Cfg::STAGE;
@@ -146,10 +156,12 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
   __shared__ float most[2][128];  // gated: the largest of a half row's 64 values
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = PAIR ? (int)cluster_ctarank() : 0;
-  const int unit = PAIR ? blockIdx.x >> 1 : blockIdx.x, units = PAIR ? gridDim.x >> 1 : gridDim.x;
-  const int n_tiles = (a.N + FL_BN - 1) / FL_BN, blocks = a.blocks;
+  const int split = SPLIT ? (int)cluster_ctarank() : 0, share = PAIR ? 2 : SPLIT ? a.splits : 1;  // share: CTAs to a tile
+  const int unit = blockIdx.x / share, units = gridDim.x / share;
+  const int n_tiles = (a.N + BN - 1) / BN, blocks = a.blocks;
+  const int b_begin = SPLIT ? split * blocks / a.splits : 0, b_end = SPLIT ? (split + 1) * blocks / a.splits : blocks;
   // the i-th box of a stage begins so many rows of W behind the tile's first
-  auto w_box = [&](int i) { return PAIR ? (GATED ? rank * 128 + i * 64 : i * 128 + rank * 64) : GATED ? (i & 1) * 128 + (i >> 1) * 64 : 0; };
+  auto w_box = [&](int i) { return PAIR ? (GATED ? rank * 128 + i * 64 : (i * 2 + rank) * Cfg::BOX) : GATED ? (i & 1) * 128 + (i >> 1) * 64 : 0; };
 
   if (warp == 0 && lane == 0) {
     dead = 0;
@@ -179,9 +191,9 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
   if (!GROUPED && warp == 0 && lane == 0) {  // the first weights into L2 while the kernel before this one ends
-    const int m_tiles = (a.M + BM - 1) / BM, n0 = unit / m_tiles * FL_BN;
-    for (int b = 0; b < min(STAGES, blocks); ++b)
-      for (int i = 0; i < Cfg::BOXES; ++i) tma_prefetch_2d(&tmap_w, b * 64, n0 + w_box(i));
+    const int m_tiles = (a.M + BM - 1) / BM, n0 = unit / m_tiles * BN;
+    for (int b = 0; b < min(STAGES, b_end - b_begin); ++b)
+      for (int i = 0; i < Cfg::BOXES; ++i) tma_prefetch_2d(&tmap_w, (b_begin + b) * 64, n0 + w_box(i));
   }
   __syncwarp();
   const float *as = a.as, *ws = a.ws;
@@ -193,7 +205,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
   // a tile: columns n0 .., rows row0 .. row_end of a group
   auto tile_of = [&](int tile, int& g, int& row0, int& row_end, int& n0) {
     const int mt = tile % m_tiles;
-    n0 = tile / m_tiles * FL_BN;
+    n0 = tile / m_tiles * BN;
     if constexpr (GROUPED) {
       const int4 e = tab[mt];  // (kept within the matrices, whatever the table says)
       g = min(max(e.x, 0), a.groups - 1);
@@ -216,17 +228,17 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
           int g, row0, row_end, n0;
           tile_of(tile, g, row0, row_end, n0);
           const int wrow = g * a.N + n0;
-          for (int b = 0; b < blocks; ++b) {
+          for (int b = b_begin; b < b_end; ++b) {
             uint8_t* to = smem + stage * Cfg::STAGE;
             f8_wait(empty + stage, phase ^ 1u, &dead, a.failed);
             if constexpr (PAIR) {
               const uint32_t bar = mapa_shared(full + stage, 0);
-              f8_expect_tx(bar, Cfg::STAGE);
+              f8_expect_tx(bar, Cfg::STAGE - F8_STAGE_W + a.a_bytes);
 #pragma unroll
               for (int i = 0; i < Cfg::BOXES; ++i) f8_load_2sm(to + F8_STAGE_W + i * Cfg::BOX * 128, &tmap_w, b * 64, wrow + w_box(i), bar);
               f8_load_2sm(to, &tmap_a, b * 64, row0, bar);
             } else {
-              mbar_expect_tx(full + stage, Cfg::STAGE);
+              mbar_expect_tx(full + stage, Cfg::STAGE - F8_STAGE_W + a.a_bytes);
 #pragma unroll
               for (int i = 0; i < Cfg::BOXES; ++i) tma_load_2d(to + F8_STAGE_W + i * Cfg::BOX * 128, &tmap_w, b * 64, wrow + w_box(i), full + stage);
               tma_load_2d(to, &tmap_a, b * 64, row0, full + stage);
@@ -242,18 +254,18 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
       __syncwarp();
     } else if (warp < 3 && rank == 0) {  // a warp to the products of each half
       const int h = warp - 1;
-      constexpr uint32_t idesc = fp8_idesc(BM, 128);
+      constexpr uint32_t idesc = fp8_idesc(BM, BN / 2);
       const uint32_t ring = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       if (elect_one())
         for (int tile = unit; tile < num_tiles; tile += units) {
-          for (int b = 0; b < blocks; ++b) {
+          for (int b = b_begin; b < b_end; ++b) {
             f8_wait(full + stage, phase, &dead, a.failed);
             f8_wait(acc_empty[h] + acc, acc_phase ^ 1u, &dead, a.failed);
             tc_fence_after();
-            const uint32_t sa = ring + (uint32_t)(stage * Cfg::STAGE), sw = sa + F8_STAGE_W + h * (PAIR ? 64 : 128) * 128;
-            const uint32_t d = tmem + (uint32_t)(acc * FL_BN + h * 128);
+            const uint32_t sa = ring + (uint32_t)(stage * Cfg::STAGE), sw = sa + F8_STAGE_W + h * (Cfg::W_ROWS / 2) * FP8_BLOCK;
+            const uint32_t d = tmem + (uint32_t)(acc * 256 + h * 128);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               if constexpr (PAIR)
@@ -279,9 +291,10 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
         }
       __syncwarp();
     }
+    if constexpr (SPLIT) cluster_sync_all();  // (as the other warps do where their sums are in shared memory)
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(FL_REGS_MANY));
-    // rows quarter * 32 + lane; columns: plain half * 128 + 0 .. 127, gated half * 64 + 0 .. 63 of the gates and of what they gate
+    // rows quarter * 32 + lane; columns: half of the tile's, gated: half * 64 + 0 .. 63 of the gates and of what they gate
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
     uint8_t* const patch = patches + (warp - 4) * FL_PATCH;
@@ -294,64 +307,124 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
       tile_of(tile, g, row0, row_end, n0);
       const int row = row0 + quarter * 32 + lane;
       const bool live = row < row_end;
-      // weights' scales: this lane's of 32 blocks, handed round by shuffles; gated: of the gates and of what they gate
-      const int nb0 = GATED ? n0 / 128 : min(n0 / 128 + half, a.n_blocks - 1);
-      const float* w0 = ws + ((long long)g * a.n_blocks + nb0) * blocks;
+      if (!SPLIT && row0 + quarter * 32 >= row_end) {  // no rows: the accumulators only have to be passed on
+        for (int b = b_begin; b < b_end; ++b) {
+          f8_wait(acc_full[half] + acc, acc_phase, &dead, a.failed);
+          __syncwarp();
+          if (lane == 0) f8_arrive(empty0 + acc * 8);
+          acc ^= 1;
+          if (acc == 0) acc_phase ^= 1u;
+        }
+        continue;
+      }
+      // weights' scales: this lane's of 32 blocks of the reduction, handed round by shuffles.  A tile's columns lie in up to two blocks of 128 (gated:
+      // the gates' and that of what they gate); 32 neighbouring columns lie in one
+      const int col0 = GATED ? 0 : n0 % 128 + half * (BN / 2), nb0 = n0 / 128 + (CH == 4 && !GATED ? half : 0);
+      const float* w0 = ws + ((long long)g * a.n_blocks + min(nb0, a.n_blocks - 1)) * blocks;
+      const bool two = GATED || (CH == 3 && nb0 + 1 < a.n_blocks);
+      auto scale_of = [&](int c) { return GATED ? c >> 1 : CH == 3 ? (col0 + 32 * c) >> 7 : 0; };
       float sw[2] = {0.f, 0.f}, sa[4], sa_next[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sa_next[i] = live && i < blocks ? as[(long long)i * a.ld_as + row] : 0.f;
-      f32x2 sum[4][16];
+      for (int i = 0; i < 4; ++i) sa_next[i] = live && b_begin + i < b_end ? as[(long long)(b_begin + i) * a.ld_as + row] : 0.f;
+      f32x2 sum[CH][16];
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < CH; ++c)
 #pragma unroll
         for (int j = 0; j < 16; ++j) sum[c][j] = 0ull;
       uint32_t v[2][32];
       f8_wait(acc_full[half] + acc, acc_phase, &dead, a.failed);
       __syncwarp();
       tc_fence_after();
-      tmem_ld32(lanes + (uint32_t)(acc * FL_BN), v[0]);
-      for (int b0 = 0; b0 < blocks; b0 += 4) {
+      tmem_ld32(lanes + (uint32_t)(acc * 256), v[0]);
+      // (a block is an odd number of loads where CH is 3: its first goes to v[i & 1] there, four blocks to a round)
+      for (int b0 = b_begin; b0 < b_end; b0 += 4) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           sa[i] = sa_next[i];
-          sa_next[i] = live && b0 + 4 + i < blocks ? as[(long long)(b0 + 4 + i) * a.ld_as + row] : 0.f;
+          sa_next[i] = live && b0 + 4 + i < b_end ? as[(long long)(b0 + 4 + i) * a.ld_as + row] : 0.f;
         }
-        if (b0 % 32 == 0 && b0 + lane < blocks) {
+        if ((b0 - b_begin) % 32 == 0 && b0 + lane < b_end) {
           sw[0] = w0[b0 + lane];
-          if constexpr (GATED) sw[1] = w0[blocks + b0 + lane];
+          if (two) sw[1] = w0[blocks + b0 + lane];
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (b0 + i < blocks) {
+          if (b0 + i < b_end) {
             f32x2 s[2];
 #pragma unroll
-            for (int h = 0; h < (GATED ? 2 : 1); ++h) {
-              const float x = sa[i] * __shfl_sync(0xffffffffu, sw[h], (b0 + i) & 31);
+            for (int h = 0; h < (GATED || CH == 3 ? 2 : 1); ++h) {
+              const float x = sa[i] * __shfl_sync(0xffffffffu, sw[h], (b0 + i - b_begin) & 31);
               s[h] = pair_of(x, x);
             }
-            const uint32_t from = lanes + (uint32_t)(acc * FL_BN);
+            const uint32_t from = lanes + (uint32_t)(acc * 256);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              tmem_ld_wait_for(v[c & 1]);
-              if (c < 3) {
-                tmem_ld32(from + (uint32_t)(c * 32 + 32), v[(c + 1) & 1]);
+            for (int c = 0; c < CH; ++c) {
+              constexpr int ODD = CH & 1;
+              uint32_t(&now)[32] = v[(c + ODD * i) & 1];
+              uint32_t(&next)[32] = v[(c + 1 + ODD * i) & 1];
+              tmem_ld_wait_for(now);
+              if (c < CH - 1) {
+                tmem_ld32(from + (uint32_t)(c * 32 + 32), next);
               } else {  // the accumulator is free; the next one's first columns while the last of this are added
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) f8_arrive(empty0 + acc * 8);
                 acc ^= 1;
                 if (acc == 0) acc_phase ^= 1u;
-                if (b0 + i + 1 < blocks) {
+                if (b0 + i + 1 < b_end) {
                   f8_wait(acc_full[half] + acc, acc_phase, &dead, a.failed);
                   __syncwarp();
                   tc_fence_after();
-                  tmem_ld32(lanes + (uint32_t)(acc * FL_BN), v[0]);
+                  tmem_ld32(lanes + (uint32_t)(acc * 256), next);
                 }
               }
-              promote(sum[c], v[c & 1], s[GATED ? c >> 1 : 0]);
+              promote(sum[c], now, GATED || CH == 3 ? (scale_of(c) ? s[1] : s[0]) : s[0]);
             }
           }
         }
+      }
+      if constexpr (SPLIT) {
+        // pieces of 32 x 32 sums, [piece][column / 4][row][4]; of all CTAs' a CTA adds up every `splits`-th, a warp to a piece
+        float4* red = reinterpret_cast<float4*>(smem) + lane;
+        asm volatile("bar.sync 5, 256;" ::: "memory");  // (both halves' products have read the ring)
+        if (*(volatile int*)&dead == 0) {
+#pragma unroll
+          for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float2 x = halves_of(sum[c][2 * j]), y = halves_of(sum[c][2 * j + 1]);
+              red[(((quarter * 2 + half) * CH + c) * 8 + j) * 32] = make_float4(x.x, x.y, y.x, y.y);
+            }
+        }
+        cluster_sync_all();
+        for (int piece = split + (warp - 4) * a.splits; piece < 8 * CH; piece += 8 * a.splits) {
+          float4 x[8], total[8];
+          for (int p = 0; p < a.splits; ++p) {
+            const uint32_t at = mapa_shared(red + piece * 256, p);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = ld_cluster_v4(at + j * 512);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              total[j] = p == 0 ? x[j] : make_float4(total[j].x + x[j].x, total[j].y + x[j].y, total[j].z + x[j].z, total[j].w + x[j].w);
+          }
+          const int r = row0 + piece / (2 * CH) * 32 + lane, n = n0 + piece % (2 * CH) * 32;
+          if (r < row_end) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (n + j * 8 < a.N) {
+                const float4 lo = total[2 * j], hi = total[2 * j + 1];
+                if (a.out_f32) {
+                  float4* to = reinterpret_cast<float4*>((float*)a.C + (long long)r * a.N + n + j * 8);
+                  to[0] = lo;
+                  to[1] = hi;
+                } else {
+                  st_v4((bf16*)a.C + (long long)r * a.N + n + j * 8,
+                        make_uint4(pack_bf16x2(lo.x, lo.y), pack_bf16x2(lo.z, lo.w), pack_bf16x2(hi.x, hi.y), pack_bf16x2(hi.z, hi.w)));
+                }
+              }
+          }
+        }
+        continue;  // (a tile to a CTA: the loop ends)
       }
       // ---- the sums leave ----
       if constexpr (GATED) {
@@ -401,11 +474,11 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
         }
         parity ^= 1;
       } else if (a.out_f32) {
-        float* to = (float*)a.C + (long long)row * a.N + n0 + half * 128;
-        const int cols = a.N - n0 - half * 128;
+        float* to = (float*)a.C + (long long)row * a.N + n0 + half * (BN / 2);
+        const int cols = a.N - n0 - half * (BN / 2);
         if (live) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < CH; ++c)
 #pragma unroll
             for (int j = 0; j < 8; ++j)
               if (c * 32 + j * 4 < cols) {
@@ -414,14 +487,16 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
               }
         }
       } else {
-        const int r0 = row0 + quarter * 32, n = n0 + half * 128;
+        const int r0 = row0 + quarter * 32, n = n0 + half * (BN / 2);
+        constexpr int WIDE = CH % 2 ? 32 : 64;              // columns at a time
+        constexpr bool COPIES = !GROUPED && WIDE == 64;     // by the copy engine, which takes 64
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {  // 64 columns at a time
-          if (!GROUPED && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        for (int h = 0; h < 32 * CH / WIDE; ++h) {
+          if (COPIES && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
           __syncwarp();
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const f32x2* x = sum[2 * h + j / 4] + 4 * (j & 3);
+          for (int j = 0; j < WIDE / 8; ++j) {
+            const f32x2* x = sum[h * (WIDE / 32) + j / 4] + 4 * (j & 3);
             uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -432,7 +507,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
                          "r"(w[2]), "r"(w[3])
                          : "memory");
           }
-          if constexpr (!GROUPED) {
+          if constexpr (COPIES) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0 && n + 64 * h < a.N && r0 < a.M) {
@@ -442,8 +517,9 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
           } else {
             __syncwarp();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int r = i * 4 + (lane >> 3), c = lane & 7, col = n + 64 * h + c * 8;
+            for (int i = 0; i < WIDE / 8; ++i) {
+              constexpr int ACROSS = WIDE / 8;  // lanes to a row
+              const int r = i * (32 / ACROSS) + lane / ACROSS, c = lane % ACROSS, col = n + WIDE * h + c * 8;
               if (r0 + r < row_end && col < a.N) st_v4((bf16*)a.C + (long long)(r0 + r) * a.N + col, lds_v4(patch_s + r * 128 + ((c ^ (r & 7)) << 4)));
             }
             __syncwarp();
@@ -457,7 +533,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
   tc_fence_before();
   __syncthreads();
   if (dead) f8_let_copies_end();
-  if constexpr (PAIR) cluster_sync_all();
+  if constexpr (PAIR || SPLIT) f8_leave_cluster();  // nobody leaves with what a peer still reads or signals
   if (warp == 1) {
     tc_fence_after();
     if constexpr (PAIR)
@@ -468,40 +544,36 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
 }
 
 // ---- small ---------------------------------------------------------------------------------------------------------------------
-constexpr int FS_MAX_STAGES = 8, FS_MAX_SPLITS = 8, FS_SCALES = 576;  // bytes of a stage's scales of rows: up to 132, from a multiple of four on
+constexpr int FS_MAX_STAGES = 8, FS_MAX_SPLITS = 8, FS_MAX_ACCS = 4, FS_SCALES = 512;  // bytes of a stage's scales of rows
 constexpr int FS_RING_ALONE = 208 * 1024, FS_RING_SHARED = 106 * 1024;
 
 // CTAs of a tile to an SM: registers for the sums and the loads, tensor memory and the ring allow two where the rows are few
 template <bool GATED>
 constexpr int small_resident(int most_rows) { return most_rows <= (GATED ? 32 : 64) ? 2 : 1; }
 
-// GATED: 128 gates and the 128 that they gate, else 128 rows of W; MOST: rows of A at most (a thread's sums)
-template <bool GATED, int MOST, bool GROUPED>
-__global__ void __launch_bounds__(GATED ? 320 : 192, small_resident<GATED>(MOST))
+// groups of four warps that share an accumulator's columns (rows of A), 64 each
+constexpr int small_groups(int most_rows) { return most_rows > 64 ? 2 : 1; }
+template <bool GATED>
+constexpr int small_threads(int most_rows) { return 64 + 128 * (GATED ? 2 : 1) * small_groups(most_rows); }
+
+// GATED: 128 gates and the 128 that they gate, else 128 rows of W; MOST: rows of A at most
+template <bool GATED, int MOST>
+__global__ void __launch_bounds__(small_threads<GATED>(MOST), small_resident<GATED>(MOST))
     gemm_fp8_small_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
                           const __grid_constant__ Fp8Args a) {
-  constexpr int WT = GATED ? 2 : 1, NT = WT * 128, EPI = 4 * WT, THREADS = 64 + 32 * EPI;
+  constexpr int WT = GATED ? 2 : 1, NT = WT * 128, CG = small_groups(MOST), EPI = 4 * WT * CG, THREADS = 64 + 32 * EPI;
+  constexpr int CHUNKS = MOST / CG / 32;               // of 32 columns to a warp
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  __shared__ __align__(8) uint64_t full[FS_MAX_STAGES], empty[FS_MAX_STAGES], acc_full[2], acc_empty[2];
+  __shared__ __align__(8) uint64_t full[FS_MAX_STAGES], empty[FS_MAX_STAGES], acc_full[FS_MAX_ACCS], acc_empty[FS_MAX_ACCS];
   __shared__ __align__(16) float scales[FS_MAX_STAGES][FS_SCALES / 4];
   __shared__ uint32_t tmem_slot;
   __shared__ int dead;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int splits = a.splits, split = blockIdx.x, n0 = blockIdx.y * NT;
   const float *as = a.as, *ws = a.ws;
-  int g = 0, row0 = blockIdx.z * a.rows, row_end = a.M;
-  if constexpr (GROUPED) {
-    wait_for_previous();
-    if ((int)blockIdx.z >= min(*a.n_mt, a.max_mt)) return;
-    const int4 e = a.tab[blockIdx.z];
-    g = min(max(e.x, 0), a.groups - 1);
-    row0 = max(e.y, 0);
-    row_end = min(e.z, a.M);
-    if (row0 >= row_end) return;
-  }
-  const int rows = min(row_end - row0, a.rows), mp = (rows + 15) & ~15, stride = (rows + 31) & ~31;  // stride: columns of an accumulator
-  const int boxes = GROUPED ? (rows + a.box_rows - 1) / a.box_rows : 1;
+  const int row0 = blockIdx.z * a.rows;
+  const int rows = min(a.M - row0, a.rows), mp = (rows + 15) & ~15, stride = (rows + 31) & ~31;  // stride: columns of an accumulator
   const int b0 = split * a.blocks / splits, b1 = (split + 1) * a.blocks / splits;
   const int a_room = (a.rows + 31) / 32 * 32 * FP8_BLOCK, stage_bytes = WT * F8_STAGE_W + a_room;
 
@@ -513,7 +585,7 @@ __global__ void __launch_bounds__(GATED ? 320 : 192, small_resident<GATED>(MOST)
       mbar_init(full + s, 1);
       mbar_init(empty + s, 1 + EPI);  // the products', and the warps that have read the scales
     }
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < a.accs; ++s) {
       mbar_init(acc_full + s, 1);
       mbar_init(acc_empty + s, EPI);
     }
@@ -524,17 +596,15 @@ __global__ void __launch_bounds__(GATED ? 320 : 192, small_resident<GATED>(MOST)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
-  const int w_row = g * a.N + n0;
-  if (!GROUPED && warp == 0 && lane == 0)  // the first weights into L2 while the kernel before this one ends
-    for (int i = 0; i < min(a.stages, b1 - b0); ++i) tma_prefetch_2d(&tmap_w, (b0 + i) * 64, w_row);
+  if (warp == 0 && lane == 0)  // the first weights into L2 while the kernel before this one ends
+    for (int i = 0; i < min(a.stages, b1 - b0); ++i) tma_prefetch_2d(&tmap_w, (b0 + i) * 64, n0);
   __syncwarp();
   follow_previous(as, ws);
 
   if (warp == 0) {
     if (lane == 0) {
-      // scales of the rows: from a multiple of four on, no further than their line goes
-      const int s0 = row0 & ~3, n_scales = min((row0 - s0 + mp + 3) & ~3, a.ld_as - s0);
-      const uint32_t bytes = (uint32_t)(WT * F8_STAGE_W + boxes * a.box_rows * FP8_BLOCK + n_scales * 4);
+      const int n_scales = min(mp, a.ld_as - row0);  // (no further than their line goes: a multiple of four, as row0 is)
+      const uint32_t bytes = (uint32_t)(WT * F8_STAGE_W + a.box_rows * FP8_BLOCK + n_scales * 4);
       int stage = 0;
       uint32_t phase = 0;
       for (int b = b0; b < b1; ++b) {
@@ -542,10 +612,9 @@ __global__ void __launch_bounds__(GATED ? 320 : 192, small_resident<GATED>(MOST)
         f8_wait(empty + stage, phase ^ 1u, &dead, a.failed);
         if (*(volatile int*)&dead) break;
         mbar_expect_tx(full + stage, bytes);
-        tma_load_2d(to, &tmap_w, b * 64, w_row, full + stage);
-        for (int x = 0; x < boxes; ++x)
-          tma_load_2d(to + WT * F8_STAGE_W + x * a.box_rows * FP8_BLOCK, &tmap_a, b * 64, row0 + x * a.box_rows, full + stage);
-        tma_bulk_g2s(scales[stage], as + (long long)b * a.ld_as + s0, n_scales * 4, full + stage);
+        tma_load_2d(to, &tmap_w, b * 64, n0, full + stage);
+        tma_load_2d(to + WT * F8_STAGE_W, &tmap_a, b * 64, row0, full + stage);
+        tma_bulk_g2s(scales[stage], as + (long long)b * a.ld_as + row0, n_scales * 4, full + stage);
         if (++stage == a.stages) {
           stage = 0;
           phase ^= 1u;
@@ -558,45 +627,45 @@ __global__ void __launch_bounds__(GATED ? 320 : 192, small_resident<GATED>(MOST)
     const uint32_t ring = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
     int stage = 0, acc = 0;
     uint32_t phase = 0, acc_phase = 0;
-    for (int b = b0; b < b1; ++b) {
-      if (!mbar_wait_warp(acc_empty + acc, acc_phase ^ 1u, &dead, a.failed, WAIT_CYCLES)) break;
-      if (!mbar_wait_warp(full + stage, phase, &dead, a.failed, WAIT_CYCLES)) break;
-      tc_fence_after();
-      if (elect_one()) {
+    if (elect_one())
+      for (int b = b0; b < b1; ++b) {
+        f8_wait(acc_empty + acc, acc_phase ^ 1u, &dead, a.failed);
+        f8_wait(full + stage, phase, &dead, a.failed);
+        if (*(volatile int*)&dead) break;
+        tc_fence_after();
         const uint32_t sw = ring + (uint32_t)(stage * stage_bytes), sa = sw + WT * F8_STAGE_W, d = tmem + (uint32_t)(acc * WT * stride);
 #pragma unroll
         for (int h = 0; h < WT; ++h)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             umma_fp8(d + (uint32_t)(h * stride), make_smem_desc(sw + h * F8_STAGE_W + k * 32), make_smem_desc(sa + k * 32), idesc, k > 0);
-        umma_commit(empty + stage);
         umma_commit(acc_full + acc);
+        umma_commit(empty + stage);
+        if (++stage == a.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+        if (++acc == a.accs) {
+          acc = 0;
+          acc_phase ^= 1u;
+        }
       }
-      __syncwarp();
-      if (++stage == a.stages) {
-        stage = 0;
-        phase ^= 1u;
-      }
-      acc ^= 1;
-      if (acc == 0) acc_phase ^= 1u;
-    }
     __syncwarp();
   }
 
   // ---- lane = row of W, column = row of A ----
   float* red = reinterpret_cast<float*>(smem);
   if (warp >= 2) {
-    const int quarter = warp & 3, which = (warp - 2) >> 2;  // which: gates, or what they gate
-    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(which * stride);
-    const float* w0 = ws + ((long long)g * a.n_blocks + blockIdx.y * WT + which) * a.blocks;
-    f32x2 sum[MOST / 32][16];
+    const int quarter = warp & 3, which = (warp - 2) / 4 % WT, col0 = (warp - 2) / (4 * WT) * (MOST / CG);  // which: gates, or what they gate
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(which * stride + col0);
+    const float* w0 = ws + (long long)(blockIdx.y * WT + which) * a.blocks;
+    f32x2 sum[CHUNKS][16];
 #pragma unroll
-    for (int c = 0; c < MOST / 32; ++c)
+    for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
       for (int j = 0; j < 16; ++j) sum[c][j] = 0ull;
     int stage = 0, acc = 0;
     uint32_t phase = 0, acc_phase = 0;
-    const int shift = row0 & 3;
     float sw = 0.f;
     for (int b = b0; b < b1; ++b) {
       if ((b - b0) % 32 == 0 && b + lane < b1) sw = w0[b + lane];
@@ -606,24 +675,20 @@ __global__ void __launch_bounds__(GATED ? 320 : 192, small_resident<GATED>(MOST)
       f8_wait(acc_full + acc, acc_phase, &dead, a.failed);
       __syncwarp();
       tc_fence_after();
+      uint32_t v[CHUNKS][32];
 #pragma unroll
-      for (int c = 0; c < MOST / 32; ++c)
-        if (c * 32 < rows) {
-          uint32_t v[32];
-          tmem_ld32(lanes + (uint32_t)(acc * WT * stride + c * 32), v);
-          tmem_ld_wait_for(v);
+      for (int c = 0; c < CHUNKS; ++c)
+        if (col0 + c * 32 < rows) tmem_ld32(lanes + (uint32_t)(acc * WT * stride + c * 32), v[c]);
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c)
+        if (col0 + c * 32 < rows) {
+          tmem_ld_wait_for(v[c]);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            float4 s;
-            if constexpr (GROUPED) {
-              const float* p = scales[stage] + shift + c * 32 + j * 4;
-              s = make_float4(p[0], p[1], p[2], p[3]);
-            } else {
-              s = *reinterpret_cast<const float4*>(scales[stage] + c * 32 + j * 4);
-            }
-            sum[c][2 * j] = fma2(pair_of(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1])), mul2(pair_of(s.x, s.y), by), sum[c][2 * j]);
+            const float4 s = *reinterpret_cast<const float4*>(scales[stage] + col0 + c * 32 + j * 4);
+            sum[c][2 * j] = fma2(pair_of(__uint_as_float(v[c][4 * j]), __uint_as_float(v[c][4 * j + 1])), mul2(pair_of(s.x, s.y), by), sum[c][2 * j]);
             sum[c][2 * j + 1] =
-                fma2(pair_of(__uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3])), mul2(pair_of(s.z, s.w), by), sum[c][2 * j + 1]);
+                fma2(pair_of(__uint_as_float(v[c][4 * j + 2]), __uint_as_float(v[c][4 * j + 3])), mul2(pair_of(s.z, s.w), by), sum[c][2 * j + 1]);
           }
         }
       tc_fence_before();
@@ -636,21 +701,23 @@ __global__ void __launch_bounds__(GATED ? 320 : 192, small_resident<GATED>(MOST)
         stage = 0;
         phase ^= 1u;
       }
-      acc ^= 1;
-      if (acc == 0) acc_phase ^= 1u;
+      if (++acc == a.accs) {
+        acc = 0;
+        acc_phase ^= 1u;
+      }
     }
     // (every warp has seen the last products, which have read the ring; a CTA that gave up leaves the ring alone)
     asm volatile("bar.sync 1, %0;" ::"n"(32 * EPI) : "memory");
     if (*(volatile int*)&dead == 0) {
       const int at = which * 128 + quarter * 32 + lane;
 #pragma unroll
-      for (int c = 0; c < MOST / 32; ++c)
-        if (c * 32 < rows) {
+      for (int c = 0; c < CHUNKS; ++c)
+        if (col0 + c * 32 < rows) {
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             const float2 f = halves_of(sum[c][j]);
-            red[(c * 32 + 2 * j) * NT + at] = f.x;
-            red[(c * 32 + 2 * j + 1) * NT + at] = f.y;
+            red[(col0 + c * 32 + 2 * j) * NT + at] = f.x;
+            red[(col0 + c * 32 + 2 * j + 1) * NT + at] = f.y;
           }
         }
     }
@@ -700,7 +767,7 @@ __global__ void __launch_bounds__(GATED ? 320 : 192, small_resident<GATED>(MOST)
         *reinterpret_cast<uint2*>((bf16*)a.C + row * a.N + n0 + lane * 4) = make_uint2(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w));
     }
   }
-  if (splits > 1) cluster_sync_all();  // nobody leaves with what a peer still reads
+  if (splits > 1) f8_leave_cluster();  // nobody leaves with what a peer still reads
   tc_fence_before();
   __syncthreads();
   if (dead) f8_let_copies_end();
@@ -743,10 +810,11 @@ static int clusters_that_fit(K kern, int cluster, int threads, int smem) {
   return n < num_sms() / cluster ? n : num_sms() / cluster;
 }
 
-template <bool PAIR, bool GATED, bool GROUPED>
+// splits > 1 (SPLIT): CTAs to a tile
+template <bool PAIR, int CH, bool GATED, bool GROUPED, bool SPLIT>
 static int launch_large(const void* A, long long a_rows, const void* W, long long w_rows, Fp8Args a, cudaStream_t st) {
-  using Cfg = LargeCfg<PAIR, GATED>;
-  auto kern = gemm_fp8_large_kernel<PAIR, GATED, GROUPED>;
+  using Cfg = LargeCfg<PAIR, CH, GATED>;
+  auto kern = gemm_fp8_large_kernel<PAIR, CH, GATED, GROUPED, SPLIT>;
   static uint64_t seen[2];
   int rc = once_per_device(seen, [&]() -> int {
     B200Q_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
@@ -754,26 +822,30 @@ static int launch_large(const void* A, long long a_rows, const void* W, long lon
   });
   CUtensorMap ta, tw, tc = {};
   // (two codes are one element of the maps; a box is 128 codes wide)
-  if (!rc) rc = get_tmap(A, a_rows, a.K / 2, 128, &ta);
+  const int box = !GROUPED && a_rows < 128 ? ((int)a_rows + 7) & ~7 : 128;  // rows of A that travel
+  a.a_bytes = box * FP8_BLOCK;
+  if (!rc) rc = get_tmap(A, a_rows, a.K / 2, box, &ta);
   if (!rc) rc = get_tmap(W, w_rows, a.K / 2, Cfg::BOX, &tw);
   if (!rc && !GROUPED && GATED) rc = get_tmap(a.C, a.M, a.N / 4, 32, &tc);
   if (!rc && !GROUPED && !GATED && !a.out_f32) rc = get_tmap(a.C, a.M, a.N, 32, &tc);
   if (rc) return rc;
-  const long long n_tiles = (a.N + FL_BN - 1) / FL_BN, m_tiles = GROUPED ? a.max_mt : (a.M + (PAIR ? 255 : 127)) / (PAIR ? 256 : 128);
-  B200Q_CHECK_ARG(n_tiles * m_tiles < (1ll << 31), "gemm_fp8: too many tiles (M=%d N=%d)", a.M, a.N);
+  const long long n_tiles = (a.N + Cfg::BN - 1) / Cfg::BN, m_tiles = GROUPED ? a.max_mt : (a.M + (PAIR ? 255 : 127)) / (PAIR ? 256 : 128);
+  const long long tiles = n_tiles * m_tiles;
+  B200Q_CHECK_ARG(tiles < (1ll << 27), "gemm_fp8: too many tiles (M=%d N=%d)", a.M, a.N);
   static int pairs = 0;
   if (PAIR && pairs == 0) pairs = clusters_that_fit(kern, 2, FL_THREADS, Cfg::SMEM);
-  const long long units = PAIR ? pairs : num_sms(), grid = (n_tiles * m_tiles < units ? n_tiles * m_tiles : units) * (PAIR ? 2 : 1);
-  B200Q_CUDA(launch_early(kern, (int)grid, FL_THREADS, Cfg::SMEM, st, PAIR ? 2 : 1, ta, tw, tc, a));
+  const long long units = PAIR ? pairs : num_sms(), at_once = SPLIT || tiles < units ? tiles : units;
+  const int cluster = PAIR ? 2 : SPLIT ? a.splits : 1;
+  B200Q_CUDA(launch_early(kern, (int)(at_once * cluster), FL_THREADS, Cfg::SMEM, st, cluster, ta, tw, tc, a));
   count_launch();
   return B200Q_OK;
 }
 
-template <bool GATED, int MOST, bool GROUPED>
-static int launch_small(const void* A, long long a_rows, const void* W, long long w_rows, Fp8Args a, cudaStream_t st) {
-  constexpr int NT = GATED ? 256 : 128, THREADS = GATED ? 320 : 192, RESIDENT = small_resident<GATED>(MOST);
+template <bool GATED, int MOST>
+static int launch_small(const void* A, const void* W, Fp8Args a, cudaStream_t st) {
+  constexpr int NT = GATED ? 256 : 128, THREADS = small_threads<GATED>(MOST), RESIDENT = small_resident<GATED>(MOST);
   constexpr int RING = RESIDENT == 2 ? FS_RING_SHARED : FS_RING_ALONE;
-  auto kern = gemm_fp8_small_kernel<GATED, MOST, GROUPED>;
+  auto kern = gemm_fp8_small_kernel<GATED, MOST>;
   static uint64_t seen[2];
   static int fit[FS_MAX_SPLITS + 1];
   int rc = once_per_device(seen, [&]() -> int {
@@ -781,14 +853,16 @@ static int launch_small(const void* A, long long a_rows, const void* W, long lon
     return B200Q_OK;
   });
   if (rc) return rc;
-  const int n_tiles = (a.N + NT - 1) / NT, m_tiles = GROUPED ? a.max_mt : (a.M + a.rows - 1) / a.rows;
+  const int n_tiles = (a.N + NT - 1) / NT, m_tiles = (a.M + a.rows - 1) / a.rows;
   B200Q_CHECK_ARG(n_tiles <= 65535 && m_tiles <= 65535, "gemm_fp8: too many tiles (M=%d N=%d)", a.M, a.N);
-  a.box_rows = GROUPED ? 32 : (a.rows + 7) & ~7;
-  if (!GROUPED && a.M < a.box_rows) a.box_rows = (a.M + 7) & ~7;
+  a.box_rows = a.M < a.rows ? (a.M + 7) & ~7 : a.rows;
   const int stage = (GATED ? 2 : 1) * F8_STAGE_W + (a.rows + 31) / 32 * 32 * FP8_BLOCK;
   a.stages = RING / stage < FS_MAX_STAGES ? RING / stage : FS_MAX_STAGES;
+  // accumulators: four where they fit the CTA's share of tensor memory, so that no role waits for the round through the others
+  const int each = (GATED ? 2 : 1) * ((a.rows + 31) / 32 * 32);
+  a.accs = FS_MAX_ACCS * each <= 512 / RESIDENT ? FS_MAX_ACCS : 512 / RESIDENT / each;
   a.cols = 32;
-  while (a.cols < 2 * (GATED ? 2 : 1) * ((a.rows + 31) / 32 * 32)) a.cols *= 2;
+  while (a.cols < a.accs * each) a.cols *= 2;
   // splits: as many as leave every cluster resident, three blocks each at least
   a.splits = 1;
   if (!batch_invariant())
@@ -797,22 +871,25 @@ static int launch_small(const void* A, long long a_rows, const void* W, long lon
       if ((long long)n_tiles * m_tiles <= (long long)fit[s] * RESIDENT) a.splits = s;
     }
   CUtensorMap ta, tw;
-  rc = get_tmap(A, a_rows, a.K / 2, a.box_rows, &ta);
-  if (!rc) rc = get_tmap(W, w_rows, a.K / 2, NT, &tw);
+  rc = get_tmap(A, a.M, a.K / 2, a.box_rows, &ta);
+  if (!rc) rc = get_tmap(W, a.N, a.K / 2, NT, &tw);
   if (rc) return rc;
   B200Q_CUDA(launch_early(kern, dim3(a.splits, n_tiles, m_tiles), THREADS, RING + 1024, st, a.splits, ta, tw, a));
   count_launch();
   return B200Q_OK;
 }
 
-template <bool GATED, bool GROUPED>
-static int launch_small(const void* A, long long a_rows, const void* W, long long w_rows, const Fp8Args& a, cudaStream_t st) {
-  if (a.rows <= 32) return launch_small<GATED, 32, GROUPED>(A, a_rows, W, w_rows, a, st);
-  if (a.rows <= 64) return launch_small<GATED, 64, GROUPED>(A, a_rows, W, w_rows, a, st);
-  return launch_small<GATED, 128, GROUPED>(A, a_rows, W, w_rows, a, st);
+template <bool GATED>
+static int launch_small(const void* A, const void* W, const Fp8Args& a, cudaStream_t st) {
+  if (a.rows <= 32) return launch_small<GATED, 32>(A, W, a, st);
+  if constexpr (GATED) {
+    return launch_small<GATED, 64>(A, W, a, st);
+  } else {
+    return a.rows <= 64 ? launch_small<GATED, 64>(A, W, a, st) : launch_small<GATED, 128>(A, W, a, st);
+  }
 }
 
-int g_fp8_mode = 0;  // test hook: 1 = small tiles, 2 = large ones of one CTA, 3 = of a pair
+int g_fp8_mode = 0;  // test hook: 1 = small tiles; large ones of 64 * (mode / 10 % 10) columns (dense), 2 = of one CTA, 3 = of a pair, 4 = in mode / 100 parts
 
 static int finish_args(Fp8Args& a) {
   a.blocks = (a.K + FP8_BLOCK - 1) / FP8_BLOCK;
@@ -828,14 +905,33 @@ template <bool GATED>
 static int dense(const void* A, const void* W, Fp8Args a, cudaStream_t st) {
   int rc = finish_args(a);
   if (rc) return rc;
-  int mode = g_fp8_mode;
-  if (mode == 0) mode = a.M <= 128 ? 1 : a.M <= 256 ? 2 : 3;
-  if (mode == 1) {
-    const int tiles = (a.M + 127) / 128;
-    a.rows = ((a.M + tiles - 1) / tiles + 15) / 16 * 16;
-    return launch_small<GATED, false>(A, a.M, W, a.N, a, st);
+  int mode = g_fp8_mode % 10, ch = g_fp8_mode / 10 % 10, splits = g_fp8_mode / 100;
+  if (mode == 0) {
+    mode = a.M <= (GATED ? 64 : 128) ? 1 : a.M <= 256 ? 2 : 3;
+    ch = 4;
   }
-  return mode == 2 ? launch_large<false, GATED, false>(A, a.M, W, a.N, a, st) : launch_large<true, GATED, false>(A, a.M, W, a.N, a, st);
+  if (GATED || ch == 0) ch = 4;
+  if (mode == 1) {
+    const int most = GATED ? 64 : 128, tiles = (a.M + most - 1) / most;
+    a.rows = ((a.M + tiles - 1) / tiles + 15) / 16 * 16;
+    return launch_small<GATED>(A, W, a, st);
+  }
+  auto large = [&](auto pair, auto columns, auto split) {
+    return launch_large<decltype(pair)::value, decltype(columns)::value, GATED, false, decltype(split)::value>(A, a.M, W, a.N, a, st);
+  };
+  const std::integral_constant<int, 4> all;
+  const std::true_type yes;
+  const std::false_type no;
+  if constexpr (!GATED) {
+    if (mode == 4 && (a.splits = splits < a.blocks ? splits : a.blocks) > 1) {
+      if (ch == 2) return large(no, std::integral_constant<int, 2>{}, yes);
+      return ch == 3 ? large(no, std::integral_constant<int, 3>{}, yes) : large(no, all, yes);
+    }
+    if (mode == 3 && ch == 3) return large(yes, std::integral_constant<int, 3>{}, no);
+    if (mode != 3 && ch == 3) return large(no, std::integral_constant<int, 3>{}, no);
+    if (mode != 3 && ch == 2) return large(no, std::integral_constant<int, 2>{}, no);
+  }
+  return mode == 3 ? large(yes, all, no) : large(no, all, no);
 }
 
 template <bool GATED>
@@ -843,13 +939,7 @@ static int grouped(const void* A, long long a_rows, const void* W, int groups, F
   int rc = finish_args(a);
   if (rc) return rc;
   a.groups = groups;
-  int mode = g_fp8_mode;
-  if (mode == 0) mode = a_rows <= 64ll * groups ? 1 : 2;
-  if (mode == 1) {
-    a.rows = 128;
-    return launch_small<GATED, true>(A, a_rows, W, (long long)groups * a.N, a, st);
-  }
-  return launch_large<false, GATED, true>(A, a_rows, W, (long long)groups * a.N, a, st);
+  return launch_large<false, 4, GATED, true, false>(A, a_rows, W, (long long)groups * a.N, a, st);
 }
 
 static bool fp8_aligned(const void* a, const void* b, const void* c, const void* d) {
@@ -960,9 +1050,12 @@ int b200q_gemm_grouped_gated_fp8(const void* A, int a_rows, const float* a_scale
   return grouped<true>(A, a_rows, W, groups, a, as_stream(stream));
 }
 
-// test hook: 0 = by size, 1 = small tiles, 2 = large tiles of one CTA, 3 = of a pair (dense products)
+// test hook: 0 = by size, 1 = small tiles, 2 = large tiles of one CTA, 3 = of a pair, 4 = of one CTA, in mode / 100 parts; mode / 10 % 10: 64
+// columns each to a dense product's tile (2, 3, 4 = 0)
 int b200q_gemm_fp8_set_mode(int mode) {
-  B200Q_CHECK_ARG(mode >= 0 && mode <= 3, "gemm_fp8_set_mode: mode=%d", mode);
+  const int kind = mode % 10, ch = mode / 10 % 10, splits = mode / 100;
+  B200Q_CHECK_ARG(mode >= 0 && kind <= 4 && (ch == 0 || (ch >= 2 && ch <= 4)) && splits <= FL_MAX_SPLITS && (splits > 0) == (kind == 4),
+                  "gemm_fp8_set_mode: mode=%d", mode);
   g_fp8_mode = mode;
   bump_tuning_epoch();
   return B200Q_OK;
