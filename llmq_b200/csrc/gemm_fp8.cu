@@ -323,9 +323,16 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
       const float* w0 = ws + ((long long)g * a.n_blocks + min(nb0, a.n_blocks - 1)) * blocks;
       const bool two = GATED || (CH == 3 && nb0 + 1 < a.n_blocks);
       auto scale_of = [&](int c) { return GATED ? c >> 1 : CH == 3 ? (col0 + 32 * c) >> 7 : 0; };
-      float sw[2] = {0.f, 0.f}, sa[4], sa_next[4];
+      // (without a condition: a load that may not be made is waited for where it is made.  Rows and blocks that do not exist take the last ones')
+      const float* own_scales = as + min(row, row_end - 1);
+      auto row_scale = [&](int b) { return own_scales[(long long)min(b, b_end - 1) * a.ld_as]; };
+      auto column_scale = [&](int b, int h) { return w0[(h && two ? blocks : 0) + min(b + lane, b_end - 1)]; };
+      constexpr int SCALES = GATED || CH == 3 ? 2 : 1;
+      float sw[SCALES], sa[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sa_next[i] = live && b_begin + i < b_end ? as[(long long)(b_begin + i) * a.ld_as + row] : 0.f;
+      for (int h = 0; h < SCALES; ++h) sw[h] = column_scale(b_begin, h);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sa[i] = row_scale(b_begin + i);
       f32x2 sum[CH][16];
 #pragma unroll
       for (int c = 0; c < CH; ++c)
@@ -338,24 +345,24 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
       tmem_ld32(lanes + (uint32_t)(acc * 256), v[0]);
       // (a block is an odd number of loads where CH is 3: its first goes to v[i & 1] there, four blocks to a round)
       for (int b0 = b_begin; b0 < b_end; b0 += 4) {
+        // four blocks' factors, and only then the loads of the next four: a wait for a load is one for all that were issued before it
+        float x[4][SCALES];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          sa[i] = sa_next[i];
-          sa_next[i] = live && b0 + 4 + i < b_end ? as[(long long)(b0 + 4 + i) * a.ld_as + row] : 0.f;
-        }
-        if ((b0 - b_begin) % 32 == 0 && b0 + lane < b_end) {
-          sw[0] = w0[b0 + lane];
-          if (two) sw[1] = w0[blocks + b0 + lane];
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int h = 0; h < SCALES; ++h) x[i][h] = sa[i] * __shfl_sync(0xffffffffu, sw[h], (b0 + i - b_begin) & 31);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sa[i] = row_scale(b0 + 4 + i);
+        if ((b0 + 4 - b_begin) % 32 == 0) {
+#pragma unroll
+          for (int h = 0; h < SCALES; ++h) sw[h] = column_scale(b0 + 4, h);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if (b0 + i < b_end) {
-            f32x2 s[2];
+            f32x2 s[SCALES];
 #pragma unroll
-            for (int h = 0; h < (GATED || CH == 3 ? 2 : 1); ++h) {
-              const float x = sa[i] * __shfl_sync(0xffffffffu, sw[h], (b0 + i - b_begin) & 31);
-              s[h] = pair_of(x, x);
-            }
+            for (int h = 0; h < SCALES; ++h) s[h] = pair_of(x[i][h], x[i][h]);
             const uint32_t from = lanes + (uint32_t)(acc * 256);
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
@@ -378,7 +385,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
                   tmem_ld32(lanes + (uint32_t)(acc * 256), next);
                 }
               }
-              promote(sum[c], now, GATED || CH == 3 ? (scale_of(c) ? s[1] : s[0]) : s[0]);
+              promote(sum[c], now, SCALES == 2 && scale_of(c) ? s[SCALES - 1] : s[0]);
             }
           }
         }
