@@ -77,9 +77,9 @@ __device__ __forceinline__ void f8_load_2sm(void* to, const void* tmap, int c0, 
 __device__ __forceinline__ void f8_store(const void* tmap, int c0, int c1, uint32_t from) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(tmap), "r"(c0), "r"(c1), "r"(from) : "memory");
 }
-__device__ __forceinline__ void f8_commit_2sm(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
-               "h"((uint16_t)3)
+// arrive on the barrier at this place in both CTAs of the pair, `pair` (a bit to a CTA of the cluster)
+__device__ __forceinline__ void f8_commit_2sm(uint64_t* bar, uint16_t pair) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"(pair)
                : "memory");
 }
 // the last barrier of a cluster: what the others have read of this CTA's memory they have used, and nothing else is handed over (an arrival that
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
                           const __grid_constant__ CUtensorMap tmap_c, const __grid_constant__ Fp8Args a) {
   using Cfg = LargeCfg<PAIR, CH, GATED>;
   static_assert(!GATED || CH == 4, "a gated tile has 128 gates");
-  static_assert(!SPLIT || !(PAIR || GROUPED || GATED), "parts of dense products of single CTAs");
+  static_assert(!SPLIT || !(GROUPED || GATED), "parts of dense products");
   constexpr int STAGES = Cfg::STAGES, BM = PAIR ? 256 : 128, BN = Cfg::BN;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -155,8 +155,9 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
   __shared__ int dead;
   __shared__ float most[2][128];  // gated: the largest of a half row's 64 values
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int rank = PAIR ? (int)cluster_ctarank() : 0;
-  const int split = SPLIT ? (int)cluster_ctarank() : 0, share = PAIR ? 2 : SPLIT ? a.splits : 1;  // share: CTAs to a tile
+  constexpr int CTAS = PAIR ? 2 : 1;  // that make a tile's products together
+  const int in_cluster = PAIR || SPLIT ? (int)cluster_ctarank() : 0, rank = in_cluster % CTAS, leader = in_cluster - rank;
+  const int split = in_cluster / CTAS, share = SPLIT ? CTAS * a.splits : CTAS;  // share: CTAs to a tile
   const int unit = blockIdx.x / share, units = gridDim.x / share;
   const int n_tiles = (a.N + BN - 1) / BN, blocks = a.blocks;
   const int b_begin = SPLIT ? split * blocks / a.splits : 0, b_end = SPLIT ? (split + 1) * blocks / a.splits : blocks;
@@ -232,7 +233,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
             uint8_t* to = smem + stage * Cfg::STAGE;
             f8_wait(empty + stage, phase ^ 1u, &dead, a.failed);
             if constexpr (PAIR) {
-              const uint32_t bar = mapa_shared(full + stage, 0);
+              const uint32_t bar = mapa_shared(full + stage, leader);
               f8_expect_tx(bar, Cfg::STAGE - F8_STAGE_W + a.a_bytes);
 #pragma unroll
               for (int i = 0; i < Cfg::BOXES; ++i) f8_load_2sm(to + F8_STAGE_W + i * Cfg::BOX * 128, &tmap_w, b * 64, wrow + w_box(i), bar);
@@ -274,8 +275,8 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
                 umma_fp8(d, make_smem_desc(sa + k * 32), make_smem_desc(sw + k * 32), idesc, k > 0);
             }
             if constexpr (PAIR) {
-              f8_commit_2sm(acc_full[h] + acc);
-              f8_commit_2sm(empty + stage);
+              f8_commit_2sm(acc_full[h] + acc, (uint16_t)(3 << leader));
+              f8_commit_2sm(empty + stage, (uint16_t)(3 << leader));
             } else {
               umma_commit(acc_full[h] + acc);
               umma_commit(empty + stage);
@@ -299,7 +300,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
     uint8_t* const patch = patches + (warp - 4) * FL_PATCH;
     const uint32_t patch_s = smem_u32(patch);
-    const uint32_t empty0 = PAIR ? mapa_shared(acc_empty[half], 0) : smem_u32(acc_empty[half]);
+    const uint32_t empty0 = PAIR ? mapa_shared(acc_empty[half], leader) : smem_u32(acc_empty[half]);
     int acc = 0, parity = 0;
     uint32_t acc_phase = 0;
     for (int tile = unit; tile < num_tiles; tile += units) {
@@ -391,7 +392,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
         }
       }
       if constexpr (SPLIT) {
-        // pieces of 32 x 32 sums, [piece][column / 4][row][4]; of all CTAs' a CTA adds up every `splits`-th, a warp to a piece
+        // [32 rows][column / 4][row][4] sums; of the tile's pieces of 32 rows x 16 columns a CTA adds up every `splits`-th, a warp to a piece
         float4* red = reinterpret_cast<float4*>(smem) + lane;
         asm volatile("bar.sync 5, 256;" ::: "memory");  // (both halves' products have read the ring)
         if (*(volatile int*)&dead == 0) {
@@ -404,29 +405,41 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
             }
         }
         cluster_sync_all();
-        for (int piece = split + (warp - 4) * a.splits; piece < 8 * CH; piece += 8 * a.splits) {
-          float4 x[8], total[8];
-          for (int p = 0; p < a.splits; ++p) {
-            const uint32_t at = mapa_shared(red + piece * 256, p);
+        for (int piece = split + (warp - 4) * a.splits; piece < 16 * CH; piece += 8 * a.splits) {
+          const int r0 = row0 + piece / (4 * CH) * 32, n = n0 + piece % (4 * CH) * 16;
+          if (r0 >= row_end) break;
+          float4 total[4];
+          constexpr int AT_ONCE = CH == 2 ? 4 : 1;  // parts whose reads are under way together (more registers than there are beside wider tiles)
+#pragma unroll 1
+          for (int p0 = 0; p0 < a.splits; p0 += AT_ONCE) {
+            float4 x[AT_ONCE][4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = ld_cluster_v4(at + j * 512);
+            for (int p = 0; p < AT_ONCE; ++p)
+              if (p0 + p < a.splits) {
+                const uint32_t at = mapa_shared(red + piece * 128, (p0 + p) * CTAS + rank);
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              total[j] = p == 0 ? x[j] : make_float4(total[j].x + x[j].x, total[j].y + x[j].y, total[j].z + x[j].z, total[j].w + x[j].w);
+                for (int j = 0; j < 4; ++j) x[p][j] = ld_cluster_v4(at + j * 512);
+              }
+#pragma unroll
+            for (int p = 0; p < AT_ONCE; ++p)
+              if (p0 + p < a.splits) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  total[j] = p0 + p == 0 ? x[p][j]
+                                         : make_float4(total[j].x + x[p][j].x, total[j].y + x[p][j].y, total[j].z + x[p][j].z, total[j].w + x[p][j].w);
+              }
           }
-          const int r = row0 + piece / (2 * CH) * 32 + lane, n = n0 + piece % (2 * CH) * 32;
-          if (r < row_end) {
+          if (r0 + lane < row_end) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < 2; ++j)
               if (n + j * 8 < a.N) {
                 const float4 lo = total[2 * j], hi = total[2 * j + 1];
+                const long long to = (long long)(r0 + lane) * a.N + n + j * 8;
                 if (a.out_f32) {
-                  float4* to = reinterpret_cast<float4*>((float*)a.C + (long long)r * a.N + n + j * 8);
-                  to[0] = lo;
-                  to[1] = hi;
+                  *reinterpret_cast<float4*>((float*)a.C + to) = lo;
+                  *reinterpret_cast<float4*>((float*)a.C + to + 4) = hi;
                 } else {
-                  st_v4((bf16*)a.C + (long long)r * a.N + n + j * 8,
-                        make_uint4(pack_bf16x2(lo.x, lo.y), pack_bf16x2(lo.z, lo.w), pack_bf16x2(hi.x, hi.y), pack_bf16x2(hi.z, hi.w)));
+                  st_v4((bf16*)a.C + to, make_uint4(pack_bf16x2(lo.x, lo.y), pack_bf16x2(lo.z, lo.w), pack_bf16x2(hi.x, hi.y), pack_bf16x2(hi.z, hi.w)));
                 }
               }
           }
@@ -842,7 +855,7 @@ static int launch_large(const void* A, long long a_rows, const void* W, long lon
   static int pairs = 0;
   if (PAIR && pairs == 0) pairs = clusters_that_fit(kern, 2, FL_THREADS, Cfg::SMEM);
   const long long units = PAIR ? pairs : num_sms(), at_once = SPLIT || tiles < units ? tiles : units;
-  const int cluster = PAIR ? 2 : SPLIT ? a.splits : 1;
+  const int cluster = (PAIR ? 2 : 1) * (SPLIT ? a.splits : 1);
   B200Q_CUDA(launch_early(kern, (int)(at_once * cluster), FL_THREADS, Cfg::SMEM, st, cluster, ta, tw, tc, a));
   count_launch();
   return B200Q_OK;
@@ -896,7 +909,7 @@ static int launch_small(const void* A, const void* W, const Fp8Args& a, cudaStre
   }
 }
 
-int g_fp8_mode = 0;  // test hook: 1 = small tiles; large ones of 64 * (mode / 10 % 10) columns (dense), 2 = of one CTA, 3 = of a pair, 4 = in mode / 100 parts
+int g_fp8_mode = 0;  // test hook: 1 = small tiles; large ones of 64 * (mode / 10 % 10) columns (dense), 2 = of one CTA, 3 = of a pair, 4 and 5 = the same in mode / 100 parts
 
 static int finish_args(Fp8Args& a) {
   a.blocks = (a.K + FP8_BLOCK - 1) / FP8_BLOCK;
@@ -934,11 +947,12 @@ static int dense(const void* A, const void* W, Fp8Args a, cudaStream_t st) {
       if (ch == 2) return large(no, std::integral_constant<int, 2>{}, yes);
       return ch == 3 ? large(no, std::integral_constant<int, 3>{}, yes) : large(no, all, yes);
     }
+    if (mode == 5 && (a.splits = splits < a.blocks ? splits : a.blocks) > 1) return large(yes, all, yes);
     if (mode == 3 && ch == 3) return large(yes, std::integral_constant<int, 3>{}, no);
     if (mode != 3 && ch == 3) return large(no, std::integral_constant<int, 3>{}, no);
     if (mode != 3 && ch == 2) return large(no, std::integral_constant<int, 2>{}, no);
   }
-  return mode == 3 ? large(yes, all, no) : large(no, all, no);
+  return mode == 3 || mode == 5 ? large(yes, all, no) : large(no, all, no);
 }
 
 template <bool GATED>
@@ -1057,11 +1071,11 @@ int b200q_gemm_grouped_gated_fp8(const void* A, int a_rows, const float* a_scale
   return grouped<true>(A, a_rows, W, groups, a, as_stream(stream));
 }
 
-// test hook: 0 = by size, 1 = small tiles, 2 = large tiles of one CTA, 3 = of a pair, 4 = of one CTA, in mode / 100 parts; mode / 10 % 10: 64
-// columns each to a dense product's tile (2, 3, 4 = 0)
+// test hook: 0 = by size, 1 = small tiles, 2 = large tiles of one CTA, 3 = of a pair, 4 and 5 = the same in mode / 100 parts of the
+// reduction; mode / 10 % 10: 64 columns each to a dense product's tile (2, 3, 4 = 0)
 int b200q_gemm_fp8_set_mode(int mode) {
   const int kind = mode % 10, ch = mode / 10 % 10, splits = mode / 100;
-  B200Q_CHECK_ARG(mode >= 0 && kind <= 4 && (ch == 0 || (ch >= 2 && ch <= 4)) && splits <= FL_MAX_SPLITS && (splits > 0) == (kind == 4),
+  B200Q_CHECK_ARG(mode >= 0 && kind <= 5 && (ch == 0 || (ch >= 2 && ch <= 4)) && splits <= (kind == 5 ? FL_MAX_SPLITS / 2 : FL_MAX_SPLITS) && (splits > 0) == (kind >= 4),
                   "gemm_fp8_set_mode: mode=%d", mode);
   g_fp8_mode = mode;
   bump_tuning_epoch();

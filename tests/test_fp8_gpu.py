@@ -157,14 +157,14 @@ def test_product(cuda, mode, M, N, K, which, out):
 # large tiles of 128 and 192 columns, and parts of the reduction: the test hook's mode is parts * 100 + columns / 64 * 10 + kernel
 @pytest.mark.parametrize("M,N,K", [(1, 8, 16), (1, 4096, 4096), (100, 200, 272), (128, 384, 14336), (129, 512, 512), (200, 2304, 1152), (257, 264, 272),
                                    (300, 1000, 2064), (513, 2048, 2048), (1001, 3584, 640)])
-@pytest.mark.parametrize("which", [22, 32, 33, 204, 304, 804, 224, 524])
+@pytest.mark.parametrize("which", [22, 32, 33, 204, 304, 804, 224, 524, 334, 205, 405])
 @pytest.mark.parametrize("out", ["bf16", "f32"])
 def test_product_of_other_tiles(cuda, mode, M, N, K, which, out):
     test_product(cuda, mode, M, N, K, which, out)
 
 
 @pytest.mark.parametrize("M,N,K", [(3, 264, 400), (300, 520, 512), (1001, 768, 1024)])
-@pytest.mark.parametrize("which", [22, 32, 33, 204, 804, 324])
+@pytest.mark.parametrize("which", [22, 32, 33, 204, 804, 324, 305])
 def test_whole_numbers_of_other_tiles(cuda, mode, M, N, K, which):
     test_whole_numbers(cuda, mode, M, N, K, which)
 

@@ -92,7 +92,7 @@ def test_grouped_gated(change, word):
 
 def test_mode():
     from llmq_b200 import lib
-    for mode in (-1, 5, 12, 53, 4, 103, 904):
+    for mode in (-1, 6, 12, 53, 4, 103, 904, 605):
         refused(lib.load().b200q_gemm_fp8_set_mode(mode), f"mode={mode}")
 
 
