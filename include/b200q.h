@@ -759,9 +759,10 @@ int b200q_gemm_grouped_fp8(const void* A_dev, int a_rows, const float* a_scales_
 int b200q_gemm_grouped_gated_fp8(const void* A_dev, int a_rows, const float* a_scales_dev, int ld_a_scales, const void* W_dev,
                                  const float* w_scales_dev, int groups, void* Y_dev, float* y_scales_dev, int ld_y_scales, int N, int K,
                                  const void* tab_dev, const int32_t* n_mt_dev, int max_mtiles, int act, void* stream);
-/* test hook: 0 = by size, 1 = small tiles, 2 = large tiles of one CTA, 3 = of a pair, 4 and 5 = the same in mode / 100 parts of the
- *     reduction; mode / 10 % 10: 64 columns each to a dense product's tile (2, 3, 4 = 0) */
+/* test hooks: 0 = by size, 1 = small tiles, 2 = large tiles of single CTAs, 3 = of pairs, 4 and 5 = these in mode / 100 parts of the reduction;
+ *     mode / 10 % 10: 64 columns each to a dense product's tile.  The mode that stands for what a dense product takes. */
 int b200q_gemm_fp8_set_mode(int mode);
+int b200q_gemm_fp8_choice(int M, int N, int K, int gated);
 
 /* nonzero once a kernel's bounded wait has run out in this process (its outputs are then missing or wrong); engine steps report
  * it as B200Q_ECUDA.  Calls return before their kernels run: who calls b200q_gemm_* (up to 128 rows), b200q_prefill_attn* or the

@@ -12,6 +12,7 @@
 //     which fetches half of the weights.
 //   * small, up to 128 rows to a tile: the weights are the M side and the rows, padded to 16, the N side; the reduction is split over a
 //     cluster whose partial sums meet in distributed shared memory in the order of the splits.
+#include <atomic>
 #include <type_traits>
 
 #include "fp8.cuh"
@@ -798,20 +799,26 @@ __global__ void __launch_bounds__(small_threads<GATED>(MOST), small_resident<GAT
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------------
-// once for each device that a kernel runs on
+// once for each device that a kernel runs on (twice at most where two threads meet)
 template <typename F>
-static int once_per_device(uint64_t (&seen)[2], F&& f) {
+static int once_per_device(std::atomic<uint64_t> (&seen)[2], F&& f) {
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 128 && (seen[dev / 64] >> (dev % 64) & 1)) return B200Q_OK;
+  const bool counted = dev >= 0 && dev < 128;
+  if (counted && (seen[dev / 64].load() >> (dev % 64) & 1)) return B200Q_OK;
   const int rc = f();
-  if (!rc && dev >= 0 && dev < 128) seen[dev / 64] |= 1ull << (dev % 64);
+  if (!rc && counted) seen[dev / 64].fetch_or(1ull << (dev % 64));
   return rc;
 }
 
-// as many clusters as can be resident at once, one CTA to an SM
-template <typename K>
-static int clusters_that_fit(K kern, int cluster, int threads, int smem) {
+// As many clusters of so many CTAs as can be resident at once, by their shared memory (one of 225 KiB to an SM, or two of 107): asked of a
+// kernel that is never launched, since the query knows one CTA to an SM for kernels that hold tensor memory.
+__global__ void fp8_probe_kernel() {}
+constexpr int F8_WHOLE_SM = 230400, F8_HALF_SM = 109568;
+static int clusters_that_fit(int cluster, int smem, int threads) {
+  static std::atomic<int> known[2][FL_MAX_SPLITS + 1];
+  std::atomic<int>& kept = known[smem == F8_HALF_SM][cluster];
+  if (int n = kept.load()) return n;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(cluster, 148);
   cfg.blockDim = dim3(threads);
@@ -823,11 +830,13 @@ static int clusters_that_fit(K kern, int cluster, int threads, int smem) {
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
+  if (cudaFuncSetAttribute(fp8_probe_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F8_WHOLE_SM) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, fp8_probe_kernel, &cfg) != cudaSuccess || n <= 0) {
     cudaGetLastError();
-    n = num_sms() / cluster;
+    n = num_sms() * (smem == F8_HALF_SM ? 2 : 1) / cluster;
   }
-  return n < num_sms() / cluster ? n : num_sms() / cluster;
+  kept.store(n);
+  return n;
 }
 
 // splits > 1 (SPLIT): CTAs to a tile
@@ -835,7 +844,7 @@ template <bool PAIR, int CH, bool GATED, bool GROUPED, bool SPLIT>
 static int launch_large(const void* A, long long a_rows, const void* W, long long w_rows, Fp8Args a, cudaStream_t st) {
   using Cfg = LargeCfg<PAIR, CH, GATED>;
   auto kern = gemm_fp8_large_kernel<PAIR, CH, GATED, GROUPED, SPLIT>;
-  static uint64_t seen[2];
+  static std::atomic<uint64_t> seen[2];
   int rc = once_per_device(seen, [&]() -> int {
     B200Q_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
     return B200Q_OK;
@@ -852,64 +861,140 @@ static int launch_large(const void* A, long long a_rows, const void* W, long lon
   const long long n_tiles = (a.N + Cfg::BN - 1) / Cfg::BN, m_tiles = GROUPED ? a.max_mt : (a.M + (PAIR ? 255 : 127)) / (PAIR ? 256 : 128);
   const long long tiles = n_tiles * m_tiles;
   B200Q_CHECK_ARG(tiles < (1ll << 27), "gemm_fp8: too many tiles (M=%d N=%d)", a.M, a.N);
-  static int pairs = 0;
-  if (PAIR && pairs == 0) pairs = clusters_that_fit(kern, 2, FL_THREADS, Cfg::SMEM);
-  const long long units = PAIR ? pairs : num_sms(), at_once = SPLIT || tiles < units ? tiles : units;
+  const long long units = PAIR ? clusters_that_fit(2, F8_WHOLE_SM, FL_THREADS) : num_sms(), at_once = SPLIT || tiles < units ? tiles : units;
   const int cluster = (PAIR ? 2 : 1) * (SPLIT ? a.splits : 1);
   B200Q_CUDA(launch_early(kern, (int)(at_once * cluster), FL_THREADS, Cfg::SMEM, st, cluster, ta, tw, tc, a));
   count_launch();
   return B200Q_OK;
 }
 
+// small tiles of a product: rows of each, parts of the reduction (as many as leave every cluster resident, three blocks each at least)
+struct SmallPlan {
+  int rows, m_tiles, n_tiles, splits, resident;
+};
+template <bool GATED>
+static SmallPlan small_plan(int M, int N, int blocks) {
+  const int most = GATED ? 64 : 128;
+  SmallPlan p{};
+  p.m_tiles = (M + most - 1) / most;
+  p.rows = ((M + p.m_tiles - 1) / p.m_tiles + 15) / 16 * 16;
+  p.m_tiles = (M + p.rows - 1) / p.rows;
+  p.n_tiles = (N + (GATED ? 255 : 127)) / (GATED ? 256 : 128);
+  p.resident = small_resident<GATED>(p.rows <= 32 ? 32 : p.rows <= 64 ? 64 : 128);
+  p.splits = 1;
+  if (!batch_invariant())
+    for (int s = 2; s <= FS_MAX_SPLITS && blocks / s >= 3; ++s)
+      if ((long long)p.n_tiles * p.m_tiles <= clusters_that_fit(s, p.resident == 2 ? F8_HALF_SM : F8_WHOLE_SM, 192)) p.splits = s;
+  return p;
+}
+
 template <bool GATED, int MOST>
-static int launch_small(const void* A, const void* W, Fp8Args a, cudaStream_t st) {
+static int launch_small(const void* A, const void* W, const SmallPlan& p, Fp8Args a, cudaStream_t st) {
   constexpr int NT = GATED ? 256 : 128, THREADS = small_threads<GATED>(MOST), RESIDENT = small_resident<GATED>(MOST);
   constexpr int RING = RESIDENT == 2 ? FS_RING_SHARED : FS_RING_ALONE;
   auto kern = gemm_fp8_small_kernel<GATED, MOST>;
-  static uint64_t seen[2];
-  static int fit[FS_MAX_SPLITS + 1];
+  static std::atomic<uint64_t> seen[2];
   int rc = once_per_device(seen, [&]() -> int {
     B200Q_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, RING + 1024));
     return B200Q_OK;
   });
   if (rc) return rc;
-  const int n_tiles = (a.N + NT - 1) / NT, m_tiles = (a.M + a.rows - 1) / a.rows;
-  B200Q_CHECK_ARG(n_tiles <= 65535 && m_tiles <= 65535, "gemm_fp8: too many tiles (M=%d N=%d)", a.M, a.N);
+  B200Q_CHECK_ARG(p.n_tiles <= 65535 && p.m_tiles <= 65535, "gemm_fp8: too many tiles (M=%d N=%d)", a.M, a.N);
+  a.rows = p.rows;
+  a.splits = p.splits;
   a.box_rows = a.M < a.rows ? (a.M + 7) & ~7 : a.rows;
-  const int stage = (GATED ? 2 : 1) * F8_STAGE_W + (a.rows + 31) / 32 * 32 * FP8_BLOCK;
+  const int padded = (a.rows + 31) / 32 * 32, stage = (GATED ? 2 : 1) * F8_STAGE_W + padded * FP8_BLOCK;
   a.stages = RING / stage < FS_MAX_STAGES ? RING / stage : FS_MAX_STAGES;
   // accumulators: four where they fit the CTA's share of tensor memory, so that no role waits for the round through the others
-  const int each = (GATED ? 2 : 1) * ((a.rows + 31) / 32 * 32);
+  const int each = (GATED ? 2 : 1) * padded;
   a.accs = FS_MAX_ACCS * each <= 512 / RESIDENT ? FS_MAX_ACCS : 512 / RESIDENT / each;
   a.cols = 32;
   while (a.cols < a.accs * each) a.cols *= 2;
-  // splits: as many as leave every cluster resident, three blocks each at least
-  a.splits = 1;
-  if (!batch_invariant())
-    for (int s = 2; s <= FS_MAX_SPLITS && a.blocks / s >= 3; ++s) {
-      if (fit[s] == 0) fit[s] = clusters_that_fit(kern, s, THREADS, FS_RING_ALONE + 1024 < RING + 1024 ? FS_RING_ALONE + 1024 : RING + 1024);
-      if ((long long)n_tiles * m_tiles <= (long long)fit[s] * RESIDENT) a.splits = s;
-    }
   CUtensorMap ta, tw;
   rc = get_tmap(A, a.M, a.K / 2, a.box_rows, &ta);
   if (!rc) rc = get_tmap(W, a.N, a.K / 2, NT, &tw);
   if (rc) return rc;
-  B200Q_CUDA(launch_early(kern, dim3(a.splits, n_tiles, m_tiles), THREADS, RING + 1024, st, a.splits, ta, tw, a));
+  B200Q_CUDA(launch_early(kern, dim3(a.splits, p.n_tiles, p.m_tiles), THREADS, RING + 1024, st, a.splits, ta, tw, a));
   count_launch();
   return B200Q_OK;
 }
 
 template <bool GATED>
 static int launch_small(const void* A, const void* W, const Fp8Args& a, cudaStream_t st) {
-  if (a.rows <= 32) return launch_small<GATED, 32>(A, W, a, st);
+  const SmallPlan p = small_plan<GATED>(a.M, a.N, a.blocks);
+  if (p.rows <= 32) return launch_small<GATED, 32>(A, W, p, a, st);
   if constexpr (GATED) {
-    return launch_small<GATED, 64>(A, W, a, st);
+    return launch_small<GATED, 64>(A, W, p, a, st);
   } else {
-    return a.rows <= 64 ? launch_small<GATED, 64>(A, W, a, st) : launch_small<GATED, 128>(A, W, a, st);
+    return p.rows <= 64 ? launch_small<GATED, 64>(A, W, p, a, st) : launch_small<GATED, 128>(A, W, p, a, st);
   }
 }
 
-int g_fp8_mode = 0;  // test hook: 1 = small tiles; large ones of 64 * (mode / 10 % 10) columns (dense), 2 = of one CTA, 3 = of a pair, 4 and 5 = the same in mode / 100 parts
+int g_fp8_mode = 0;  // test hook: see b200q_gemm_fp8_set_mode
+
+// Which kernel and tile: the least of what each is expected to take, us.  A round of tiles (as many as are resident at once) costs so much for
+// its start and end and so much a block; no kernel takes less than the weights do to come from memory; parts cost their exchange.  Fitted to
+// 450 sizes (15 shapes of 1024 to 16384 columns x 1024 to 14336, 30 row counts from 1 to 4608, weights from HBM, back to back in a graph) and
+// every kernel: what is taken is 1 % slower than the best on average and 21 % at worst (129 x 1024 x 4096: 9.1 us, 7.5).  us, the choice / the
+// others: 1 x 4096 x 4096 small 6.3 / four parts of 128 columns 8.8; 48 x 4096 x 14336 small 15.2 / 16.2; 128 x 4096 x 14336 four parts of
+// 128 columns 17.5 / small 22.8, whole tiles 48; 200 x 4096 x 14336 three parts of 192 columns 23.7 / two of 128 25.7, a pair's whole tiles 42;
+// 300 x 8192 x 3584 pairs of 256 columns 15.4 / single CTAs 16.0, of 128 columns 23.8; 450 x 4096 x 14336 pairs in two parts 37 / of 128
+// columns 41; 768 x 4096 x 4096 pairs of 192 columns 16.1 / 256 17.2; 4608 x 4096 x 14336 pairs of 256 254 / single CTAs 277.
+// Gated (184 sizes, 8 shapes; 0.3 % and 7 %): 7 x 16384 x 2048 small 9.6 / 12.5 / pairs 12.5; 48 x 28672 x 4096 small 28.8 / 26.0 / 36.3;
+// 200 x 28672 x 4096 96 / 39.8 / 34.3; 300 110 / 59.9 / 67.4; 4608 497 / 445.
+struct Fp8Tile {
+  int kind, ch, splits;  // as the hook's
+};
+template <bool GATED>
+static Fp8Tile choose_fp8_tile(int M, int N, int blocks) {
+  const double weights = 1.6e-7 * N * FP8_BLOCK * blocks;
+  Fp8Tile best{1, 4, 1};
+  double least = 1e30;
+  auto offer = [&](Fp8Tile t, double us) {
+    if (us < least) {
+      least = us;
+      best = t;
+    }
+  };
+  auto larger = [](double a, double b) { return a > b ? a : b; };
+  if (M <= 512) {
+    const SmallPlan p = small_plan<GATED>(M, N, blocks);
+    const int fit = p.splits > 1 ? clusters_that_fit(p.splits, p.resident == 2 ? F8_HALF_SM : F8_WHOLE_SM, 192) : num_sms() * p.resident;
+    const int rounds = (p.n_tiles * p.m_tiles + fit - 1) / fit, each = (blocks + p.splits - 1) / p.splits;
+    const double parts = p.splits - 1;
+    if (GATED)
+      offer({1, 4, 1}, p.resident == 2 ? 5.5 + larger(rounds * (0.27 + 0.053 * each), 1.09 * weights) : 3.6 + larger(rounds * (1.4 + 0.69 * each), 1.38 * weights));
+    else if (p.rows <= 32)
+      offer({1, 4, 1}, 2.9 + larger(rounds * 0.466 * each, 1.13 * weights) + 0.1 * parts);
+    else if (p.rows <= 64)
+      offer({1, 4, 1}, 3.95 + larger(rounds * 0.519 * each, 1.19 * weights) + 0.17 * parts);
+    else if (rounds == 1 && each <= 16)
+      offer({1, 4, 1}, 4.94 + larger(0.564 * each, weights) + 0.024 * parts);
+  }
+  const struct {
+    Fp8Tile tile;  // splits: the most
+    double fixed, round, block, part, weights;
+  } plain[6] = {{{2, 2, 1}, 2.0, 1.55, 0.340, 0, 1}, {{2, 4, 1}, 0, 4.0, 0.403, 0, 1}, {{3, 3, 1}, 0, 3.9, 0.340, 0, 1}, {{3, 4, 1}, 0, 4.5, 0.352, 0, 1},
+                {{4, 2, 6}, 0, 5.5, 0.359, 0.13, 1}, {{4, 3, 4}, 0, 6.8, 0.391, 0.17, 1.77}},
+    pair_parts = {{5, 4, 3}, 0, 8.5, 0.387, 0.07, 1},
+    gated[2] = {{{2, 4, 1}, 2.8, 2.0, 0.53, 0, 1.21}, {{3, 4, 1}, 2.75, 2.46, 0.43, 0, 1.06}};
+  auto large = [&](const auto& c) {
+    const bool pair = c.tile.kind == 3 || c.tile.kind == 5;
+    const long long tiles = (long long)((M + (pair ? 255 : 127)) / (pair ? 256 : 128)) * ((N + 64 * c.tile.ch - 1) / (64 * c.tile.ch));
+    for (int s = c.tile.splits > 1 ? 2 : 1; s <= c.tile.splits && (s == 1 || blocks / s >= 2); ++s) {
+      const int ctas = s * (pair ? 2 : 1), fit = ctas > 1 ? clusters_that_fit(ctas, F8_WHOLE_SM, FL_THREADS) : num_sms();
+      const double rounds = (double)((tiles + fit - 1) / fit);
+      offer({c.tile.kind, c.tile.ch, s}, c.fixed + larger(rounds * (c.round + c.block * ((blocks + s - 1) / s)), c.weights * weights) + c.part * (s - 1));
+    }
+  };
+  if (GATED) {
+    for (const auto& c : gated) large(c);
+  } else {
+    for (int i = 0; i < (batch_invariant() ? 4 : 6); ++i) large(plain[i]);
+    if (!batch_invariant()) large(pair_parts);
+  }
+  return best;
+}
 
 static int finish_args(Fp8Args& a) {
   a.blocks = (a.K + FP8_BLOCK - 1) / FP8_BLOCK;
@@ -925,34 +1010,25 @@ template <bool GATED>
 static int dense(const void* A, const void* W, Fp8Args a, cudaStream_t st) {
   int rc = finish_args(a);
   if (rc) return rc;
-  int mode = g_fp8_mode % 10, ch = g_fp8_mode / 10 % 10, splits = g_fp8_mode / 100;
-  if (mode == 0) {
-    mode = a.M <= (GATED ? 64 : 128) ? 1 : a.M <= 256 ? 2 : 3;
-    ch = 4;
-  }
-  if (GATED || ch == 0) ch = 4;
-  if (mode == 1) {
-    const int most = GATED ? 64 : 128, tiles = (a.M + most - 1) / most;
-    a.rows = ((a.M + tiles - 1) / tiles + 15) / 16 * 16;
-    return launch_small<GATED>(A, W, a, st);
-  }
+  Fp8Tile t{g_fp8_mode % 10, g_fp8_mode / 10 % 10, g_fp8_mode / 100};
+  if (t.kind == 0) t = choose_fp8_tile<GATED>(a.M, a.N, a.blocks);
+  if (t.kind == 1) return launch_small<GATED>(A, W, a, st);
+  a.splits = t.splits < a.blocks ? t.splits : a.blocks;
+  const bool pair = t.kind == 3 || t.kind == 5;
   auto large = [&](auto pair, auto columns, auto split) {
     return launch_large<decltype(pair)::value, decltype(columns)::value, GATED, false, decltype(split)::value>(A, a.M, W, a.N, a, st);
   };
-  const std::integral_constant<int, 4> all;
+  const std::integral_constant<int, 2> c128;
+  const std::integral_constant<int, 3> c192;
+  const std::integral_constant<int, 4> c256;
   const std::true_type yes;
   const std::false_type no;
   if constexpr (!GATED) {
-    if (mode == 4 && (a.splits = splits < a.blocks ? splits : a.blocks) > 1) {
-      if (ch == 2) return large(no, std::integral_constant<int, 2>{}, yes);
-      return ch == 3 ? large(no, std::integral_constant<int, 3>{}, yes) : large(no, all, yes);
-    }
-    if (mode == 5 && (a.splits = splits < a.blocks ? splits : a.blocks) > 1) return large(yes, all, yes);
-    if (mode == 3 && ch == 3) return large(yes, std::integral_constant<int, 3>{}, no);
-    if (mode != 3 && ch == 3) return large(no, std::integral_constant<int, 3>{}, no);
-    if (mode != 3 && ch == 2) return large(no, std::integral_constant<int, 2>{}, no);
+    if (a.splits > 1 && t.kind >= 4) return pair ? large(yes, c256, yes) : t.ch == 2 ? large(no, c128, yes) : large(no, c192, yes);
+    if (pair && t.ch == 3) return large(yes, c192, no);
+    if (!pair && t.ch == 2) return large(no, c128, no);
   }
-  return mode == 3 || mode == 5 ? large(yes, all, no) : large(no, all, no);
+  return pair ? large(yes, c256, no) : large(no, c256, no);
 }
 
 template <bool GATED>
@@ -1071,8 +1147,9 @@ int b200q_gemm_grouped_gated_fp8(const void* A, int a_rows, const float* a_scale
   return grouped<true>(A, a_rows, W, groups, a, as_stream(stream));
 }
 
-// test hook: 0 = by size, 1 = small tiles, 2 = large tiles of one CTA, 3 = of a pair, 4 and 5 = the same in mode / 100 parts of the
-// reduction; mode / 10 % 10: 64 columns each to a dense product's tile (2, 3, 4 = 0)
+// test hook: 0 = by size, 1 = small tiles, 2 = large tiles of single CTAs, 3 = of pairs; 4 and 5 = these in mode / 100 parts of the reduction.
+// mode / 10 % 10: 64 columns each to a dense product's tile, 0 and what there is no kernel of = 4 (2: single CTAs; 3: pairs; parts: 2 or 3 for
+// single CTAs, 4 for pairs)
 int b200q_gemm_fp8_set_mode(int mode) {
   const int kind = mode % 10, ch = mode / 10 % 10, splits = mode / 100;
   B200Q_CHECK_ARG(mode >= 0 && kind <= 5 && (ch == 0 || (ch >= 2 && ch <= 4)) && splits <= (kind == 5 ? FL_MAX_SPLITS / 2 : FL_MAX_SPLITS) && (splits > 0) == (kind >= 4),
@@ -1080,6 +1157,12 @@ int b200q_gemm_fp8_set_mode(int mode) {
   g_fp8_mode = mode;
   bump_tuning_epoch();
   return B200Q_OK;
+}
+
+// test hook: the mode that stands for what a dense product takes
+int b200q_gemm_fp8_choice(int M, int N, int K, int gated) {
+  const Fp8Tile t = gated ? choose_fp8_tile<true>(M, N, (K + FP8_BLOCK - 1) / FP8_BLOCK) : choose_fp8_tile<false>(M, N, (K + FP8_BLOCK - 1) / FP8_BLOCK);
+  return t.kind == 1 ? 1 : t.kind + 10 * t.ch + (t.splits > 1 ? 100 * t.splits : 0);
 }
 
 }  // extern "C"
