@@ -118,7 +118,7 @@ __device__ __noinline__ void f8_let_copies_end() {
 }
 
 // ---- large ---------------------------------------------------------------------------------------------------------------------
-constexpr int FL_THREADS = 384, FL_PATCH = 4096, FL_MAX_SPLITS = 8;
+constexpr int FL_THREADS = 384, FL_MAX_SPLITS = 8;
 // registers: 384 threads begin with 168; four warps give back 128 each and eight take 64 more (40 x 128 + 232 x 256 = 168 x 384)
 constexpr int FL_REGS_FEW = 40, FL_REGS_MANY = 232;
 // A tile has 64 CH columns.  The products of a block are two, to a half of them each, whose accumulators are filled and emptied on their own: a
@@ -128,9 +128,11 @@ template <bool PAIR, int CH, bool GATED>
 struct LargeCfg {
   static constexpr int BN = 64 * CH, W_ROWS = PAIR ? BN / 2 : BN;                // columns of a tile; rows of W that a CTA fetches
   static constexpr int STAGE = F8_STAGE_W + W_ROWS * FP8_BLOCK;                  // behind 128 rows of A
-  static constexpr int STAGES = 196608 / STAGE < 8 ? 196608 / STAGE : 8;
+  // a warp's columns of C on their way out: all of them where a wide tile of a pair leaves room, else 64 (gated: 128 codes of two tiles for two warps)
+  static constexpr int PATCH = PAIR && CH == 4 && !GATED ? 8192 : 4096;
+  static constexpr int STAGES = (229376 - 8 * PATCH) / STAGE < 8 ? (229376 - 8 * PATCH) / STAGE : 8;
   static constexpr int BOX = PAIR ? 16 * CH : GATED ? 64 : BN, BOXES = W_ROWS / BOX;
-  static constexpr int SMEM = STAGES * STAGE + 8 * FL_PATCH + 1024;
+  static constexpr int SMEM = STAGES * STAGE + 8 * PATCH + 1024;
 };
 
 // 32 of a thread's sums (its row, columns in turn) += scale * what has come from tensor memory
@@ -205,11 +207,11 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
   const int m_tiles = GROUPED ? min(*n_mt, a.max_mt) : (a.M + BM - 1) / BM;
   const int num_tiles = m_tiles * n_tiles;
   // a tile: columns n0 .., rows row0 .. row_end of a group
-  auto tile_of = [&](int tile, int& g, int& row0, int& row_end, int& n0) {
+  auto entry_of = [&](int tile) { return GROUPED ? tab[tile % m_tiles] : make_int4(0, 0, 0, 0); };
+  auto tile_of = [&](int tile, int4 e, int& g, int& row0, int& row_end, int& n0) {
     const int mt = tile % m_tiles;
     n0 = tile / m_tiles * BN;
-    if constexpr (GROUPED) {
-      const int4 e = tab[mt];  // (kept within the matrices, whatever the table says)
+    if constexpr (GROUPED) {  // (kept within the matrices, whatever the table says)
       g = min(max(e.x, 0), a.groups - 1);
       row0 = max(e.y, 0);
       row_end = min(e.z, a.M);
@@ -228,7 +230,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
         uint32_t phase = 0;
         for (int tile = unit; tile < num_tiles; tile += units) {
           int g, row0, row_end, n0;
-          tile_of(tile, g, row0, row_end, n0);
+          tile_of(tile, entry_of(tile), g, row0, row_end, n0);
           const int wrow = g * a.N + n0;
           for (int b = b_begin; b < b_end; ++b) {
             uint8_t* to = smem + stage * Cfg::STAGE;
@@ -299,14 +301,43 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
     // rows quarter * 32 + lane; columns: half of the tile's, gated: half * 64 + 0 .. 63 of the gates and of what they gate
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
-    uint8_t* const patch = patches + (warp - 4) * FL_PATCH;
+    uint8_t* const patch = patches + (warp - 4) * Cfg::PATCH;
     const uint32_t patch_s = smem_u32(patch);
     const uint32_t empty0 = PAIR ? mapa_shared(acc_empty[half], leader) : smem_u32(acc_empty[half]);
     int acc = 0, parity = 0;
     uint32_t acc_phase = 0;
+    // Weights' scales: a lane's of 32 blocks of the reduction, handed round by shuffles.  A tile's columns lie in up to two blocks of 128 (gated:
+    // the gates' and that of what they gate); 32 neighbouring columns lie in one.  Rows' scales: four blocks'.  A tile's first are asked for
+    // while the one before it leaves.  (Without a condition: a load that may not be made is waited for where it is made.  Rows and blocks that do
+    // not exist take the last ones', or the first.)
+    constexpr int SCALES = GATED || CH == 3 ? 2 : 1;
+    float sw[SCALES], sa[4];
+    auto row_scales = [&](int row0, int row_end) { return as + max(min(row0 + quarter * 32 + lane, row_end - 1), 0); };
+    auto row_scale = [&](const float* rows, int b) { return rows[(long long)min(b, b_end - 1) * a.ld_as]; };
+    auto column_scales = [&](int g, int n0) {
+      return ws + ((long long)g * a.n_blocks + min(n0 / 128 + (CH == 4 && !GATED ? half : 0), a.n_blocks - 1)) * blocks;
+    };
+    auto column_scale = [&](const float* columns, int n0, int b, int h) {
+      return columns[(h && n0 / 128 + 1 < a.n_blocks ? blocks : 0) + min(b + lane, b_end - 1)];
+    };
+    auto first_scales = [&](int tile, int4 e) {
+      int g, row0, row_end, n0;
+      tile_of(tile, e, g, row0, row_end, n0);
+#pragma unroll
+      for (int h = 0; h < SCALES; ++h) sw[h] = column_scale(column_scales(g, n0), n0, b_begin, h);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sa[i] = row_scale(row_scales(row0, row_end), b_begin + i);
+    };
+    int4 entry = make_int4(0, 0, 0, 0), next_entry = entry;
+    if (unit < num_tiles) {
+      next_entry = entry_of(unit);
+      first_scales(unit, next_entry);
+    }
     for (int tile = unit; tile < num_tiles; tile += units) {
       int g, row0, row_end, n0;
-      tile_of(tile, g, row0, row_end, n0);
+      entry = next_entry;
+      if (tile + units < num_tiles) next_entry = entry_of(tile + units);
+      tile_of(tile, entry, g, row0, row_end, n0);
       const int row = row0 + quarter * 32 + lane;
       const bool live = row < row_end;
       if (!SPLIT && row0 + quarter * 32 >= row_end) {  // no rows: the accumulators only have to be passed on
@@ -317,24 +348,12 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
           acc ^= 1;
           if (acc == 0) acc_phase ^= 1u;
         }
+        if (tile + units < num_tiles) first_scales(tile + units, next_entry);
         continue;
       }
-      // weights' scales: this lane's of 32 blocks of the reduction, handed round by shuffles.  A tile's columns lie in up to two blocks of 128 (gated:
-      // the gates' and that of what they gate); 32 neighbouring columns lie in one
-      const int col0 = GATED ? 0 : n0 % 128 + half * (BN / 2), nb0 = n0 / 128 + (CH == 4 && !GATED ? half : 0);
-      const float* w0 = ws + ((long long)g * a.n_blocks + min(nb0, a.n_blocks - 1)) * blocks;
-      const bool two = GATED || (CH == 3 && nb0 + 1 < a.n_blocks);
+      const int col0 = GATED ? 0 : n0 % 128 + half * (BN / 2);
       auto scale_of = [&](int c) { return GATED ? c >> 1 : CH == 3 ? (col0 + 32 * c) >> 7 : 0; };
-      // (without a condition: a load that may not be made is waited for where it is made.  Rows and blocks that do not exist take the last ones')
-      const float* own_scales = as + min(row, row_end - 1);
-      auto row_scale = [&](int b) { return own_scales[(long long)min(b, b_end - 1) * a.ld_as]; };
-      auto column_scale = [&](int b, int h) { return w0[(h && two ? blocks : 0) + min(b + lane, b_end - 1)]; };
-      constexpr int SCALES = GATED || CH == 3 ? 2 : 1;
-      float sw[SCALES], sa[4];
-#pragma unroll
-      for (int h = 0; h < SCALES; ++h) sw[h] = column_scale(b_begin, h);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sa[i] = row_scale(b_begin + i);
+      const float *own_rows = row_scales(row0, row_end), *columns = column_scales(g, n0);
       f32x2 sum[CH][16];
 #pragma unroll
       for (int c = 0; c < CH; ++c)
@@ -354,10 +373,10 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
 #pragma unroll
           for (int h = 0; h < SCALES; ++h) x[i][h] = sa[i] * __shfl_sync(0xffffffffu, sw[h], (b0 + i - b_begin) & 31);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sa[i] = row_scale(b0 + 4 + i);
+        for (int i = 0; i < 4; ++i) sa[i] = row_scale(own_rows, b0 + 4 + i);
         if ((b0 + 4 - b_begin) % 32 == 0) {
 #pragma unroll
-          for (int h = 0; h < SCALES; ++h) sw[h] = column_scale(b0 + 4, h);
+          for (int h = 0; h < SCALES; ++h) sw[h] = column_scale(columns, n0, b0 + 4, h);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -447,6 +466,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
         }
         continue;  // (a tile to a CTA: the loop ends)
       }
+      if (tile + units < num_tiles) first_scales(tile + units, next_entry);
       // ---- the sums leave ----
       if constexpr (GATED) {
         float y[64];
@@ -463,8 +483,8 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
         for (int j = 0; j < 64; ++j) m = max_or_nan(m, fabsf(y[j]));
         most[half][quarter * 32 + lane] = m;
         // (two warps share a quarter's rows, and a patch of 32 rows x 128 codes for each parity of the tile)
-        uint8_t* const out = patches + (2 * quarter + parity) * FL_PATCH;
-        const bool copies = !GROUPED && half == 0 && lane == 0;
+        uint8_t* const out = patches + (2 * quarter + parity) * Cfg::PATCH;
+        const bool copies = half == 0 && lane == 0, engine = !GROUPED || row0 + quarter * 32 + 32 <= row_end;  // (no rows that are another group's)
         if (copies) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
         asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
         const float scale = fp8_scale(max_or_nan(m, most[half ^ 1][quarter * 32 + lane])), by = fp8_inverse(scale);
@@ -479,13 +499,13 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
           }
           st_v4(out + lane * 128 + (((half * 4 + j) ^ (lane & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
         }
-        if constexpr (!GROUPED) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
-        if (copies) {  // (rows that do not exist leave an empty group, as the wait counts turns)
-          if (row0 + quarter * 32 < a.M) f8_store(&tmap_c, n0 / 4, row0 + quarter * 32, smem_u32(out));
+        if (copies) {  // (rows that are not copied so leave an empty group, as the wait counts turns)
+          if (engine && row0 + quarter * 32 < a.M) f8_store(&tmap_c, n0 / 4, row0 + quarter * 32, smem_u32(out));
           asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
-        if constexpr (GROUPED) {
+        if (!engine) {
           uint8_t* to = (uint8_t*)a.C + (long long)(row0 + quarter * 32) * (a.N / 2) + n0 / 2;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -509,12 +529,17 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
         }
       } else {
         const int r0 = row0 + quarter * 32, n = n0 + half * (BN / 2);
-        constexpr int WIDE = CH % 2 ? 32 : 64;              // columns at a time
-        constexpr bool COPIES = !GROUPED && WIDE == 64;     // by the copy engine, which takes 64
+        constexpr int WIDE = CH % 2 ? 32 : 64;  // columns at a time
+        // by the copy engine, which takes 64 columns of 32 rows, and none that are another group's; else by this warp
+        constexpr bool ENGINE = WIDE == 64, ROOM = Cfg::PATCH > 4096;
+        const bool copies = ENGINE && (!GROUPED || r0 + 32 <= row_end);
 #pragma unroll
         for (int h = 0; h < 32 * CH / WIDE; ++h) {
-          if (COPIES && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-          __syncwarp();
+          const uint32_t to = patch_s + (ROOM ? h * 4096 : 0);
+          if (ENGINE && (!ROOM || h == 0)) {
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            __syncwarp();
+          }
 #pragma unroll
           for (int j = 0; j < WIDE / 8; ++j) {
             const f32x2* x = sum[h * (WIDE / 32) + j / 4] + 4 * (j & 3);
@@ -524,15 +549,15 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
               const float2 f = halves_of(x[i]);
               w[i] = pack_bf16x2(f.x, f.y);
             }
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(patch_s + lane * 128 + ((j ^ (lane & 7)) << 4)), "r"(w[0]), "r"(w[1]),
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + lane * 128 + ((j ^ (lane & 7)) << 4)), "r"(w[0]), "r"(w[1]),
                          "r"(w[2]), "r"(w[3])
                          : "memory");
           }
-          if constexpr (COPIES) {
+          if (copies) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0 && n + 64 * h < a.N && r0 < a.M) {
-              f8_store(&tmap_c, n + 64 * h, r0, patch_s);
+              f8_store(&tmap_c, n + 64 * h, r0, to);
               asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
           } else {
@@ -541,14 +566,14 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
             for (int i = 0; i < WIDE / 8; ++i) {
               constexpr int ACROSS = WIDE / 8;  // lanes to a row
               const int r = i * (32 / ACROSS) + lane / ACROSS, c = lane % ACROSS, col = n + WIDE * h + c * 8;
-              if (r0 + r < row_end && col < a.N) st_v4((bf16*)a.C + (long long)(r0 + r) * a.N + col, lds_v4(patch_s + r * 128 + ((c ^ (r & 7)) << 4)));
+              if (r0 + r < row_end && col < a.N) st_v4((bf16*)a.C + (long long)(r0 + r) * a.N + col, lds_v4(to + r * 128 + ((c ^ (r & 7)) << 4)));
             }
             __syncwarp();
           }
         }
       }
     }
-    if (!GROUPED && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
 
   tc_fence_before();
@@ -855,8 +880,8 @@ static int launch_large(const void* A, long long a_rows, const void* W, long lon
   a.a_bytes = box * FP8_BLOCK;
   if (!rc) rc = get_tmap(A, a_rows, a.K / 2, box, &ta);
   if (!rc) rc = get_tmap(W, w_rows, a.K / 2, Cfg::BOX, &tw);
-  if (!rc && !GROUPED && GATED) rc = get_tmap(a.C, a.M, a.N / 4, 32, &tc);
-  if (!rc && !GROUPED && !GATED && !a.out_f32) rc = get_tmap(a.C, a.M, a.N, 32, &tc);
+  if (!rc && GATED) rc = get_tmap(a.C, a.M, a.N / 4, 32, &tc);
+  if (!rc && !GATED && !a.out_f32) rc = get_tmap(a.C, a.M, a.N, 32, &tc);
   if (rc) return rc;
   const long long n_tiles = (a.N + Cfg::BN - 1) / Cfg::BN, m_tiles = GROUPED ? a.max_mt : (a.M + (PAIR ? 255 : 127)) / (PAIR ? 256 : 128);
   const long long tiles = n_tiles * m_tiles;
