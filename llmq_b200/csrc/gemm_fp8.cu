@@ -30,7 +30,7 @@ struct Fp8Args {
   const int4* tab;   // [*n_mt] {group, first row, end of its rows, 0}, or NULL: the rows are one group
   const int32_t* n_mt;
   int* failed;
-  int ld_as, ld_ys, M, N, K, blocks, n_blocks, max_mt, groups, out_f32, gelu, a_bytes;
+  int ld_as, ld_ys, M, N, K, blocks, n_blocks, max_mt, groups, ahead, out_f32, gelu, a_bytes;
   // small tiles
   int rows, box_rows, stages, accs, cols, splits;
 };
@@ -194,8 +194,9 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
   if constexpr (PAIR) cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
-  if (!GROUPED && warp == 0 && lane == 0) {  // the first weights into L2 while the kernel before this one ends
-    const int m_tiles = (a.M + BM - 1) / BM, n0 = unit / m_tiles * BN;
+  if (warp == 0 && lane == 0 && (!GROUPED || unit < a.ahead)) {
+    // the first weights into L2 while the kernel before this one ends (the table is not known yet: as if every group had one tile)
+    const int m_tiles = GROUPED ? a.groups : (a.M + BM - 1) / BM, n0 = unit / m_tiles * BN + (GROUPED ? unit % m_tiles * a.N : 0);
     for (int b = 0; b < min(STAGES, b_end - b_begin); ++b)
       for (int i = 0; i < Cfg::BOXES; ++i) tma_prefetch_2d(&tmap_w, (b_begin + b) * 64, n0 + w_box(i));
   }
@@ -1061,6 +1062,8 @@ static int grouped(const void* A, long long a_rows, const void* W, int groups, F
   int rc = finish_args(a);
   if (rc) return rc;
   a.groups = groups;
+  // weights are asked for before the table is known where most groups have one tile: two rows or more to a group on average, one tile at most
+  if (a_rows >= 2ll * groups && a_rows <= 128ll * groups) a.ahead = (int)((long long)groups * ((a.N + 255) / 256) < (1 << 30) ? groups * ((a.N + 255) / 256) : 1 << 30);
   return launch_large<false, 4, GATED, true, false>(A, a_rows, W, (long long)groups * a.N, a, st);
 }
 
