@@ -784,6 +784,13 @@ def fp8_row_scales(rows, K, device="cuda"):
     return torch.empty((K + 127) // 128, (rows + 3) // 4 * 4, dtype=torch.float32, device=device)
 
 
+def _codes(t, what, dev):
+    """data_ptr of codes"""
+    if t.dtype is not (_TORCH or _types())["e"] or t.get_device() != dev or not t.is_contiguous():
+        _refuse(t, "e", what, dev)
+    return t.data_ptr()
+
+
 def _row_scales(t, rows, K, what, dev):
     """(data_ptr, ld) of scales of rows"""
     blocks, ld = t.shape
@@ -792,89 +799,110 @@ def _row_scales(t, rows, K, what, dev):
     return _arg(t, "f", what, dev), ld
 
 
-def _weight_scales(t, w, dev):
-    *groups, N, K = w.shape
-    if t.shape != (*groups, (N + 127) >> 7, (K + 127) >> 7):
-        raise ValueError(f"w_scales: {tuple(t.shape)} does not fit {tuple(w.shape)}")
-    return _arg(t, "f", "w_scales", dev)
+def _weights(w, scales, K, dev):
+    """data_ptr of weights [N, K] and of their scales, N"""
+    (N, Kw), (down, across) = w.shape, scales.shape
+    if Kw != K or down != (N + 127) >> 7 or across != (K + 127) >> 7:
+        raise ValueError(f"w and w_scales: {tuple(w.shape)} and {tuple(scales.shape)} do not fit each other, or not K = {K}")
+    return _codes(w, "w", dev), _arg(scales, "f", "w_scales", dev), N
 
 
-def _float(t, what):
-    """dtype code of a bf16 or fp32 tensor"""
+def _expert_weights(w, scales, K, dev):
+    """data_ptr of weights [E, N, K] and of their scales, E, N"""
+    (E, N, Kw), (Es, down, across) = w.shape, scales.shape
+    if Kw != K or Es != E or down != (N + 127) >> 7 or across != (K + 127) >> 7:
+        raise ValueError(f"w and w_scales: {tuple(w.shape)} and {tuple(scales.shape)} do not fit each other, or not K = {K}")
+    return _codes(w, "w", dev), _arg(scales, "f", "w_scales", dev), E, N
+
+
+def _tiles(tile_tab, n_tiles, dev):
+    """data_ptr of moe_route's table and of its length, its room"""
+    room, four = tile_tab.shape
+    _want(four == 4 and n_tiles.numel() > 0, "tile_tab is [room, 4], n_tiles [1]")
+    return _arg(tile_tab, "i", "tile_tab", dev), _arg(n_tiles, "i", "n_tiles", dev), room
+
+
+def _float(t, what, dev):
+    """data_ptr and dtype code of a bf16 or fp32 tensor"""
     kinds, have = _TORCH or _types(), t.dtype
-    if have is kinds["h"]:
-        return "h", DTYPE_BF16
-    if have is not kinds["f"]:
+    if have is not kinds["h"] and have is not kinds["f"]:
         raise ValueError(f"{what}: {have}, neither bfloat16 nor float32")
-    return "f", DTYPE_F32
+    if t.get_device() != dev or not t.is_contiguous():
+        _refuse(t, None, what, dev)
+    return t.data_ptr(), DTYPE_BF16 if have is kinds["h"] else DTYPE_F32
 
 
 def rmsnorm_fp8(x, w, y, scales, eps, residual=None, stream=None):
     """residual <- x + residual (None: x alone); y, scales = that, RMS-normed and times w, in 8 bits.  x is not written."""
-    (T, H), (s, dev), (kind, dtype) = x.shape, _here(stream), _float(x, "x")
-    _want(w.numel() == H and y.shape == x.shape and (residual is None or residual.shape == x.shape), "rmsnorm_fp8: w, y or residual do not fit x")
-    ps, ld = _row_scales(scales, T, H, "scales", dev)
-    check(load().b200q_rmsnorm_fp8(_arg(x, kind, "x", dev), 0 if residual is None else _arg(residual, kind, "residual", dev), _arg(w, kind, "w", dev),
-                                   _arg(y, "e", "y", dev), ps, ld, T, H, eps, dtype, s))
+    (T, H), (s, dev) = x.shape, _here(stream)
+    (px, dtype), (ps, ld) = _float(x, "x", dev), _row_scales(scales, T, H, "scales", dev)
+    kind = "f" if dtype else "h"
+    if w.numel() != H or y.shape != (T, H) or (residual is not None and residual.shape != (T, H)):
+        raise ValueError("rmsnorm_fp8: w, y or residual do not fit x")
+    check(load().b200q_rmsnorm_fp8(px, 0 if residual is None else _arg(residual, kind, "residual", dev), _arg(w, kind, "w", dev), _codes(y, "y", dev), ps,
+                                   ld, T, H, eps, dtype, s))
 
 
 def quantize_fp8(x, y, scales, rows=None, stream=None):
     """y, scales = the rows of x (of x[rows]) in 8 bits; x may be a slice of wider rows"""
-    (n, K), (T, Ky), (s, dev), (kind, dtype) = x.shape, y.shape, _here(stream), _float(x, "x")
-    _want(K == Ky and (T <= n if rows is None else rows.numel() == T), "quantize_fp8: y or rows do not fit x")
-    if x.get_device() != dev or x.stride(1) != 1:
-        raise ValueError(f"x: rows on device {dev}, the current one, are wanted")
+    (n, K), (T, Ky), (s, dev) = x.shape, y.shape, _here(stream)
+    kinds, have = _TORCH or _types(), x.dtype
+    if K != Ky or (T > n if rows is None else rows.numel() != T):
+        raise ValueError("quantize_fp8: y or rows do not fit x")
+    if x.get_device() != dev or x.stride(1) != 1 or (have is not kinds["h"] and have is not kinds["f"]):
+        raise ValueError(f"x: bfloat16 or float32 rows on device {dev}, the current one, are wanted")
     ps, ld = _row_scales(scales, T, K, "scales", dev)
-    ld_x = x.stride(0) if n > 1 else (K + 7) // 8 * 8
-    check(load().b200q_quantize_fp8(x.data_ptr(), ld_x, 0 if rows is None else _arg(rows, "i", "rows", dev), _arg(y, "e", "y", dev), ps, ld, T, K,
-                                    dtype, s))
+    check(load().b200q_quantize_fp8(x.data_ptr(), x.stride(0) if n > 1 else (K + 7) // 8 * 8, 0 if rows is None else _arg(rows, "i", "rows", dev),
+                                    _codes(y, "y", dev), ps, ld, T, K, DTYPE_BF16 if have is kinds["h"] else DTYPE_F32, s))
 
 
 def quantize_fp8_weight(w, q, scales, stream=None):
     """q, scales = weights [N, K] or [groups, N, K] in 8 bits"""
-    (s, dev), (kind, dtype) = _here(stream), _float(w, "w")
+    s, dev = _here(stream)
     _want(w.dim() in (2, 3) and q.shape == w.shape, "quantize_fp8_weight: w is [N, K] or [groups, N, K], q of its shape")
-    N, K = w.shape[-2:]
-    check(load().b200q_quantize_fp8_weight(_arg(w, kind, "w", dev), _arg(q, "e", "q", dev), _weight_scales(scales, w, dev),
-                                           w.shape[0] if w.dim() == 3 else 1, N, K, dtype, s))
+    *groups, N, K = w.shape
+    _want(scales.shape == (*groups, (N + 127) >> 7, (K + 127) >> 7), "quantize_fp8_weight: scales do not fit w")
+    pw, dtype = _float(w, "w", dev)
+    check(load().b200q_quantize_fp8_weight(pw, _codes(q, "q", dev), _arg(scales, "f", "scales", dev), groups[0] if groups else 1, N, K, dtype, s))
 
 
 def gemm_fp8(a, a_scales, w, w_scales, c, stream=None):
     """c [M, N] (bf16 or fp32) = a [M, K] * w [N, K]^T, both in 8 bits"""
-    (M, K), (N, Kw), (s, dev), (kind, dtype) = a.shape, w.shape, _here(stream), _float(c, "c")
-    _want(K == Kw and c.shape == (M, N), "gemm_fp8: shapes do not fit")
-    ps, ld = _row_scales(a_scales, M, K, "a_scales", dev)
-    check(load().b200q_gemm_fp8(_arg(a, "e", "a", dev), ps, ld, _arg(w, "e", "w", dev), _weight_scales(w_scales, w, dev), _arg(c, kind, "c", dev), M, N,
-                                K, dtype, s))
+    (M, K), (s, dev) = a.shape, _here(stream)
+    (ps, ld), (pw, pws, N), (pc, dtype) = _row_scales(a_scales, M, K, "a_scales", dev), _weights(w, w_scales, K, dev), _float(c, "c", dev)
+    if c.shape != (M, N):
+        raise ValueError(f"gemm_fp8: c is [{M}, {N}], not {tuple(c.shape)}")
+    check(load().b200q_gemm_fp8(_codes(a, "a", dev), ps, ld, pw, pws, pc, M, N, K, dtype, s))
 
 
 def gemm_gated_fp8(a, a_scales, w, w_scales, y, y_scales, act="silu", stream=None):
     """y [M, N / 2], y_scales = act(gate) * up of a * w^T in 8 bits; rows of w: gate and up in turns of 128"""
-    (M, K), (N, Kw), (s, dev) = a.shape, w.shape, _here(stream)
-    _want(K == Kw and y.shape == (M, N // 2), "gemm_gated_fp8: shapes do not fit")
-    (ps, ld), (py, ldy) = _row_scales(a_scales, M, K, "a_scales", dev), _row_scales(y_scales, M, N // 2, "y_scales", dev)
-    check(load().b200q_gemm_gated_fp8(_arg(a, "e", "a", dev), ps, ld, _arg(w, "e", "w", dev), _weight_scales(w_scales, w, dev), _arg(y, "e", "y", dev), py,
-                                      ldy, M, N, K, ACTS[act], s))
+    (M, K), (s, dev) = a.shape, _here(stream)
+    (ps, ld), (pw, pws, N) = _row_scales(a_scales, M, K, "a_scales", dev), _weights(w, w_scales, K, dev)
+    py, ldy = _row_scales(y_scales, M, N // 2, "y_scales", dev)
+    if y.shape != (M, N // 2):
+        raise ValueError(f"gemm_gated_fp8: y is [{M}, {N // 2}], not {tuple(y.shape)}")
+    check(load().b200q_gemm_gated_fp8(_codes(a, "a", dev), ps, ld, pw, pws, _codes(y, "y", dev), py, ldy, M, N, K, ACTS[act], s))
 
 
 def gemm_grouped_fp8(a, a_scales, w, w_scales, c, tile_tab, n_tiles, stream=None):
     """c [rows, N] (bf16 or fp32): row r of a, which is sorted by expert, times the w [E, N, K] of its expert; tile_tab, n_tiles: moe_route's"""
-    (M, K), (E, N, Kw), (mt, four), (s, dev), (kind, dtype) = a.shape, w.shape, tile_tab.shape, _here(stream), _float(c, "c")
-    _want(K == Kw and c.shape == (M, N) and four == 4 and n_tiles.numel() >= 1, "gemm_grouped_fp8: shapes do not fit")
-    ps, ld = _row_scales(a_scales, M, K, "a_scales", dev)
-    check(load().b200q_gemm_grouped_fp8(_arg(a, "e", "a", dev), M, ps, ld, _arg(w, "e", "w", dev), _weight_scales(w_scales, w, dev), E,
-                                        _arg(c, kind, "c", dev), N, K, _arg(tile_tab, "i", "tile_tab", dev), _arg(n_tiles, "i", "n_tiles", dev), mt,
-                                        dtype, s))
+    (M, K), (s, dev) = a.shape, _here(stream)
+    (ps, ld), (pw, pws, E, N), (pc, dtype) = _row_scales(a_scales, M, K, "a_scales", dev), _expert_weights(w, w_scales, K, dev), _float(c, "c", dev)
+    if c.shape != (M, N):
+        raise ValueError(f"gemm_grouped_fp8: c is [{M}, {N}], not {tuple(c.shape)}")
+    check(load().b200q_gemm_grouped_fp8(_codes(a, "a", dev), M, ps, ld, pw, pws, E, pc, N, K, *_tiles(tile_tab, n_tiles, dev), dtype, s))
 
 
 def gemm_grouped_gated_fp8(a, a_scales, w, w_scales, y, y_scales, tile_tab, n_tiles, act="silu", stream=None):
     """gemm_gated_fp8 by expert, arguments as of gemm_grouped_fp8"""
-    (M, K), (E, N, Kw), (mt, four), (s, dev) = a.shape, w.shape, tile_tab.shape, _here(stream)
-    _want(K == Kw and y.shape == (M, N // 2) and four == 4 and n_tiles.numel() >= 1, "gemm_grouped_gated_fp8: shapes do not fit")
-    (ps, ld), (py, ldy) = _row_scales(a_scales, M, K, "a_scales", dev), _row_scales(y_scales, M, N // 2, "y_scales", dev)
-    check(load().b200q_gemm_grouped_gated_fp8(_arg(a, "e", "a", dev), M, ps, ld, _arg(w, "e", "w", dev), _weight_scales(w_scales, w, dev), E,
-                                              _arg(y, "e", "y", dev), py, ldy, N, K, _arg(tile_tab, "i", "tile_tab", dev),
-                                              _arg(n_tiles, "i", "n_tiles", dev), mt, ACTS[act], s))
+    (M, K), (s, dev) = a.shape, _here(stream)
+    (ps, ld), (pw, pws, E, N) = _row_scales(a_scales, M, K, "a_scales", dev), _expert_weights(w, w_scales, K, dev)
+    py, ldy = _row_scales(y_scales, M, N // 2, "y_scales", dev)
+    if y.shape != (M, N // 2):
+        raise ValueError(f"gemm_grouped_gated_fp8: y is [{M}, {N // 2}], not {tuple(y.shape)}")
+    check(load().b200q_gemm_grouped_gated_fp8(_codes(a, "a", dev), M, ps, ld, pw, pws, E, _codes(y, "y", dev), py, ldy, N, K,
+                                              *_tiles(tile_tab, n_tiles, dev), ACTS[act], s))
 
 
 def gemm_fp8_set_mode(mode: int):
