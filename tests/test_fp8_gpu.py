@@ -455,3 +455,76 @@ def test_offsets_beyond_32_bits(cuda):
     ref, size = product(part, torch.ones(blocks_of(K), 9, device="cuda"), w, sw)
     assert ((c[rows.cuda()].double() - ref).abs() <= product_off(size, K) + ref.abs() * 2.0 ** -8).all()
     assert (c[3:M // 2:997] == 0).all()
+
+
+def test_rule_reaches_every_kernel(cuda):
+    """over the matrices of the built-in models every kernel and tile is taken somewhere"""
+    from llmq_b200 import lib
+    L = lib.load()
+    shapes = ((6144, 4096), (4096, 4096), (4096, 14336), (2048, 2048), (2048, 8192), (8192, 3584), (3584, 4096), (3584, 14336), (4096, 2304), (2304, 9216))
+    taken = {L.b200q_gemm_fp8_choice(m, N, K, 0) for N, K in shapes for m in range(1, 4609, 13)}
+    assert {1, 22, 42, 33, 43} <= taken and {24, 34, 45} <= {t % 100 for t in taken if t > 100}, sorted(taken)
+    assert {L.b200q_gemm_fp8_choice(m, 16384, 2048, 1) % 10 for m in range(1, 4609, 7)} == {1, 2, 3}
+
+
+def test_first_call_in_a_capture(cuda):
+    """a process whose first product is captured"""
+    import subprocess
+    import sys
+    code = """
+import torch
+from llmq_b200 import lib
+from tests.fp8_util import random_held, product, product_off
+g = torch.Generator(device="cuda").manual_seed(0)
+(a, sa), (w, sw) = random_held(g, 300, 1024, 1), random_held(g, 512, 1024, 128)
+c = torch.zeros(300, 512, device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    lib.gemm_fp8(a, sa, w, sw, c)
+graph.replay()
+torch.cuda.synchronize()
+ref, size = product(a, sa, w, sw)
+assert ((c.double() - ref).abs() <= product_off(size, 1024)).all()
+print("fine")
+"""
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=root, timeout=120)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_units_far_from_zero(cuda, mode, act):
+    """gates of hundreds, of either sign, and of next to nothing: what a row of 128 is held as stays right"""
+    from llmq_b200 import lib
+    for which in (1, 2, 3):
+        mode(which)
+        a = torch.zeros(6, 128, device="cuda")
+        a[:, 0] = torch.tensor([1.0, -1.0, 0.25, -0.25, 2.0 ** -9, 0.0])
+        a, sa = a.to(F8), torch.ones(1, 8, device="cuda")
+        w = torch.zeros(256, 128, device="cuda")
+        w[:128, 0] = torch.linspace(-448, 448, 128)
+        w[128:, 0] = torch.linspace(1, 3, 128)
+        w, sw = w.to(F8), torch.ones(2, 1, device="cuda")
+        y, ys = torch.empty(6, 128, dtype=F8, device="cuda"), lib.fp8_row_scales(6, 128)
+        lib.gemm_gated_fp8(a, sa, w, sw, y, ys, act)
+        sums, size = product(a, sa, w, sw)
+        held_close(y, ys[:, :6], unit(sums, act), unit_off(sums, product_off(size, 128), act) + 1e-13, what=f"mode {which}")
+
+
+def test_repeated_rows_and_layers_in_place(cuda):
+    """the same row many times in a gather; a residual that is normed again and again"""
+    from llmq_b200 import lib
+    g = gen(3)
+    x = torch.randn(7, 256, generator=g, device="cuda").to(BF)
+    rows = torch.full((500,), 6, dtype=torch.int32, device="cuda")
+    y, s = torch.empty(500, 256, dtype=F8, device="cuda"), lib.fp8_row_scales(500, 256)
+    lib.quantize_fp8(x, y, s, rows=rows)
+    assert (y.view(torch.uint8) == y.view(torch.uint8)[0]).all() and (s[:, :500] == s[:, :1]).all()
+    r, w = torch.zeros(7, 256, dtype=BF, device="cuda"), torch.ones(256, dtype=BF, device="cuda")
+    y, s = torch.empty(7, 256, dtype=F8, device="cuda"), lib.fp8_row_scales(7, 256)
+    want = r.clone()
+    for _ in range(5):
+        lib.rmsnorm_fp8(x, w, y, s, 1e-5, residual=r)
+        want = (x.float() + want.float()).to(BF)
+    assert torch.equal(r, want)
