@@ -127,6 +127,7 @@ constexpr int FL_REGS_FEW = 40, FL_REGS_MANY = 232;
 template <bool PAIR, int CH, bool GATED>
 struct LargeCfg {
   static constexpr int BN = 64 * CH, W_ROWS = PAIR ? BN / 2 : BN;                // columns of a tile; rows of W that a CTA fetches
+  static constexpr int ACCS = 512 / BN < 4 ? 2 : 4;                              // accumulators of each half in tensor memory
   static constexpr int STAGE = F8_STAGE_W + W_ROWS * FP8_BLOCK;                  // behind 128 rows of A
   // a warp's columns of C on their way out: all of them where a wide tile of a pair leaves room, else 64 (gated: 128 codes of two tiles for two warps)
   static constexpr int PATCH = PAIR && CH == 4 && !GATED ? 8192 : 4096;
@@ -153,7 +154,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* patches = smem + STAGES * Cfg::STAGE;
-  __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], acc_full[2][2], acc_empty[2][2];  // of accumulators: [half of the columns][turn]
+  __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], acc_full[2][Cfg::ACCS], acc_empty[2][Cfg::ACCS];  // of accumulators: [half of the columns][turn]
   __shared__ uint32_t tmem_slot;
   __shared__ int dead;
   __shared__ float most[2][128];  // gated: the largest of a half row's 64 values
@@ -164,6 +165,12 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
   const int unit = blockIdx.x / share, units = gridDim.x / share;
   const int n_tiles = (a.N + BN - 1) / BN, blocks = a.blocks;
   const int b_begin = SPLIT ? split * blocks / a.splits : 0, b_end = SPLIT ? (split + 1) * blocks / a.splits : blocks;
+  auto next_acc = [](int& acc, uint32_t& phase) {
+    if (++acc == Cfg::ACCS) {
+      acc = 0;
+      phase ^= 1u;
+    }
+  };
   // the i-th box of a stage begins so many rows of W behind the tile's first
   auto w_box = [&](int i) { return PAIR ? (GATED ? rank * 128 + i * 64 : (i * 2 + rank) * Cfg::BOX) : GATED ? (i & 1) * 128 + (i >> 1) * 64 : 0; };
 
@@ -175,9 +182,9 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
       mbar_init(full + s, PAIR ? 2 : 1);
       mbar_init(empty + s, 2);  // both halves' products
     }
-    for (int s = 0; s < 4; ++s) {
-      mbar_init(acc_full[s >> 1] + (s & 1), 1);
-      mbar_init(acc_empty[s >> 1] + (s & 1), PAIR ? 8 : 4);  // (the leader's) the warps that promote
+    for (int s = 0; s < 2 * Cfg::ACCS; ++s) {
+      mbar_init(acc_full[0] + s, 1);
+      mbar_init(acc_empty[0] + s, PAIR ? 8 : 4);  // (the leader's) the warps that promote
     }
     mbar_fence_init();
   }
@@ -270,7 +277,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
             f8_wait(acc_empty[h] + acc, acc_phase ^ 1u, &dead, a.failed);
             tc_fence_after();
             const uint32_t sa = ring + (uint32_t)(stage * Cfg::STAGE), sw = sa + F8_STAGE_W + h * (Cfg::W_ROWS / 2) * FP8_BLOCK;
-            const uint32_t d = tmem + (uint32_t)(acc * 256 + h * 128);
+            const uint32_t d = tmem + (uint32_t)(acc * BN + h * (BN / 2));
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               if constexpr (PAIR)
@@ -289,8 +296,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
               stage = 0;
               phase ^= 1u;
             }
-            acc ^= 1;
-            if (acc == 0) acc_phase ^= 1u;
+            next_acc(acc, acc_phase);
           }
           if (*(volatile int*)&dead) break;
         }
@@ -301,7 +307,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(FL_REGS_MANY));
     // rows quarter * 32 + lane; columns: half of the tile's, gated: half * 64 + 0 .. 63 of the gates and of what they gate
     const int quarter = warp & 3, half = (warp - 4) >> 2;
-    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * (BN / 2));
     uint8_t* const patch = patches + (warp - 4) * Cfg::PATCH;
     const uint32_t patch_s = smem_u32(patch);
     const uint32_t empty0 = PAIR ? mapa_shared(acc_empty[half], leader) : smem_u32(acc_empty[half]);
@@ -346,8 +352,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
           f8_wait(acc_full[half] + acc, acc_phase, &dead, a.failed);
           __syncwarp();
           if (lane == 0) f8_arrive(empty0 + acc * 8);
-          acc ^= 1;
-          if (acc == 0) acc_phase ^= 1u;
+          next_acc(acc, acc_phase);
         }
         if (tile + units < num_tiles) first_scales(tile + units, next_entry);
         continue;
@@ -364,7 +369,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
       f8_wait(acc_full[half] + acc, acc_phase, &dead, a.failed);
       __syncwarp();
       tc_fence_after();
-      tmem_ld32(lanes + (uint32_t)(acc * 256), v[0]);
+      tmem_ld32(lanes + (uint32_t)(acc * BN), v[0]);
       // (a block is an odd number of loads where CH is 3: its first goes to v[i & 1] there, four blocks to a round)
       for (int b0 = b_begin; b0 < b_end; b0 += 4) {
         // four blocks' factors, and only then the loads of the next four: a wait for a load is one for all that were issued before it
@@ -385,7 +390,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
             f32x2 s[SCALES];
 #pragma unroll
             for (int h = 0; h < SCALES; ++h) s[h] = pair_of(x[i][h], x[i][h]);
-            const uint32_t from = lanes + (uint32_t)(acc * 256);
+            const uint32_t from = lanes + (uint32_t)(acc * BN);
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
               constexpr int ODD = CH & 1;
@@ -398,13 +403,12 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) f8_arrive(empty0 + acc * 8);
-                acc ^= 1;
-                if (acc == 0) acc_phase ^= 1u;
+                next_acc(acc, acc_phase);
                 if (b0 + i + 1 < b_end) {
                   f8_wait(acc_full[half] + acc, acc_phase, &dead, a.failed);
                   __syncwarp();
                   tc_fence_after();
-                  tmem_ld32(lanes + (uint32_t)(acc * 256), next);
+                  tmem_ld32(lanes + (uint32_t)(acc * BN), next);
                 }
               }
               promote(sum[c], now, SCALES == 2 && scale_of(c) ? s[SCALES - 1] : s[0]);
