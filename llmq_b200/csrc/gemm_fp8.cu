@@ -268,6 +268,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
       const int h = warp - 1;
       constexpr uint32_t idesc = fp8_idesc(BM, BN / 2);
       const uint32_t ring = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
+      const uint64_t rows = make_smem_desc(ring), columns = make_smem_desc(ring + F8_STAGE_W + h * (Cfg::W_ROWS / 2) * FP8_BLOCK);
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       if (elect_one())
@@ -276,14 +277,14 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
             f8_wait(full + stage, phase, &dead, a.failed);
             f8_wait(acc_empty[h] + acc, acc_phase ^ 1u, &dead, a.failed);
             tc_fence_after();
-            const uint32_t sa = ring + (uint32_t)(stage * Cfg::STAGE), sw = sa + F8_STAGE_W + h * (Cfg::W_ROWS / 2) * FP8_BLOCK;
+            const uint64_t at = (uint64_t)(stage * (Cfg::STAGE / 16));  // (addresses in descriptors count 16 bytes)
             const uint32_t d = tmem + (uint32_t)(acc * BN + h * (BN / 2));
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               if constexpr (PAIR)
-                umma_fp8_2sm(d, make_smem_desc(sa + k * 32), make_smem_desc(sw + k * 32), idesc, k > 0);
+                umma_fp8_2sm(d, rows + at + 2 * k, columns + at + 2 * k, idesc, k > 0);
               else
-                umma_fp8(d, make_smem_desc(sa + k * 32), make_smem_desc(sw + k * 32), idesc, k > 0);
+                umma_fp8(d, rows + at + 2 * k, columns + at + 2 * k, idesc, k > 0);
             }
             if constexpr (PAIR) {
               f8_commit_2sm(acc_full[h] + acc, (uint16_t)(3 << leader));
@@ -679,6 +680,7 @@ __global__ void __launch_bounds__(small_threads<GATED>(MOST), small_resident<GAT
   } else if (warp == 1) {
     const uint32_t idesc = fp8_idesc(128, mp);
     const uint32_t ring = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
+    const uint64_t weights = make_smem_desc(ring), rows_of_a = make_smem_desc(ring + WT * F8_STAGE_W);
     int stage = 0, acc = 0;
     uint32_t phase = 0, acc_phase = 0;
     if (elect_one())
@@ -687,12 +689,12 @@ __global__ void __launch_bounds__(small_threads<GATED>(MOST), small_resident<GAT
         f8_wait(full + stage, phase, &dead, a.failed);
         if (*(volatile int*)&dead) break;
         tc_fence_after();
-        const uint32_t sw = ring + (uint32_t)(stage * stage_bytes), sa = sw + WT * F8_STAGE_W, d = tmem + (uint32_t)(acc * WT * stride);
+        const uint64_t at = (uint64_t)(uint32_t)(stage * (stage_bytes / 16));  // (addresses in descriptors count 16 bytes)
+        const uint32_t d = tmem + (uint32_t)(acc * WT * stride);
 #pragma unroll
         for (int h = 0; h < WT; ++h)
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_fp8(d + (uint32_t)(h * stride), make_smem_desc(sw + h * F8_STAGE_W + k * 32), make_smem_desc(sa + k * 32), idesc, k > 0);
+          for (int k = 0; k < 4; ++k) umma_fp8(d + (uint32_t)(h * stride), weights + at + (h * (F8_STAGE_W / 16) + 2 * k), rows_of_a + at + 2 * k, idesc, k > 0);
         umma_commit(acc_full + acc);
         umma_commit(empty + stage);
         if (++stage == a.stages) {
