@@ -970,13 +970,14 @@ int g_fp8_mode = 0;  // test hook: see b200q_gemm_fp8_set_mode
 // Which kernel and tile: the least of what each is expected to take, us.  A round of tiles (as many as are resident at once) costs so much for
 // its start and end and so much a block; no kernel takes less than the weights do to come from memory; parts cost their exchange.  Fitted to
 // 450 sizes (15 shapes of 1024 to 16384 columns x 1024 to 14336, 30 row counts from 1 to 4608, weights from HBM, back to back in a graph) and
-// every kernel: what is taken is 1 % slower than the best on average and 21 % at worst (129 x 1024 x 4096: 9.1 us, 7.5).  us, the choice / the
-// others: 1 x 4096 x 4096 small 6.3 / four parts of 128 columns 8.8; 48 x 4096 x 14336 small 15.2 / 16.2; 128 x 4096 x 14336 four parts of
-// 128 columns 17.5 / small 22.8, whole tiles 48; 200 x 4096 x 14336 three parts of 192 columns 23.7 / two of 128 25.7, a pair's whole tiles 42;
-// 300 x 8192 x 3584 pairs of 256 columns 15.4 / single CTAs 16.0, of 128 columns 23.8; 450 x 4096 x 14336 pairs in two parts 37 / of 128
-// columns 41; 768 x 4096 x 4096 pairs of 192 columns 16.1 / 256 17.2; 4608 x 4096 x 14336 pairs of 256 254 / single CTAs 277.
-// Gated (184 sizes, 8 shapes; 0.3 % and 7 %): 7 x 16384 x 2048 small 9.6 / 12.5 / pairs 12.5; 48 x 28672 x 4096 small 28.8 / 26.0 / 36.3;
-// 200 x 28672 x 4096 96 / 39.8 / 34.3; 300 110 / 59.9 / 67.4; 4608 497 / 445.
+// every kernel: what is taken is 0.6 % slower than the best on average, more than 5 % at 15 of them, and 12 % at 33 x 3584 x 14336 (four parts
+// 15.3 us, small tiles 13.7).  us, the choice / others: 1 x 4096 x 4096 small 6.3 / four parts of 128 columns 8.3; 48 x 4096 x 14336 small 14.7 / four
+// parts 15.5; 128 x 4096 x 14336 four parts of 128 columns 16.7 / small 22.5, whole tiles 43; 200 x 4096 x 14336 three parts of 192 columns
+// 23.0 / two of 128 23.4, whole 43; 300 x 8192 x 3584 pairs of 256 columns 15.7 / single CTAs 16.3, of 128 columns 21.1; 450 x 4096 x 14336 pairs
+// in two parts 35.1 / 128 columns 37.8; 768 x 4096 x 4096 pairs of 256 17.2 / of 192 17.4, 128 columns 23.1; 4608 x 4096 x 14336 pairs of 256
+// 252 / single CTAs 251 to 277.
+// Gated (184 sizes, 8 shapes; 0.2 % on average): 16 x 16384 x 2048 small 10.6 / 13.4 / pairs 13.5; 48 x 28672 x 4096 small 27.7 / 25.2 / 35.9;
+// 200 x 28672 x 4096 99 / 42 / 37; 300 110 / 62 / 69; 4608 single CTAs 586 / pairs 507.
 struct Fp8Tile {
   int kind, ch, splits;  // as the hook's
 };
@@ -998,21 +999,21 @@ static Fp8Tile choose_fp8_tile(int M, int N, int blocks) {
     const int rounds = (p.n_tiles * p.m_tiles + fit - 1) / fit, each = (blocks + p.splits - 1) / p.splits;
     const double parts = p.splits - 1;
     if (GATED)
-      offer({1, 4, 1}, p.resident == 2 ? 5.5 + larger(rounds * (0.27 + 0.053 * each), 1.09 * weights) : 3.6 + larger(rounds * (1.4 + 0.69 * each), 1.38 * weights));
+      offer({1, 4, 1}, p.resident == 2 ? 5.5 + larger(rounds * (0.29 + 0.093 * each), 1.05 * weights) : 2.5 + larger(rounds * (2.55 + 0.677 * each), 1.4 * weights));
     else if (p.rows <= 32)
-      offer({1, 4, 1}, 2.9 + larger(rounds * 0.466 * each, 1.13 * weights) + 0.1 * parts);
+      offer({1, 4, 1}, 2.9 + larger(rounds * 0.464 * each, 1.14 * weights) + 0.13 * parts);
     else if (p.rows <= 64)
-      offer({1, 4, 1}, 3.95 + larger(rounds * 0.519 * each, 1.19 * weights) + 0.17 * parts);
+      offer({1, 4, 1}, 3.77 + larger(rounds * 0.516 * each, 1.2 * weights) + 0.2 * parts);
     else if (rounds == 1 && each <= 16)
-      offer({1, 4, 1}, 4.94 + larger(0.564 * each, weights) + 0.024 * parts);
+      offer({1, 4, 1}, 4.5 + larger(0.5 * each, weights) + 0.024 * parts);
   }
   const struct {
     Fp8Tile tile;  // splits: the most
     double fixed, round, block, part, weights;
-  } plain[6] = {{{2, 2, 1}, 2.0, 1.55, 0.340, 0, 1}, {{2, 4, 1}, 0, 4.0, 0.403, 0, 1}, {{3, 3, 1}, 0, 3.9, 0.340, 0, 1}, {{3, 4, 1}, 0, 4.5, 0.352, 0, 1},
-                {{4, 2, 6}, 0, 5.5, 0.359, 0.13, 1}, {{4, 3, 4}, 0, 6.8, 0.391, 0.17, 1.77}},
-    pair_parts = {{5, 4, 3}, 0, 8.5, 0.387, 0.07, 1},
-    gated[2] = {{{2, 4, 1}, 2.8, 2.0, 0.53, 0, 1.21}, {{3, 4, 1}, 2.75, 2.46, 0.43, 0, 1.06}};
+  } plain[6] = {{{2, 2, 1}, 2.0, 1.45, 0.307, 0, 1.19}, {{2, 4, 1}, 0, 4.16, 0.406, 0, 1}, {{3, 3, 1}, 0, 4.4, 0.342, 0, 1}, {{3, 4, 1}, 0, 4.63, 0.359, 0, 1},
+                {{4, 2, 6}, 0, 5.5, 0.325, 0.12, 1}, {{4, 3, 4}, 0, 6.9, 0.384, 0.1, 1.87}},
+    pair_parts = {{5, 4, 3}, 0, 9.05, 0.429, 0, 1},
+    gated[2] = {{{2, 4, 1}, 2.1, 2.72, 0.53, 0, 1.25}, {{3, 4, 1}, 2.4, 3.24, 0.435, 0, 1.06}};
   auto large = [&](const auto& c) {
     const bool pair = c.tile.kind == 3 || c.tile.kind == 5;
     const long long tiles = (long long)((M + (pair ? 255 : 127)) / (pair ? 256 : 128)) * ((N + 64 * c.tile.ch - 1) / (64 * c.tile.ch));
