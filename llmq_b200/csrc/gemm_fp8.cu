@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
     n0 = tile / m_tiles * BN;
     if constexpr (GROUPED) {  // (kept within the matrices, whatever the table says)
       g = min(max(e.x, 0), a.groups - 1);
-      row0 = max(e.y, 0);
+      row0 = min(max(e.y, 0), a.M);
       row_end = min(e.z, a.M);
     } else {
       g = 0;

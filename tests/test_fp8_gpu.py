@@ -528,3 +528,27 @@ def test_repeated_rows_and_layers_in_place(cuda):
         lib.rmsnorm_fp8(x, w, y, s, 1e-5, residual=r)
         want = (x.float() + want.float()).to(BF)
     assert torch.equal(r, want)
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_rows_of_a_table_stay_within_the_matrices(cuda, gated):
+    """entries whose rows lie far outside are no rows at all, in whichever quarter of a tile their sum with the first row would turn over"""
+    from llmq_b200 import lib
+    g = gen(5)
+    (a, sa), (w, sw) = random_held(g, 130, 256, 1), random_held(g, 256, 256, 128)
+    last = 2 ** 31 - 1
+    tab = torch.tensor([[0, last, last, 0], [0, last - 40, last, 0], [0, last - 100, 130, 0], [0, 130, last, 0], [0, 64, 100, 0]], dtype=torch.int32, device="cuda")
+    n = torch.tensor([5], dtype=torch.int32, device="cuda")
+    w, sw = w[None], sw[None]
+    if gated:
+        y, ys = torch.zeros(130, 128, dtype=F8, device="cuda"), lib.fp8_row_scales(130, 128)
+        ys.fill_(-3.0)
+        lib.gemm_grouped_gated_fp8(a, sa / 60, w, sw, y, ys, tab, n)
+        out, none = ys[0, :130], -3.0
+        assert (y[:64].float() == 0.0).all() and (y[100:].float() == 0.0).all()
+    else:
+        c = torch.full((130, 256), 7.0, device="cuda")
+        lib.gemm_grouped_fp8(a, sa, w, sw, c, tab, n)
+        out, none = c[:, 0], 7.0
+        assert (c[:64] == 7.0).all() and (c[100:] == 7.0).all()
+    assert (out[:64] == none).all() and (out[100:130] == none).all() and (out[64:100] != none).all()
