@@ -71,9 +71,10 @@ __global__ void __launch_bounds__(256)
 template <typename T>
 __global__ void __launch_bounds__(256)
     quantize_fp8_kernel(const T* __restrict__ x, long long ld_x, const int32_t* __restrict__ rows, uint2* __restrict__ y,
-                        float* __restrict__ scales, int ld_scales, int K, uint32_t blocks, uint32_t total) {
+                        float* __restrict__ scales, int ld_scales, int K, uint32_t blocks, uint32_t by_blocks, int shift, uint32_t total) {
   follow_previous(x, rows, y, scales);
-  const uint32_t item = blockIdx.x * 32 + (threadIdx.x >> 3), row = item / blocks, block = item - row * blocks;
+  // item / blocks (by_blocks: 2^shift / blocks and less than 2^(shift - 31) more, so exact for items below 2^31)
+  const uint32_t item = blockIdx.x * 32 + (threadIdx.x >> 3), row = (uint32_t)((uint64_t)item * by_blocks >> shift), block = item - row * blocks;
   const int lane = threadIdx.x & 7, k = (int)block * FP8_BLOCK + lane * 8;
   const bool live = item < total;
   const T* from = x + (live ? (rows ? (long long)rows[row] : (long long)row) : 0ll) * ld_x + k;
@@ -163,10 +164,13 @@ int b200q_quantize_fp8(const void* x, int64_t ld_x, const int32_t* rows, void* y
   const int blocks = (K + FP8_BLOCK - 1) / FP8_BLOCK;
   const long long total = (long long)T_ * blocks;
   B200Q_CHECK_ARG(total < (1ll << 31), "quantize_fp8: too much at once (T=%d K=%d)", T_, K);
+  int up = 0;  // 2^up >= blocks
+  while ((1 << up) < blocks) ++up;
+  const uint32_t by_blocks = (uint32_t)((1ull << (31 + up)) / (uint32_t)blocks + 1);
   auto launch = [&](auto type) -> int {
     using T = decltype(type);
     B200Q_CUDA(launch_early(quantize_fp8_kernel<T>, dim3((unsigned)((total + 31) / 32)), 256, 0, as_stream(stream), 1, (const T*)x, (long long)ld_x, rows,
-                            (uint2*)y, scales, ld_scales, K, (uint32_t)blocks, (uint32_t)total));
+                            (uint2*)y, scales, ld_scales, K, (uint32_t)blocks, by_blocks, 31 + up, (uint32_t)total));
     count_launch();
     return B200Q_OK;
   };
