@@ -3,15 +3,20 @@
 //
 // A block of 128 codes is one swizzle span, one stage of the ring and four tcgen05.mma (kind::f8f6f4, 32 codes each) whose fp32 sums start from
 // zero; the block's scales are then multiplied in while the sums leave tensor memory for the registers that hold the running total ("promoted").
-// Two accumulators in tensor memory let the tensor core work on block b + 1 meanwhile.  Bounds: the weight stream (N K bytes) for few rows; for many
-// the tensor core at twice the bf16 rate, and, close behind it, the promotion, which reads 4 bytes of tensor memory and does one multiply-add
-// for every 128 products.
+// Two or four accumulators let the tensor core work on the next blocks meanwhile.
 //
-//   * large: rows of A are the tensor core's M side (a lane has a row, so that its scale is one number to a thread), 256 columns to a CTA, eight
-//     warps that promote 128 columns each in 128 registers a thread.  Persistent.  One CTA to 128 rows, or a pair (cta_group::2) to 256, each of
-//     which fetches half of the weights.
-//   * small, up to 128 rows to a tile: the weights are the M side and the rows, padded to 16, the N side; the reduction is split over a
-//     cluster whose partial sums meet in distributed shared memory in the order of the splits.
+// Bounds: for few rows the weight stream (N K bytes); for many the tensor core at twice the bf16 rate and, as near, tensor memory, which products
+// fill while the promotion reads it (32 columns: some 165 cycles beside products, 16 to 30 alone), two packed multiply-adds to four sums; at the
+// largest sizes the clock as well, which the power limit holds at 1.2 to 1.3 GHz.  us, back to back in a graph, weights from HBM: 1 x 4096 x 4096 6.3,
+// 48 x 4096 x 14336 14.5 (4.1 TB/s of weights; bf16 24.7), 1001 x 8192 x 3584 33.5 (1.76 PFLOP/s; bf16 50), 4608 x 4096 x 14336 252 to 260
+// (2.1 PFLOP/s; bf16 413 to 422; the library's product of the same codes with one scale for all of them 196, of zeros 133); gated 7 x 16384 x 2048
+// 9.4 to 10.5, 4608 x 28672 x 4096 520 to 526 (bf16 770); 16 experts of 2048 x 2048, 64 tokens to four of them 17 (3.9 TB/s of weights).
+//
+//   * large: rows of A are the tensor core's M side (a lane has a row, so that its scale is one number to a thread), up to 256 columns to a CTA,
+//     eight warps that promote half of them each in up to 128 registers a thread.  Persistent.  One CTA to 128 rows, or a pair (cta_group::2) to
+//     256, each of which fetches half of the weights; or a cluster to a tile, with a part of the reduction to each CTA or pair.
+//   * small, up to 128 rows to a tile (gated: 64): the weights are the M side and the rows, padded to 16, the N side; the reduction is split over
+//     a cluster whose partial sums meet in distributed shared memory in the order of the splits.
 #include <atomic>
 #include <type_traits>
 
@@ -970,9 +975,9 @@ int g_fp8_mode = 0;  // test hook: see b200q_gemm_fp8_set_mode
 // Which kernel and tile: the least of what each is expected to take, us.  A round of tiles (as many as are resident at once) costs so much for
 // its start and end and so much a block; no kernel takes less than the weights do to come from memory; parts cost their exchange.  Fitted to
 // 450 sizes (15 shapes of 1024 to 16384 columns x 1024 to 14336, 30 row counts from 1 to 4608, weights from HBM, back to back in a graph) and
-// every kernel: what is taken is 0.6 % slower than the best on average, more than 5 % at 15 of them, and 12 % at 33 x 3584 x 14336 (four parts
-// 15.3 us, small tiles 13.7).  us, the choice / others: 1 x 4096 x 4096 small 6.3 / four parts of 128 columns 8.3; 48 x 4096 x 14336 small 14.7 / four
-// parts 15.5; 128 x 4096 x 14336 four parts of 128 columns 16.7 / small 22.5, whole tiles 43; 200 x 4096 x 14336 three parts of 192 columns
+// every kernel: what is taken is 0.5 % slower than the best on average, more than 5 % at 9 of them, and 10 % at 3000 x 2304 x 9216 (pairs of 192
+// columns 68.9 us, of 256 62.7).  us, the choice / others: 1 x 4096 x 4096 small 6.3 / four parts of 128 columns 8.3; 48 x 4096 x 14336 small 14.5 / four
+// parts 15.9; 128 x 4096 x 14336 four parts of 128 columns 16.7 / small 22.5, whole tiles 43; 200 x 4096 x 14336 three parts of 192 columns
 // 23.0 / two of 128 23.4, whole 43; 300 x 8192 x 3584 pairs of 256 columns 15.7 / single CTAs 16.3, of 128 columns 21.1; 450 x 4096 x 14336 pairs
 // in two parts 35.1 / 128 columns 37.8; 768 x 4096 x 4096 pairs of 256 17.2 / of 192 17.4, 128 columns 23.1; 4608 x 4096 x 14336 pairs of 256
 // 252 / single CTAs 251 to 277.
@@ -1003,7 +1008,7 @@ static Fp8Tile choose_fp8_tile(int M, int N, int blocks) {
     else if (p.rows <= 32)
       offer({1, 4, 1}, 2.9 + larger(rounds * 0.464 * each, 1.14 * weights) + 0.13 * parts);
     else if (p.rows <= 64)
-      offer({1, 4, 1}, 3.77 + larger(rounds * 0.516 * each, 1.2 * weights) + 0.2 * parts);
+      offer({1, 4, 1}, 2.4 + larger(rounds * 0.78 * each, weights) + 0.07 * parts + 0.025 * (M - 33));
     else if (rounds == 1 && each <= 16)
       offer({1, 4, 1}, 4.5 + larger(0.5 * each, weights) + 0.024 * parts);
   }
