@@ -10,7 +10,7 @@
 // largest sizes the clock as well, which the power limit holds at 1.2 to 1.3 GHz.  us, back to back in a graph, weights from HBM: 1 x 4096 x 4096 6.3,
 // 48 x 4096 x 14336 14.5 (4.1 TB/s of weights; bf16 24.7), 1001 x 8192 x 3584 33.5 (1.76 PFLOP/s; bf16 50), 4608 x 4096 x 14336 252 to 260
 // (2.1 PFLOP/s; bf16 413 to 422; the library's product of the same codes with one scale for all of them 196, of zeros 133); gated 7 x 16384 x 2048
-// 9.4 to 10.5, 4608 x 28672 x 4096 520 to 526 (bf16 770); 16 experts of 2048 x 2048, 64 tokens to four of them 17 (3.9 TB/s of weights).
+// 9.4 to 10.5, 4608 x 28672 x 4096 516 to 522 (bf16 770); 16 experts of 2048 x 2048, 64 tokens to four of them 17 (3.9 TB/s of weights).
 //
 //   * large: rows of A are the tensor core's M side (a lane has a row, so that its scale is one number to a thread), up to 256 columns to a CTA,
 //     eight warps that promote half of them each in up to 128 registers a thread.  Persistent.  One CTA to 128 rows, or a pair (cta_group::2) to
@@ -96,8 +96,13 @@ __device__ __forceinline__ void f8_leave_cluster() {
 }
 // the unit of a gate and what it gates, fp32 from the sums on: g sigmoid(g) u, or tanh GELU, 0.5 g (1 + tanh t) = g sigmoid(2 t)
 __device__ __forceinline__ float fp8_unit(float g, float u, int gelu) {
-  const float t = gelu ? 1.5957691216057308f * (g + 0.044715f * (g * g * g)) : g;
-  return __fdividef(g, 1.f + __expf(-t)) * u;
+  // (the exponent is for base 2, its rounding 2^-24 of it; the two instructions are off by 2^-22 and 2^-23 at most; the same through __expf and
+  // __fdividef, which look at subnormal numbers: 4608 x 16384 x 2048 174 us for 170)
+  const float t = gelu ? g * fmaf(-0.10294324f, g * g, -2.3022082f) : g * -1.4426950f;
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return g * r * u;
 }
 // (dead: another role of the CTA has given up; flag and clock are looked at every 64 tries)
 __device__ __forceinline__ void f8_wait(uint64_t* bar, uint32_t parity, volatile int* dead, int* failed) {
