@@ -736,7 +736,7 @@ int b200q_decode_attn_q4_set_whole(int whole);
 int b200q_rmsnorm_fp8(const void* x_dev, void* residual_dev, const void* w_dev, void* y_dev, float* scales_dev, int ld_scales, int T, int H,
                       float eps, int dtype, void* stream);
 /* rows of x (ld_x elements apart, a multiple of 8) in 8 bits; rows != NULL: row i of y is row rows[i] of x (tokens sorted by expert: perm_tok
- *     of b200q_moe_route) */
+ *     of b200q_moe_route), which is not looked at: it has to be one of x */
 int b200q_quantize_fp8(const void* x_dev, int64_t ld_x, const int32_t* rows_dev, void* y_dev, float* scales_dev, int ld_scales, int T, int K,
                        int dtype, void* stream);
 /* weights [groups][N, K] in 8 bits */

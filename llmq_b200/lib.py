@@ -882,7 +882,7 @@ def gemm_gated_fp8(a, a_scales, w, w_scales, y, y_scales, act="silu", stream=Non
     py, ldy = _row_scales(y_scales, M, N // 2, "y_scales", dev)
     if y.shape != (M, N // 2):
         raise ValueError(f"gemm_gated_fp8: y is [{M}, {N // 2}], not {tuple(y.shape)}")
-    check(load().b200q_gemm_gated_fp8(_codes(a, "a", dev), ps, ld, pw, pws, _codes(y, "y", dev), py, ldy, M, N, K, ACTS[act], s))
+    check(load().b200q_gemm_gated_fp8(_codes(a, "a", dev), ps, ld, pw, pws, _codes(y, "y", dev), py, ldy, M, N, K, ACTS.get(act, -1), s))
 
 
 def gemm_grouped_fp8(a, a_scales, w, w_scales, c, tile_tab, n_tiles, stream=None):
@@ -902,7 +902,7 @@ def gemm_grouped_gated_fp8(a, a_scales, w, w_scales, y, y_scales, tile_tab, n_ti
     if y.shape != (M, N // 2):
         raise ValueError(f"gemm_grouped_gated_fp8: y is [{M}, {N // 2}], not {tuple(y.shape)}")
     check(load().b200q_gemm_grouped_gated_fp8(_codes(a, "a", dev), M, ps, ld, pw, pws, E, _codes(y, "y", dev), py, ldy, N, K,
-                                              *_tiles(tile_tab, n_tiles, dev), ACTS[act], s))
+                                              *_tiles(tile_tab, n_tiles, dev), ACTS.get(act, -1), s))
 
 
 def gemm_fp8_set_mode(mode: int):

@@ -552,3 +552,12 @@ def test_rows_of_a_table_stay_within_the_matrices(cuda, gated):
         out, none = c[:, 0], 7.0
         assert (c[:64] == 7.0).all() and (c[100:] == 7.0).all()
     assert (out[:64] == none).all() and (out[100:130] == none).all() and (out[64:100] != none).all()
+
+
+def test_unknown_units_are_refused(cuda):
+    from llmq_b200 import lib
+    (a, sa), (w, sw) = random_held(gen(1), 4, 128, 1), random_held(gen(2), 256, 128, 128)
+    y, ys = torch.zeros(4, 128, dtype=F8, device="cuda"), lib.fp8_row_scales(4, 128)
+    with pytest.raises(lib.B200QError, match="act=-1"):
+        lib.gemm_gated_fp8(a, sa, w, sw, y, ys, act="relu")
+    assert (y.float() == 0.0).all()
