@@ -546,16 +546,18 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
       } else {
         const int r0 = row0 + quarter * 32, n = n0 + half * (BN / 2);
         constexpr int WIDE = CH % 2 ? 32 : 64;  // columns at a time
-        // by the copy engine, which takes 64 columns of 32 rows, and none that are another group's; else by this warp
+        // by the copy engine, which takes 64 columns of 32 rows, and none that are another group's; else by this warp, as all but the last 64
+        // where the patch has room for no more: the engine takes some 1000 cycles to read it (64 tokens, 16 experts of 2048 x 1024 9.0 -> 8.7 us)
         constexpr bool ENGINE = WIDE == 64, ROOM = Cfg::PATCH > 4096;
+        constexpr int LAST = 32 * CH / WIDE - 1;
         const bool copies = ENGINE && (!GROUPED || r0 + 32 <= row_end);
+        if (ENGINE) {  // (what the tile before left has been read)
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          __syncwarp();
+        }
 #pragma unroll
-        for (int h = 0; h < 32 * CH / WIDE; ++h) {
+        for (int h = 0; h <= LAST; ++h) {
           const uint32_t to = patch_s + (ROOM ? h * 4096 : 0);
-          if (ENGINE && (!ROOM || h == 0)) {
-            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-            __syncwarp();
-          }
 #pragma unroll
           for (int j = 0; j < WIDE / 8; ++j) {
             const f32x2* x = sum[h * (WIDE / 32) + j / 4] + 4 * (j & 3);
@@ -569,7 +571,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
                          "r"(w[2]), "r"(w[3])
                          : "memory");
           }
-          if (copies) {
+          if (copies && (ROOM || h == LAST)) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0 && n + 64 * h < a.N && r0 < a.M) {
