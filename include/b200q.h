@@ -729,7 +729,8 @@ int b200q_decode_attn_q4_set_whole(int whole);
  * codes[t, k] * scales[k / 128][t]; ld >= T, for products a multiple of 4.  Weights: codes [N, K], scales [ceil(N / 128)]
  * [ceil(K / 128)], one for a square of 128 x 128.  K is a multiple of 16.  A scale is a 448th of its block's largest magnitude (2^-100 at
  * least), codes are rounded to nearest (even).  A block with a NaN or an infinity reads back as NaN throughout.  Matrices are
- * 16-byte aligned; scales behind the last row are neither written nor do they count.  The activations' scales of products are 16-byte aligned too. */
+ * 16-byte aligned; scales behind the last row are neither written nor do they count.  The activations' scales of products are 16-byte aligned too.  No output
+ * overlaps an input. */
 
 /* b200q_rmsnorm / b200q_add_rmsnorm with an output in 8 bits: residual <- x + residual (rounded to its type; NULL: x alone), y = that
  *     / sqrt(mean of its squares + eps) * w, not rounded before it is quantised.  dtype: of x, residual and w.  x is not written; H <= 16384. */

@@ -7,7 +7,7 @@
 //
 // Bounds: for few rows the weight stream (N K bytes); for many the tensor core at twice the bf16 rate and, as near, tensor memory, which products
 // fill while the promotion reads it (32 columns: some 165 cycles beside products, 16 to 30 alone), two packed multiply-adds to four sums; at the
-// largest sizes the clock as well, which the power limit holds at 1.2 to 1.3 GHz.  us, back to back in a graph, weights from HBM: 1 x 4096 x 4096 6.3,
+// largest sizes the clock as well, which the power limit holds at 1.2 to 1.3 GHz.  us, back to back in a graph, weights from HBM: 1 x 4096 x 4096 6.1,
 // 48 x 4096 x 14336 14.5 (4.1 TB/s of weights; bf16 24.7), 1001 x 8192 x 3584 33.5 (1.76 PFLOP/s; bf16 50), 4608 x 4096 x 14336 252 to 260
 // (2.1 PFLOP/s; bf16 413 to 422; the library's product of the same codes with one scale for all of them 196, of zeros 133); gated 7 x 16384 x 2048
 // 9.4 to 10.5, 4608 x 28672 x 4096 516 to 522 (bf16 770); 16 experts of 2048 x 2048, 64 tokens to four of them 17 (3.9 TB/s of weights).
@@ -198,6 +198,13 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
     }
     mbar_fence_init();
   }
+  if (warp == 3 && lane == 0 && (!GROUPED || unit < a.ahead)) {
+    // the first weights into L2 while the kernel before this one ends and this one makes ready (behind that: 1 to 2 % more for few rows).  The table
+    // is not known yet: as if every group had one tile
+    const int m_tiles = GROUPED ? a.groups : (a.M + BM - 1) / BM, n0 = unit / m_tiles * BN + (GROUPED ? unit % m_tiles * a.N : 0);
+    for (int b = 0; b < min(STAGES, b_end - b_begin); ++b)
+      for (int i = 0; i < Cfg::BOXES; ++i) tma_prefetch_2d(&tmap_w, (b_begin + b) * 64, n0 + w_box(i));
+  }
   if (warp == 1) {
     if constexpr (PAIR) {
       asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_slot)) : "memory");
@@ -211,13 +218,6 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
   if constexpr (PAIR) cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
-  if (warp == 0 && lane == 0 && (!GROUPED || unit < a.ahead)) {
-    // the first weights into L2 while the kernel before this one ends (the table is not known yet: as if every group had one tile)
-    const int m_tiles = GROUPED ? a.groups : (a.M + BM - 1) / BM, n0 = unit / m_tiles * BN + (GROUPED ? unit % m_tiles * a.N : 0);
-    for (int b = 0; b < min(STAGES, b_end - b_begin); ++b)
-      for (int i = 0; i < Cfg::BOXES; ++i) tma_prefetch_2d(&tmap_w, (b_begin + b) * 64, n0 + w_box(i));
-  }
-  __syncwarp();
   const float *as = a.as, *ws = a.ws;
   const int4* tab = a.tab;
   const int32_t* n_mt = a.n_mt;
@@ -659,13 +659,12 @@ __global__ void __launch_bounds__(small_threads<GATED>(MOST), small_resident<GAT
     mbar_fence_init();
   }
   if (warp == 1) tmem_alloc(&tmem_slot, a.cols);
+  if (warp == 2 && lane == 0)  // the first weights into L2 while the kernel before this one ends and this one makes ready
+    for (int i = 0; i < min(a.stages, b1 - b0); ++i) tma_prefetch_2d(&tmap_w, (b0 + i) * 64, n0);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
-  if (warp == 0 && lane == 0)  // the first weights into L2 while the kernel before this one ends
-    for (int i = 0; i < min(a.stages, b1 - b0); ++i) tma_prefetch_2d(&tmap_w, (b0 + i) * 64, n0);
-  __syncwarp();
   follow_previous(as, ws);
 
   if (warp == 0) {
