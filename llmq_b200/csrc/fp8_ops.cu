@@ -1,7 +1,8 @@
 // fp8_ops.cu — rows and weights in 8 bits (format: fp8.cuh): RMS norm with the residual's addition, rows as they are or gathered, weights.
 // All three are bound by memory: every value is read once and leaves as one byte.  Next to that bound are their instructions, so that eight lanes
-// have a block of 128 (two pieces of eight values each: three exchanges for the largest), pairs of bf16 are added and compared at once, and the
-// norm's factor is multiplied in together with the scale's reciprocal.
+// have a block of 128 (two pieces of eight values each: three exchanges for the largest), and pairs of bf16 are added and compared at once.  (The
+// norm's factor is multiplied in on its own: its product with a scale's reciprocal, up to 2^109, can pass fp32's range where a row is next to zero,
+// and 0 times that is no zero.  4608 x 4096 24.2 us for 24.0.)
 #include "fp8.cuh"
 
 namespace b200q {
@@ -57,8 +58,8 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
     for (int p = 0; p < 2; ++p)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) n[p].w[i] = v[j][p].get(i) * u[j][p].get(i);
-    const float scale = fp8_scale(max_of_8_lanes(max_or_nan(n[0].largest(), n[1].largest())) * inv), by = fp8_inverse(scale) * inv;
+      for (int i = 0; i < 8; ++i) n[p].w[i] = v[j][p].get(i) * inv * u[j][p].get(i);
+    const float scale = fp8_scale(max_of_8_lanes(max_or_nan(n[0].largest(), n[1].largest()))), by = fp8_inverse(scale);
 #pragma unroll
     for (int p = 0; p < 2; ++p)
       if (place(j, p) < H) y[(row * H + place(j, p)) >> 3] = fp8_eight(n[p], by);
