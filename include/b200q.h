@@ -747,7 +747,8 @@ int b200q_quantize_fp8_weight(const void* w_dev, void* q_dev, float* scales_dev,
 int b200q_gemm_fp8(const void* A_dev, const float* a_scales_dev, int ld_a_scales, const void* W_dev, const float* w_scales_dev, void* C_dev,
                    int M, int N, int K, int out_f32, void* stream);
 /* the same with a gated unit, whose values leave in 8 bits: Y [M, N/2] = act(gate) * up, act 0 = SiLU, 1 = tanh GELU; rows of W in turns of
- *     128 as for b200q_gemm_swiglu_bf16 (N % 256 == 0).  Sums are not rounded before the unit, nor its values before they are quantised. */
+ *     128 as for b200q_gemm_swiglu_bf16 (N % 256 == 0).  Sums are not rounded before the unit, nor its values before they are quantised.  A gate
+ *     whose exponential passes fp32's range (below -88.7, tanh GELU -10.06) lets nothing through. */
 int b200q_gemm_gated_fp8(const void* A_dev, const float* a_scales_dev, int ld_a_scales, const void* W_dev, const float* w_scales_dev, void* Y_dev,
                          float* y_scales_dev, int ld_y_scales, int M, int N, int K, int act, void* stream);
 /* both by expert: the rows of A and of the output are sorted by group, W is [groups][N, K] (scales [groups][ceil(N/128)][ceil(K/128)]);

@@ -95,14 +95,16 @@ __device__ __forceinline__ void f8_leave_cluster() {
   asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
 // the unit of a gate and what it gates, fp32 from the sums on: g sigmoid(g) u, or tanh GELU, 0.5 g (1 + tanh t) = g sigmoid(2 t)
+// (the exponent is for base 2, its rounding 2^-24 of it; the two instructions are off by 2^-22 and 2^-23 at most; the same through __expf and
+// __fdividef, which look at subnormal numbers: 4608 x 16384 x 2048 174 us for 170)
+// The reciprocal is that of a quarter and is multiplied by a quarter of the gate: fp32 has it in full up to where the exponential passes its range,
+// 2^128 (gates below -88.7, tanh GELU -10.06), and nothing is let through.  (That of 1 + e ends at 2^126: what gates from -87.3 on let through was 0.)
 __device__ __forceinline__ float fp8_unit(float g, float u, int gelu) {
-  // (the exponent is for base 2, its rounding 2^-24 of it; the two instructions are off by 2^-22 and 2^-23 at most; the same through __expf and
-  // __fdividef, which look at subnormal numbers: 4608 x 16384 x 2048 174 us for 170)
-  const float t = gelu ? g * fmaf(-0.10294324f, g * g, -2.3022082f) : g * -1.4426950f;
+  const float q = 0.25f * g, t = gelu ? q * fmaf(64.f * -0.10294324f, q * q, 4.f * -2.3022082f) : q * (4.f * -1.4426950f);
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-  return g * r * u;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(e, 0.25f, 0.25f)));
+  return q * r * u;
 }
 // (dead: another role of the CTA has given up; flag and clock are looked at every 64 tries)
 __device__ __forceinline__ void f8_wait(uint64_t* bar, uint32_t parity, volatile int* dead, int* failed) {
