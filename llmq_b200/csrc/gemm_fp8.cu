@@ -614,6 +614,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
 
 // ---- small ---------------------------------------------------------------------------------------------------------------------
 constexpr int FS_MAX_STAGES = 8, FS_MAX_SPLITS = 8, FS_MAX_ACCS = 4, FS_SCALES = 512;  // bytes of a stage's scales of rows
+constexpr int FS_MAX_TILES = 65535;  // in each of the grid's directions
 constexpr int FS_RING_ALONE = 208 * 1024, FS_RING_SHARED = 106 * 1024;
 
 // CTAs of a tile to an SM: registers for the sums and the loads, tensor memory and the ring allow two where the rows are few
@@ -947,7 +948,7 @@ static int launch_small(const void* A, const void* W, const SmallPlan& p, Fp8Arg
     return B200Q_OK;
   });
   if (rc) return rc;
-  B200Q_CHECK_ARG(p.n_tiles <= 65535 && p.m_tiles <= 65535, "gemm_fp8: too many tiles (M=%d N=%d)", a.M, a.N);
+  B200Q_CHECK_ARG(p.n_tiles <= FS_MAX_TILES && p.m_tiles <= FS_MAX_TILES, "gemm_fp8: too many tiles (M=%d N=%d)", a.M, a.N);
   a.rows = p.rows;
   a.splits = p.splits;
   a.box_rows = a.M < a.rows ? (a.M + 7) & ~7 : a.rows;
@@ -1006,7 +1007,7 @@ static Fp8Tile choose_fp8_tile(int M, int N, int blocks) {
     }
   };
   auto larger = [](double a, double b) { return a > b ? a : b; };
-  if (M <= 512) {
+  if (M <= 512 && N <= FS_MAX_TILES * (GATED ? 256 : 128)) {
     const SmallPlan p = small_plan<GATED>(M, N, blocks);
     const int fit = p.splits > 1 ? clusters_that_fit(p.splits, p.resident == 2 ? F8_HALF_SM : F8_WHOLE_SM, 192) : num_sms() * p.resident;
     const int rounds = (p.n_tiles * p.m_tiles + fit - 1) / fit, each = (blocks + p.splits - 1) / p.splits;

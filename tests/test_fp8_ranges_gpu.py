@@ -91,3 +91,16 @@ def test_units_of_gates_that_next_to_nothing_is_left_of(cuda, mode, which, act):
     want[:, 256:] = 0.0
     held(y, ys[:, :M], want, want.abs() * 2.0 ** -19 * (1 + t.abs()) + 1e-30, what=str(which))
     assert (want[:, :256].abs() > 2.0 ** -10).all() and (y[:, :128].float() != 0.0).all()
+
+
+@pytest.mark.parametrize("M", [1, 40])
+def test_more_columns_than_small_tiles_go_round(cuda, M):
+    """65536 tiles of 128 columns and eight columns more: small tiles are counted in a grid's second direction, which ends at 65535"""
+    from llmq_b200 import lib
+    N, K, g = 65536 * 128 + 8, 16, gen(M)
+    a, sa = random_held(g, M, K, 1)
+    w, sw = random_held(g, N, K, 128)
+    c = torch.full((M, N), float("nan"), device="cuda")
+    lib.gemm_fp8(a, sa, w, sw, c)
+    ref, size = product(a, sa, w, sw)
+    assert ((c.double() - ref).abs() <= product_off(size, K) + 1e-30).all()
