@@ -727,7 +727,7 @@ int b200q_decode_attn_q4_set_whole(int whole);
 /* ---- linear layers in 8 bits (fp8_ops.cu, gemm_fp8.cu; conversions: fp8.cuh) --------------------------------------------------
  * A value is an e4m3 code times an fp32 scale.  Activations: codes [T, K], scales [ceil(K / 128)][ld]: element (t, k) is
  * codes[t, k] * scales[k / 128][t]; ld >= T, for products a multiple of 4.  Weights: codes [N, K], scales [ceil(N / 128)]
- * [ceil(K / 128)], one for a square of 128 x 128.  K is a multiple of 16.  A scale is a 448th of its block's largest magnitude (2^-100 at
+ * [ceil(K / 128)], one for a square of 128 x 128.  K is a multiple of 16.  Rows, N (of all groups together) and K are 2^31 - 1024 at most.  A scale is a 448th of its block's largest magnitude (2^-100 at
  * least), codes are rounded to nearest (even).  A block with a NaN or an infinity reads back as NaN throughout.  Matrices are
  * 16-byte aligned; scales behind the last row are neither written nor do they count.  The activations' scales of products are 16-byte aligned too.  No output
  * overlaps an input. */
@@ -740,7 +740,7 @@ int b200q_rmsnorm_fp8(const void* x_dev, void* residual_dev, const void* w_dev, 
  *     of b200q_moe_route), which is not looked at: it has to be one of x */
 int b200q_quantize_fp8(const void* x_dev, int64_t ld_x, const int32_t* rows_dev, void* y_dev, float* scales_dev, int ld_scales, int T, int K,
                        int dtype, void* stream);
-/* weights [groups][N, K] in 8 bits */
+/* weights [groups][N, K] in 8 bits; N <= 8388480, groups <= 65535 */
 int b200q_quantize_fp8_weight(const void* w_dev, void* q_dev, float* scales_dev, int groups, int N, int K, int dtype, void* stream);
 /* C[M,N] = A[M,K] * W[N,K]^T of values in 8 bits, fp32 sums, C bf16 or (out_f32) fp32; N % 8 == 0.  Waits are bounded
  *     (b200q_wait_failures), for the products below too.  No scratch. */

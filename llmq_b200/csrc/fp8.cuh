@@ -10,6 +10,7 @@
 namespace b200q {
 
 constexpr int FP8_BLOCK = 128;
+constexpr int FP8_MOST = 2147483647 - 1023;  // rows, columns, lengths at most: rounded up to whole tiles they are still 32-bit numbers
 
 __device__ __forceinline__ float max_or_nan(float a, float b) {
   float r;

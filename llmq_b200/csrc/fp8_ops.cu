@@ -157,7 +157,7 @@ int b200q_rmsnorm_fp8(const void* x, void* residual, const void* w, void* y, flo
 
 int b200q_quantize_fp8(const void* x, int64_t ld_x, const int32_t* rows, void* y, float* scales, int ld_scales, int T_, int K, int dtype,
                        void* stream) {
-  B200Q_CHECK_ARG(T_ >= 0 && K > 0 && K % 16 == 0 && is_dtype(dtype), "quantize_fp8: bad shape T=%d K=%d or dtype=%d", T_, K, dtype);
+  B200Q_CHECK_ARG(T_ >= 0 && K > 0 && K <= FP8_MOST && K % 16 == 0 && is_dtype(dtype), "quantize_fp8: bad shape T=%d K=%d or dtype=%d", T_, K, dtype);
   B200Q_CHECK_ARG(ld_scales >= T_ && ld_x >= K && ld_x % 8 == 0, "quantize_fp8: ld_scales=%d or ld_x=%lld does not fit", ld_scales, (long long)ld_x);
   if (T_ == 0) return B200Q_OK;
   B200Q_CHECK_ARG(x && y && scales, "quantize_fp8: null argument");
@@ -179,7 +179,7 @@ int b200q_quantize_fp8(const void* x, int64_t ld_x, const int32_t* rows, void* y
 }
 
 int b200q_quantize_fp8_weight(const void* w, void* q, float* scales, int groups, int N, int K, int dtype, void* stream) {
-  B200Q_CHECK_ARG(groups >= 0 && groups <= 65535 && N > 0 && K > 0 && K % 16 == 0 && is_dtype(dtype) && (N + 127) / 128 <= 65535,
+  B200Q_CHECK_ARG(groups >= 0 && groups <= 65535 && N > 0 && N <= 65535 * 128 && K > 0 && K <= FP8_MOST && K % 16 == 0 && is_dtype(dtype),
                   "quantize_fp8_weight: bad shape groups=%d N=%d K=%d or dtype=%d", groups, N, K, dtype);
   if (groups == 0) return B200Q_OK;
   B200Q_CHECK_ARG(w && q && scales, "quantize_fp8_weight: null argument");

@@ -1098,8 +1098,8 @@ static bool fp8_aligned(const void* a, const void* b, const void* c, const void*
 // what all products ask of their arguments
 static int check_product(const char* what, const void* A, const float* as, int ld_as, const void* W, const float* ws, const void* C, int M, int N,
                          int K, bool gated) {
-  B200Q_CHECK_ARG(M >= 0 && N > 0 && K > 0 && K % 16 == 0 && N % (gated ? 256 : 8) == 0, "%s: unsupported shape M=%d N=%d K=%d (K%%16==0, N%%%d==0)", what,
-                  M, N, K, gated ? 256 : 8);
+  B200Q_CHECK_ARG(M >= 0 && N > 0 && K > 0 && K % 16 == 0 && N % (gated ? 256 : 8) == 0 && M <= FP8_MOST && N <= FP8_MOST && K <= FP8_MOST,
+                  "%s: unsupported shape M=%d N=%d K=%d (K%%16==0, N%%%d==0, each up to 2^31 - 1024)", what, M, N, K, gated ? 256 : 8);
   B200Q_CHECK_ARG(ld_as >= M && ld_as % 4 == 0, "%s: ld_a_scales=%d is less than M=%d or no multiple of 4", what, ld_as, M);
   if (M == 0) return B200Q_OK;
   B200Q_CHECK_ARG(A && as && W && ws && C, "%s: null argument", what);
@@ -1154,7 +1154,7 @@ int b200q_gemm_grouped_fp8(const void* A, int a_rows, const float* a_scales, int
                            int N, int K, const void* tab, const int32_t* n_mt, int max_mtiles, int out_f32, void* stream) {
   int rc = check_product("gemm_grouped_fp8", A, a_scales, ld_a_scales, W, w_scales, C, a_rows, N, K, false);
   if (rc) return rc;
-  B200Q_CHECK_ARG(groups > 0 && max_mtiles >= 0 && (long long)groups * N < (1ll << 31), "gemm_grouped_fp8: groups=%d max_mtiles=%d", groups, max_mtiles);
+  B200Q_CHECK_ARG(groups > 0 && max_mtiles >= 0 && (long long)groups * N <= FP8_MOST, "gemm_grouped_fp8: groups=%d max_mtiles=%d", groups, max_mtiles);
   if (a_rows == 0 || max_mtiles == 0) return B200Q_OK;
   B200Q_CHECK_ARG(tab && n_mt && (reinterpret_cast<uintptr_t>(tab) & 15) == 0, "gemm_grouped_fp8: the table of tiles is missing or not aligned");
   Fp8Args a{};
@@ -1178,7 +1178,7 @@ int b200q_gemm_grouped_gated_fp8(const void* A, int a_rows, const float* a_scale
   int rc = check_product("gemm_grouped_gated_fp8", A, a_scales, ld_a_scales, W, w_scales, Y, a_rows, N, K, true);
   if (rc) return rc;
   B200Q_CHECK_ARG((act == 0 || act == 1) && ld_y_scales >= a_rows, "gemm_grouped_gated_fp8: act=%d or ld_y_scales=%d unknown or too small", act, ld_y_scales);
-  B200Q_CHECK_ARG(groups > 0 && max_mtiles >= 0 && (long long)groups * N < (1ll << 31), "gemm_grouped_gated_fp8: groups=%d max_mtiles=%d", groups, max_mtiles);
+  B200Q_CHECK_ARG(groups > 0 && max_mtiles >= 0 && (long long)groups * N <= FP8_MOST, "gemm_grouped_gated_fp8: groups=%d max_mtiles=%d", groups, max_mtiles);
   if (a_rows == 0 || max_mtiles == 0) return B200Q_OK;
   B200Q_CHECK_ARG(tab && n_mt && y_scales && (reinterpret_cast<uintptr_t>(tab) & 15) == 0,
                   "gemm_grouped_gated_fp8: the table of tiles or y_scales is missing or not aligned");
