@@ -764,6 +764,8 @@ int b200q_gemm_grouped_gated_fp8(const void* A_dev, int a_rows, const float* a_s
 /* test hooks: 0 = by size, 1 = small tiles, 2 = large tiles of single CTAs, 3 = of pairs, 4 and 5 = these in mode / 100 parts of the reduction;
  *     mode / 10 % 10: 64 columns each to a dense product's tile.  The mode that stands for what a dense product takes. */
 int b200q_gemm_fp8_set_mode(int mode);
+/*     n > 0 = every warp of products gives up before its n-th block: outputs are missing or wrong, and b200q_wait_failures says so; 0 = normal */
+int b200q_gemm_fp8_set_give_up(int n);
 int b200q_gemm_fp8_choice(int M, int N, int K, int gated);
 
 /* nonzero once a kernel's bounded wait has run out in this process (its outputs are then missing or wrong); engine steps report

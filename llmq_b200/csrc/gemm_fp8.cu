@@ -38,6 +38,10 @@ struct Fp8Args {
   int ld_as, ld_ys, M, N, K, blocks, n_blocks, max_mt, groups, ahead, out_f32, gelu, a_bytes;
   // small tiles
   int rows, box_rows, stages, accs, cols, splits;
+  // blocks that a warp of products makes before it gives up (a test's; else more than there are); large: cycles that a wait lasts (read from here the
+  // small kernel's cost 48 x 4096 x 14336 0.4 us)
+  long long patience;
+  int give_up;
 };
 
 __device__ __forceinline__ void umma_fp8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
@@ -106,20 +110,28 @@ __device__ __forceinline__ float fp8_unit(float g, float u, int gelu) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(e, 0.25f, 0.25f)));
   return q * r * u;
 }
-// (dead: another role of the CTA has given up; flag and clock are looked at every 64 tries)
-__device__ __forceinline__ void f8_wait(uint64_t* bar, uint32_t parity, volatile int* dead, int* failed) {
+// A wait with a limit: false where it has run out, or another role of the CTA has given up (dead; flag and clock are looked at every 64 tries).  Who
+// is told so issues nothing more: a load would come to a place that is still read, or arm a barrier that is armed, a product would read what has not
+// come.
+__device__ __forceinline__ bool f8_give_up(volatile int* dead, int* failed) {
+  *dead = 1;
+  __threadfence_block();
+  *(volatile int*)failed = 1;
+  return false;
+}
+[[nodiscard]] __device__ __forceinline__ bool f8_wait(uint64_t* bar, uint32_t parity, volatile int* dead, int* failed, long long limit = WAIT_CYCLES) {
   long long t0 = 0;
   for (int n = 0; !mbar_try_wait(bar, parity); ++n) {
     if (n % 64 != 63) continue;
     if (n == 63) t0 = clock64();
-    if (*dead) return;
-    if (clock64() - t0 > WAIT_CYCLES) {
-      *dead = 1;
-      __threadfence_block();
-      *(volatile int*)failed = 1;
-      return;
-    }
+    if (*dead) return false;
+    if (clock64() - t0 > limit) return f8_give_up(dead, failed);
   }
+  return true;
+}
+// the same of who looks at `dead` itself before anything is issued, or issues nothing
+__device__ __forceinline__ void f8_await(uint64_t* bar, uint32_t parity, volatile int* dead, int* failed, long long limit = WAIT_CYCLES) {
+  (void)f8_wait(bar, parity, dead, failed, limit);
 }
 // copies in flight end before a block that gave up returns its memory
 __device__ __noinline__ void f8_let_copies_end() {
@@ -248,13 +260,15 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
       if (lane == 0) {
         int stage = 0;
         uint32_t phase = 0;
-        for (int tile = unit; tile < num_tiles; tile += units) {
+        bool on = true;
+        for (int tile = unit; on && tile < num_tiles; tile += units) {
           int g, row0, row_end, n0;
           tile_of(tile, entry_of(tile), g, row0, row_end, n0);
           const int wrow = g * a.N + n0;
           for (int b = b_begin; b < b_end; ++b) {
             uint8_t* to = smem + stage * Cfg::STAGE;
-            f8_wait(empty + stage, phase ^ 1u, &dead, a.failed);
+            on = f8_wait(empty + stage, phase ^ 1u, &dead, a.failed, a.patience);
+            if (!on) break;
             if constexpr (PAIR) {
               const uint32_t bar = mapa_shared(full + stage, leader);
               f8_expect_tx(bar, Cfg::STAGE - F8_STAGE_W + a.a_bytes);
@@ -272,7 +286,6 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
               phase ^= 1u;
             }
           }
-          if (*(volatile int*)&dead) break;
         }
       }
       __syncwarp();
@@ -283,11 +296,15 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
       const uint64_t rows = make_smem_desc(ring), columns = make_smem_desc(ring + F8_STAGE_W + h * (Cfg::W_ROWS / 2) * FP8_BLOCK);
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
+      int left = a.give_up;
+      bool on = true;
       if (elect_one())
-        for (int tile = unit; tile < num_tiles; tile += units) {
-          for (int b = b_begin; b < b_end; ++b) {
-            f8_wait(full + stage, phase, &dead, a.failed);
-            f8_wait(acc_empty[h] + acc, acc_phase ^ 1u, &dead, a.failed);
+        for (int tile = unit; on && tile < num_tiles; tile += units) {
+          const int b_stop = left < b_end - b_begin ? b_begin + left : b_end;
+          left -= b_stop - b_begin;
+          for (int b = b_begin; b < b_stop; ++b) {
+            on = f8_wait(full + stage, phase, &dead, a.failed, a.patience) && f8_wait(acc_empty[h] + acc, acc_phase ^ 1u, &dead, a.failed, a.patience);
+            if (!on) break;
             tc_fence_after();
             const uint64_t at = (uint64_t)(stage * (Cfg::STAGE / 16));  // (addresses in descriptors count 16 bytes)
             const uint32_t d = tmem + (uint32_t)(acc * BN + h * (BN / 2));
@@ -311,7 +328,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
             }
             next_acc(acc, acc_phase);
           }
-          if (*(volatile int*)&dead) break;
+          if (b_stop < b_end) on = f8_give_up(&dead, a.failed);
         }
       __syncwarp();
     }
@@ -326,6 +343,10 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
     const uint32_t empty0 = PAIR ? mapa_shared(acc_empty[half], leader) : smem_u32(acc_empty[half]);
     int acc = 0, parity = 0;
     uint32_t acc_phase = 0;
+    auto await_sums = [&]() {
+      f8_await(acc_full[half] + acc, acc_phase, &dead, a.failed, a.patience);
+      __syncwarp();
+    };
     // Weights' scales: a lane's of 32 blocks of the reduction, handed round by shuffles.  A tile's columns lie in up to two blocks of 128 (gated:
     // the gates' and that of what they gate); 32 neighbouring columns lie in one.  Rows' scales: four blocks'.  A tile's first are asked for
     // while the one before it leaves.  (Without a condition: a load that may not be made is waited for where it is made.  Rows and blocks that do
@@ -362,8 +383,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
       const bool live = row < row_end;
       if (!SPLIT && row0 + quarter * 32 >= row_end) {  // no rows: the accumulators only have to be passed on
         for (int b = b_begin; b < b_end; ++b) {
-          f8_wait(acc_full[half] + acc, acc_phase, &dead, a.failed);
-          __syncwarp();
+          await_sums();
           if (lane == 0) f8_arrive(empty0 + acc * 8);
           next_acc(acc, acc_phase);
         }
@@ -379,8 +399,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
 #pragma unroll
         for (int j = 0; j < 16; ++j) sum[c][j] = 0ull;
       uint32_t v[2][32];
-      f8_wait(acc_full[half] + acc, acc_phase, &dead, a.failed);
-      __syncwarp();
+      await_sums();
       tc_fence_after();
       tmem_ld32(lanes + (uint32_t)(acc * BN), v[0]);
       // (a block is an odd number of loads where CH is 3: its first goes to v[i & 1] there, four blocks to a round)
@@ -418,8 +437,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
                 if (lane == 0) f8_arrive(empty0 + acc * 8);
                 next_acc(acc, acc_phase);
                 if (b0 + i + 1 < b_end) {
-                  f8_wait(acc_full[half] + acc, acc_phase, &dead, a.failed);
-                  __syncwarp();
+                  await_sums();
                   tc_fence_after();
                   tmem_ld32(lanes + (uint32_t)(acc * BN), next);
                 }
@@ -443,7 +461,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
             }
         }
         cluster_sync_all();
-        for (int piece = split + (warp - 4) * a.splits; piece < 16 * CH; piece += 8 * a.splits) {
+        for (int piece = dead ? 16 * CH : split + (warp - 4) * a.splits; piece < 16 * CH; piece += 8 * a.splits) {
           const int r0 = row0 + piece / (4 * CH) * 32, n = n0 + piece % (4 * CH) * 16;
           if (r0 >= row_end) break;
           float4 total[4];
@@ -504,7 +522,18 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
         uint8_t* const out = patches + (2 * quarter + parity) * Cfg::PATCH;
         const bool copies = half == 0 && lane == 0, engine = !GROUPED || row0 + quarter * 32 + 32 <= row_end;  // (no rows that are another group's)
         if (copies) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-        asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+        uint32_t gone = *(volatile int*)&dead;  // (for both warps, which meet again below)
+        asm volatile(
+            "{\n\t"
+            ".reg .pred p;\n\t"
+            "setp.ne.b32 p, %0, 0;\n\t"
+            "bar.red.or.pred p, %1, 64, p;\n\t"
+            "selp.b32 %0, 1, 0, p;\n\t"
+            "}\n"
+            : "+r"(gone)
+            : "r"(1 + quarter)
+            : "memory");
+        if (gone) break;
         const float scale = fp8_scale(max_or_nan(m, most[half ^ 1][quarter * 32 + lane])), by = fp8_inverse(scale);
         if (half == 0 && live) a.ys[(long long)(n0 / 256) * a.ld_ys + row] = scale;
 #pragma unroll
@@ -532,6 +561,8 @@ __global__ void __launch_bounds__(FL_THREADS, 1)
           }
         }
         parity ^= 1;
+      } else if (__any_sync(0xffffffffu, *(volatile int*)&dead)) {
+        break;
       } else if (a.out_f32) {
         float* to = (float*)a.C + (long long)row * a.N + n0 + half * (BN / 2);
         const int cols = a.N - n0 - half * (BN / 2);
@@ -678,8 +709,8 @@ __global__ void __launch_bounds__(small_threads<GATED>(MOST), small_resident<GAT
       uint32_t phase = 0;
       for (int b = b0; b < b1; ++b) {
         uint8_t* to = smem + stage * stage_bytes;
-        f8_wait(empty + stage, phase ^ 1u, &dead, a.failed);
-        if (*(volatile int*)&dead) break;
+        f8_await(empty + stage, phase ^ 1u, &dead, a.failed);
+        if (*(volatile int*)&dead) break;  // (warps whose waits have run out arrive all the same, behind the flag)
         mbar_expect_tx(full + stage, bytes);
         tma_load_2d(to, &tmap_w, b * 64, n0, full + stage);
         tma_load_2d(to + WT * F8_STAGE_W, &tmap_a, b * 64, row0, full + stage);
@@ -697,10 +728,11 @@ __global__ void __launch_bounds__(small_threads<GATED>(MOST), small_resident<GAT
     const uint64_t weights = make_smem_desc(ring), rows_of_a = make_smem_desc(ring + WT * F8_STAGE_W);
     int stage = 0, acc = 0;
     uint32_t phase = 0, acc_phase = 0;
-    if (elect_one())
-      for (int b = b0; b < b1; ++b) {
-        f8_wait(acc_empty + acc, acc_phase ^ 1u, &dead, a.failed);
-        f8_wait(full + stage, phase, &dead, a.failed);
+    const int b_stop = a.give_up < b1 - b0 ? b0 + a.give_up : b1;
+    if (elect_one()) {
+      for (int b = b0; b < b_stop; ++b) {
+        f8_await(acc_empty + acc, acc_phase ^ 1u, &dead, a.failed);
+        f8_await(full + stage, phase, &dead, a.failed);
         if (*(volatile int*)&dead) break;
         tc_fence_after();
         const uint64_t at = (uint64_t)(uint32_t)(stage * (stage_bytes / 16));  // (addresses in descriptors count 16 bytes)
@@ -720,6 +752,8 @@ __global__ void __launch_bounds__(small_threads<GATED>(MOST), small_resident<GAT
           acc_phase ^= 1u;
         }
       }
+      if (b_stop < b1) f8_give_up(&dead, a.failed);
+    }
     __syncwarp();
   }
 
@@ -741,8 +775,8 @@ __global__ void __launch_bounds__(small_threads<GATED>(MOST), small_resident<GAT
       if ((b - b0) % 32 == 0 && b + lane < b1) sw = w0[b + lane];
       const float x = __shfl_sync(0xffffffffu, sw, (b - b0) & 31);
       const f32x2 by = pair_of(x, x);
-      f8_wait(full + stage, phase, &dead, a.failed);  // (the scales)
-      f8_wait(acc_full + acc, acc_phase, &dead, a.failed);
+      f8_await(full + stage, phase, &dead, a.failed);  // (the scales)
+      f8_await(acc_full + acc, acc_phase, &dead, a.failed);
       __syncwarp();
       tc_fence_after();
       uint32_t v[CHUNKS][32];
@@ -980,6 +1014,7 @@ static int launch_small(const void* A, const void* W, const Fp8Args& a, cudaStre
 }
 
 int g_fp8_mode = 0;  // test hook: see b200q_gemm_fp8_set_mode
+int g_fp8_give_up = 0;
 
 // Which kernel and tile: the least of what each is expected to take, us.  A round of tiles (as many as are resident at once) costs so much for
 // its start and end and so much a block; no kernel takes less than the weights do to come from memory; parts cost their exchange.  Fitted to
@@ -1049,6 +1084,8 @@ static Fp8Tile choose_fp8_tile(int M, int N, int blocks) {
 static int finish_args(Fp8Args& a) {
   a.blocks = (a.K + FP8_BLOCK - 1) / FP8_BLOCK;
   a.n_blocks = (a.N + 127) / 128;
+  a.patience = g_fp8_give_up ? 200000 : WAIT_CYCLES;
+  a.give_up = g_fp8_give_up ? g_fp8_give_up - 1 : 2147483647;
   if (!wait_flag(&a.failed)) {
     set_error("gemm_fp8: no host-visible flag for bounded waits");
     return B200Q_ECUDA;
@@ -1207,6 +1244,15 @@ int b200q_gemm_fp8_set_mode(int mode) {
   B200Q_CHECK_ARG(mode >= 0 && kind <= 5 && (ch == 0 || (ch >= 2 && ch <= 4)) && splits <= (kind == 5 ? FL_MAX_SPLITS / 2 : FL_MAX_SPLITS) && (splits > 0) == (kind >= 4),
                   "gemm_fp8_set_mode: mode=%d", mode);
   g_fp8_mode = mode;
+  bump_tuning_epoch();
+  return B200Q_OK;
+}
+
+// test hook: n > 0 = every warp of products gives up before its n-th block (b200q_wait_failures says so; what large
+// tiles had no sums for is not stored, small ones are wrong) and waits of pairs last some 100 us, 0 = normal
+int b200q_gemm_fp8_set_give_up(int n) {
+  B200Q_CHECK_ARG(n >= 0, "gemm_fp8_set_give_up: n=%d", n);
+  g_fp8_give_up = n;
   bump_tuning_epoch();
   return B200Q_OK;
 }

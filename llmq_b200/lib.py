@@ -325,6 +325,7 @@ SIGNATURES = {
     "b200q_gemm_grouped_fp8": (_i, [_vp, _i, _vp, _i, _vp, _vp, _i, _vp, _i, _i, _vp, _vp, _i, _i, _vp]),
     "b200q_gemm_grouped_gated_fp8": (_i, [_vp, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _vp, _vp, _i, _i, _vp]),
     "b200q_gemm_fp8_set_mode": (_i, [_i]),
+    "b200q_gemm_fp8_set_give_up": (_i, [_i]),
     "b200q_gemm_fp8_choice": (_i, [_i, _i, _i, _i]),
     "b200q_pages_fork": (_i, [_vp, _vp, _i, _vp, _i, _i, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp]),
     "b200q_pages_free": (_i, [_vp, _vp, _vp, _i, _i, _vp, _i, _i, _vp]),
