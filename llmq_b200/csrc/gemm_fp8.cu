@@ -895,13 +895,18 @@ static int once_per_device(std::atomic<uint64_t> (&seen)[2], F&& f) {
 }
 
 // As many clusters of so many CTAs as can be resident at once, by their shared memory (one of 225 KiB to an SM, or two of 107): asked of a
-// kernel that is never launched, since the query knows one CTA to an SM for kernels that hold tensor memory.
+// kernel that is never launched, since the query knows one CTA to an SM for kernels that hold tensor memory.  Asked once on each device (which SMs a
+// device has, and so how many clusters fit, is its own); where the query fails, by the number of SMs, and again the next time.
 __global__ void fp8_probe_kernel() {}
 constexpr int F8_WHOLE_SM = 230400, F8_HALF_SM = 109568;
 static int clusters_that_fit(int cluster, int smem, int threads) {
-  static std::atomic<int> known[2][FL_MAX_SPLITS + 1];
-  std::atomic<int>& kept = known[smem == F8_HALF_SM][cluster];
-  if (int n = kept.load()) return n;
+  constexpr int DEVICES = 64;
+  static std::atomic<int> known[DEVICES][2][FL_MAX_SPLITS + 1];
+  int dev = -1;
+  cudaGetDevice(&dev);
+  std::atomic<int>* const kept = dev >= 0 && dev < DEVICES ? &known[dev][smem == F8_HALF_SM][cluster] : nullptr;
+  if (kept)
+    if (int n = kept->load()) return n;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(cluster, 148);
   cfg.blockDim = dim3(threads);
@@ -916,9 +921,9 @@ static int clusters_that_fit(int cluster, int smem, int threads) {
   if (cudaFuncSetAttribute(fp8_probe_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F8_WHOLE_SM) != cudaSuccess ||
       cudaOccupancyMaxActiveClusters(&n, fp8_probe_kernel, &cfg) != cudaSuccess || n <= 0) {
     cudaGetLastError();
-    n = num_sms() * (smem == F8_HALF_SM ? 2 : 1) / cluster;
+    return num_sms() * (smem == F8_HALF_SM ? 2 : 1) / cluster;
   }
-  kept.store(n);
+  if (kept) kept->store(n);
   return n;
 }
 
