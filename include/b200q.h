@@ -727,13 +727,14 @@ int b200q_decode_attn_q4_set_whole(int whole);
 /* ---- linear layers in 8 bits (fp8_ops.cu, gemm_fp8.cu; conversions: fp8.cuh) --------------------------------------------------
  * A value is an e4m3 code times an fp32 scale.  Activations: codes [T, K], scales [ceil(K / 128)][ld]: element (t, k) is
  * codes[t, k] * scales[k / 128][t]; ld >= T, for products a multiple of 4.  Weights: codes [N, K], scales [ceil(N / 128)]
- * [ceil(K / 128)], one for a square of 128 x 128.  K is a multiple of 16.  Rows, N (of all groups together) and K are 2^31 - 1024 at most.  A scale is a 448th of its block's largest magnitude (2^-100 at
- * least), codes are rounded to nearest (even).  A block with a NaN or an infinity reads back as NaN throughout.  Matrices are
- * 16-byte aligned; scales behind the last row are neither written nor do they count.  The activations' scales of products are 16-byte aligned too.  No output
- * overlaps an input. */
+ * [ceil(K / 128)], one for a square of 128 x 128.  K is a multiple of 16.  Rows, N (of all groups together) and K are 2^31 - 1024 at
+ * most.  A scale is a 448th of its block's largest magnitude (2^-100 at least), codes are rounded to nearest (even).  A block with a NaN
+ * or an infinity reads back as NaN throughout.  Matrices are 16-byte aligned, the activations' scales of products too; scales behind the
+ * last row are neither written nor do they count.  No output overlaps an input. */
 
 /* b200q_rmsnorm / b200q_add_rmsnorm with an output in 8 bits: residual <- x + residual (rounded to its type; NULL: x alone), y = that
- *     / sqrt(mean of its squares + eps) * w, not rounded before it is quantised.  dtype: of x, residual and w.  x is not written; H <= 16384. */
+ *     / sqrt(mean of its squares + eps) * w, not rounded before it is quantised.  dtype: of x, residual and w.  x is not written; H <= 16384.
+ *     Squares and their sum are fp32's: rows of magnitudes from 2^-60 to 2^60. */
 int b200q_rmsnorm_fp8(const void* x_dev, void* residual_dev, const void* w_dev, void* y_dev, float* scales_dev, int ld_scales, int T, int H,
                       float eps, int dtype, void* stream);
 /* rows of x (ld_x elements apart, a multiple of 8) in 8 bits; rows != NULL: row i of y is row rows[i] of x (tokens sorted by expert: perm_tok
@@ -762,10 +763,11 @@ int b200q_gemm_grouped_gated_fp8(const void* A_dev, int a_rows, const float* a_s
                                  const float* w_scales_dev, int groups, void* Y_dev, float* y_scales_dev, int ld_y_scales, int N, int K,
                                  const void* tab_dev, const int32_t* n_mt_dev, int max_mtiles, int act, void* stream);
 /* test hooks: 0 = by size, 1 = small tiles, 2 = large tiles of single CTAs, 3 = of pairs, 4 and 5 = these in mode / 100 parts of the reduction;
- *     mode / 10 % 10: 64 columns each to a dense product's tile.  The mode that stands for what a dense product takes. */
+ *     mode / 10 % 10: 64 columns each to a dense product's tile.  Products by expert take large tiles of single CTAs whatever it is. */
 int b200q_gemm_fp8_set_mode(int mode);
 /*     n > 0 = every warp of products gives up before its n-th block: outputs are missing or wrong, and b200q_wait_failures says so; 0 = normal */
 int b200q_gemm_fp8_set_give_up(int n);
+/*     the mode that stands for what a dense product takes */
 int b200q_gemm_fp8_choice(int M, int N, int K, int gated);
 
 /* nonzero once a kernel's bounded wait has run out in this process (its outputs are then missing or wrong); engine steps report

@@ -68,7 +68,8 @@ __global__ void __launch_bounds__(256)
 }
 
 // y[i] = row rows[i] (NULL: i) of x in 8 bits.  Eight lanes to a block of 128 values, and no more than one block: many short CTAs keep more reads
-// under way than longer ones (4608 x 4096: 10.3 us, two blocks 11.8, four 12.3; 4004 gathered rows of 2048 4.7 / 5.9 / 5.9).
+// under way than longer ones (one measurement: 4608 x 4096 10.3 us, two blocks 11.8, four 12.3; 4004 gathered rows of 2048 4.7 / 5.9 / 5.9.  Others, inputs
+// from HBM: 10.5 to 10.8 and 5.2 to 5.3).
 template <typename T>
 __global__ void __launch_bounds__(256)
     quantize_fp8_kernel(const T* __restrict__ x, long long ld_x, const int32_t* __restrict__ rows, uint2* __restrict__ y,

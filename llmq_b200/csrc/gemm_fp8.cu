@@ -6,11 +6,12 @@
 // Two or four accumulators let the tensor core work on the next blocks meanwhile.
 //
 // Bounds: for few rows the weight stream (N K bytes); for many the tensor core at twice the bf16 rate and, as near, tensor memory, which products
-// fill while the promotion reads it (32 columns: some 165 cycles beside products, 16 to 30 alone), two packed multiply-adds to four sums; at the
-// largest sizes the clock as well, which the power limit holds at 1.2 to 1.3 GHz.  us, back to back in a graph, weights from HBM: 1 x 4096 x 4096 6.1,
-// 48 x 4096 x 14336 14.5 (4.1 TB/s of weights; bf16 24.7), 1001 x 8192 x 3584 33.5 (1.76 PFLOP/s; bf16 50), 4608 x 4096 x 14336 252 to 260
-// (2.1 PFLOP/s; bf16 413 to 422; the library's product of the same codes with one scale for all of them 196, of zeros 133); gated 7 x 16384 x 2048
-// 9.4 to 10.5, 4608 x 28672 x 4096 516 to 522 (bf16 770); 16 experts of 2048 x 2048, 64 tokens to four of them 17 (3.9 TB/s of weights).
+// fill while the promotion reads it (32 columns: some 165 cycles beside products, 16 to 30 alone), two packed multiply-adds to four sums; over a second
+// of them the clock, which the power limit holds at 1.2 to 1.5 GHz.  us, back to back in a graph, weights from HBM (the first milliseconds / over a
+// second): 1 x 4096 x 4096 6.3, 48 x 4096 x 14336 14.7 (4.0 TB/s of weights; bf16 24), 1001 x 8192 x 3584 29.9 / 34.7 (1.97 / 1.70 PFLOP/s; bf16
+// 44.9 / 51.7), 4608 x 4096 x 14336 231 / 265 (2.34 / 2.04 PFLOP/s; bf16 370 / 428; over a second the library's product of the same codes with one scale
+// for all of them 196, of zeros 133); gated 7 x 16384 x 2048 9.3, 4608 x 28672 x 4096 463 / 529 (bf16 684 / 781); 16 experts of 2048 x 2048, 64
+// tokens to four of them 16.1 / 17.2 (4.2 TB/s of weights).
 //
 //   * large: rows of A are the tensor core's M side (a lane has a row, so that its scale is one number to a thread), up to 256 columns to a CTA,
 //     eight warps that promote half of them each in up to 128 registers a thread.  Persistent.  One CTA to 128 rows, or a pair (cta_group::2) to
@@ -1023,9 +1024,10 @@ int g_fp8_give_up = 0;
 
 // Which kernel and tile: the least of what each is expected to take, us.  A round of tiles (as many as are resident at once) costs so much for
 // its start and end and so much a block; no kernel takes less than the weights do to come from memory; parts cost their exchange.  Fitted to
-// 450 sizes (15 shapes of 1024 to 16384 columns x 1024 to 14336, 30 row counts from 1 to 4608, weights from HBM, back to back in a graph) and
-// every kernel: what is taken is 0.5 % slower than the best on average, more than 5 % at 9 of them, and 10 % at 3000 x 2304 x 9216 (pairs of 192
-// columns 68.9 us, of 256 62.7).  us, the choice / others: 1 x 4096 x 4096 small 6.3 / four parts of 128 columns 8.3; 48 x 4096 x 14336 small 14.5 / four
+// 450 sizes (15 shapes of 1024 to 16384 columns x 1024 to 14336, 30 row counts from 1 to 4608, weights from HBM, bf16 outputs, back to back in a
+// graph) and every kernel: what is taken is 0.5 % slower than the best on average, more than 5 % at 9 of them, and 10 % at 3000 x 2304 x 9216 (pairs
+// of 192 columns 68.9 us, of 256 62.7).  us (of that measurement: one card, its large products at the power limit), the choice / others:
+// 1 x 4096 x 4096 small 6.3 / four parts of 128 columns 8.3; 48 x 4096 x 14336 small 14.5 / four
 // parts 15.9; 128 x 4096 x 14336 four parts of 128 columns 16.7 / small 22.5, whole tiles 43; 200 x 4096 x 14336 three parts of 192 columns
 // 23.0 / two of 128 23.4, whole 43; 300 x 8192 x 3584 pairs of 256 columns 15.7 / single CTAs 16.3, of 128 columns 21.1; 450 x 4096 x 14336 pairs
 // in two parts 35.1 / 128 columns 37.8; 768 x 4096 x 4096 pairs of 256 17.2 / of 192 17.4, 128 columns 23.1; 4608 x 4096 x 14336 pairs of 256

@@ -38,8 +38,9 @@ def half_step(r):
 
 def held_close(code, scales, x, off, tall=1, what=""):
     """codes and scales (of weights, or of rows cut to [blocks, rows]) are those of x, of which the kernel knew values that were `off` away (a
-    tensor or number).  The scale is a quotient rounded once, the code a product with a reciprocal: 2^-24 each for the scale, the reciprocal and
-    the product, which count as 2^-22; behind them a rounding of half a step of e4m3."""
+    tensor or number).  The scale is a product with 1 / 448: the constant off by 0.38 x 2^-23, the product by 2^-24, 0.88 x 2^-23 together, for which
+    2^-23 is allowed.  The code is a product with the reciprocal of the scale that is given here: 2^-23 and 2^-24, for which 2^-22 is allowed; behind
+    them a rounding of half a step of e4m3.  (What a norm multiplies by beforehand is part of `off`.)"""
     rows, K = x.shape
     x = x.double()
     off = torch.as_tensor(off, dtype=torch.float64, device=x.device).expand(x.shape)
